@@ -63,7 +63,9 @@ enum {
   PA_STATUS_BAD_POSITION = 2,
   PA_STATUS_BAD_NUM_BLOCKS = 4,
   PA_STATUS_BAD_SEQ_INDEX = 8,
-  PA_STATUS_PEER_TIMEOUT = 32
+  PA_STATUS_PEER_TIMEOUT = 32,
+  PA_STATUS_COPY_OVERLAP = 64, /* a page copy into another copy's source or target  */
+  PA_STATUS_BAD_POOL = 128     /* block pool arrays that contradict each other      */
 };
 
 /*
@@ -421,6 +423,130 @@ int block_pool_step(const pa_block_pool_t* pool, const int32_t* seq_slot, const 
                     const int32_t* cu_seqlens, int32_t num_seqs, int32_t* block_table, int64_t bt_stride,
                     int32_t bt_cols, int32_t* num_blocks, int32_t* positions, int32_t* token_seq,
                     int32_t total_tokens, int32_t* status, void* stream);
+
+/*
+ * Copies of pages inside the pools of num_layers layers, in one launch (per 64
+ * layers): block src[i] to block dst[i], K, V and an INT8 pool's scales.  The
+ * caches differ in their pointers only; layer 0's shape and strides hold for
+ * all.  num_slots int32 [num_pairs] copies the first num_slots[i] slots of a
+ * block (0: none) and leaves the others as they are; NULL copies whole blocks.
+ * A scale per block goes with any number of slots.  src, dst and num_slots are
+ * device pointers.  The copies act at once, so a pair whose target is another
+ * pair's source, or an earlier pair's target, is skipped and reported as
+ * PA_STATUS_COPY_OVERLAP; ids outside the pool are skipped as
+ * PA_STATUS_BAD_BLOCK_ID, num_slots outside 0..block_size as
+ * PA_STATUS_BAD_POSITION; a pair with src[i] == dst[i] does nothing.
+ * The reference has no page copies (its blocks belong to one sequence each,
+ * core/block_manager.py:19-68).
+ */
+int kv_copy_blocks(const pa_kv_cache_t* caches, int32_t num_layers, const int32_t* src, const int32_t* dst,
+                   const int32_t* num_slots, int32_t num_pairs, int32_t* status, void* stream);
+
+/*
+ * Blocks shared between sequences: a count of holders beside the block pool.
+ *   ref_count      int32 [num_blocks], 0 = free
+ *   scratch        int32 [scratch_words], zero before its first use; the calls
+ *                  below leave it ready for the next.  One pool's calls must
+ *                  not overlap, as with the pool itself.
+ *   scratch_words  >= block_pool_scratch_words(num_blocks)
+ *                  (16 + 3 * num_blocks + ceil(num_blocks / 32))
+ * A block is written only while one sequence holds it: forks share the blocks
+ * that their tokens fill and copy a partly filled last one.
+ */
+typedef struct {
+  int32_t* ref_count;
+  int32_t* scratch;
+  int64_t scratch_words;
+} pa_block_share_t;
+
+int64_t block_pool_scratch_words(int32_t num_blocks);
+
+/* block_pool_init, with no holders and zeroed scratch. */
+int block_pool_init_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, void* stream);
+
+/*
+ * block_pool_apply with holders counted, ops int32 [n_ops][4] = (kind, slot, n,
+ * parent): PA_POOL_ALLOCATE and PA_POOL_RELEASE as there (a release frees, in
+ * list order, the blocks without another holder), and
+ *   PA_POOL_FORK  slot (without an entry) becomes a copy of `parent` at n
+ *                 tokens: it shares the n / block_size full blocks, and gets a
+ *                 new block for a partly filled last one.  FAILURE when slot
+ *                 has an entry or parent none, ROW_FULL when parent holds fewer
+ *                 blocks, INSUFFICIENT_SPACE when no block is free.
+ * copy_src / copy_dst / copy_slots (int32 [n_ops] each, or all NULL) receive
+ * the page copy that operation i needs, for kv_copy_blocks; equal ids where it
+ * needs none.
+ */
+enum { PA_POOL_FORK = 2 };
+int block_pool_apply_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* ops,
+                            int32_t n_ops, int32_t block_size, int32_t* results, int32_t* copy_src, int32_t* copy_dst,
+                            int32_t* copy_slots, void* stream);
+
+/*
+ * Beams take over their parents' state.  Group g's beams hold pool rows
+ * slots[g][0..num_beams), all with num_tokens[g] tokens (and equally many
+ * blocks); beam j continues beam parents[g][j].  The first child of a parent
+ * keeps its row, the other children take the rows of the beams without
+ * children (both in ascending order); slots_out[g][j] is beam j's row
+ * afterwards (another array than slots).  A row taken over shares the parent's
+ * full blocks, and the tokens of a partly filled last block are copied, in
+ * every layer, into the row's own; blocks past it stay with their row.
+ * Blocks without holders are pushed in ascending order.  One launch (per 64
+ * layers), nothing is read back; all arrays int32 on the device.  Every row
+ * belongs to one beam of one group.  A group with a bad or repeated row, a bad
+ * parent (PA_STATUS_BAD_SEQ_INDEX), or rows whose blocks do not hold its
+ * tokens or are not equally many (PA_STATUS_BAD_POSITION) is left as it is.
+ * Limits: 1 <= num_beams <= 32.
+ */
+int block_pool_reorder(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* slots,
+                       const int32_t* parents, const int32_t* num_tokens, int32_t num_groups, int32_t num_beams,
+                       int32_t* slots_out, const pa_kv_cache_t* caches, int32_t num_layers, int32_t* status,
+                       void* stream);
+
+/*
+ * Move the blocks in use to the lowest ids: those at or above the number L in
+ * use go, in ascending order, to the free ids below it; every row, the holder
+ * counts and the pages of every layer follow.  The free list becomes
+ * num_blocks_after - 1 .. L (L is handed out next), so that no id at or above
+ * num_blocks_after is in use or handed out again and that memory can be given
+ * up.  live (int32 [1], device, may be NULL) receives L.  More blocks in use
+ * than num_blocks_after: nothing changes, PA_STATUS_BAD_POOL.
+ */
+int block_pool_compact(const pa_block_pool_t* pool, const pa_block_share_t* share, int32_t num_blocks_after,
+                       int32_t* live, const pa_kv_cache_t* caches, int32_t num_layers, int32_t* status, void* stream);
+
+/*
+ * The best continuations of every sequence's beams over the vocabulary:
+ *   score(b, k, v) = scores[b][k] + x[b][k][v] - log sum_u exp(x[b][k][u])
+ * and out_* [num_seqs][num_out] hold the num_out largest, in the order of
+ * score, then lower beam, then larger logit, then lower token.
+ *   logits    [num_seqs, num_beams, vocab] PA_DTYPE_F32, F16 or BF16, vocab
+ *             contiguous, any alignment; NaN counts as -inf, +inf as FLT_MAX
+ *   scores    fp32 [num_seqs, num_beams]; NaN counts as -inf
+ *   finished  uint8 [num_seqs, num_beams] or NULL: a finished beam's logits are
+ *             not read; its log-probabilities are 0 at eos_id and -inf elsewhere
+ * Sums are held in fp32 per split and joined in 64 bits; scores are compared
+ * in 64 bits and rounded once to fp32.
+ * Limits: num_beams <= 32, num_out <= min(32, num_beams * vocab).
+ */
+typedef struct {
+  const void* logits;
+  const float* scores;
+  const uint8_t* finished;
+  int64_t stride_seq, stride_beam;
+  int32_t dtype;
+  int32_t num_seqs;
+  int32_t num_beams;
+  int32_t vocab;
+  int32_t eos_id;
+  int32_t num_out;
+  float* out_scores;
+  int32_t* out_tokens;
+  int32_t* out_parents;
+} pa_beam_select_t;
+
+int beam_select_workspace_size(const pa_beam_select_t* args, size_t* bytes);
+int beam_select(const pa_beam_select_t* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Message for the last failing call on this thread ("" if none). */
 const char* paged_attn_error_string(void);

@@ -979,6 +979,276 @@ int block_pool_step(const pa_block_pool_t* pool, const int32_t* seq_slot, const 
   return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_step launch");
 }
 
+// ---- shared blocks, page copies, beams -------------------------------------------
+// Pages of every layer, as kernel parameters: the layers [first, first + 64).
+static int page_params(const pa_kv_cache_t* caches, int32_t num_layers, int32_t first, pa::PageParams& g) {
+  memset(&g, 0, sizeof(g));
+  const pa_kv_cache_t& a = caches[0];
+  const int e = elt_size(a.dtype), H = a.num_kv_heads, D = a.head_dim, BS = a.block_size;
+  g.layers = num_layers - first < pa::kMaxLayers ? num_layers - first : pa::kMaxLayers;
+  g.num_blocks = a.num_blocks;
+  g.block_size = BS;
+  g.heads = H;
+  g.row_vecs_log2 = ilog2(D * e / 16);
+  g.scale_bytes = a.scale_dtype == PA_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < g.layers; ++i) {
+    const pa_kv_cache_t& c = caches[first + i];
+    g.page[0][i] = static_cast<char*>(c.k);
+    g.page[1][i] = static_cast<char*>(c.v);
+    if (a.dtype == PA_DTYPE_I8) {
+      g.scale[0][i] = static_cast<char*>(c.k_scale);
+      g.scale[1][i] = static_cast<char*>(c.v_scale);
+    }
+  }
+  const int64_t st[2][6] = {{a.k_stride_block, a.k_stride_slot, a.k_stride_head, a.ks_stride_block, a.ks_stride_slot,
+                             a.ks_stride_head},
+                            {a.v_stride_block, a.v_stride_slot, a.v_stride_head, a.vs_stride_block, a.vs_stride_slot,
+                             a.vs_stride_head}};
+  for (int kv = 0; kv < 2; ++kv) {
+    pa::PageSide& s = g.side[kv];
+    s.blk = st[kv][0] * e;
+    s.slot = st[kv][1] * e;
+    s.head = st[kv][2] * e;
+    s.sblk = st[kv][3] * g.scale_bytes;
+    s.sslot = st[kv][4] * g.scale_bytes;
+    s.shead = st[kv][5] * g.scale_bytes;
+    s.linear = (H == 1 || s.head == D * e) && (BS == 1 || s.slot == static_cast<long long>(H) * D * e);
+    s.dense = s.linear || ((BS == 1 || s.slot == D * e) && (H == 1 || s.head == static_cast<long long>(BS) * D * e));
+    s.slot_fast = s.slot < s.head;
+  }
+  return PA_OK;
+}
+
+// Pieces of a page: 16 KB (four loads a thread), and down to 4 KB (one) where
+// `copies` pages of K or V would leave SMs idle.
+static int page_parts(const pa_kv_cache_t& a, long long copies) {
+  const long long bytes = static_cast<long long>(a.block_size) * a.num_kv_heads * a.head_dim * elt_size(a.dtype);
+  const long long least = (bytes + 16383) / 16384, most = (bytes + 4095) / 4096;
+  long long parts = copies > 0 ? (2LL * pa::device_sm_count() + copies - 1) / copies : least;
+  parts = parts < least ? least : parts > most ? most : parts;
+  return static_cast<int>(parts);
+}
+
+static int check_layers(const pa_kv_cache_t* caches, int32_t num_layers) {
+  if (num_layers < 1 || !caches) return fail(PA_ERR_INVALID, "the caches of at least one layer are needed");
+  for (int i = 0; i < num_layers; ++i) {
+    int rc = check_cache(&caches[i]);
+    if (rc) return rc;
+    pa_kv_cache_t c = caches[i];  // the same but for the pointers
+    c.k = caches[0].k;
+    c.v = caches[0].v;
+    c.k_scale = caches[0].k_scale;
+    c.v_scale = caches[0].v_scale;
+    const pa_kv_cache_t& a = caches[0];
+    const bool pools = c.dtype == a.dtype && c.num_blocks == a.num_blocks && c.block_size == a.block_size &&
+                       c.num_kv_heads == a.num_kv_heads && c.head_dim == a.head_dim &&
+                       c.k_stride_block == a.k_stride_block && c.k_stride_slot == a.k_stride_slot &&
+                       c.k_stride_head == a.k_stride_head && c.v_stride_block == a.v_stride_block &&
+                       c.v_stride_slot == a.v_stride_slot && c.v_stride_head == a.v_stride_head;
+    const bool scales = a.dtype != PA_DTYPE_I8 ||
+                        (c.scale_dtype == a.scale_dtype && c.ks_stride_block == a.ks_stride_block &&
+                         c.ks_stride_slot == a.ks_stride_slot && c.ks_stride_head == a.ks_stride_head &&
+                         c.vs_stride_block == a.vs_stride_block && c.vs_stride_slot == a.vs_stride_slot &&
+                         c.vs_stride_head == a.vs_stride_head);
+    if (!pools || !scales) return fail(PA_ERR_INVALID, "layer %d's pools differ from layer 0's in type, shape or strides", i);
+  }
+  return PA_OK;
+}
+
+int kv_copy_blocks(const pa_kv_cache_t* caches, int32_t num_layers, const int32_t* src, const int32_t* dst,
+                   const int32_t* num_slots, int32_t num_pairs, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  int rc = check_layers(caches, num_layers);
+  if (rc) return rc;
+  if (num_pairs < 0) return fail(PA_ERR_INVALID, "num_pairs < 0");
+  if (num_pairs == 0) return PA_OK;
+  if (!src || !dst) return fail(PA_ERR_INVALID, "kv_copy_blocks: src / dst is NULL");
+  for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
+    pa::PageParams g;
+    page_params(caches, num_layers, first, g);
+    g.parts = page_parts(caches[0], 2LL * num_pairs * g.layers);
+    cudaError_t e = pa::launch_copy_blocks(g, src, dst, num_slots, num_pairs, status, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv_copy_blocks launch");
+  }
+  return PA_OK;
+}
+
+int64_t block_pool_scratch_words(int32_t num_blocks) {
+  const int64_t n = num_blocks > 0 ? num_blocks : 0;
+  return pa::kShareHead + 3 * n + (n + 31) / 32;
+}
+
+static int block_share_check(const pa_block_pool_t* pool, const pa_block_share_t* share, pa::PoolParams& p,
+                             pa::ShareParams& s) {
+  int rc = block_pool_check(pool, p);
+  if (rc) return rc;
+  if (!share || !share->ref_count || !share->scratch)
+    return fail(PA_ERR_INVALID, "block sharing needs ref_count and scratch");
+  if (share->scratch_words < block_pool_scratch_words(pool->num_blocks))
+    return fail(PA_ERR_WORKSPACE, "block sharing: scratch holds %lld words, %lld are needed",
+                static_cast<long long>(share->scratch_words),
+                static_cast<long long>(block_pool_scratch_words(pool->num_blocks)));
+  s.ref = share->ref_count;
+  s.scratch = share->scratch;
+  return PA_OK;
+}
+
+int block_pool_init_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, void* stream) {
+  g_err[0] = 0;
+  pa::PoolParams p;
+  pa::ShareParams s;
+  int rc = block_share_check(pool, share, p, s);
+  if (rc) return rc;
+  cudaError_t e = pa::launch_block_pool_init_shared(p, s, share->scratch_words, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_init_shared launch");
+}
+
+int block_pool_apply_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* ops,
+                            int32_t n_ops, int32_t block_size, int32_t* results, int32_t* copy_src, int32_t* copy_dst,
+                            int32_t* copy_slots, void* stream) {
+  g_err[0] = 0;
+  pa::PoolParams p;
+  pa::ShareParams s;
+  int rc = block_share_check(pool, share, p, s);
+  if (rc) return rc;
+  if (n_ops < 0) return fail(PA_ERR_INVALID, "n_ops < 0");
+  if (n_ops > 0 && !ops) return fail(PA_ERR_INVALID, "ops is NULL");
+  if (!is_pow2(block_size)) return fail(PA_ERR_INVALID, "block_size %d must be a power of two", block_size);
+  if ((copy_src != nullptr) != (copy_dst != nullptr) || (copy_src != nullptr) != (copy_slots != nullptr))
+    return fail(PA_ERR_INVALID, "copy_src, copy_dst and copy_slots come together");
+  cudaError_t e = pa::launch_block_pool_apply_shared(p, s, ops, n_ops, ilog2(block_size), results, copy_src, copy_dst,
+                                                     copy_slots, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_apply_shared launch");
+}
+
+int block_pool_reorder(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* slots,
+                       const int32_t* parents, const int32_t* num_tokens, int32_t num_groups, int32_t num_beams,
+                       int32_t* slots_out, const pa_kv_cache_t* caches, int32_t num_layers, int32_t* status,
+                       void* stream) {
+  g_err[0] = 0;
+  pa::PoolParams p;
+  pa::ShareParams s;
+  int rc = block_share_check(pool, share, p, s);
+  if (rc) return rc;
+  rc = check_layers(caches, num_layers);
+  if (rc) return rc;
+  if (caches[0].num_blocks < pool->num_blocks)
+    return fail(PA_ERR_INVALID, "the caches hold %d blocks, the pool hands out %d", caches[0].num_blocks, pool->num_blocks);
+  if (num_groups < 0) return fail(PA_ERR_INVALID, "num_groups < 0");
+  if (num_beams < 1 || num_beams > pa::kMaxBeams)
+    return fail(PA_ERR_UNSUPPORTED, "num_beams %d is outside 1..%d", num_beams, pa::kMaxBeams);
+  if (num_groups == 0) return PA_OK;
+  if (!slots || !parents || !num_tokens || !slots_out) return fail(PA_ERR_INVALID, "block_pool_reorder: NULL argument");
+  if (slots_out == slots) return fail(PA_ERR_INVALID, "slots_out must not be slots: the launch reads one while it writes the other");
+  pa::ReorderParams r{};
+  r.slots = slots;
+  r.parents = parents;
+  r.num_tokens = num_tokens;
+  r.slots_out = slots_out;
+  r.groups = num_groups;
+  r.beams = num_beams;
+  r.status = status;
+  for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
+    pa::PageParams g;
+    page_params(caches, num_layers, first, g);
+    g.parts = page_parts(caches[0], 2LL * num_groups * (num_beams - 1) * g.layers);
+    const long long ctas = static_cast<long long>(num_groups) *
+                           (p.max_blocks_per_seq / 1024 + 1LL + (num_beams - 1LL) * g.layers * 2 * g.parts);
+    if (ctas > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "block_pool_reorder: %lld CTAs in one launch", ctas);
+    cudaError_t e = pa::launch_block_pool_reorder(p, s, r, g, static_cast<cudaStream_t>(stream), first == 0);
+    if (e != cudaSuccess) return cuda_fail(e, "block_pool_reorder launch");
+  }
+  return PA_OK;
+}
+
+int block_pool_compact(const pa_block_pool_t* pool, const pa_block_share_t* share, int32_t num_blocks_after,
+                       int32_t* live, const pa_kv_cache_t* caches, int32_t num_layers, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  pa::PoolParams p;
+  pa::ShareParams s;
+  int rc = block_share_check(pool, share, p, s);
+  if (rc) return rc;
+  rc = check_layers(caches, num_layers);
+  if (rc) return rc;
+  if (caches[0].num_blocks < pool->num_blocks)
+    return fail(PA_ERR_INVALID, "the caches hold %d blocks, the pool hands out %d", caches[0].num_blocks, pool->num_blocks);
+  if (num_blocks_after < 0 || num_blocks_after > pool->num_blocks)
+    return fail(PA_ERR_INVALID, "num_blocks_after %d is outside 0..%d", num_blocks_after, pool->num_blocks);
+  for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
+    pa::PageParams g;
+    page_params(caches, num_layers, first, g);
+    g.parts = page_parts(caches[0], 0);
+    cudaError_t e = pa::launch_block_pool_compact(p, s, num_blocks_after, live, g, status,
+                                                  static_cast<cudaStream_t>(stream), first == 0);
+    if (e != cudaSuccess) return cuda_fail(e, "block_pool_compact launch");
+  }
+  return PA_OK;
+}
+
+static int beam_params(const pa_beam_select_t* a, pa::BeamParams& p, size_t& bytes) {
+  if (!a) return fail(PA_ERR_INVALID, "beam_select: NULL descriptor");
+  const int e = a->dtype == PA_DTYPE_I8 ? 0 : elt_size(a->dtype);
+  if (!e) return fail(PA_ERR_INVALID, "logits dtype must be fp32, fp16 or bf16");
+  if (a->num_seqs < 0 || a->vocab < 1) return fail(PA_ERR_INVALID, "beam_select: bad num_seqs or vocab");
+  if (a->num_beams < 1 || a->num_beams > pa::kMaxBeams)
+    return fail(PA_ERR_UNSUPPORTED, "num_beams %d is outside 1..%d", a->num_beams, pa::kMaxBeams);
+  if (a->num_out < 1 || a->num_out > pa::kMaxBeamOut)
+    return fail(PA_ERR_UNSUPPORTED, "num_out %d is outside 1..%d", a->num_out, pa::kMaxBeamOut);
+  if (a->num_out > static_cast<long long>(a->num_beams) * a->vocab)
+    return fail(PA_ERR_INVALID, "num_out %d exceeds num_beams * vocab", a->num_out);
+  if (a->finished && (a->eos_id < 0 || a->eos_id >= a->vocab))
+    return fail(PA_ERR_INVALID, "eos_id %d is outside the vocabulary", a->eos_id);
+  if (a->stride_seq < 0 || a->stride_beam < 0) return fail(PA_ERR_INVALID, "beam_select: negative strides");
+  if (a->vocab > 0x7fffffff - 64) return fail(PA_ERR_UNSUPPORTED, "vocab %d is too large", a->vocab);
+  const long long rows = static_cast<long long>(a->num_seqs) * a->num_beams;
+  if (rows > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "beam_select: too many rows");
+  p = pa::BeamParams{};
+  p.logits = a->logits;
+  p.stride_seq = a->stride_seq;
+  p.stride_beam = a->stride_beam;
+  p.scores = a->scores;
+  p.finished = a->finished;
+  p.seqs = a->num_seqs;
+  p.beams = a->num_beams;
+  p.vocab = a->vocab;
+  p.num_out = a->num_out;
+  p.eos = a->eos_id;
+  p.out_scores = a->out_scores;
+  p.out_tokens = a->out_tokens;
+  p.out_parents = a->out_parents;
+  const int aligned = al(a->logits, 16) && row_al(a->stride_seq, e, 16) && row_al(a->stride_beam, e, 16);
+  p.splits = rows ? pa::beam_splits(static_cast<int>(rows), p.beams, p.num_out, p.vocab, a->dtype, aligned, &p.split_vecs) : 1;
+  bytes = static_cast<size_t>(rows) * p.splits * (8 * static_cast<size_t>(p.num_out) + 8);
+  return PA_OK;
+}
+
+int beam_select_workspace_size(const pa_beam_select_t* a, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(PA_ERR_INVALID, "bytes is NULL");
+  pa::BeamParams p;
+  return beam_params(a, p, *bytes);
+}
+
+int beam_select(const pa_beam_select_t* a, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  pa::BeamParams p;
+  size_t bytes = 0;
+  int rc = beam_params(a, p, bytes);
+  if (rc) return rc;
+  if (p.seqs == 0) return PA_OK;
+  if (!p.logits || !p.scores || !p.out_scores || !p.out_tokens || !p.out_parents)
+    return fail(PA_ERR_INVALID, "beam_select: NULL pointer");
+  if (!al(p.logits, elt_size(a->dtype))) return fail(PA_ERR_INVALID, "logits misaligned");
+  if (!workspace || workspace_bytes < bytes || !al(workspace, 16))
+    return fail(PA_ERR_WORKSPACE, "beam_select: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, bytes);
+  const size_t lists = static_cast<size_t>(p.seqs) * p.beams * p.splits;
+  p.part_key = static_cast<unsigned long long*>(workspace);
+  p.part_max = reinterpret_cast<float*>(p.part_key + lists * p.num_out);
+  p.part_sum = p.part_max + lists;
+  cudaError_t e = pa::launch_beam_select(p, a->dtype, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PA_OK : cuda_fail(e, "beam_select launch");
+}
+
 const char* paged_attn_error_string(void) { return g_err; }
 
 const char* paged_attn_version(void) { return "0.1.0"; }

@@ -23,6 +23,8 @@ enum : int {
   ST_BAD_SEQ_INDEX = 8,    // token -> sequence index outside [0, num_seqs)
   ST_WAIT_TIMEOUT = 16,    // a bounded wait on an asynchronous copy gave up
   ST_PEER_TIMEOUT = 32,    // the cross-GPU barrier gave up waiting for a peer's flag
+  ST_COPY_OVERLAP = 64,    // a page copy whose target is another copy's source or target
+  ST_BAD_POOL = 128,       // block pool arrays that contradict each other
 };
 constexpr int kMaxPeers = 8;  // GPUs of one box taking part in a peer output exchange
 
@@ -144,6 +146,73 @@ cudaError_t launch_block_pool_init(const PoolParams& p, cudaStream_t stream);
 cudaError_t launch_block_pool_apply(const PoolParams& p, const int* ops, int n_ops, int* results,
                                     cudaStream_t stream);
 cudaError_t launch_block_pool_step(const PoolParams& p, const StepParams& s, cudaStream_t stream);
+
+
+// Page copies (csrc/page_copy.cuh).  One K or V page is `rows` = slots * heads
+// rows of head_dim elements; strides are in bytes.
+constexpr int kMaxLayers = 64;  // layers of one launch (their pointers are kernel parameters)
+struct PageSide {
+  long long blk, slot, head;     // K or V rows
+  long long sblk, sslot, shead;  // scales (sslot 0: one per block and head)
+  int linear;     // the rows of a page are one run of memory, slot after slot
+  int dense;      // they are one run of memory, in any order
+  int slot_fast;  // neighbouring slots lie nearer in memory than neighbouring heads
+};
+struct PageParams {
+  char* page[2][kMaxLayers];   // K, V
+  char* scale[2][kMaxLayers];  // NULL: no scales
+  PageSide side[2];
+  int layers, num_blocks, block_size, heads, row_vecs_log2, scale_bytes;
+  int parts;  // pieces a page is cut into
+};
+cudaError_t launch_copy_blocks(const PageParams& g, const int* src, const int* dst, const int* num_slots, int pairs,
+                               int* status, cudaStream_t stream);
+
+// Shared blocks (csrc/block_share.cu): reference counts beside the pool, and
+// scratch that holds a launch ticket, counters, a bitmap and page lists.
+enum : int { POOL_FORK = 2 };
+struct ShareParams {
+  int* ref;
+  int* scratch;
+};
+constexpr int kShareHead = 16;  // scratch words before the page lists
+cudaError_t launch_block_pool_init_shared(const PoolParams& p, const ShareParams& s, long long scratch_words,
+                                          cudaStream_t stream);
+cudaError_t launch_block_pool_apply_shared(const PoolParams& p, const ShareParams& s, const int* ops, int n_ops,
+                                           int log2BS, int* results, int* copy_src, int* copy_dst, int* copy_slots,
+                                           cudaStream_t stream);
+struct ReorderParams {
+  const int* slots;       // [groups, beams] pool row of each beam
+  const int* parents;     // [groups, beams]
+  const int* num_tokens;  // [groups]
+  int* slots_out;         // [groups, beams]
+  int groups, beams;
+  int* status;
+};
+cudaError_t launch_block_pool_reorder(const PoolParams& p, const ShareParams& s, const ReorderParams& r,
+                                      const PageParams& g, cudaStream_t stream, bool first);
+cudaError_t launch_block_pool_compact(const PoolParams& p, const ShareParams& s, int num_blocks_after, int* live,
+                                      const PageParams& g, int* status, cudaStream_t stream, bool first);
+
+// Beam selection (csrc/beam_select.cu).
+constexpr int kMaxBeams = 32;
+constexpr int kMaxBeamOut = 32;
+struct BeamParams {
+  const void* logits;
+  long long stride_seq, stride_beam;  // elements
+  const float* scores;                // [seqs, beams]
+  const unsigned char* finished;      // [seqs, beams] or NULL
+  int seqs, beams, vocab, num_out, eos;
+  int splits, split_vecs;
+  unsigned long long* part_key;  // [rows, splits, num_out]
+  float* part_max;               // [rows, splits]
+  float* part_sum;
+  float* out_scores;
+  int* out_tokens;
+  int* out_parents;
+};
+int beam_splits(int rows, int beams, int num_out, int vocab, int dtype, int aligned, int* split_vecs);
+cudaError_t launch_beam_select(const BeamParams& p, int dtype, cudaStream_t stream);
 
 // K/V projection with the cache write in its epilogue (kv_project.cu): the
 // destination fields of WriteParams plus the projection's inner dimension and bias.

@@ -8,6 +8,11 @@
 //                                           K/V rows (transformer/model.py:85-122)
 //   pie_b200::project_write_kv              the K/V projection with that write in
 //                                           its epilogue (transformer/model.py:75-122)
+//   pie_b200::copy_blocks                   page copies inside the pools of all layers
+//   pie_b200::reorder_beams                 beams take over their parents' pool rows
+//   pie_b200::compact_blocks                the blocks in use move to the lowest ids
+//   pie_b200::beam_select                   the best continuations of every
+//                                           sequence's beams
 //
 // Each op reads pointers, sizes and element strides from its tensors, fills the
 // C structs of include/paged_attn_b200.h and calls the library on the current
@@ -380,7 +385,204 @@ void project_write_kv(const at::Tensor& x, const at::Tensor& w, const std::optio
   check_rc(kv_project_write(&pj, &kv, &pg, opt_ptr<int32_t>(status), stream), "kv_project_write");
 }
 
+// ---- shared blocks, page copies, beams ---------------------------------------
+void check_vec(const at::Tensor& ref, const at::Tensor& t, const char* name) {
+  check_device(ref, t, name);
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous(), "pie_b200: ", name, " must be contiguous int32");
+}
+
+void check_status(const at::Tensor& ref, const std::optional<at::Tensor>& status) {
+  if (status.has_value()) {
+    check_vec(ref, *status, "status");
+    TORCH_CHECK_VALUE(status->numel() >= 1, "pie_b200: status holds no word");
+  }
+}
+
+// One descriptor per layer; the scale lists are empty but for int8 pools.
+std::vector<pa_kv_cache_t> layer_descs(at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs) {
+  TORCH_CHECK_VALUE(!k.empty() && k.size() == v.size(), "pie_b200: as many K as V pools are needed, one at least (got ",
+                    k.size(), " and ", v.size(), ")");
+  const bool i8 = k[0].scalar_type() == at::kChar;
+  TORCH_CHECK_VALUE(!i8 || (ks.size() == k.size() && vs.size() == k.size()),
+                    "pie_b200: int8 KV pools need k_scale and v_scale for every layer");
+  TORCH_CHECK_VALUE(k[0].is_cuda(), "pie_b200: the pools must be CUDA tensors");
+  std::vector<pa_kv_cache_t> d;
+  d.reserve(k.size());
+  for (size_t i = 0; i < k.size(); ++i) {
+    check_device(k[0], k[i], "K");
+    if (i8) d.push_back(kv_desc(k[i], v[i], ks[i], vs[i]));
+    else d.push_back(kv_desc(k[i], v[i], std::nullopt, std::nullopt));
+  }
+  return d;
+}
+
+void copy_blocks(at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs, const at::Tensor& src,
+                 const at::Tensor& dst, const std::optional<at::Tensor>& num_slots,
+                 const std::optional<at::Tensor>& status) {
+  const std::vector<pa_kv_cache_t> d = layer_descs(k, v, ks, vs);
+  const int64_t n = src.numel();
+  check_i32(k[0], src, "src", n);
+  check_i32(k[0], dst, "dst", n);
+  if (num_slots.has_value()) check_i32(k[0], *num_slots, "num_slots", n);
+  check_status(k[0], status);
+  const c10::cuda::CUDAGuard guard(k[0].device());
+  void* stream = c10::cuda::getCurrentCUDAStream(k[0].device().index()).stream();
+  check_rc(kv_copy_blocks(d.data(), static_cast<int32_t>(d.size()), static_cast<const int32_t*>(src.data_ptr()),
+                          static_cast<const int32_t*>(dst.data_ptr()), opt_ptr<const int32_t>(num_slots),
+                          static_cast<int32_t>(n), opt_ptr<int32_t>(status), stream),
+           "kv_copy_blocks");
+}
+
+struct SharedPool {
+  pa_block_pool_t pool{};
+  pa_block_share_t share{};
+};
+
+SharedPool pool_desc(const at::Tensor& ref, const at::Tensor& free_stack, const at::Tensor& free_top,
+                     const at::Tensor& table, const at::Tensor& count, const at::Tensor& ref_count,
+                     const at::Tensor& scratch) {
+  check_vec(ref, free_stack, "free_stack");
+  check_vec(ref, free_top, "free_top");
+  check_vec(ref, count, "count");
+  check_vec(ref, ref_count, "ref_count");
+  check_vec(ref, scratch, "scratch");
+  check_device(ref, table, "table");
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) < 2 || table.stride(1) == 1),
+                    "pie_b200: table must be int32 [max_seqs, max_blocks_per_seq] with contiguous rows");
+  TORCH_CHECK_VALUE(free_top.numel() >= 1 && count.numel() == table.size(0),
+                    "pie_b200: count needs one entry per table row, free_top one entry");
+  TORCH_CHECK_VALUE(free_stack.numel() >= ref_count.numel(), "pie_b200: free_stack needs an entry per block");
+  SharedPool s;
+  s.pool.free_stack = static_cast<int32_t*>(free_stack.data_ptr());
+  s.pool.free_top = static_cast<int32_t*>(free_top.data_ptr());
+  s.pool.table = static_cast<int32_t*>(table.data_ptr());
+  s.pool.count = static_cast<int32_t*>(count.data_ptr());
+  s.pool.table_stride = table.size(0) > 1 ? table.stride(0) : table.size(1);
+  s.pool.num_blocks = static_cast<int32_t>(ref_count.numel());
+  s.pool.max_seqs = static_cast<int32_t>(table.size(0));
+  s.pool.max_blocks_per_seq = static_cast<int32_t>(table.size(1));
+  s.share.ref_count = static_cast<int32_t*>(ref_count.data_ptr());
+  s.share.scratch = static_cast<int32_t*>(scratch.data_ptr());
+  s.share.scratch_words = scratch.numel();
+  return s;
+}
+
+at::Tensor reorder_beams(const at::Tensor& free_stack, const at::Tensor& free_top, const at::Tensor& table,
+                         const at::Tensor& count, const at::Tensor& ref_count, const at::Tensor& scratch,
+                         const at::Tensor& slots, const at::Tensor& parents, const at::Tensor& num_tokens,
+                         at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs,
+                         const std::optional<at::Tensor>& status) {
+  const std::vector<pa_kv_cache_t> d = layer_descs(k, v, ks, vs);
+  SharedPool s = pool_desc(k[0], free_stack, free_top, table, count, ref_count, scratch);
+  check_vec(k[0], slots, "slots");
+  check_vec(k[0], parents, "parents");
+  TORCH_CHECK_VALUE(slots.dim() == 2 && parents.sizes() == slots.sizes(),
+                    "pie_b200: slots and parents must be [num_groups, num_beams]");
+  check_i32(k[0], num_tokens, "num_tokens", slots.size(0));
+  check_status(k[0], status);
+  const c10::cuda::CUDAGuard guard(k[0].device());
+  at::Tensor out = at::empty(slots.sizes(), slots.options());
+  void* stream = c10::cuda::getCurrentCUDAStream(k[0].device().index()).stream();
+  check_rc(block_pool_reorder(&s.pool, &s.share, static_cast<const int32_t*>(slots.data_ptr()),
+                              static_cast<const int32_t*>(parents.data_ptr()),
+                              static_cast<const int32_t*>(num_tokens.data_ptr()), static_cast<int32_t>(slots.size(0)),
+                              static_cast<int32_t>(slots.size(1)), static_cast<int32_t*>(out.data_ptr()), d.data(),
+                              static_cast<int32_t>(d.size()), opt_ptr<int32_t>(status), stream),
+           "block_pool_reorder");
+  return out;
+}
+
+at::Tensor compact_blocks(const at::Tensor& free_stack, const at::Tensor& free_top, const at::Tensor& table,
+                          const at::Tensor& count, const at::Tensor& ref_count, const at::Tensor& scratch,
+                          int64_t num_blocks_after, at::TensorList k, at::TensorList v, at::TensorList ks,
+                          at::TensorList vs, const std::optional<at::Tensor>& status) {
+  const std::vector<pa_kv_cache_t> d = layer_descs(k, v, ks, vs);
+  SharedPool s = pool_desc(k[0], free_stack, free_top, table, count, ref_count, scratch);
+  check_status(k[0], status);
+  TORCH_CHECK_VALUE(num_blocks_after <= s.pool.num_blocks, "pie_b200: num_blocks ", num_blocks_after, " exceeds the pool's ",
+                    s.pool.num_blocks);
+  const c10::cuda::CUDAGuard guard(k[0].device());
+  at::Tensor live = at::empty({1}, free_top.options());
+  void* stream = c10::cuda::getCurrentCUDAStream(k[0].device().index()).stream();
+  check_rc(block_pool_compact(&s.pool, &s.share,
+                              num_blocks_after < 0 ? s.pool.num_blocks : static_cast<int32_t>(num_blocks_after),
+                              static_cast<int32_t*>(live.data_ptr()), d.data(), static_cast<int32_t>(d.size()),
+                              opt_ptr<int32_t>(status), stream),
+           "block_pool_compact");
+  return live;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_outputs(const at::Tensor& scores, int64_t num_out) {
+  const auto i32 = scores.options().dtype(at::kInt);
+  const int64_t B = scores.size(0);
+  return {at::empty({B, num_out}, scores.options()), at::empty({B, num_out}, i32), at::empty({B, num_out}, i32)};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_op(const at::Tensor& logits, const at::Tensor& scores,
+                                                              int64_t num_out,
+                                                              const std::optional<at::Tensor>& finished,
+                                                              int64_t eos_id) {
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 3 && (logits.size(2) < 2 || logits.stride(2) == 1),
+                    "pie_b200: logits must be a CUDA tensor [num_seqs, num_beams, vocab] with a contiguous vocabulary");
+  check_device(logits, scores, "beam_scores");
+  TORCH_CHECK_VALUE(scores.scalar_type() == at::kFloat && scores.is_contiguous() && scores.dim() == 2 &&
+                        scores.size(0) == logits.size(0) && scores.size(1) == logits.size(1),
+                    "pie_b200: beam_scores must be contiguous float32 [num_seqs, num_beams]");
+  if (finished.has_value()) {
+    check_device(logits, *finished, "finished");
+    TORCH_CHECK_VALUE((finished->scalar_type() == at::kBool || finished->scalar_type() == at::kByte) &&
+                          finished->is_contiguous() && finished->sizes() == scores.sizes(),
+                      "pie_b200: finished must be contiguous bool [num_seqs, num_beams]");
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  pa_beam_select_t a{};
+  a.logits = logits.data_ptr();
+  a.scores = static_cast<const float*>(scores.data_ptr());
+  a.finished = opt_ptr<const uint8_t>(finished);
+  a.stride_seq = logits.stride(0);
+  a.stride_beam = logits.stride(1);
+  a.dtype = pa_dtype(logits.scalar_type());
+  TORCH_CHECK_VALUE(logits.size(2) >= 1 && logits.size(2) < (int64_t{1} << 31) && logits.size(0) < (int64_t{1} << 31) &&
+                        logits.size(1) < (int64_t{1} << 31) && num_out < (int64_t{1} << 31) && eos_id < (int64_t{1} << 31),
+                    "pie_b200: beam_select sizes out of range");
+  a.num_seqs = static_cast<int32_t>(logits.size(0));
+  a.num_beams = static_cast<int32_t>(logits.size(1));
+  a.vocab = static_cast<int32_t>(logits.size(2));
+  a.eos_id = static_cast<int32_t>(eos_id);
+  a.num_out = static_cast<int32_t>(num_out);
+  size_t bytes = 0;
+  check_rc(beam_select_workspace_size(&a, &bytes), "beam_select");
+  // a workspace of this call's own: calls on other streams and captured graphs do not share it
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, logits.options().dtype(at::kByte));
+  auto out = beam_outputs(scores, num_out);
+  a.out_scores = static_cast<float*>(std::get<0>(out).data_ptr());
+  a.out_tokens = static_cast<int32_t*>(std::get<1>(out).data_ptr());
+  a.out_parents = static_cast<int32_t*>(std::get<2>(out).data_ptr());
+  void* stream = c10::cuda::getCurrentCUDAStream(logits.device().index()).stream();
+  check_rc(beam_select(&a, ws.data_ptr(), bytes, stream), "beam_select");
+  return out;
+}
+
 // ---- shapes only (fake / meta tensors) ------------------------------------
+at::Tensor reorder_beams_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                              const at::Tensor&, const at::Tensor&, const at::Tensor& slots, const at::Tensor&,
+                              const at::Tensor&, at::TensorList, at::TensorList, at::TensorList, at::TensorList,
+                              const std::optional<at::Tensor>&) {
+  return at::empty(slots.sizes(), slots.options());
+}
+
+at::Tensor compact_blocks_meta(const at::Tensor&, const at::Tensor& free_top, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, const at::Tensor&, int64_t, at::TensorList, at::TensorList,
+                               at::TensorList, at::TensorList, const std::optional<at::Tensor>&) {
+  return at::empty({1}, free_top.options());
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_meta(const at::Tensor&, const at::Tensor& scores,
+                                                                int64_t num_out, const std::optional<at::Tensor>&,
+                                                                int64_t) {
+  return beam_outputs(scores, num_out);
+}
+
 std::tuple<at::Tensor, at::Tensor> paged_attention_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&,
                                                         const at::Tensor&, const at::Tensor&, const at::Tensor&,
                                                         const at::Tensor&, const std::optional<at::Tensor>&,
@@ -417,6 +619,17 @@ TORCH_LIBRARY(pie_b200, m) {
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
   m.def("project_write_kv(Tensor x, Tensor w, Tensor? bias, Tensor block_table, Tensor seq_index, Tensor positions, "
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
+  m.def("copy_blocks(Tensor(a!)[] k_caches, Tensor(b!)[] v_caches, Tensor(c!)[] k_scales, Tensor(d!)[] v_scales, "
+        "Tensor src, Tensor dst, Tensor? num_slots, Tensor(s!)? status) -> ()");
+  m.def("reorder_beams(Tensor(a!) free_stack, Tensor(b!) free_top, Tensor(c!) table, Tensor(d!) count, "
+        "Tensor(e!) ref_count, Tensor(f!) scratch, Tensor slots, Tensor parents, Tensor num_tokens, "
+        "Tensor(g!)[] k_caches, Tensor(h!)[] v_caches, Tensor(i!)[] k_scales, Tensor(j!)[] v_scales, "
+        "Tensor(s!)? status) -> Tensor");
+  m.def("compact_blocks(Tensor(a!) free_stack, Tensor(b!) free_top, Tensor(c!) table, Tensor(d!) count, "
+        "Tensor(e!) ref_count, Tensor(f!) scratch, int num_blocks_after, Tensor(g!)[] k_caches, "
+        "Tensor(h!)[] v_caches, Tensor(i!)[] k_scales, Tensor(j!)[] v_scales, Tensor(s!)? status) -> Tensor");
+  m.def("beam_select(Tensor logits, Tensor beam_scores, int num_out, Tensor? finished, int eos_id) -> "
+        "(Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(pie_b200, CUDA, m) {
@@ -426,9 +639,16 @@ TORCH_LIBRARY_IMPL(pie_b200, CUDA, m) {
   m.impl("paged_attention_varlen_out", &paged_attention_varlen_out);
   m.impl("write_kv", &write_kv);
   m.impl("project_write_kv", &project_write_kv);
+  m.impl("copy_blocks", &copy_blocks);
+  m.impl("reorder_beams", &reorder_beams);
+  m.impl("compact_blocks", &compact_blocks);
+  m.impl("beam_select", &beam_select_op);
 }
 
 TORCH_LIBRARY_IMPL(pie_b200, Meta, m) {
   m.impl("paged_attention", &paged_attention_meta);
   m.impl("paged_attention_varlen", &paged_attention_varlen_meta);
+  m.impl("reorder_beams", &reorder_beams_meta);
+  m.impl("compact_blocks", &compact_blocks_meta);
+  m.impl("beam_select", &beam_select_meta);
 }

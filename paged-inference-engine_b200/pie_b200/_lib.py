@@ -29,6 +29,8 @@ PA_STATUS_BAD_POSITION = 2
 PA_STATUS_BAD_NUM_BLOCKS = 4
 PA_STATUS_BAD_SEQ_INDEX = 8
 PA_STATUS_PEER_TIMEOUT = 32
+PA_STATUS_COPY_OVERLAP = 64
+PA_STATUS_BAD_POOL = 128
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -91,6 +93,22 @@ class PaKvProj(ctypes.Structure):
     ]
 
 
+class PaBlockShare(ctypes.Structure):
+    """Mirror of pa_block_share_t."""
+
+    _fields_ = [("ref_count", _vp), ("scratch", _vp), ("scratch_words", _i64)]
+
+
+class PaBeamSelect(ctypes.Structure):
+    """Mirror of pa_beam_select_t."""
+
+    _fields_ = [
+        ("logits", _vp), ("scores", _vp), ("finished", _vp), ("stride_seq", _i64), ("stride_beam", _i64),
+        ("dtype", _i32), ("num_seqs", _i32), ("num_beams", _i32), ("vocab", _i32), ("eos_id", _i32),
+        ("num_out", _i32), ("out_scores", _vp), ("out_tokens", _vp), ("out_parents", _vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/paged_attn_b200.h declares.
 SIGNATURES = {
     "paged_attn_workspace_size": (ctypes.c_int, [ctypes.POINTER(PaAttnIO), ctypes.POINTER(PaKvCache),
@@ -129,6 +147,17 @@ SIGNATURES = {
     "block_pool_apply": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, _vp, _vp]),
     "block_pool_step": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_int64, ctypes.c_int32,
                                        _vp, _vp, _vp, ctypes.c_int32, _vp, _vp]),
+    "kv_copy_blocks": (ctypes.c_int, [ctypes.POINTER(PaKvCache), _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "block_pool_scratch_words": (_i64, [_i32]),
+    "block_pool_init_shared": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp]),
+    "block_pool_apply_shared": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp, _i32, _i32, _vp, _vp, _vp, _vp,
+                                               _vp]),
+    "block_pool_reorder": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp, _vp, _vp, _i32, _i32, _vp,
+                                          ctypes.POINTER(PaKvCache), _i32, _vp, _vp]),
+    "block_pool_compact": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _i32, _vp, ctypes.POINTER(PaKvCache), _i32,
+                                          _vp, _vp]),
+    "beam_select_workspace_size": (ctypes.c_int, [ctypes.POINTER(PaBeamSelect), ctypes.POINTER(ctypes.c_size_t)]),
+    "beam_select": (ctypes.c_int, [ctypes.POINTER(PaBeamSelect), _vp, ctypes.c_size_t, _vp]),
     "paged_attn_error_string": (ctypes.c_char_p, []),
     "paged_attn_version": (ctypes.c_char_p, []),
 }

@@ -16,7 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-from typing import Optional
+from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -229,6 +229,10 @@ def _raise_status_value(fn: str, v: int) -> None:
             bits.append("sequence index outside the block table")
         if v & _lib.PA_STATUS_PEER_TIMEOUT:
             bits.append("a peer GPU never reached the output-exchange barrier")
+        if v & _lib.PA_STATUS_COPY_OVERLAP:
+            bits.append("a page copy into another copy's source or target")
+        if v & _lib.PA_STATUS_BAD_POOL:
+            bits.append("block pool arrays that contradict each other, or more blocks in use than may stay")
         raise IndexError(f"{fn}: device status {v:#x}: " + "; ".join(bits))
 
 
@@ -561,3 +565,239 @@ def project_write_kv(x: torch.Tensor, w_kv: torch.Tensor, bias: Optional[torch.T
                                                                 torch.cuda.current_stream(dev).cuda_stream))
     if _CHECK and status is not None:
         _raise_status("project_write_kv", status)
+
+
+class PoolState(NamedTuple):
+    """The device arrays of a block pool whose blocks sequences share (all int32, see pa_block_share_t).
+
+    ``free_stack`` [num_blocks], ``free_top`` [1], ``table`` [max_seqs, max_blocks_per_seq], ``count`` [max_seqs]
+    (-1: no entry), ``ref_count`` [num_blocks] holders of each block, ``scratch`` (``pool_scratch_words`` words,
+    zero before its first use).
+    """
+
+    free_stack: torch.Tensor
+    free_top: torch.Tensor
+    table: torch.Tensor
+    count: torch.Tensor
+    ref_count: torch.Tensor
+    scratch: torch.Tensor
+
+
+def pool_scratch_words(num_blocks: int) -> int:
+    """Words of a PoolState's ``scratch``: 16 + 3 * num_blocks + ceil(num_blocks / 32)."""
+    return 16 + 3 * num_blocks + (num_blocks + 31) // 32
+
+
+Caches = Union[torch.Tensor, Sequence[torch.Tensor]]
+
+
+def _layers(t: Optional[Caches]) -> Sequence[torch.Tensor]:
+    return () if t is None else (t,) if isinstance(t, torch.Tensor) else t
+
+
+def layer_descs(k_cache: Caches, v_cache: Caches, k_scale: Optional[Caches] = None,
+                v_scale: Optional[Caches] = None) -> ctypes.Array:
+    """One descriptor per layer; layers differ in their pointers only."""
+    k, v, ks, vs = _layers(k_cache), _layers(v_cache), _layers(k_scale), _layers(v_scale)
+    if not k or len(k) != len(v):
+        raise ValueError(f"as many K as V pools are needed, one at least (got {len(k)} and {len(v)})")
+    if k[0].dtype == torch.int8 and not len(k) == len(ks) == len(vs):
+        raise ValueError("int8 KV pools need k_scale and v_scale for every layer")
+    if any(t.device != k[0].device for t in (*k, *v, *ks, *vs)):
+        raise ValueError("the pools and scales of all layers must be on one device")
+    descs = (PaKvCache * len(k))()
+    for i in range(len(k)):
+        if k[i].dtype == torch.int8:
+            descs[i] = kv_cache_desc(k[i], v[i], ks[i], vs[i])
+        else:
+            descs[i] = kv_cache_desc(k[i], v[i])
+    return descs
+
+
+def _check_vectors(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, got {t.device}")
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32")
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def copy_blocks(k_cache: Caches, v_cache: Caches, src: torch.Tensor, dst: torch.Tensor,
+                k_scale: Optional[Caches] = None, v_scale: Optional[Caches] = None, *,
+                num_slots: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """Copy block ``src[i]`` to ``dst[i]`` in the pools of one layer (tensors) or of all layers (lists).
+
+    ``src`` / ``dst`` int32 [n] on the device; ``num_slots`` int32 [n] copies only the first slots of each block.
+    The copies act at once: a pair whose target another pair reads, or an earlier pair writes, is skipped (and
+    reported in ``status``), as is one with an id outside the pool.
+    """
+    k, v = _layers(k_cache), _layers(v_cache)
+    if not k:
+        raise ValueError("as many K as V pools are needed, one at least (got none)")
+    dev = k[0].device
+    src, dst = _i32(src), _i32(dst)
+    if num_slots is not None:
+        num_slots = _i32(num_slots)
+    if src.dim() != 1 or dst.shape != src.shape or (num_slots is not None and num_slots.shape != src.shape):
+        raise ValueError("src, dst and num_slots must be vectors of one length")
+    if status is None and _CHECK:
+        status = status_word(dev)
+    if BACKEND == "torch":
+        _op("copy_blocks")(k, v, _layers(k_scale), _layers(v_scale), src, dst, num_slots, status)
+    else:
+        descs = layer_descs(k, v, k_scale, v_scale)
+        _check_vectors(dev, src=src, dst=dst, num_slots=num_slots, status=status)
+        with torch.cuda.device(dev):
+            _lib.check("kv_copy_blocks", _lib.load().kv_copy_blocks(
+                descs, len(descs), src.data_ptr(), dst.data_ptr(), _ptr(num_slots), src.numel(), _ptr(status),
+                _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("copy_blocks", status)
+
+
+def pool_descs(pool: PoolState):
+    """The C descriptors (pa_block_pool_t, pa_block_share_t) of a pool's arrays."""
+    from .block_pool import PaBlockPool
+
+    dev = pool.ref_count.device
+    _check_vectors(dev, free_stack=pool.free_stack, free_top=pool.free_top, count=pool.count, ref_count=pool.ref_count,
+                   scratch=pool.scratch)
+    t = pool.table
+    if t.device != dev or t.dtype != torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("table must be int32 [max_seqs, max_blocks_per_seq] with contiguous rows")
+    if pool.count.numel() != t.shape[0] or pool.free_top.numel() < 1:
+        raise ValueError("count needs one entry per table row, free_top one entry")
+    if pool.free_stack.numel() < pool.ref_count.numel():
+        raise ValueError("free_stack needs an entry per block")
+    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return (PaBlockPool(pool.free_stack.data_ptr(), pool.free_top.data_ptr(), t.data_ptr(), pool.count.data_ptr(), stride,
+                        pool.ref_count.numel(), t.shape[0], t.shape[1], 0),
+            _lib.PaBlockShare(pool.ref_count.data_ptr(), pool.scratch.data_ptr(), pool.scratch.numel()))
+
+
+def reorder_beams(pool: PoolState, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor,
+                  k_cache: Caches, v_cache: Caches, k_scale: Optional[Caches] = None,
+                  v_scale: Optional[Caches] = None, *, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Beams take over their parents' state in the paged cache; returns the beams' pool rows afterwards.
+
+    ``slots`` [G, K] are the pool rows of each group's beams, ``parents`` [G, K] the beam that beam j continues,
+    ``num_tokens`` [G] the tokens in the cache (int32, on the device).  Full blocks are shared, a partly filled
+    last block is copied in every layer, blocks that no beam continues are freed; see block_pool_reorder.
+    """
+    k, v = _layers(k_cache), _layers(v_cache)
+    if not k:
+        raise ValueError("as many K as V pools are needed, one at least (got none)")
+    dev = k[0].device
+    slots, parents, num_tokens = _i32(slots), _i32(parents), _i32(num_tokens)
+    if status is None and _CHECK:
+        status = status_word(dev)
+    if BACKEND == "torch":
+        out = _op("reorder_beams")(*pool, slots, parents, num_tokens, k, v, _layers(k_scale), _layers(v_scale), status)
+    else:
+        descs = layer_descs(k, v, k_scale, v_scale)
+        desc, share = pool_descs(pool)
+        if slots.dim() != 2 or parents.shape != slots.shape or num_tokens.shape != slots.shape[:1]:
+            raise ValueError("slots and parents must be [num_groups, num_beams], num_tokens [num_groups]")
+        _check_vectors(dev, slots=slots, parents=parents, num_tokens=num_tokens, status=status, ref_count=pool.ref_count)
+        out = torch.empty_like(slots)
+        with torch.cuda.device(dev):
+            _lib.check("block_pool_reorder", _lib.load().block_pool_reorder(
+                ctypes.byref(desc), ctypes.byref(share), slots.data_ptr(), parents.data_ptr(), num_tokens.data_ptr(),
+                slots.shape[0], slots.shape[1], out.data_ptr(), descs, len(descs), _ptr(status), _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("reorder_beams", status)
+    return out
+
+
+def compact_blocks(pool: PoolState, k_cache: Caches, v_cache: Caches, k_scale: Optional[Caches] = None,
+                   v_scale: Optional[Caches] = None, *, num_blocks: Optional[int] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Move the blocks in use to the lowest ids (pages, rows, holder counts, free list); see block_pool_compact.
+
+    Afterwards only ids below ``num_blocks`` (default: all of the pool's) are in use or handed out.  Returns the
+    number of blocks in use, int32 [1] on the device.
+    """
+    k, v = _layers(k_cache), _layers(v_cache)
+    if not k:
+        raise ValueError("as many K as V pools are needed, one at least (got none)")
+    if num_blocks is not None and num_blocks < 0:
+        raise ValueError("num_blocks must be >= 0")
+    dev = k[0].device
+    if status is None and _CHECK:
+        status = status_word(dev)
+    if BACKEND == "torch":
+        live = _op("compact_blocks")(*pool, -1 if num_blocks is None else num_blocks, k, v, _layers(k_scale),
+                                     _layers(v_scale), status)
+    else:
+        descs = layer_descs(k, v, k_scale, v_scale)
+        desc, share = pool_descs(pool)
+        _check_vectors(dev, status=status, ref_count=pool.ref_count)
+        live = torch.empty(1, dtype=torch.int32, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check("block_pool_compact", _lib.load().block_pool_compact(
+                ctypes.byref(desc), ctypes.byref(share), desc.num_blocks if num_blocks is None else num_blocks,
+                live.data_ptr(), descs, len(descs), _ptr(status), _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("compact_blocks", status)
+    return live
+
+
+def beam_select(logits: torch.Tensor, beam_scores: torch.Tensor, num_out: Optional[int] = None, *,
+                finished: Optional[torch.Tensor] = None,
+                eos_id: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``num_out`` best continuations of every sequence's beams; returns (scores, tokens, parents) [B, num_out].
+
+    ``logits`` [B, K, V] (float32, float16 or bfloat16, any strides with a contiguous vocabulary), ``beam_scores``
+    [B, K] float32: the candidate (k, v) scores ``beam_scores[k] + log_softmax(logits[k])[v]``.  Ordered by score, then
+    lower beam, then larger logit, then lower token.  ``finished`` [B, K] (bool): such a beam is not read; it
+    continues with ``eos_id`` at its own score.  ``num_out`` defaults to K; scores float32, tokens and
+    parents int32.  See beam_select in the C header for NaN and infinities.
+    """
+    if logits.dim() != 3 or beam_scores.dim() != 2:
+        raise ValueError("logits must be [num_seqs, num_beams, vocab] and beam_scores [num_seqs, num_beams]")
+    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    if finished is not None and eos_id is None:
+        raise ValueError("finished beams need eos_id")
+    B, K, V = logits.shape
+    n = K if num_out is None else int(num_out)
+    if V < 1 or not 1 <= n <= max(1, K) * V:
+        raise ValueError(f"num_out {n} is outside 1..num_beams * vocab ({K} * {V})")
+    if finished is not None and not 0 <= eos_id < V:
+        raise ValueError(f"eos_id {eos_id} is outside the vocabulary of {V}")
+    if logits.stride(2) != 1 and V > 1:
+        logits = logits.contiguous()
+    if not beam_scores.is_contiguous():
+        beam_scores = beam_scores.contiguous()
+    if finished is not None and not finished.is_contiguous():
+        finished = finished.contiguous()
+    if BACKEND == "torch":
+        return _op("beam_select")(logits, beam_scores, n, finished, -1 if eos_id is None else int(eos_id))
+    dev = logits.device
+    if tuple(beam_scores.shape) != (B, K) or beam_scores.dtype != torch.float32 or beam_scores.device != dev:
+        raise ValueError(f"beam_scores must be float32 [{B}, {K}] on {dev}")
+    if finished is not None and (tuple(finished.shape) != (B, K) or finished.dtype not in (torch.bool, torch.uint8)
+                                 or finished.device != dev):
+        raise ValueError(f"finished must be bool [{B}, {K}] on {dev}")
+    a = _lib.PaBeamSelect()
+    a.logits, a.scores, a.finished = logits.data_ptr(), beam_scores.data_ptr(), _ptr(finished)
+    a.stride_seq, a.stride_beam, a.dtype = logits.stride(0), logits.stride(1), _TORCH2PA[logits.dtype]
+    a.num_seqs, a.num_beams, a.vocab, a.num_out = B, K, V, n
+    a.eos_id = -1 if eos_id is None else int(eos_id)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        _lib.check("beam_select", lib.beam_select_workspace_size(a, ctypes.byref(nbytes)))
+        ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=dev)
+        scores = torch.empty(B, n, dtype=torch.float32, device=dev)
+        tokens = torch.empty(B, n, dtype=torch.int32, device=dev)
+        parents = torch.empty(B, n, dtype=torch.int32, device=dev)
+        a.out_scores, a.out_tokens, a.out_parents = scores.data_ptr(), tokens.data_ptr(), parents.data_ptr()
+        _lib.check("beam_select", lib.beam_select(a, ws.data_ptr(), nbytes.value, _stream(dev)))
+    return scores, tokens, parents
