@@ -446,8 +446,9 @@ int kv_copy_blocks(const pa_kv_cache_t* caches, int32_t num_layers, const int32_
  * Blocks shared between sequences: a count of holders beside the block pool.
  *   ref_count      int32 [num_blocks], 0 = free
  *   scratch        int32 [scratch_words], zero before its first use; the calls
- *                  below leave it ready for the next.  One pool's calls must
- *                  not overlap, as with the pool itself.
+ *                  below leave it ready for the next.  It belongs to one pool,
+ *                  whose num_blocks may shrink but not grow, and one pool's
+ *                  calls must not overlap, as with the pool itself.
  *   scratch_words  >= block_pool_scratch_words(num_blocks)
  *                  (16 + 3 * num_blocks + ceil(num_blocks / 32))
  * A block is written only while one sequence holds it: forks share the blocks

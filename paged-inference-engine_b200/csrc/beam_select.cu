@@ -9,32 +9,50 @@
 // count as -inf, +inf as the largest float.
 //
 // Bound: every logit is read once, so the floor is rows * vocab * size bytes
-// of HBM.  Two launches: `beam_rows_kernel` streams each row in S splits, with
-// the running maximum, the sum of exponentials and the best num_out logits of
-// its split kept on chip; `beam_merge_kernel` joins the splits and the beams of
-// one sequence.  Row selection compares (logit, token) as one 64-bit integer,
-// so it is exact whatever the order of the threads.
+// of HBM; next comes the one exponential per logit (16 a clock and SM: 0.77 of
+// the HBM time for 16-bit logits).  Two launches: `beam_rows_kernel` streams a
+// split of a row through registers, each thread with its own running maximum
+// and sum, and no barrier until the split's end; `beam_merge_kernel` joins the
+// splits and the beams of one sequence.
+//
+// The best logits come from the maxima that the softmax needs anyway.  The
+// threads' maxima are joined in groups; with T the num_out-th largest of the
+// groups' maxima, num_out logits are at least T, so the best are among the
+// logits that are, and only the threads whose maximum reaches T have their
+// logits looked at again (for 16 of 32768 independent logits: 22 threads of
+// 256; each remembers the maxima of 8 spans, so it reads one of them, from L2).  Selection compares (logit, token) as one 64-bit integer, so it
+// is exact whatever the order of the threads; the sum's order depends on the
+// logits' places in the row alone, not on its address, so equal rows have equal
+// sums.
 #include "pa_common.cuh"
 
+#include <atomic>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace pa {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kRowCtas = 5;             // resident on an SM
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kVec = 4;             // 16-byte loads a thread has in flight per tile
+constexpr int kLaneRuns = 4;            // runs of 16 bytes of a lane per chunk
+constexpr int kLogLaneRuns = 2;
+constexpr int kChunkRuns = 32 * kLaneRuns;
+constexpr int kUnitRuns = kRowWarps * kChunkRuns;  // a chunk of every warp: the grain in which rows are split
+constexpr int kStages = 2;    // chunks of a warp in shared memory
+constexpr int kSpans = 8;              // a thread's units are remembered in so many spans, by their maxima
+constexpr int kHits = kRowWarps * kMaxBeamOut;  // logits at T that a split may have; with more its warps keep sorted lists
 constexpr int kMergeThreads = 512;
-constexpr int kMaxSplits = 32;      // one lane per split when sums are joined
+constexpr int kMergeWarps = kMergeThreads / 32;
+constexpr int kMergeKeys = 8192;        // candidates that the merge holds in shared memory (20 bytes each)
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DT>
-struct Logit {
-  static constexpr int kBytes = DT == PA_DTYPE_F32 ? 4 : 2;
-  static constexpr int kPer = 16 / kBytes;      // logits of a 16-byte load
-  static constexpr int kMine = kVec * kPer;     // logits of a thread per tile
-};
+constexpr int logit_bytes() {
+  return DT == PA_DTYPE_F32 ? 4 : 2;
+}
 
 __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX) + 0.f; }  // NaN, +inf, -0
 
@@ -52,312 +70,484 @@ __device__ __forceinline__ int key_token(unsigned long long k) {
   return static_cast<int>(0xffffffffu - static_cast<unsigned>(k));
 }
 
+// The logits of a 4-byte word: one in fp32 (the second counts as -inf), two in 16 bits.
 template <int DT>
-__device__ __forceinline__ float load_one(const void* row, long long i) {
-  if constexpr (DT == PA_DTYPE_F32) return static_cast<const float*>(row)[i];
-  else if constexpr (DT == PA_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
-  else return __half2float(static_cast<const __half*>(row)[i]);
+__device__ __forceinline__ float2 word_logits(uint32_t w) {
+  if constexpr (DT == PA_DTYPE_F32) return make_float2(__uint_as_float(w), -INFINITY);
+  else if constexpr (DT == PA_DTYPE_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {  // NaN gives way
+  if constexpr (DT == PA_DTYPE_F32) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  } else if constexpr (DT == PA_DTYPE_BF16) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+template <int DT>
+constexpr uint32_t word_lowest() {  // -inf
+  return DT == PA_DTYPE_F32 ? 0xff800000u : DT == PA_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
 }
 
-template <int DT>
-__device__ __forceinline__ void unpack(const uint4& w, float* f) {
-  const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+// 32 values, one per lane, from large to small.
+__device__ __forceinline__ float sort_lanes(float v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (DT == PA_DTYPE_F32) {
-      f[i] = __uint_as_float(a[i]);
-    } else if constexpr (DT == PA_DTYPE_BF16) {
-      f[2 * i] = __uint_as_float(a[i] << 16);
-      f[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
-    } else {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, v, step);
+      v = (((lane & size) == 0) == ((lane & step) == 0)) ? fmaxf(v, o) : fminf(v, o);
     }
   }
-}
-
-// Position of `key` in a list sorted from large to small: entries above it.
-__device__ __forceinline__ int count_above(const unsigned long long* list, int n, unsigned long long key) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] > key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
+  return v;
 }
 
 struct RowShared {
-  unsigned long long sorted[kRowWarps][32];
-  unsigned long long buf[(kMaxBeamOut + 1) * 33];  // at most kMaxBeamOut threads' logits and the list
-  unsigned long long top[kMaxBeamOut];
-  unsigned long long limit;
-  float m[kRowWarps], s[kRowWarps];
-  int count;
+  unsigned long long hit[kHits];
+  float peak[kRowWarps][32], sum[kRowWarps];  // peak: the threads' maxima
+  float top, limit;
+  int count;                                  // of hit
 };
 
-// Vector `vec` of a row whose first logit is number `lead` of its 16-byte
-// aligned vector 0.  A vector that reaches over an end of the row or of the
-// split is left to loads of single logits (`edge`).
-template <int DT>
-__device__ __forceinline__ void load_vec(const char* base, int vec, int vend, int lead, int vocab, uint4& raw, bool& edge) {
-  constexpr int PER = Logit<DT>::kPer;
-  const int first = vec * PER - lead;
-  edge = vec >= vend || first < 0 || first + PER > vocab;
-  if (!edge) raw = __ldcs(reinterpret_cast<const uint4*>(base) + vec);
+// The n-th largest of groups' maxima: a group for each lane, of all warps, for
+// n <= 16, else two, of the even and the odd warps (the n-th of n groups would
+// be their smallest, and four times n logits reach it).  By lane, so that a part
+// which leaves warps without logits still has every group.  `top`: the largest.
+__device__ __forceinline__ float nth_peak(const float (*peak)[32], int n, float& top) {
+  const int lane = threadIdx.x & 31;
+  float a = peak[0][lane], b = peak[1][lane];
+#pragma unroll
+  for (int w = 2; w < kRowWarps; w += 2) {
+    a = fmaxf(a, peak[w][lane]);
+    b = fmaxf(b, peak[w + 1][lane]);
+  }
+  float v;
+  if (n <= 16) {
+    v = sort_lanes(fmaxf(a, b));
+  } else {
+    v = fmaxf(sort_lanes(a), __shfl_sync(0xffffffffu, sort_lanes(b), 31 - lane));  // the 32 largest, falling and rising
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, v, step);
+      v = (lane & step) == 0 ? fmaxf(v, o) : fminf(v, o);
+    }
+  }
+  top = __shfl_sync(0xffffffffu, v, 0);
+  return __shfl_sync(0xffffffffu, v, n - 1);
+}
+
+// Run j of a row is its 16 bytes with logits [j PER, (j + 1) PER).  `base` is the
+// row's start rounded down to 16 bytes and `lead` (in bytes) what that left
+// off: run j lies in the aligned pieces j and j + 1 of base.
+__device__ __forceinline__ uint4 shift_run(const uint4& a, const uint4& b, int lead) {
+  uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) x[i] = lead & 8 ? x[i + 2] : x[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) x[i] = lead & 4 ? x[i + 1] : x[i];
+  const unsigned pick = lead & 2 ? 0x5432 : 0x3210;
+  return make_uint4(__byte_perm(x[0], x[1], pick), __byte_perm(x[1], x[2], pick), __byte_perm(x[2], x[3], pick),
+                    __byte_perm(x[3], x[4], pick));
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamParams p) {
+struct Row {
+  static constexpr int SZ = logit_bytes<DT>();
+  static constexpr int PER = 16 / SZ;
+  const char* first;
+  const uint4* base;
+  int lead, vocab;
+  int safe0, safe1;  // runs [safe0, safe1) lie in pieces that belong to the row entirely
+
+  __device__ __forceinline__ Row(const BeamParams& p, int row) {
+    const int b = row / p.beams;
+    first = static_cast<const char*>(p.logits) +
+            (b * p.stride_seq + static_cast<long long>(row - b * p.beams) * p.stride_beam) * SZ;
+    lead = static_cast<int>(reinterpret_cast<uintptr_t>(first) & 15);
+    base = reinterpret_cast<const uint4*>(first - lead);
+    vocab = p.vocab;
+    safe0 = lead ? 1 : 0;
+    safe1 = (vocab + lead / SZ) / PER - safe0;
+  }
+  __device__ __forceinline__ float one(int i) const {
+    if constexpr (DT == PA_DTYPE_F32) return reinterpret_cast<const float*>(first)[i];
+    else if constexpr (DT == PA_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(first)[i]);
+    else return __half2float(reinterpret_cast<const __half*>(first)[i]);
+  }
+  // Run j, with -inf past the row's end.
+  __device__ __forceinline__ uint4 run(int j) const {
+    if (j >= safe0 && j < safe1) return lead ? shift_run(__ldg(base + j), __ldg(base + j + 1), lead) : __ldg(base + j);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (SZ == 4) {
+        const int i = j * PER + k;
+        w[k] = i < vocab ? reinterpret_cast<const uint32_t*>(first)[i] : word_lowest<DT>();
+      } else {
+        const int i = j * PER + 2 * k;
+        const uint16_t* r = reinterpret_cast<const uint16_t*>(first);
+        const uint32_t low = word_lowest<DT>() & 0xffffu;
+        w[k] = (i < vocab ? r[i] : low) | (i + 1 < vocab ? r[i + 1] : low) << 16;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// N runs into a thread's maximum m and its sum s of exp(x - m); returns their maximum.
+template <int DT, int N>
+__device__ __forceinline__ float take_runs(const uint4 (&u)[N], float& m, float& s) {
+  uint32_t a = word_max<DT>(u[0].x, u[0].y), b = word_max<DT>(u[0].z, u[0].w);
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    a = word_max<DT>(word_max<DT>(a, u[i].x), u[i].y);
+    b = word_max<DT>(word_max<DT>(b, u[i].z), u[i].w);
+  }
+  const float2 f = word_logits<DT>(word_max<DT>(a, b));
+  const float top = fminf(fmaxf(f.x, f.y), FLT_MAX);
+  if (top > m) {
+    s *= ex2((m - top) * kLog2e);
+    m = top;
+  }
+  const float ref = fmaxf(m, -FLT_MAX);
+  auto all = [&](auto&& term) {  // term: of two logits, as a pair
+    uint64_t part[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      if constexpr (DT == PA_DTYPE_F32) {
+        part[0] = f2_add(part[0], term(__uint_as_float(w[0]), __uint_as_float(w[1])));
+        part[1] = f2_add(part[1], term(__uint_as_float(w[2]), __uint_as_float(w[3])));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 g = word_logits<DT>(w[k]);
+          part[k & 1] = f2_add(part[k & 1], term(g.x, g.y));
+        }
+      }
+    }
+    float a, b;
+    f2_unpack(f2_add(part[0], part[1]), a, b);
+    return a + b;
+  };
+  // exp(x - ref) = 2^(x L + c) 2^e with c = -ref L rounded and e what that left off
+  const float c = -ref * kLog2e, e = fmaf(-ref, kLog2e, -c);
+  float sum = NAN;
+  if (fabsf(ref) < 1e30f) {
+    const uint64_t scale = f2_pack(kLog2e, kLog2e), shift = f2_pack(c, c);
+    sum = all([&](float x, float y) {
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(x, y), scale, shift), a, b);
+      return f2_pack(ex2(a), ex2(b));
+    });
+    sum = fmaf(sum, e * 0.6931472f, sum);
+  }
+  if (!(sum <= FLT_MAX)) {  // NaN, +inf, or a maximum that x L would pass the largest float for
+    sum = all([&](float x, float y) { return f2_pack(ex2((clean(x) - ref) * kLog2e), ex2((clean(y) - ref) * kLog2e)); });
+  }
+  s += sum;
+  return top;
+}
+
+// The warp's list (lane i: the i-th largest key) takes the lanes' keys above its n-th.
+__device__ __forceinline__ void insert_keys(unsigned long long& list, int n, bool hit, unsigned long long key) {
+  const int lane = threadIdx.x & 31;
+  unsigned long long last = __shfl_sync(0xffffffffu, list, n - 1);
+  unsigned todo = __ballot_sync(0xffffffffu, hit && key > last);
+  while (todo) {
+    const int from = __ffs(todo) - 1;
+    const unsigned long long k = __shfl_sync(0xffffffffu, key, from);
+    const int place = __popc(__ballot_sync(0xffffffffu, list > k));
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
+    if (lane == place) list = k;
+    else if (lane > place) list = up;
+    last = __shfl_sync(0xffffffffu, list, n - 1);
+    todo = __ballot_sync(0xffffffffu, hit && key > last) & ~((2u << from) - 1);
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas) beam_rows_kernel(const BeamParams p) {
   pdl_enter();
-  using L = Logit<DT>;
+  constexpr int PER = Row<DT>::PER, SZ = Row<DT>::SZ;
+  extern __shared__ uint4 ring[];  // [warp][stage][kChunkRuns + 1] pieces, then spans' maxima [span][thread]
   __shared__ RowShared sh;
-  const int row = blockIdx.x, split = blockIdx.y;
-  if (p.finished && p.finished[row]) return;
-  const int b = row / p.beams;
-  const long long at = b * p.stride_seq + static_cast<long long>(row - b * p.beams) * p.stride_beam;
-  const char* first = static_cast<const char*>(p.logits) + at * L::kBytes;
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15) / L::kBytes);
-  const char* base = first - lead * L::kBytes;
-  const int vecs = static_cast<int>((static_cast<long long>(lead) + p.vocab + L::kPer - 1) / L::kPer);
-  const int v0 = split * p.split_vecs;
-  const int vend = min(vecs, v0 + p.split_vecs);
   const int n = p.num_out;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int out = row * p.splits + split;
-
-  if (tid == 0) sh.limit = 0;
-  for (int i = tid; i < n; i += kRowThreads) sh.top[i] = 0;
-  float m = -INFINITY, s = 0.f;  // this thread's maximum and sum of exp(x - m)
-  __syncthreads();
-
-  for (int t0 = v0; t0 < vend; t0 += kRowThreads * kVec) {
-    float x[L::kMine];
-    uint4 raw[kVec];
-    bool edge[kVec];
+  const int runs = (p.vocab + PER - 1) / PER;
+  uint4* const mine = ring + warp * kStages * (kChunkRuns + 1);
+  const int row = blockIdx.x, out = row * p.parts + blockIdx.y;
+  if (p.finished && p.finished[row]) return;
+  const Row<DT> r(p, row);
+  const int u0 = blockIdx.y * p.part_units, u1 = min(p.row_units, u0 + p.part_units);
+  if (tid == 0) sh.count = 0;
+  // ---- maximum and sum over the units [u0, u1) of the row, in each a chunk for
+  // every warp.  Chunks whose pieces all belong to the row come through the
+  // warp's own ring of asynchronous copies; the row's ends are read run by run.
+  __nv_bfloat16* const peaks = reinterpret_cast<__nv_bfloat16*>(ring + kRowWarps * kStages * (kChunkRuns + 1));
+  float m = -INFINITY, s = 0.f, span = -INFINITY;
+  auto start = [&](int u) { return u * kUnitRuns + warp * kChunkRuns; };
+  auto ringed = [&](int u) { return start(u) >= r.safe0 && start(u) + kChunkRuns <= r.safe1; };
+  auto stream = [&](auto shifts) {  // shifts: the row starts off a 16-byte boundary
+    auto fetch = [&](int u, int stage) {  // one commit group, empty where there is nothing to fetch
+      if (u < u1 && ringed(u)) {
+        const uint4* src = r.base + start(u) + lane;
+        const uint32_t dst = smem_u32(mine + stage * (kChunkRuns + 1) + lane);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) load_vec<DT>(base, t0 + j * kRowThreads + tid, vend, lead, p.vocab, raw[j], edge[j]);
+        for (int k = 0; k < kLaneRuns; ++k) cp_async_16(dst + 512 * k, src + 32 * k, 16);
+        if (shifts && lane == 0) cp_async_16(dst + 512 * kLaneRuns, src + kChunkRuns, 16);
+      }
+      cp_async_commit();
+    };
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      if (!edge[j]) {
-        unpack<DT>(raw[j], x + j * L::kPer);
+    for (int i = 0; i < kStages - 1; ++i) fetch(u0 + i, i);
+    int stage = 0;
+    for (int u = u0; u < u1; ++u) {
+      __syncwarp();  // the stage before this one has been read
+      fetch(u + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      uint4 x[kLaneRuns];
+      if (ringed(u)) {
+        const uint4* src = mine + stage * (kChunkRuns + 1) + lane;
+#pragma unroll
+        for (int k = 0; k < kLaneRuns; ++k) x[k] = src[32 * k];
+        if (shifts) {
+#pragma unroll
+          for (int k = 0; k < kLaneRuns; ++k) x[k] = shift_run(x[k], src[32 * k + 1], r.lead);
+        }
       } else {
-        const int vec = t0 + j * kRowThreads + tid;
 #pragma unroll
-        for (int e = 0; e < L::kPer; ++e) {
-          const int i = vec * L::kPer - lead + e;
-          x[j * L::kPer + e] = (vec < vend && i >= 0 && i < p.vocab) ? load_one<DT>(first, i) : -INFINITY;
-        }
+        for (int k = 0; k < kLaneRuns; ++k) x[k] = r.run(start(u) + 32 * k + lane);
       }
+      const float top = take_runs<DT, kLaneRuns>(x, m, s);
+      span = ((u - u0) & ((1 << p.log_span) - 1)) == 0 ? top : fmaxf(span, top);
+      peaks[((u - u0) >> p.log_span) * kRowThreads + tid] = __float2bfloat16_ru(span);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    // ---- sum of exponentials -------------------------------------------------
-    float tmax = x[0];
-#pragma unroll
-    for (int e = 1; e < L::kMine; ++e) tmax = fmaxf(tmax, x[e]);  // fmaxf drops NaN
-    tmax = fminf(fmaxf(tmax, -INFINITY), FLT_MAX);
-    if (tmax > m) {
-      s *= ex2((m - tmax) * kLog2e);  // m = -inf gives 0
-      m = tmax;
+  };
+  if (r.lead) stream(std::true_type());
+  else stream(std::false_type());
+  sh.peak[warp][lane] = m;
+  __syncthreads();
+  if (warp == 0) {
+    float top;
+    const float limit = nth_peak(sh.peak, n, top);
+    if (lane == 0) {
+      sh.top = fminf(top, FLT_MAX);
+      sh.limit = limit;
     }
-    const float ref = fmaxf(m, -FLT_MAX);
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < L::kMine; ++e) part[e & 3] += ex2((x[e] - ref) * kLog2e);
-    float sum = (part[0] + part[1]) + (part[2] + part[3]);
-    if (!(sum <= FLT_MAX)) {  // a NaN or +inf among them
-      sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < L::kMine; ++e) sum += ex2((clean(x[e]) - ref) * kLog2e);
-    }
-    s += sum;
-    // ---- the best n logits so far ----------------------------------------------
-    const unsigned long long limit = sh.limit;
-    const int token0 = (t0 + tid) * L::kPer - lead;
-    auto token_of = [&](int j, int e) { return token0 + j * kRowThreads * L::kPer + e; };
-    auto valid = [&](int j, int tok) { return t0 + j * kRowThreads + tid < vend && tok >= 0 && tok < p.vocab; };
-    unsigned long long best = 0;  // this thread's largest key, where it may pass the limit
-    if (limit == 0 || tmax >= key_logit(limit)) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-#pragma unroll
-        for (int e = 0; e < L::kPer; ++e) {
-          const int tok = token_of(j, e);
-          const float v = x[j * L::kPer + e];
-          if ((v >= tmax || tmax == -INFINITY) && valid(j, tok)) {  // a NaN counts as -inf
-            const unsigned long long k = make_key(v, tok);
-            best = k > best ? k : best;
-          }
-        }
-    }
-    if (!__syncthreads_or(best > limit)) continue;
-    // The n-th largest of the threads' best keys bounds the candidates from
-    // below, and only the n threads at or above it can hold any.
-    {
-      unsigned long long k = best;
-#pragma unroll
-      for (int size = 2; size <= 32; size <<= 1) {
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-          const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, step);
-          const bool larger = ((lane & size) == 0) == ((lane & step) == 0);
-          k = (larger == (o > k)) ? o : k;
-        }
-      }
-      sh.sorted[warp][lane] = k;
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      int rank = lane;
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w)
-        if (w != warp) {
-          int a = count_above(sh.sorted[w], 32, k);
-          if (k == 0 && w < warp) a = 32;  // zeros stand for absent keys: any order among them
-          rank += a;
-        }
-      if (rank == n - 1) sh.limit = k > limit ? k : limit;
-      for (int i = tid; i < n; i += kRowThreads) {
-        const unsigned long long k0 = sh.top[i];
-        if (k0) sh.buf[atomicAdd(&sh.count, 1)] = k0;
-      }
-      __syncthreads();
-    }
-    const unsigned long long low = sh.limit;
-    if (best && best >= low) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-#pragma unroll
-        for (int e = 0; e < L::kPer; ++e) {
-          const int tok = token_of(j, e);
-          if (valid(j, tok)) {
-            const unsigned long long k = make_key(x[j * L::kPer + e], tok);
-            if (k >= low && k > limit) sh.buf[atomicAdd(&sh.count, 1)] = k;
-          }
-        }
-    }
-    __syncthreads();
-    const int have = sh.count;
-    for (int i = tid; i < have; i += kRowThreads) {
-      const unsigned long long k = sh.buf[i];
-      int r = 0;
-      for (int q = 0; q < have; ++q) r += sh.buf[q] > k;
-      if (r < n) sh.top[r] = k;
-    }
-    __syncthreads();
-    if (tid == 0) sh.limit = sh.top[n - 1];
-    __syncthreads();
   }
-
-  // ---- join the threads' sums ---------------------------------------------------
-  float mm = m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  s *= ex2((m - fmaxf(mm, -FLT_MAX)) * kLog2e);
+  __syncthreads();
+  // ---- the spans whose maximum reaches T, of this warp's threads whose own does
+  const float top = sh.top, limit = sh.limit;
+  unsigned short* const list = reinterpret_cast<unsigned short*>(mine);  // the warp is through with its ring
+  const int spans = ((u1 - u0 - 1) >> p.log_span) + 1;
+  int listed = 0;
+  for (unsigned todo = __ballot_sync(0xffffffffu, m >= limit); todo; todo &= todo - 1) {
+    const int t = __ffs(todo) - 1;
+    const bool in = lane < spans && __bfloat162float(peaks[lane * kRowThreads + warp * 32 + t]) >= limit;
+    const unsigned some = __ballot_sync(0xffffffffu, in);
+    if (in) list[listed + __popc(some & ((1u << lane) - 1))] = static_cast<unsigned short>(lane * 32 + t);
+    listed += __popc(some);
+  }
+  __syncwarp();
+  // ---- their runs once more, a lane for each; few hold a logit at T
+  const int log_each = p.log_span + kLogLaneRuns, items = listed << log_each;
+  auto run_of = [&](int i) {  // of item i; past every row where there is none
+    if (i >= items) return runs;
+    const int entry = list[i >> log_each], e = i & ((1 << log_each) - 1);
+    const int u = u0 + (entry / 32 << p.log_span) + (e >> kLogLaneRuns);
+    return u < u1 ? start(u) + e % kLaneRuns * 32 + entry % 32 : runs;
+  };
+  int j = run_of(lane);
+  uint4 x = make_uint4(0, 0, 0, 0);
+  if (j < runs) x = r.run(j);
+  s *= ex2((m - fmaxf(top, -FLT_MAX)) * kLog2e);  // the part's sum, while that comes
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) {
-    sh.m[warp] = mm;
-    sh.s[warp] = s;
+  if (lane == 0) sh.sum[warp] = s;
+  for (int i0 = 0; i0 < items; i0 += 32) {
+    if (i0) {
+      j = run_of(i0 + lane);
+      if (j < runs) x = r.run(j);
+    }
+    const float2 f = word_logits<DT>(word_max<DT>(word_max<DT>(x.x, x.y), word_max<DT>(x.z, x.w)));
+    if (j >= runs || fmaxf(f.x, f.y) < limit) continue;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const float2 g = word_logits<DT>(w[e * SZ / 4]);
+      const float v = SZ == 2 && (e & 1) ? g.y : g.x;
+      if ((v >= limit || limit == -INFINITY) && j * PER + e < p.vocab) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kHits) sh.hit[at] = make_key(v, j * PER + e);
+      }
+    }
   }
   __syncthreads();
-  if (tid == 0) {
-    float M = sh.m[0], S = 0.f;
-    for (int w = 1; w < kRowWarps; ++w) M = fmaxf(M, sh.m[w]);
-    for (int w = 0; w < kRowWarps; ++w) S += sh.s[w] * ex2((sh.m[w] - fmaxf(M, -FLT_MAX)) * kLog2e);
-    p.part_max[out] = M;
-    p.part_sum[out] = S;
+  int count = sh.count;
+  if (count > kHits) {  // many equal logits: each warp keeps its n best
+    unsigned long long best = 0;
+    for (int i0 = 0; i0 < items; i0 += 32 / PER) {  // a lane for each logit of 32 / PER runs
+      const int j = run_of(i0 + lane / PER);
+      const int i = j < runs ? j * PER + lane % PER : p.vocab;
+      const float v = i < p.vocab ? r.one(i) : 0.f;
+      insert_keys(best, n, i < p.vocab && (v >= limit || limit == -INFINITY), make_key(v, i));
+    }
+    __syncthreads();
+    if (lane < n) sh.hit[warp * n + lane] = best;
+    count = kRowWarps * n;
+    __syncthreads();
   }
-  for (int i = tid; i < n; i += kRowThreads) p.part_key[static_cast<long long>(out) * n + i] = sh.top[i];
+  if (tid == 0) {
+    float total = 0.f;
+    for (int w = 0; w < kRowWarps; ++w) total += sh.sum[w];
+    p.part_max[out] = top;
+    p.part_sum[out] = total;
+  }
+  // ---- a key's place is the number of keys above it, counted by eight lanes
+  unsigned long long* keys = p.part_key + static_cast<long long>(out) * n;
+  if (tid < n && tid >= count) keys[tid] = 0;
+  for (int i0 = warp * 4; i0 < count; i0 += kRowThreads / 8) {
+    const int i = i0 + (lane >> 3);
+    const unsigned long long key = i < count ? sh.hit[i] : 0;
+    int place = 0;
+    for (int q = lane & 7; q < count; q += 8) place += sh.hit[q] > key || (sh.hit[q] == key && q < i);
+#pragma unroll
+    for (int o = 4; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (i < count && place < n && (lane & 7) == 0) keys[place] = key;
+  }
 }
 
-// One CTA per sequence: the splits' lists of each beam, then the beams.  An
-// entry's place is the number of entries above it, found by binary search in
-// the other sorted lists.  Scores are formed in 64 bits: candidates of
-// different beams lie as near as their logits' rounding, and -50 + x - lse in
-// 32 bits would swap them.
+// One CTA per sequence: the n best of its beams' parts.  Scores are compared in
+// 64 bits: candidates of different beams lie as near as their logits' rounding,
+// and -50 + x - lse in 32 bits would swap them.  Only candidates that may be
+// among the n best get there: as in the rows, T is the n-th largest of 32 groups'
+// maxima, here of scores in fp32 and less their rounding.  A part's list is
+// sorted, so the groups mix ranks and lists.
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamParams p) {
-  pdl_enter();
   extern __shared__ unsigned long long dyn[];
-  const int b = blockIdx.x, K = p.beams, S = p.splits, n = p.num_out;
+  const int b = blockIdx.x, K = p.beams, S = p.parts, n = p.num_out;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  unsigned long long* keys = dyn;                                // [K][S][n]
-  unsigned long long* rows = keys + K * S * n;                   // [K][n]
-  double* score = reinterpret_cast<double*>(rows + K * n);       // [K][n]
-  __shared__ double lse[kMaxBeams];
-  __shared__ unsigned char done[kMaxBeams];
+  const int per = S * n, total = K * per;
+  unsigned long long* keys = dyn;                             // every candidate's
+  double* score = reinterpret_cast<double*>(keys + total);    // of the candidates at T
+  int* which = reinterpret_cast<int*>(score + total);
+  __shared__ double top[kMaxBeams], logsum[kMaxBeams];  // apart: beside a maximum of 1e30 the logarithm would vanish
+  __shared__ float ftop[kMaxBeams], offset[kMaxBeams];
+  __shared__ int group[32], count;
+  __shared__ float limit_of_all;
   const int row0 = b * K;
-  for (int i = tid; i < K * S * n; i += kMergeThreads) {
-    const int k = i / (S * n);
+  if (tid < 32) group[tid] = static_cast<int>(0x80000000u);
+  if (tid == 0) count = 0;
+  pdl_enter();
+  // rows and lists of candidate i, by multiplication (total < 2^14: exact)
+  const unsigned per_inv = (1u << 28) / per + 1, n_inv = (1u << 28) / n + 1;
+  auto over = [](int i, unsigned inv) { return static_cast<int>((static_cast<unsigned long long>(i) * inv) >> 28); };
+  for (int k = warp; k < K; k += kMergeWarps) {
     const bool fin = p.finished && p.finished[row0 + k];
-    keys[i] = fin ? 0 : p.part_key[static_cast<long long>(row0) * S * n + i];
-  }
-  for (int i = tid; i < K * n; i += kMergeThreads) rows[i] = 0;
-  for (int k = warp; k < K; k += kMergeThreads / 32) {
-    const bool fin = p.finished && p.finished[row0 + k];
-    float m = -INFINITY, s = 0.f;
-    if (!fin && lane < S) {
-      m = p.part_max[(row0 + k) * S + lane];
-      s = p.part_sum[(row0 + k) * S + lane];
-    }
+    const int parts = fin ? 0 : S, at = (row0 + k) * S;
+    float m = lane < parts ? p.part_max[at + lane] : -INFINITY;
+    float t = lane < parts ? p.part_sum[at + lane] : 0.f;
+    const float base = p.scores[row0 + k];
     float M = m;
+    for (int i = lane + 32; i < parts; i += 32) M = fmaxf(M, p.part_max[at + i]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    double sum = s > 0.f ? static_cast<double>(s) * exp(static_cast<double>(m) - static_cast<double>(M)) : 0.0;
+    double sum = t > 0.f ? t * exp(static_cast<double>(m) - static_cast<double>(M)) : 0.0;
+    for (int i = lane + 32; i < parts; i += 32) {
+      t = p.part_sum[at + i];
+      if (t > 0.f) sum += t * exp(static_cast<double>(p.part_max[at + i]) - static_cast<double>(M));
+    }
+    if (S > 1) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
     if (lane == 0) {
-      lse[k] = sum > 0.0 ? static_cast<double>(M) + log(sum) : 0.0;  // a row of -inf: every score is -inf
-      done[k] = fin;
+      // a row of -inf has no sum: all its scores are -inf; a finished beam's are 0 and -inf
+      const double log_sum = sum > 0.0 ? log(sum) : 0.0;
+      top[k] = sum > 0.0 ? M : 0.0;
+      ftop[k] = sum > 0.0 ? M : 0.f;
+      logsum[k] = log_sum;
+      offset[k] = static_cast<float>(base - log_sum);
     }
   }
+  for (int i = tid; i < total; i += kMergeThreads) {
+    const int k = over(i, per_inv), r = i - k * per;
+    unsigned long long key;
+    if (p.finished && p.finished[row0 + k]) {  // eos, then the other tokens at -inf
+      key = 0;
+      if (r < n && r < p.vocab) key = make_key(r == 0 ? 0.f : -INFINITY, r == 0 ? p.eos : r - 1 + (r - 1 >= p.eos));
+    } else {
+      key = p.part_key[static_cast<long long>(row0) * per + i];
+    }
+    keys[i] = key;
+  }
   __syncthreads();
-  for (int i = tid; i < K * S * n; i += kMergeThreads) {
+  auto rough = [&](int i, int k) {
+    const float v = (key_logit(keys[i]) - ftop[k]) + offset[k];
+    return v == v ? v : -INFINITY;
+  };
+  for (int i = tid; i < total; i += kMergeThreads) {
+    if (!keys[i]) continue;
+    const int list = over(i, n_inv), r = i - list * n;
+    const int f = __float_as_int(rough(i, over(i, per_inv)) + 0.f);
+    atomicMax(&group[(r + 11 * list) & 31], f >= 0 ? f : f ^ 0x7fffffff);  // floats in their order
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int g = group[lane];
+    const float v = sort_lanes(g == static_cast<int>(0x80000000u) ? -INFINITY : __int_as_float(g >= 0 ? g : g ^ 0x7fffffff));
+    if (lane == n - 1) limit_of_all = v;
+  }
+  __syncthreads();
+  const float limit = limit_of_all;
+  for (int i = tid; i < total; i += kMergeThreads) {
     const unsigned long long key = keys[i];
-    if (!key) continue;
-    const int list = i / n, k = list / S;
-    int rank = i - list * n;
-    for (int q = k * S; q < (k + 1) * S && rank < n; ++q)
-      if (q != list) rank += count_above(keys + q * n, n, key);
-    if (rank < n) rows[k * n + rank] = key;
+    const int k = over(i, per_inv);
+    bool hit = key != 0;
+    if (hit) {
+      const float v = rough(i, k);
+      // x - top and the sum with the offset are rounded twice, the limit's too
+      const float slack = 4.f * 1.2e-7f * (fabsf(limit) + fabsf(v) + fabsf(offset[k]));
+      hit = !(v < limit) || !(limit - v > slack);
+    }
+    if (!hit) continue;
+    const int at = atomicAdd(&count, 1);
+    const double v = static_cast<double>(p.scores[row0 + k]) + ((static_cast<double>(key_logit(key)) - top[k]) - logsum[k]);
+    score[at] = v == v ? v : -INFINITY;  // NaN counts as -inf
+    which[at] = i;
   }
   __syncthreads();
-  for (int i = tid; i < K * n; i += kMergeThreads) {
-    const int k = i / n, r = i - k * n;
-    const float base = p.scores[row0 + k];
-    double v = -INFINITY;
-    if (done[k]) {
-      const int tok = r == 0 ? p.eos : r - 1 + (r - 1 >= p.eos);
-      if (r < p.vocab) {
-        rows[i] = make_key(r == 0 ? 0.f : -INFINITY, tok);
-        if (r == 0) v = base;
+  // a candidate's place is the number of candidates before it, counted by eight lanes
+  const int have = count;
+  for (int i0 = warp * 4; i0 < have; i0 += kMergeThreads / 8) {
+    const int i = i0 + (lane >> 3);
+    const bool in = i < have;
+    const double v = in ? score[i] : 0.0;
+    const int c = in ? which[i] : 0, k = over(c, per_inv);
+    int place = 0;
+    for (int q = lane & 7; q < have; q += 8) {
+      const double o = score[q];
+      if (o > v) ++place;
+      if (o == v) {
+        const int d = which[q], l = over(d, per_inv);
+        place += l < k || (l == k && keys[d] > keys[c]);
       }
-    } else if (rows[i]) {
-      v = static_cast<double>(base) + (static_cast<double>(key_logit(rows[i])) - lse[k]);
     }
-    score[i] = v == v ? v : -INFINITY;  // NaN counts as -inf
-  }
-  __syncthreads();
-  const int width = min(n, p.vocab);  // entries of a beam's list
-  for (int i = tid; i < K * n; i += kMergeThreads) {
-    const int k = i / n, r = i - k * n;
-    if (r >= width) continue;
-    const double v = score[i];
-    int rank = r;
-    for (int q = 0; q < K && rank < n; ++q) {
-      if (q == k) continue;
-      int lo = 0, hi = width;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const double o = score[q * n + mid];
-        if (o > v || (o == v && q < k)) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank < n) {
-      const long long o = static_cast<long long>(b) * n + rank;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (in && place < n && (lane & 7) == 0) {
+      const long long o = static_cast<long long>(b) * n + place;
       p.out_scores[o] = static_cast<float>(v);
-      p.out_tokens[o] = key_token(rows[i]);
+      p.out_tokens[o] = key_token(keys[c]);
       p.out_parents[o] = k;
     }
   }
@@ -365,33 +555,61 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
 
 }  // namespace
 
-// Splits of a row: enough CTAs for two rounds of the four that fit an SM, at
-// least one tile each, no more than the merge joins with a lane each and its
-// shared memory (64 KB of keys) holds.
-int beam_splits(int rows, int beams, int num_out, int vocab, int dtype, int aligned, int* split_vecs) {
+// Parts of a row: the number that leaves the fewest SMs idle at the rows
+// kernel's end, with a unit's time added to each part for its selection; the
+// merge's shared memory bounds it.
+void beam_plan(BeamParams& p, int dtype) {
   const int per = dtype == PA_DTYPE_F32 ? 4 : 8;
-  const long long vecs = (static_cast<long long>(vocab) + per - 1) / per + (aligned ? 0 : 1);  // a row may start inside its first vector
-  const long long tile = kRowThreads * kVec;
-  long long s = (2LL * 4 * device_sm_count() + rows - 1) / rows;
-  const long long most[3] = {(vecs + tile - 1) / tile, kMaxSplits, 8192 / (static_cast<long long>(beams) * num_out)};
-  for (long long m : most) s = s < m ? s : m;
-  if (s < 1) s = 1;
-  *split_vecs = static_cast<int>((vecs + s - 1) / s);
-  return static_cast<int>((vecs + *split_vecs - 1) / *split_vecs);
+  const long long rows = static_cast<long long>(p.seqs) * p.beams;
+  const long long runs = (static_cast<long long>(p.vocab) + per - 1) / per;
+  const long long units = (runs + kUnitRuns - 1) / kUnitRuns;
+  const long long slots = static_cast<long long>(kRowCtas) * device_sm_count();
+  const long long fit = kMergeKeys / (static_cast<long long>(p.beams) * p.num_out);
+  long long least = 0;
+  for (long long parts = 1; parts <= units && parts <= fit; ++parts) {
+    const long long share = (units + parts - 1) / parts, used = (units + share - 1) / share;
+    const long long cost = (rows * used + slots - 1) / slots * (share + 1);
+    if (parts == 1 || cost < least) {
+      least = cost;
+      p.part_units = static_cast<int>(share);
+      p.parts = static_cast<int>(used);
+    }
+  }
+  p.row_units = static_cast<int>(units);
+  p.log_span = 0;
+  while ((p.part_units - 1) >> p.log_span >= kSpans) ++p.log_span;
+}
+
+// Shared memory past the default, allowed once per device.
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return e;
+}
+
+template <int DT>
+cudaError_t launch_rows(const BeamParams& p, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  const int ring = kRowWarps * kStages * (kChunkRuns + 1) * 16;
+  const int smem = ring + (((p.part_units - 1) >> p.log_span) + 1) * kRowThreads * 2;
+  cudaError_t e = allow_smem(beam_rows_kernel<DT>, ring + kSpans * kRowThreads * 2, done);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(beam_rows_kernel<DT>, dim3(p.seqs * p.beams, p.parts), dim3(kRowThreads), smem, stream, p);
 }
 
 cudaError_t launch_beam_select(const BeamParams& p, int dtype, cudaStream_t stream) {
-  const dim3 grid(p.seqs * p.beams, p.splits);
-  cudaError_t e;
-  if (dtype == PA_DTYPE_F32) e = launch_pdl(beam_rows_kernel<PA_DTYPE_F32>, grid, dim3(kRowThreads), 0, stream, p);
-  else if (dtype == PA_DTYPE_BF16) e = launch_pdl(beam_rows_kernel<PA_DTYPE_BF16>, grid, dim3(kRowThreads), 0, stream, p);
-  else e = launch_pdl(beam_rows_kernel<PA_DTYPE_F16>, grid, dim3(kRowThreads), 0, stream, p);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem(beam_merge_kernel, kMergeKeys * 20 + 8, done);
   if (e != cudaSuccess) return e;
-  const size_t smem = (static_cast<size_t>(p.beams) * p.splits + 2 * p.beams) * p.num_out * 8;
-  if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  e = dtype == PA_DTYPE_F32    ? launch_rows<PA_DTYPE_F32>(p, stream)
+      : dtype == PA_DTYPE_BF16 ? launch_rows<PA_DTYPE_BF16>(p, stream)
+                               : launch_rows<PA_DTYPE_F16>(p, stream);
+  if (e != cudaSuccess) return e;
+  const size_t smem = static_cast<size_t>(p.beams) * p.parts * p.num_out * 20 + 8;
   e = launch_pdl(beam_merge_kernel, dim3(p.seqs), dim3(kMergeThreads), smem, stream, p);
   return e != cudaSuccess ? e : cudaGetLastError();
 }

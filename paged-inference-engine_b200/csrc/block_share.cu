@@ -49,7 +49,7 @@ __global__ void share_init_kernel(int* ref, int num_blocks, int* scratch, long l
 //             and the copy (copy_src[i], copy_dst[i], copy_slots[i])
 // Operations without a copy leave a pair of equal ids.
 __global__ void __launch_bounds__(kApplyThreads) apply_shared_kernel(const PoolParams p, const ShareParams s,
-                                                                     const int* ops, int n_ops, int log2BS,
+                                                                     const int* ops, int n_ops, int block_size,
                                                                      int* results, int* copy_src, int* copy_dst,
                                                                      int* copy_slots) {
   pdl_enter();
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kApplyThreads) apply_shared_kernel(const PoolP
         }
       } else {
         const int pc = parent >= 0 && parent < p.max_seqs ? p.count[parent] : -1;
-        const int full = n >> log2BS, tail = n & ((1 << log2BS) - 1);
+        const int full = n / block_size, tail = n - full * block_size;
         const int have = full + (tail > 0);
         if (pc < 0 || c >= 0) {
           res = POOL_FAILURE;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kCopyThreads) reorder_kernel(const PoolParams 
   }
 
   const int group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
-  unsigned* bitmap = reinterpret_cast<unsigned*>(s.scratch + kShareHead + 3LL * p.num_blocks);
+  unsigned* bitmap = reinterpret_cast<unsigned*>(s.scratch + kShareHead);
   if (threadIdx.x < 32) {
     const bool good = plan_group(p, r, log2BS, group, f, chunk == 0);
     if (threadIdx.x == 0) ok = good;
@@ -323,10 +323,10 @@ cudaError_t launch_block_pool_init_shared(const PoolParams& p, const ShareParams
 }
 
 cudaError_t launch_block_pool_apply_shared(const PoolParams& p, const ShareParams& s, const int* ops, int n_ops,
-                                           int log2BS, int* results, int* copy_src, int* copy_dst, int* copy_slots,
+                                           int block_size, int* results, int* copy_src, int* copy_dst, int* copy_slots,
                                            cudaStream_t stream) {
   if (n_ops <= 0) return cudaSuccess;
-  cudaError_t e = launch_pdl(apply_shared_kernel, dim3(1), dim3(kApplyThreads), 0, stream, p, s, ops, n_ops, log2BS,
+  cudaError_t e = launch_pdl(apply_shared_kernel, dim3(1), dim3(kApplyThreads), 0, stream, p, s, ops, n_ops, block_size,
                              results, copy_src, copy_dst, copy_slots);
   return e != cudaSuccess ? e : cudaGetLastError();
 }

@@ -1113,10 +1113,10 @@ int block_pool_apply_shared(const pa_block_pool_t* pool, const pa_block_share_t*
   if (rc) return rc;
   if (n_ops < 0) return fail(PA_ERR_INVALID, "n_ops < 0");
   if (n_ops > 0 && !ops) return fail(PA_ERR_INVALID, "ops is NULL");
-  if (!is_pow2(block_size)) return fail(PA_ERR_INVALID, "block_size %d must be a power of two", block_size);
+  if (block_size < 1) return fail(PA_ERR_INVALID, "block_size %d must be positive", block_size);
   if ((copy_src != nullptr) != (copy_dst != nullptr) || (copy_src != nullptr) != (copy_slots != nullptr))
     return fail(PA_ERR_INVALID, "copy_src, copy_dst and copy_slots come together");
-  cudaError_t e = pa::launch_block_pool_apply_shared(p, s, ops, n_ops, ilog2(block_size), results, copy_src, copy_dst,
+  cudaError_t e = pa::launch_block_pool_apply_shared(p, s, ops, n_ops, block_size, results, copy_src, copy_dst,
                                                      copy_slots, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_apply_shared launch");
 }
@@ -1216,9 +1216,8 @@ static int beam_params(const pa_beam_select_t* a, pa::BeamParams& p, size_t& byt
   p.out_scores = a->out_scores;
   p.out_tokens = a->out_tokens;
   p.out_parents = a->out_parents;
-  const int aligned = al(a->logits, 16) && row_al(a->stride_seq, e, 16) && row_al(a->stride_beam, e, 16);
-  p.splits = rows ? pa::beam_splits(static_cast<int>(rows), p.beams, p.num_out, p.vocab, a->dtype, aligned, &p.split_vecs) : 1;
-  bytes = static_cast<size_t>(rows) * p.splits * (8 * static_cast<size_t>(p.num_out) + 8);
+  if (rows) pa::beam_plan(p, a->dtype);
+  bytes = static_cast<size_t>(rows) * p.parts * (8 * static_cast<size_t>(p.num_out) + 8);
   return PA_OK;
 }
 
@@ -1241,7 +1240,7 @@ int beam_select(const pa_beam_select_t* a, void* workspace, size_t workspace_byt
   if (!al(p.logits, elt_size(a->dtype))) return fail(PA_ERR_INVALID, "logits misaligned");
   if (!workspace || workspace_bytes < bytes || !al(workspace, 16))
     return fail(PA_ERR_WORKSPACE, "beam_select: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, bytes);
-  const size_t lists = static_cast<size_t>(p.seqs) * p.beams * p.splits;
+  const size_t lists = static_cast<size_t>(p.seqs) * p.beams * p.parts;
   p.part_key = static_cast<unsigned long long*>(workspace);
   p.part_max = reinterpret_cast<float*>(p.part_key + lists * p.num_out);
   p.part_sum = p.part_max + lists;

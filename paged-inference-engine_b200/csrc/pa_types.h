@@ -169,17 +169,18 @@ cudaError_t launch_copy_blocks(const PageParams& g, const int* src, const int* d
                                int* status, cudaStream_t stream);
 
 // Shared blocks (csrc/block_share.cu): reference counts beside the pool, and
-// scratch that holds a launch ticket, counters, a bitmap and page lists.
+// scratch: a launch ticket and counters, a bitmap of freed blocks (zero between
+// launches; first, so that it stays zero when the pool shrinks) and page lists.
 enum : int { POOL_FORK = 2 };
 struct ShareParams {
   int* ref;
   int* scratch;
 };
-constexpr int kShareHead = 16;  // scratch words before the page lists
+constexpr int kShareHead = 16;  // scratch words before the bitmap
 cudaError_t launch_block_pool_init_shared(const PoolParams& p, const ShareParams& s, long long scratch_words,
                                           cudaStream_t stream);
 cudaError_t launch_block_pool_apply_shared(const PoolParams& p, const ShareParams& s, const int* ops, int n_ops,
-                                           int log2BS, int* results, int* copy_src, int* copy_dst, int* copy_slots,
+                                           int block_size, int* results, int* copy_src, int* copy_dst, int* copy_slots,
                                            cudaStream_t stream);
 struct ReorderParams {
   const int* slots;       // [groups, beams] pool row of each beam
@@ -203,15 +204,16 @@ struct BeamParams {
   const float* scores;                // [seqs, beams]
   const unsigned char* finished;      // [seqs, beams] or NULL
   int seqs, beams, vocab, num_out, eos;
-  int splits, split_vecs;
-  unsigned long long* part_key;  // [rows, splits, num_out]
-  float* part_max;               // [rows, splits]
+  int row_units, part_units, parts;  // units of a row and of a part of it, parts of a row
+  int log_span;                      // units of a span
+  unsigned long long* part_key;  // [rows, parts, num_out]
+  float* part_max;               // [rows, parts]
   float* part_sum;
   float* out_scores;
   int* out_tokens;
   int* out_parents;
 };
-int beam_splits(int rows, int beams, int num_out, int vocab, int dtype, int aligned, int* split_vecs);
+void beam_plan(BeamParams& p, int dtype);  // sets row_units, part_units, parts and log_span
 cudaError_t launch_beam_select(const BeamParams& p, int dtype, cudaStream_t stream);
 
 // K/V projection with the cache write in its epilogue (kv_project.cu): the

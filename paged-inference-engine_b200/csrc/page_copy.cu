@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const PagePar
 
 // ---- compaction -----------------------------------------------------------------
 // Scratch words: [2] pages to move, [3] live pages, [4] 1 when the pool was
-// refused; then map[NB] (new id of a moved page, else -1), src[NB], dst[NB].
+// refused; after the bitmap of freed blocks map[NB] (new id of a moved page, else -1), src[NB], dst[NB].
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanIds = 4;  // ids of a thread per round
 
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PoolPa
                                                                     int* live_out, int* status) {
   pdl_enter();
   __shared__ int warp_sum[32];
-  int* map = s.scratch + kShareHead;
+  int* map = s.scratch + kShareHead + (p.num_blocks + 31) / 32;
   int* src = map + p.num_blocks;
   int* dst = src + p.num_blocks;
   int mine = 0, live;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PoolPa
 __global__ void __launch_bounds__(kCopyThreads) compact_move_kernel(const PoolParams p, const ShareParams s, int after,
                                                                     const PageParams g, int* status, bool first) {
   pdl_enter();
-  const int* map = s.scratch + kShareHead;
+  const int* map = s.scratch + kShareHead + (p.num_blocks + 31) / 32;
   const int* src = map + p.num_blocks;
   const int* dst = src + p.num_blocks;
   const int moves = s.scratch[2], live = s.scratch[3];

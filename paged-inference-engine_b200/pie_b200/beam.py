@@ -1,0 +1,151 @@
+"""Beam search over the paged cache, with all decisions on the device.
+
+``BeamSearch`` keeps K beams of each of B sequences as rows of a
+``DeviceBlockManager``.  A step is: ``step_inputs()`` (a new block for beams
+whose last one is full, the beams' block tables, positions and lengths), the
+caller's model over them (``write_kv`` and ``paged_attention`` as in any
+decode step), and ``advance(logits)``: ``ops.beam_select`` picks the best
+continuations and ``reorder_beams`` makes the cache follow them: beams share
+their parents' full blocks, partly filled ones are copied.  Nothing is read
+back before ``finish()``.
+
+The reference decodes one sampled continuation per sequence
+(core/model_runner.py:28-159) and has no beams.
+"""
+from __future__ import annotations
+
+from typing import Sequence
+
+import torch
+
+from . import ops
+from .block_pool import AllocStatus, DeviceBlockManager
+
+
+class BeamSearch:
+    """``num_beams`` beams of each of ``seq_ids``, which hold ``num_tokens[i]`` prompt tokens in the cache.
+
+    ``logits`` [B, V] are those of each prompt's last token.  The beams' pool ids are ``beam_ids(i, k)``; the
+    sequences must hold exactly the blocks that their tokens fill.  A beam that emits ``eos_id`` is finished: it keeps
+    its score and competes with the others until ``finish``.
+    """
+
+    def __init__(self, pool: DeviceBlockManager, seq_ids: Sequence[int], num_tokens: Sequence[int], logits: torch.Tensor,
+                 num_beams: int, eos_id: int, max_new_tokens: int):
+        B, K = len(seq_ids), int(num_beams)
+        if logits.dim() != 2 or logits.shape[0] != B or len(num_tokens) != B:
+            raise ValueError(f"logits must be [{B}, vocab] and num_tokens hold {B} lengths")
+        if not 1 <= K <= logits.shape[1]:
+            raise ValueError(f"num_beams {K} is outside 1..vocab ({logits.shape[1]})")
+        if max_new_tokens < 1 or B < 1:
+            raise ValueError("at least one sequence and one new token are needed")
+        self.pool, self.B, self.K, self.eos = pool, B, K, int(eos_id)
+        self.seq_ids = [int(s) for s in seq_ids]
+        self.host_tokens = [int(n) for n in num_tokens]
+        dev = pool.free_top.device
+        made = []
+        try:
+            for s, n in zip(self.seq_ids, self.host_tokens):
+                st = pool.fork_beams(s, [self.beam_id(s, k) for k in range(1, K)], n)
+                if st is not AllocStatus.SUCCESS:
+                    raise RuntimeError(f"no beams for sequence {s}: {st.name}")
+                made.append(s)
+        except Exception:
+            for s in made:  # the prompts stay as they were
+                pool.dissolve_beams(s)
+            raise
+        pool.flush()
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.slots = pool.beam_slots(self.seq_ids)
+        self.num_tokens = torch.tensor(self.host_tokens, dtype=torch.int32).to(dev)
+        self.max_new = int(max_new_tokens)
+        self.history = torch.empty(2, self.max_new, B, K, **i32)  # tokens and parents of every step
+        self.q_len = torch.ones(B * K, **i32)
+        self.cu = torch.arange(B * K + 1, **i32)
+        self.scores = torch.zeros(B, 1, device=dev)
+        self.finished = torch.zeros(B, 1, dtype=torch.bool, device=dev)
+        self.steps = 0
+        self._room = False
+        self._choose(logits.unsqueeze(1))
+
+    @staticmethod
+    def beam_id(seq_id: int, k: int) -> object:
+        """The pool's id of beam k: the sequence itself, or (sequence, k)."""
+        return seq_id if k == 0 else (seq_id, k)
+
+    @property
+    def tokens(self) -> torch.Tensor:
+        """The beams' newest tokens, int32 [B, K]: the next step's inputs."""
+        return self.history[0, self.steps - 1]
+
+    def _choose(self, logits: torch.Tensor) -> torch.Tensor:
+        self.scores, tokens, parents = ops.beam_select(logits, self.scores, self.K, finished=self.finished, eos_id=self.eos)
+        self.finished = self.finished.gather(1, parents.long()) | (tokens == self.eos)
+        self.history[0, self.steps] = tokens
+        self.history[1, self.steps] = parents
+        self.steps += 1
+        return parents
+
+    def step_inputs(self) -> dict:
+        """Attention inputs of the next token of every beam (row ``b * K + k``), as ``DeviceBlockManager.step_inputs``.
+
+        The new token of a beam of sequence b goes to position ``num_tokens[b]`` and attends to one more key.
+        """
+        if self.steps >= self.max_new:
+            raise RuntimeError(f"the search was made for {self.max_new} new tokens")
+        pool, S = self.pool, self.B * self.K
+        if not self._room:
+            need = [s for s, n in zip(self.seq_ids, self.host_tokens) if n % pool.block_size == 0]
+            if pool.num_free_blocks() < len(need) * self.K:
+                raise RuntimeError(f"{len(need) * self.K} blocks are needed, {pool.num_free_blocks()} are free")
+            for s in need:
+                pool.allocate_beams(s, 1)
+            self._room = True
+        pool.flush()
+        cols = max(-(-(n + 1) // pool.block_size) for n in self.host_tokens)
+        i32 = dict(dtype=torch.int32, device=self.slots.device)
+        out = dict(block_table=torch.empty(S, cols, **i32), num_blocks_per_seq=torch.empty(S, **i32), q_len=self.q_len,
+                   kv_len=(self.num_tokens + 1).repeat_interleave(self.K), cu_seqlens=self.cu,
+                   positions=torch.empty(S, **i32), token_seq=torch.empty(S, **i32))
+        pool.step_rows(self.slots.view(-1), self.q_len, out["kv_len"], self.cu, S, out["block_table"],
+                       out["num_blocks_per_seq"], out["positions"], out["token_seq"], pool.status)
+        return out
+
+    def advance(self, logits: torch.Tensor) -> torch.Tensor:
+        """Take the next tokens from ``logits`` [B, K, V], after the step's K/V rows were written; returns ``tokens``."""
+        if not self._room:
+            raise RuntimeError("step_inputs() comes before advance()")
+        if tuple(logits.shape[:2]) != (self.B, self.K):
+            raise ValueError(f"logits must be [{self.B}, {self.K}, vocab]")
+        parents = self._choose(logits)
+        self.num_tokens += 1
+        self.host_tokens = [n + 1 for n in self.host_tokens]
+        self.slots = self.pool.reorder_beams(self.slots, parents, self.num_tokens)
+        self._room = False
+        return self.tokens
+
+    def all_finished(self) -> bool:
+        """Whether every beam has ended (reads the device: synchronises)."""
+        return bool(self.finished.all().item())
+
+    def finish(self) -> list[list[tuple[float, list[int]]]]:
+        """End the search and free its blocks: each sequence's (score, new tokens), best first, without what follows eos."""
+        tokens, parents = self.history[:, :self.steps].cpu().tolist()
+        scores = self.scores.cpu().tolist()
+        for s in self.seq_ids:
+            self.pool.release_beams(s)
+        self.pool.flush()
+        found = []
+        for b in range(self.B):
+            beams = []
+            for k in range(self.K):
+                line, j = [], k
+                for t in range(self.steps - 1, -1, -1):
+                    line.append(tokens[t][b][j])
+                    j = parents[t][b][j]
+                line.reverse()
+                if self.eos in line:
+                    line = line[:line.index(self.eos) + 1]
+                beams.append((scores[b][k], line))
+            found.append(beams)
+        return found

@@ -21,6 +21,16 @@ the padded table live in device memory:
 
 ``AllocResult.block_ids`` is a device tensor (the ids the call appended, valid
 once the queued operations have been flushed) rather than a host list.
+
+Sequences may share blocks (the reference's never do).  Every block counts its
+holders (``ref_count``); a block is written only while one sequence holds it:
+
+* ``fork(parent, child, num_tokens)`` gives the child the parent's first tokens:
+  the full blocks are shared, a partly filled last one is copied in every layer
+  of the caches named by ``attach_caches``;
+* ``fork_beams`` / ``allocate_beams`` / ``reorder_beams`` / ``release_beams``
+  keep the beams of a beam search, whose parents only the device knows;
+* ``compact`` moves the blocks in use to the lowest ids.
 """
 from __future__ import annotations
 
@@ -31,7 +41,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 
 class AllocStatus(enum.Enum):
@@ -56,7 +66,16 @@ class PaBlockPool(ctypes.Structure):
                 ("max_seqs", ctypes.c_int32), ("max_blocks_per_seq", ctypes.c_int32), ("_reserved", ctypes.c_int32)]
 
 
-POOL_ALLOCATE, POOL_RELEASE = 0, 1
+POOL_ALLOCATE, POOL_RELEASE, POOL_FORK = 0, 1, 2
+
+
+class _Prefix:
+    """Columns of a block table that sequences share: ``n`` blocks after those of ``up``, held by ``holders``."""
+
+    __slots__ = ("n", "holders", "up")
+
+    def __init__(self, n: int, holders: int, up: Optional["_Prefix"]):
+        self.n, self.holders, self.up = n, holders, up
 
 
 class BlockLedger:
@@ -76,10 +95,21 @@ class BlockLedger:
         self.blocks: dict[int, int] = {}      # seq_id -> blocks held
         self.slot: dict[int, int] = {}        # seq_id -> table row
         self.free_slots = list(range(self.max_seqs - 1, -1, -1))
-        self.ops: list[tuple[int, int, int]] = []
+        self.ops: list[tuple[int, ...]] = []
+        self.prefix: dict[int, _Prefix] = {}  # seq_id -> its last shared columns
+        self.beams: dict[int, tuple[int, ...]] = {}  # first beam -> all beams of a search
+        self.member: dict[int, int] = {}      # beam -> first beam
+
+    def _alone(self, seq_id: int) -> None:
+        if seq_id in self.member:
+            raise ValueError(f"sequence {seq_id} is a beam of {self.member[seq_id]}: beams are extended and released together")
 
     def allocate(self, seq_id: int, num_blocks: int) -> tuple[AllocStatus, int, int]:
         """Returns (status, slot, first new column); queues the operation on success."""
+        self._alone(seq_id)
+        return self._allocate(seq_id, num_blocks)
+
+    def _allocate(self, seq_id: int, num_blocks: int) -> tuple[AllocStatus, int, int]:
         num_blocks = int(num_blocks)
         if num_blocks < 0:
             raise ValueError("num_blocks must be >= 0")
@@ -101,15 +131,125 @@ class BlockLedger:
         return AllocStatus.SUCCESS, slot, base
 
     def release(self, seq_id: int) -> AllocStatus:
+        self._alone(seq_id)
+        return self._release(seq_id)
+
+    def _release(self, seq_id: int) -> AllocStatus:
         if seq_id not in self.blocks:
             return AllocStatus.FAILURE
         slot = self.slot.pop(seq_id)
         self.ops.append((POOL_RELEASE, slot, 0))
         self.free += self.blocks.pop(seq_id)
+        node = self.prefix.pop(seq_id, None)
+        while node is not None:  # columns that others hold are not free
+            node.holders -= 1
+            if node.holders:
+                self.free -= node.n
+            node = node.up
         self.free_slots.append(slot)
         return AllocStatus.SUCCESS
 
-    def take_ops(self) -> list[tuple[int, int, int]]:
+    def _shared(self, seq_id: int, columns: int) -> Optional[_Prefix]:
+        """The node that ends at ``columns`` columns of ``seq_id``, split off where there is none."""
+        if columns == 0:
+            return None
+        node = self.prefix.get(seq_id)
+        end, n = 0, node
+        while n is not None:
+            end += n.n
+            n = n.up
+        if columns > end:  # private columns become shareable
+            node = self.prefix[seq_id] = _Prefix(columns - end, 1, node)
+            return node
+        while end - node.n >= columns:
+            end -= node.n
+            node = node.up
+        if end > columns:
+            node.up = _Prefix(columns - (end - node.n), node.holders, node.up)
+            node.n = end - columns
+            node = node.up
+        return node
+
+    def fork(self, parent_id: int, child_id: int, num_tokens: int, block_size: int) -> tuple[AllocStatus, int]:
+        """The child gets the parent's first tokens: (status, the child's slot); queues the operation on success."""
+        self._alone(parent_id)
+        return self._fork(parent_id, child_id, num_tokens, block_size)
+
+    def _fork(self, parent_id: int, child_id: int, num_tokens: int, block_size: int) -> tuple[AllocStatus, int]:
+        num_tokens = int(num_tokens)
+        if num_tokens < 0:
+            raise ValueError("num_tokens must be >= 0")
+        if parent_id not in self.blocks or child_id in self.blocks:
+            return AllocStatus.FAILURE, -1
+        full, tail = divmod(num_tokens, block_size)
+        if full + (tail > 0) > self.blocks[parent_id]:
+            raise ValueError(f"sequence {parent_id} holds {self.blocks[parent_id]} blocks, fewer than {num_tokens} tokens")
+        if tail and self.free < 1:
+            return AllocStatus.INSUFFICIENT_SPACE, -1
+        if not self.free_slots:
+            raise RuntimeError(f"more than max_seqs={self.max_seqs} sequences hold blocks")
+        slot = self.slot[child_id] = self.free_slots.pop()
+        self.ops.append((POOL_FORK, slot, num_tokens, self.slot[parent_id]))
+        self.blocks[child_id] = full + (tail > 0)
+        self.free -= tail > 0
+        node = self._shared(parent_id, full)
+        if node is not None:
+            self.prefix[child_id] = node
+        while node is not None:
+            node.holders += 1
+            node = node.up
+        return AllocStatus.SUCCESS, slot
+
+    def fork_beams(self, seq_id: int, beam_ids: Sequence[int], num_tokens: int, block_size: int) -> AllocStatus:
+        """``seq_id`` and its new forks ``beam_ids`` become the beams of one search; all or none are made."""
+        self._alone(seq_id)
+        beams = (seq_id, *beam_ids)
+        if len(set(beams)) < len(beams):
+            raise ValueError("beam ids must differ")
+        if seq_id not in self.blocks or any(b in self.blocks for b in beam_ids):
+            return AllocStatus.FAILURE
+        num_tokens = int(num_tokens)
+        if self.blocks[seq_id] != -(-num_tokens // block_size):
+            raise ValueError(f"sequence {seq_id} holds {self.blocks[seq_id]} blocks: beams start with the "
+                             f"{-(-num_tokens // block_size)} that {num_tokens} tokens fill")
+        if len(self.free_slots) < len(beam_ids):
+            raise RuntimeError(f"more than max_seqs={self.max_seqs} sequences hold blocks")
+        if self.free < (len(beam_ids) if num_tokens % block_size else 0):
+            return AllocStatus.INSUFFICIENT_SPACE
+        for b in beam_ids:
+            self._fork(seq_id, b, num_tokens, block_size)
+        self.beams[seq_id] = beams
+        self.member.update((b, seq_id) for b in beams)
+        return AllocStatus.SUCCESS
+
+    def dissolve_beams(self, seq_id: int) -> None:
+        """Undo fork_beams before any reordering: the forks are released, ``seq_id`` keeps its blocks."""
+        beams = self.beams.pop(seq_id)
+        for b in beams:
+            del self.member[b]
+        for b in beams[1:]:
+            self._release(b)
+
+    def allocate_beams(self, seq_id: int, num_blocks: int) -> AllocStatus:
+        beams = self.beams[seq_id]
+        if self.free < num_blocks * len(beams):
+            return AllocStatus.INSUFFICIENT_SPACE
+        for b in beams:
+            self._allocate(b, num_blocks)
+        return AllocStatus.SUCCESS
+
+    def release_beams(self, seq_id: int) -> AllocStatus:
+        # Reordering keeps each column's blocks within those that the beams
+        # held before, so the device never uses more than is counted here, and
+        # the counts agree again when all beams are gone.
+        if seq_id not in self.beams:
+            return AllocStatus.FAILURE
+        for b in self.beams.pop(seq_id):
+            del self.member[b]
+            self._release(b)
+        return AllocStatus.SUCCESS
+
+    def take_ops(self) -> list[tuple[int, ...]]:
         ops, self.ops = self.ops, []
         return ops
 
@@ -134,15 +274,21 @@ class DeviceBlockManager:
         self.free_top = torch.empty(1, **i32)
         self.table = torch.empty(max(1, self.max_seqs), max(1, self.max_blocks_per_seq), **i32)
         self.count = torch.empty(max(1, self.max_seqs), **i32)
+        self.ref_count = torch.empty(max(1, self.num_blocks), **i32)
+        self.scratch = torch.empty(ops.pool_scratch_words(max(1, self.num_blocks)), **i32)
         self.status = torch.zeros(1, **i32)
         self._desc = PaBlockPool(self.free_stack.data_ptr(), self.free_top.data_ptr(), self.table.data_ptr(),
                                  self.count.data_ptr(), self.table.stride(0), self.num_blocks, self.max_seqs,
                                  self.max_blocks_per_seq, 0)
+        self._share = _lib.PaBlockShare(self.ref_count.data_ptr(), self.scratch.data_ptr(), self.scratch.numel())
         self.ledger = BlockLedger(self.num_blocks, self.max_seqs, self.max_blocks_per_seq)
+        self.caches: Optional[tuple] = None  # (K, V, K scales, V scales) of every layer
+        self._copies: set = set()            # sequences whose queued forks copy a page
         self._results: Optional[torch.Tensor] = None
         lib = _lib.load()
         with torch.cuda.device(self.device):
-            _lib.check("block_pool_init", lib.block_pool_init(ctypes.byref(self._desc), self._stream()))
+            _lib.check("block_pool_init_shared", lib.block_pool_init_shared(
+                ctypes.byref(self._desc), ctypes.byref(self._share), self._stream()))
 
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -156,7 +302,8 @@ class DeviceBlockManager:
         return AllocResult(st, self.table[slot, base:base + int(num_blocks)])
 
     def release_blocks(self, seq_id: int) -> AllocStatus:
-        """core/block_manager.py:47-57: return ``seq_id``'s blocks to the free list."""
+        """core/block_manager.py:47-57: return ``seq_id``'s blocks (that no other sequence holds) to the free list."""
+        self._copies_first()
         return self.ledger.release(seq_id)
 
     def num_free_blocks(self) -> int:
@@ -164,6 +311,114 @@ class DeviceBlockManager:
 
     def can_allocate(self, num_blocks: int) -> bool:
         return self.ledger.free >= num_blocks
+
+    # ---- shared blocks ------------------------------------------------------
+    def attach_caches(self, k_cache: ops.Caches, v_cache: ops.Caches, k_scale: Optional[ops.Caches] = None,
+                      v_scale: Optional[ops.Caches] = None) -> None:
+        """Name the pools whose pages this manager hands out: one layer's tensors or lists of every layer's.
+
+        Forks, beams and compaction move pages in all of them.
+        """
+        descs = ops.layer_descs(k_cache, v_cache, k_scale, v_scale)
+        if descs[0].block_size != self.block_size or descs[0].num_blocks < self.num_blocks:
+            raise ValueError(f"the caches hold {descs[0].num_blocks} blocks of {descs[0].block_size} tokens, "
+                             f"the manager hands out {self.num_blocks} of {self.block_size}")
+        lists = [list(ops._layers(c)) for c in (k_cache, v_cache, k_scale, v_scale)]
+        if lists[0][0].device.type != "cuda" or lists[0][0].device != self.free_top.device:
+            raise ValueError(f"the caches are on {lists[0][0].device}, the pool on {self.free_top.device}")
+        self.caches = tuple(lists)
+
+    @property
+    def state(self) -> ops.PoolState:
+        """The pool's device arrays, for ``ops.reorder_beams`` and ``ops.compact_blocks``."""
+        return ops.PoolState(self.free_stack, self.free_top, self.table[:self.max_seqs, :self.max_blocks_per_seq],
+                             self.count[:self.max_seqs], self.ref_count[:self.num_blocks], self.scratch)
+
+    def _need_caches(self) -> tuple:
+        if self.caches is None:
+            raise ValueError("attach_caches() names the pools whose pages are to be moved")
+        return self.caches
+
+    def _copies_first(self) -> None:
+        """A released block may be handed out again: the copies queued so far read their pages before that."""
+        if self._copies:
+            self.flush()
+
+    def _before_fork(self, parent_id: int, num_tokens: int) -> None:
+        """A fork that copies needs the caches, and its parent's own copy to be made: one launch's copies act at once."""
+        if num_tokens % self.block_size:
+            self._need_caches()
+            if parent_id in self._copies:
+                self.flush()
+
+    def fork(self, parent_id: int, child_id: int, num_tokens: int) -> AllocResult:
+        """Let ``child_id`` start with the first ``num_tokens`` tokens of ``parent_id``, sharing its full blocks.
+
+        A partly filled last block is copied when the queued calls are flushed, so the parent's tokens must be
+        written by work on the same stream before that.
+        """
+        self._before_fork(parent_id, num_tokens)
+        st, slot = self.ledger.fork(parent_id, child_id, num_tokens, self.block_size)
+        if st is not AllocStatus.SUCCESS:
+            return AllocResult(st, None)
+        if num_tokens % self.block_size:
+            self._copies.add(child_id)
+        return AllocResult(st, self.table[slot, :self.ledger.blocks[child_id]])
+
+    def fork_beams(self, seq_id: int, beam_ids: Sequence[int], num_tokens: int) -> AllocStatus:
+        """Make ``seq_id`` and new forks of it, ``beam_ids``, the beams of one search over ``num_tokens`` tokens."""
+        self._before_fork(seq_id, num_tokens)
+        st = self.ledger.fork_beams(seq_id, beam_ids, num_tokens, self.block_size)
+        if st is AllocStatus.SUCCESS and num_tokens % self.block_size:
+            self._copies.update(beam_ids)
+        return st
+
+    def allocate_beams(self, seq_id: int, num_blocks: int) -> AllocStatus:
+        """``num_blocks`` new blocks for every beam of ``seq_id``'s search, or none."""
+        return self.ledger.allocate_beams(seq_id, num_blocks)
+
+    def dissolve_beams(self, seq_id: int) -> None:
+        """Undo ``fork_beams`` before any reordering: the forks are released, ``seq_id`` is a plain sequence again."""
+        self._copies_first()
+        self.ledger.dissolve_beams(seq_id)
+
+    def beam_slots(self, seq_ids: Sequence[int]) -> torch.Tensor:
+        """The rows of the beams as ``fork_beams`` made them, int32 [len(seq_ids), num_beams] on the device."""
+        rows = [[self.ledger.slot[b] for b in self.ledger.beams[s]] for s in seq_ids]
+        return torch.tensor(rows, dtype=torch.int32).to(self.device)
+
+    def reorder_beams(self, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor) -> torch.Tensor:
+        """Beam j of group g continues beam ``parents[g, j]``: returns the beams' rows afterwards (``ops.reorder_beams``).
+
+        Which blocks became free only the device knows; ``num_free_blocks`` counts them when the beams are
+        released.  No host synchronisation: the call can be captured (with no queued calls).
+        """
+        caches = self._need_caches()
+        self.flush()
+        return ops.reorder_beams(self.state, slots, parents, num_tokens, *caches, status=self.status)
+
+    def release_beams(self, seq_id: int) -> AllocStatus:
+        """Return the blocks of all beams of ``seq_id``'s search to the free list."""
+        self._copies_first()
+        return self.ledger.release_beams(seq_id)
+
+    def compact(self, num_blocks: Optional[int] = None) -> torch.Tensor:
+        """Move the blocks in use to the lowest ids; returns their number, int32 [1] on the device.
+
+        With ``num_blocks`` the pool shrinks: ids at or above it are neither in use nor handed out any more, and
+        their memory can be given up (``attach_caches`` with smaller pools).  Raises ValueError when more blocks
+        are in use.
+        """
+        caches = self._need_caches()
+        n = self.num_blocks if num_blocks is None else int(num_blocks)
+        used = self.num_blocks - self.ledger.free
+        if not used <= n <= self.num_blocks:
+            raise ValueError(f"{used} of {self.num_blocks} blocks are in use: the pool cannot have {n}")
+        self.flush()
+        live = ops.compact_blocks(self.state, *caches, num_blocks=n, status=self.status)
+        self.ledger.free -= self.num_blocks - n
+        self.num_blocks = self.ledger.num_blocks = self._desc.num_blocks = n
+        return live
 
     # ---- device side --------------------------------------------------------
     def flush(self, keep_results: bool = False) -> None:
@@ -176,14 +431,20 @@ class DeviceBlockManager:
         if not ops_list:
             return
         n = len(ops_list)
-        host = torch.tensor(ops_list, dtype=torch.int32).pin_memory()
-        ops = host.to(self.device, non_blocking=True)
+        host = torch.tensor([(*o, 0)[:4] for o in ops_list], dtype=torch.int32).pin_memory()
+        dev_ops = host.to(self.device, non_blocking=True)
         res = torch.empty(n, dtype=torch.int32, device=self.device) if keep_results else None
+        copies = torch.empty(3, n, dtype=torch.int32, device=self.device) if self._copies else None
+        src, dst, slots = (None, None, None) if copies is None else copies
         lib = _lib.load()
         with torch.cuda.device(self.device):
-            _lib.check("block_pool_apply", lib.block_pool_apply(ctypes.byref(self._desc), ops.data_ptr(), n,
-                                                                None if res is None else res.data_ptr(),
-                                                                self._stream()))
+            _lib.check("block_pool_apply_shared", lib.block_pool_apply_shared(
+                ctypes.byref(self._desc), ctypes.byref(self._share), dev_ops.data_ptr(), n, self.block_size,
+                ops._ptr(res), ops._ptr(src), ops._ptr(dst), ops._ptr(slots), self._stream()))
+        if copies is not None:
+            k, v, ks, vs = self._need_caches()
+            ops.copy_blocks(k, v, src, dst, ks, vs, num_slots=slots, status=self.status)
+            self._copies.clear()
         self._results = res
 
     @property

@@ -1,0 +1,302 @@
+"""Block sharing on the CPU: the host ledger against the list model, and what the entry points refuse."""
+import ctypes
+import os
+import random
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import ROOT
+from oracle import beam_search as obs
+from oracle.block_sharing import SUCCESS, SharedPool
+
+
+def _apply(model, ops):
+    for kind, slot, n, *parent in ops:
+        st = (model.allocate(slot, n) if kind == 0 else model.release(slot) if kind == 1
+              else model.fork(slot, n, parent[0])[0])
+        assert st == SUCCESS
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_ledger_counts_like_the_list_model(seed):
+    """Random allocations, forks and releases: the ledger's free count and decisions are the model's."""
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    r = random.Random(seed)
+    NB, BS, seqs, cols = 60, 4, 12, 9
+    led, model = BlockLedger(NB, seqs, cols), SharedPool(NB, seqs, cols, BS)
+    nxt = 0
+    for _ in range(400):
+        live = list(led.blocks)
+        what = r.random()
+        if what < 0.4 and len(live) < seqs:
+            led.allocate(nxt, r.randint(0, 4))
+            nxt += 1
+        elif what < 0.55 and live:
+            s = r.choice(live)
+            led.allocate(s, r.randint(0, min(2, cols - led.blocks[s])))
+        elif what < 0.8 and live and len(live) < seqs:
+            s = r.choice(live)
+            st, _ = led.fork(s, nxt, r.randint(0, led.blocks[s] * BS), BS)
+            assert st in (AllocStatus.SUCCESS, AllocStatus.INSUFFICIENT_SPACE)
+            nxt += 1
+        elif live:
+            assert led.release(r.choice(live)) is AllocStatus.SUCCESS
+        _apply(model, led.take_ops())
+        model.check()
+        assert led.free == len(model.stack)
+        assert {led.slot[s]: n for s, n in led.blocks.items()} == {i: len(x) for i, x in enumerate(model.rows) if x is not None}
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_ledger_never_counts_more_free_blocks_than_beams_leave(seed):
+    """Beams whose parents the host does not know: the ledger's free count stays at or below the model's, and meets it again."""
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    r = random.Random(100 + seed)
+    NB, BS, seqs, cols = 90, 4, 14, 12
+    led, model = BlockLedger(NB, seqs, cols), SharedPool(NB, seqs, cols, BS)
+    groups, nxt = {}, 0  # first beam -> [slots, tokens]
+    plain = {}
+
+    def follow():
+        _apply(model, led.take_ops())
+        model.check()
+
+    for _ in range(250):
+        what = r.random()
+        if what < 0.2 and len(led.blocks) < seqs:
+            n = r.randint(1, 12)
+            if led.allocate(nxt, -(-n // BS))[0] is AllocStatus.SUCCESS:
+                plain[nxt] = n
+            nxt += 1
+        elif what < 0.3 and plain and len(led.blocks) < seqs:
+            s = r.choice(list(plain))
+            if led.fork(s, nxt, plain[s], BS)[0] is AllocStatus.SUCCESS:
+                plain[nxt] = plain[s]
+            nxt += 1
+        elif what < 0.4 and plain and len(led.blocks) + 3 <= seqs:
+            s = r.choice(list(plain))
+            ids = [(s, k) for k in (1, 2, 3)]
+            if led.fork_beams(s, ids, plain[s], BS) is AllocStatus.SUCCESS:
+                groups[s] = [[led.slot[b] for b in (s, *ids)], plain.pop(s)]
+                with pytest.raises(ValueError):
+                    led.release(ids[0])
+                with pytest.raises(ValueError):
+                    led.fork(s, "x", 1, BS)
+        elif what < 0.85 and groups:
+            s = r.choice(list(groups))
+            slots, n = groups[s]
+            if n % BS == 0:
+                if -(-(n + 1) // BS) > cols or led.allocate_beams(s, 1) is not AllocStatus.SUCCESS:
+                    continue
+                follow()
+            new, _, freed = model.reorder(slots, [r.randrange(4) for _ in range(4)], n + 1)
+            model.push(freed)
+            groups[s] = [new, n + 1]
+        elif what < 0.92 and groups:
+            s = r.choice(list(groups))
+            del groups[s]
+            assert led.release_beams(s) is AllocStatus.SUCCESS
+        elif plain:
+            s = r.choice(list(plain))
+            del plain[s]
+            led.release(s)
+        follow()
+        assert led.free <= len(model.stack)
+        if not groups:
+            assert led.free == len(model.stack)
+
+
+def test_ledger_refusals():
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    led = BlockLedger(10, 3, 8)
+    led.allocate(0, 3)
+    assert led.fork(5, 1, 4, 4)[0] is AllocStatus.FAILURE  # no such parent
+    assert led.fork(0, 0, 4, 4)[0] is AllocStatus.FAILURE  # the child exists
+    with pytest.raises(ValueError):
+        led.fork(0, 1, 13, 4)                              # more tokens than blocks
+    with pytest.raises(ValueError):
+        led.fork(0, 1, -1, 4)
+    with pytest.raises(ValueError):
+        led.fork_beams(0, [1, 1], 12, 4)
+    with pytest.raises(ValueError):
+        led.fork_beams(0, [1], 8, 4)                       # an unused block
+    with pytest.raises(RuntimeError):
+        led.fork_beams(0, [1, 2, 3], 12, 4)                # three rows in all
+    assert led.release_beams(0) is AllocStatus.FAILURE
+    led.allocate(1, 7)
+    assert led.fork(0, 2, 11, 4)[0] is AllocStatus.INSUFFICIENT_SPACE
+    assert led.fork_beams(0, [2], 11, 4) is AllocStatus.INSUFFICIENT_SPACE
+    assert led.fork_beams(0, [2], 12, 4) is AllocStatus.SUCCESS
+    led.dissolve_beams(0)
+    assert led.blocks == {0: 3, 1: 7} and led.free == 0
+    led.release(0)
+    led.release(1)
+    assert led.free == 10
+
+
+def test_struct_layouts_match_header(tmp_path):
+    from pie_b200 import _lib
+
+    structs = {"pa_block_share_t": _lib.PaBlockShare, "pa_beam_select_t": _lib.PaBeamSelect}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "paged_attn_b200.h"', "int main(void) {"]
+    for cname, py in structs.items():
+        lines.append(f'printf("{cname} sizeof %zu\\n", sizeof({cname}));')
+        lines += [f'printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in py._fields_]
+    lines.append("return 0; }")
+    (tmp_path / "layout.c").write_text("\n".join(lines))
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "layout.c"), "-o", str(exe)], check=True)
+    for ln in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        cname, field, val = ln.split()
+        py = structs[cname]
+        assert int(val) == (ctypes.sizeof(py) if field == "sizeof" else getattr(py, field).offset), ln
+
+
+def _cache(n=1, dtype=0, blocks=8):
+    from pie_b200 import _lib
+
+    c = (_lib.PaKvCache * n)()
+    for kv in c:
+        kv.k = kv.v = 1 << 20
+        kv.dtype = dtype
+        kv.num_blocks, kv.block_size, kv.num_kv_heads, kv.head_dim = blocks, 16, 2, 64
+        kv.k_stride_block = kv.v_stride_block = 16 * 128
+        kv.k_stride_slot = kv.v_stride_slot = 128
+        kv.k_stride_head = kv.v_stride_head = 64
+    return c
+
+
+def test_copy_blocks_validates_without_gpu():
+    from pie_b200 import _lib
+
+    lib, p = _lib.load(), 1 << 21
+    c = _cache(2)
+    assert lib.kv_copy_blocks(c, 2, p, p, None, 0, None, None) == _lib.PA_OK  # nothing to do
+    assert lib.kv_copy_blocks(None, 1, p, p, None, 1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.kv_copy_blocks(c, 0, p, p, None, 1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.kv_copy_blocks(c, 2, p, p, None, -1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.kv_copy_blocks(c, 2, None, p, None, 1, None, None) == _lib.PA_ERR_INVALID
+    for field in ("k_stride_slot", "num_blocks", "num_kv_heads", "dtype"):
+        c = _cache(2)
+        setattr(c[1], field, 16 * getattr(c[1], field) + (1 if field == "dtype" else 0))
+        assert lib.kv_copy_blocks(c, 2, p, p, None, 1, None, None) == _lib.PA_ERR_INVALID, field
+        assert b"layer 1" in lib.paged_attn_error_string()
+    c = _cache(1, dtype=_lib.PA_DTYPE_I8)  # no scales
+    assert lib.kv_copy_blocks(c, 1, p, p, None, 1, None, None) == _lib.PA_ERR_INVALID
+
+
+def test_shared_pool_calls_validate_without_gpu():
+    from pie_b200 import _lib
+    from pie_b200.block_pool import PaBlockPool
+    from pie_b200.ops import pool_scratch_words
+
+    lib, p = _lib.load(), 1 << 21
+    d = PaBlockPool(p, p, p, p, 8, 16, 8, 8, 0)
+    words = lib.block_pool_scratch_words(16)
+    assert words == pool_scratch_words(16)
+    s, B = _lib.PaBlockShare(p, p, words), ctypes.byref
+    assert lib.block_pool_init_shared(B(d), B(_lib.PaBlockShare(None, p, words)), None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_init_shared(B(d), B(_lib.PaBlockShare(p, p, words - 1)), None) == _lib.PA_ERR_WORKSPACE
+    assert lib.block_pool_apply_shared(B(d), B(s), None, 1, 16, None, None, None, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_shared(B(d), B(s), p, 1, 0, None, None, None, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_shared(B(d), B(s), p, 1, 16, None, p, None, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_shared(B(d), B(s), p, 0, 16, None, None, None, None, None) == _lib.PA_OK
+    c = _cache(1, blocks=16)
+
+    def reorder(groups=1, beams=4, out=p + 64, caches=c, slots=p):
+        return lib.block_pool_reorder(B(d), B(s), slots, p, p, groups, beams, out, caches, 1, None, None)
+
+    assert reorder(groups=0) == _lib.PA_OK
+    assert reorder(groups=-1) == _lib.PA_ERR_INVALID
+    assert reorder(beams=0) == reorder(beams=33) == _lib.PA_ERR_UNSUPPORTED
+    assert reorder(out=p) == reorder(out=None) == reorder(slots=None) == _lib.PA_ERR_INVALID
+    assert reorder(caches=_cache(1, blocks=15)) == _lib.PA_ERR_INVALID
+    for after in (-1, 17):
+        assert lib.block_pool_compact(B(d), B(s), after, None, c, 1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_compact(B(d), B(s), 16, None, None, 1, None, None) == _lib.PA_ERR_INVALID
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(dtype=2), -1), (dict(dtype=9), -1), (dict(vocab=0), -1), (dict(num_seqs=-1), -1), (dict(num_beams=0), -2),
+    (dict(num_beams=33), -2), (dict(num_out=0), -2), (dict(num_out=33), -2), (dict(vocab=7), -1), (dict(eos_id=100), -1),
+    (dict(eos_id=-1), -1), (dict(stride_seq=-4), -1), (dict(vocab=2**31 - 1), -2),
+])
+def test_beam_select_validates_without_gpu(change, code):
+    from pie_b200 import _lib
+
+    lib, n = _lib.load(), ctypes.c_size_t(0)
+    args = dict(logits=1 << 20, scores=1 << 20, finished=1 << 20, stride_seq=400, stride_beam=100, dtype=3, num_seqs=2,
+                num_beams=4, vocab=100, eos_id=3, num_out=32)
+    a = _lib.PaBeamSelect(**args)
+    assert lib.beam_select_workspace_size(a, ctypes.byref(n)) == 0 and n.value >= 2 * 4 * (32 * 8 + 8)
+    assert lib.beam_select(a, None, 0, None) == _lib.PA_ERR_INVALID  # no outputs
+    a.out_scores = a.out_tokens = a.out_parents = 1 << 22
+    assert lib.beam_select(a, None, 0, None) == _lib.PA_ERR_WORKSPACE
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert lib.beam_select(a, 1 << 23, 1 << 40, None) == code
+    assert lib.paged_attn_error_string()
+
+
+def test_front_end_refusals_without_gpu():
+    from pie_b200 import ops
+
+    x, s = torch.zeros(2, 3, 50), torch.zeros(2, 3)
+    for bad in (dict(logits=x[0]), dict(logits=x.double()), dict(num_out=0), dict(num_out=151),
+                dict(finished=torch.zeros(2, 3, dtype=torch.bool)), dict(logits=x[..., :0]),
+                dict(finished=torch.zeros(2, 3, dtype=torch.bool), eos_id=50)):
+        a = dict(logits=x, beam_scores=s, num_out=4, finished=None, eos_id=None) | bad
+        with pytest.raises(ValueError):
+            ops.beam_select(a["logits"], a["beam_scores"], a["num_out"], finished=a["finished"], eos_id=a["eos_id"])
+    K = torch.zeros(5, 16, 2, 64, dtype=torch.float16)
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.copy_blocks([], [], i, i)
+    with pytest.raises(ValueError):
+        ops.copy_blocks(K, K, i, i[:2])
+    with pytest.raises(ValueError):
+        ops.copy_blocks(K, K, i, i, num_slots=i[:1])
+    with pytest.raises(ValueError):
+        ops.layer_descs([K, K], [K])
+    with pytest.raises(ValueError):
+        ops.layer_descs(K.to(torch.int8), K.to(torch.int8))
+    with pytest.raises(ValueError):
+        ops.compact_blocks(None, K, K, num_blocks=-1)
+    for name in ("copy_blocks", "reorder_beams", "compact_blocks", "beam_select"):
+        with pytest.raises(Exception):  # no CPU path
+            if name == "beam_select":
+                ops.beam_select(x, s, 4)
+            elif name == "copy_blocks":
+                ops.copy_blocks(K, K, i, i)
+            else:
+                pool = ops.PoolState(*[torch.zeros(5, dtype=torch.int32)] * 2, torch.zeros(4, 5, dtype=torch.int32),
+                                     torch.zeros(4, dtype=torch.int32), torch.zeros(5, dtype=torch.int32),
+                                     torch.zeros(ops.pool_scratch_words(5), dtype=torch.int32))
+                if name == "reorder_beams":
+                    ops.reorder_beams(pool, i[None], i[None], i[:1], K, K)
+                else:
+                    ops.compact_blocks(pool, K, K)
+
+
+def test_meta_kernels_give_the_shapes():
+    from pie_b200 import _torch_ext
+
+    ops = _torch_ext.ops()
+    m = dict(device="meta")
+    x = torch.empty(3, 4, 100, dtype=torch.bfloat16, **m)
+    s, t, p = ops.beam_select(x, torch.empty(3, 4, **m), 7, None, -1)
+    assert s.shape == t.shape == p.shape == (3, 7) and s.dtype == torch.float32 and t.dtype == p.dtype == torch.int32
+
+
+def test_selection_oracle_on_known_values():
+    """Two beams of three tokens, by hand: log-probabilities of [0, ln 2, 0] are ln 1/4, ln 1/2, ln 1/4."""
+    x = np.array([[[0.0, np.log(2.0), 0.0], [0.0, 0.0, -np.inf]]])
+    s, t, p = obs.select(x, np.array([[0.0, np.log(0.5)]]), 5)
+    assert t.tolist() == [[1, 0, 2, 0, 1]] and p.tolist() == [[0, 0, 0, 1, 1]]
+    np.testing.assert_allclose(s, [np.log([0.5, 0.25, 0.25, 0.25, 0.25])])
