@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kApplyThreads) apply_shared_kernel(const PoolP
 // therefore never change, and a child's row changes only against its donor's.
 struct Forks {
   int child[kMaxBeams], donor[kMaxBeams];  // pool rows of the n forks
+  int src[kMaxBeams], dst[kMaxBeams];      // their partly filled blocks
   int n, full, tail;                       // full blocks and tokens of the last one
 };
 
@@ -172,7 +173,10 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
   const bool alone = __match_any_sync(0xffffffffu, slot) == (1u << lane);
   const bool named = __all_sync(0xffffffffu, in_range && alone);
   int bad = named ? 0 : ST_BAD_SEQ_INDEX;
+  const int full = tokens >> log2BS;
+  int last = 0;  // the row's partly filled block
   if (named) {
+    if (on && tokens > 0 && full < p.max_blocks_per_seq) last = p.table[slot * p.table_stride + full];
     const int c = on ? p.count[slot] : 0;
     const int c0 = __shfl_sync(0xffffffffu, c, 0);
     const long long need = tokens < 0 ? -1 : (static_cast<long long>(tokens) + bs - 1) >> log2BS;
@@ -193,13 +197,17 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
   const int donor = __shfl_sync(0xffffffffu, slot, on ? parent : 0);
   const int taken = again ? __fns(spare, 0, nth + 1) : 0;
   const int child = __shfl_sync(0xffffffffu, slot, taken & 31);
+  const int src = __shfl_sync(0xffffffffu, last, on ? parent : 0);
+  const int dst = __shfl_sync(0xffffffffu, last, taken & 31);
   if (again) {
     f.child[nth] = child;
     f.donor[nth] = donor;
+    f.src[nth] = src;
+    f.dst[nth] = dst;
   }
   if (lane == 0) {
     f.n = __popc(forks);
-    f.full = tokens >> log2BS;
+    f.full = full;
     f.tail = tokens & (bs - 1);
   }
   if (write && on) r.slots_out[g * K + lane] = again ? child : donor;
@@ -213,36 +221,31 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
 // no table change touches.  Freed blocks are marked in a bitmap, and the last
 // table CTA pushes them in ascending order, so the stack does not depend on
 // the order in which CTAs run.
-__global__ void __launch_bounds__(kCopyThreads) reorder_kernel(const PoolParams p, const ShareParams s,
+__global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolParams p, const ShareParams s,
                                                                const ReorderParams r, const PageParams g, int log2BS,
-                                                               int chunks) {
+                                                               int chunks, int shares) {
   pdl_enter();
   __shared__ Forks f;
   __shared__ bool ok, last;
   __shared__ int warp_sum[kApplyThreads / 32];
   const int tables = r.groups * chunks;
   if (static_cast<int>(blockIdx.x) >= tables) {
-    int item = blockIdx.x - tables;
-    const int part = item % g.parts;
-    item /= g.parts;
-    const int kv = item & 1;
-    item >>= 1;
-    const int layer = item % g.layers;
-    item /= g.layers;
-    const int nth = item % (r.beams - 1), group = item / (r.beams - 1);
+    const int cta = blockIdx.x - tables, share = cta % shares, fork = cta / shares;
+    const int nth = fork / r.groups, group = fork - nth * r.groups;  // groups' first forks first: few groups have K - 1
     if (threadIdx.x < 32) {
       const bool good = plan_group(p, r, log2BS, group, f, false);
       if (threadIdx.x == 0) ok = good;
     }
     __syncthreads();
     if (!ok || nth >= f.n || f.tail == 0) return;
-    const int src = p.table[f.donor[nth] * p.table_stride + f.full];
-    const int dst = p.table[f.child[nth] * p.table_stride + f.full];
+    const int src = f.src[nth], dst = f.dst[nth];
     if (src < 0 || src >= g.num_blocks || dst < 0 || dst >= g.num_blocks) {
       if (threadIdx.x == 0) set_status(r.status, ST_BAD_BLOCK_ID);
       return;
     }
-    copy_page(g, layer, kv, src, dst, f.tail, part);
+    const int items = g.layers * 2 * g.parts;
+    for (int i = items * share / shares; i < items * (share + 1) / shares; ++i)
+      copy_page<4>(g, i / g.parts >> 1, i / g.parts & 1, src, dst, f.tail, i % g.parts);
     return;
   }
 
@@ -334,12 +337,18 @@ cudaError_t launch_block_pool_apply_shared(const PoolParams& p, const ShareParam
 cudaError_t launch_block_pool_reorder(const PoolParams& p, const ShareParams& s, const ReorderParams& r,
                                       const PageParams& g, cudaStream_t stream, bool first) {
   const int chunks = !first ? 0 : p.max_blocks_per_seq > kColumns ? (p.max_blocks_per_seq + kColumns - 1) / kColumns : 1;
-  const long long ctas = static_cast<long long>(r.groups) * (chunks + (r.beams - 1LL) * g.layers * 2 * g.parts);
+  // A fork's copies are shared by so many CTAs that all forks together, half of
+  // the beams perhaps, fill every SM several times: planning a group costs a CTA
+  // about 1 us, and partly filled blocks differ in size.
+  const long long items = g.layers * 2LL * g.parts, forks = static_cast<long long>(r.groups) * (r.beams - 1);
+  long long shares = forks ? (32LL * device_sm_count() + forks - 1) / forks : 1;
+  shares = shares < items ? shares : items;
+  const long long ctas = static_cast<long long>(r.groups) * chunks + forks * shares;
   if (ctas <= 0) return cudaSuccess;
   int log2BS = 0;
   while ((1 << log2BS) < g.block_size) ++log2BS;
   cudaError_t e = launch_pdl(reorder_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kCopyThreads), 0, stream, p, s, r,
-                             g, log2BS, chunks);
+                             g, log2BS, chunks, static_cast<int>(shares));
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

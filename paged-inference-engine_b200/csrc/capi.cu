@@ -1019,15 +1019,17 @@ static int page_params(const pa_kv_cache_t* caches, int32_t num_layers, int32_t 
   return PA_OK;
 }
 
-// Pieces of a page: 16 KB (four loads a thread), and down to 4 KB (one) where
-// `copies` pages of K or V would leave SMs idle.
-static int page_parts(const pa_kv_cache_t& a, long long copies) {
+// Pieces of a page: `most_bytes` (what a CTA's loads hold in flight), and down to
+// 4 KB (a load a thread) where `copies` pages of K or V would leave SMs idle.
+static int page_parts(const pa_kv_cache_t& a, long long copies, int most_bytes) {
   const long long bytes = static_cast<long long>(a.block_size) * a.num_kv_heads * a.head_dim * elt_size(a.dtype);
-  const long long least = (bytes + 16383) / 16384, most = (bytes + 4095) / 4096;
+  const long long least = (bytes + most_bytes - 1) / most_bytes, most = (bytes + 4095) / 4096;
   long long parts = copies > 0 ? (2LL * pa::device_sm_count() + copies - 1) / copies : least;
   parts = parts < least ? least : parts > most ? most : parts;
   return static_cast<int>(parts);
 }
+// Eight loads a thread over a page that is one run of memory, else four.
+static int whole_page_bytes(const pa::PageParams& g) { return g.side[0].dense && g.side[1].dense ? 32768 : 16384; }
 
 static int check_layers(const pa_kv_cache_t* caches, int32_t num_layers) {
   if (num_layers < 1 || !caches) return fail(PA_ERR_INVALID, "the caches of at least one layer are needed");
@@ -1066,7 +1068,7 @@ int kv_copy_blocks(const pa_kv_cache_t* caches, int32_t num_layers, const int32_
   for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
     pa::PageParams g;
     page_params(caches, num_layers, first, g);
-    g.parts = page_parts(caches[0], 2LL * num_pairs * g.layers);
+    g.parts = page_parts(caches[0], 2LL * num_pairs * g.layers, whole_page_bytes(g));
     cudaError_t e = pa::launch_copy_blocks(g, src, dst, num_slots, num_pairs, status, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "kv_copy_blocks launch");
   }
@@ -1151,7 +1153,7 @@ int block_pool_reorder(const pa_block_pool_t* pool, const pa_block_share_t* shar
   for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
     pa::PageParams g;
     page_params(caches, num_layers, first, g);
-    g.parts = page_parts(caches[0], 2LL * num_groups * (num_beams - 1) * g.layers);
+    g.parts = page_parts(caches[0], 2LL * num_groups * (num_beams - 1) * g.layers, 16384);
     const long long ctas = static_cast<long long>(num_groups) *
                            (p.max_blocks_per_seq / 1024 + 1LL + (num_beams - 1LL) * g.layers * 2 * g.parts);
     if (ctas > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "block_pool_reorder: %lld CTAs in one launch", ctas);
@@ -1177,7 +1179,7 @@ int block_pool_compact(const pa_block_pool_t* pool, const pa_block_share_t* shar
   for (int first = 0; first < num_layers; first += pa::kMaxLayers) {
     pa::PageParams g;
     page_params(caches, num_layers, first, g);
-    g.parts = page_parts(caches[0], 0);
+    g.parts = page_parts(caches[0], 0, whole_page_bytes(g));
     cudaError_t e = pa::launch_block_pool_compact(p, s, num_blocks_after, live, g, status,
                                                   static_cast<cudaStream_t>(stream), first == 0);
     if (e != cudaSuccess) return cuda_fail(e, "block_pool_compact launch");

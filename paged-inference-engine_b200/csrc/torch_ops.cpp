@@ -28,6 +28,7 @@
 // scales as [num_blocks, num_kv_heads] (per block) or
 // [num_blocks, block_size, num_kv_heads] (per token).
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -398,6 +399,11 @@ void check_status(const at::Tensor& ref, const std::optional<at::Tensor>& status
   }
 }
 
+// An uninitialised tensor on the current device's allocator, without a dispatch.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, t, dev, std::nullopt));
+}
+
 // One descriptor per layer; the scale lists are empty but for int8 pools.
 std::vector<pa_kv_cache_t> layer_descs(at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs) {
   TORCH_CHECK_VALUE(!k.empty() && k.size() == v.size(), "pie_b200: as many K as V pools are needed, one at least (got ",
@@ -481,7 +487,7 @@ at::Tensor reorder_beams(const at::Tensor& free_stack, const at::Tensor& free_to
   check_i32(k[0], num_tokens, "num_tokens", slots.size(0));
   check_status(k[0], status);
   const c10::cuda::CUDAGuard guard(k[0].device());
-  at::Tensor out = at::empty(slots.sizes(), slots.options());
+  at::Tensor out = fresh(slots.sizes(), at::kInt, k[0].device());
   void* stream = c10::cuda::getCurrentCUDAStream(k[0].device().index()).stream();
   check_rc(block_pool_reorder(&s.pool, &s.share, static_cast<const int32_t*>(slots.data_ptr()),
                               static_cast<const int32_t*>(parents.data_ptr()),
@@ -502,7 +508,7 @@ at::Tensor compact_blocks(const at::Tensor& free_stack, const at::Tensor& free_t
   TORCH_CHECK_VALUE(num_blocks_after <= s.pool.num_blocks, "pie_b200: num_blocks ", num_blocks_after, " exceeds the pool's ",
                     s.pool.num_blocks);
   const c10::cuda::CUDAGuard guard(k[0].device());
-  at::Tensor live = at::empty({1}, free_top.options());
+  at::Tensor live = fresh({1}, at::kInt, k[0].device());
   void* stream = c10::cuda::getCurrentCUDAStream(k[0].device().index()).stream();
   check_rc(block_pool_compact(&s.pool, &s.share,
                               num_blocks_after < 0 ? s.pool.num_blocks : static_cast<int32_t>(num_blocks_after),
@@ -510,12 +516,6 @@ at::Tensor compact_blocks(const at::Tensor& free_stack, const at::Tensor& free_t
                               opt_ptr<int32_t>(status), stream),
            "block_pool_compact");
   return live;
-}
-
-std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_outputs(const at::Tensor& scores, int64_t num_out) {
-  const auto i32 = scores.options().dtype(at::kInt);
-  const int64_t B = scores.size(0);
-  return {at::empty({B, num_out}, scores.options()), at::empty({B, num_out}, i32), at::empty({B, num_out}, i32)};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_op(const at::Tensor& logits, const at::Tensor& scores,
@@ -553,8 +553,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_op(const at::Tensor& 
   size_t bytes = 0;
   check_rc(beam_select_workspace_size(&a, &bytes), "beam_select");
   // a workspace of this call's own: calls on other streams and captured graphs do not share it
-  at::Tensor ws = at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, logits.options().dtype(at::kByte));
-  auto out = beam_outputs(scores, num_out);
+  at::Tensor ws = fresh({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, at::kByte, logits.device());
+  const int64_t B = logits.size(0);
+  std::tuple<at::Tensor, at::Tensor, at::Tensor> out{fresh({B, num_out}, at::kFloat, logits.device()),
+                                                     fresh({B, num_out}, at::kInt, logits.device()),
+                                                     fresh({B, num_out}, at::kInt, logits.device())};
   a.out_scores = static_cast<float*>(std::get<0>(out).data_ptr());
   a.out_tokens = static_cast<int32_t*>(std::get<1>(out).data_ptr());
   a.out_parents = static_cast<int32_t*>(std::get<2>(out).data_ptr());
@@ -580,7 +583,9 @@ at::Tensor compact_blocks_meta(const at::Tensor&, const at::Tensor& free_top, co
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_meta(const at::Tensor&, const at::Tensor& scores,
                                                                 int64_t num_out, const std::optional<at::Tensor>&,
                                                                 int64_t) {
-  return beam_outputs(scores, num_out);
+  const auto i32 = scores.options().dtype(at::kInt);
+  const int64_t B = scores.size(0);
+  return {at::empty({B, num_out}, scores.options()), at::empty({B, num_out}, i32), at::empty({B, num_out}, i32)};
 }
 
 std::tuple<at::Tensor, at::Tensor> paged_attention_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&,

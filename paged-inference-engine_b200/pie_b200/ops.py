@@ -638,14 +638,17 @@ def copy_blocks(k_cache: Caches, v_cache: Caches, src: torch.Tensor, dst: torch.
     reported in ``status``), as is one with an id outside the pool.
     """
     k, v = _layers(k_cache), _layers(v_cache)
-    if not k:
-        raise ValueError("as many K as V pools are needed, one at least (got none)")
-    dev = k[0].device
     src, dst = _i32(src), _i32(dst)
     if num_slots is not None:
         num_slots = _i32(num_slots)
+    if not k:
+        raise ValueError("as many K as V pools are needed, one at least (got none)")
     if src.dim() != 1 or dst.shape != src.shape or (num_slots is not None and num_slots.shape != src.shape):
         raise ValueError("src, dst and num_slots must be vectors of one length")
+    if BACKEND == "torch" and not _CHECK:  # the op checks the rest
+        _op("copy_blocks")(k, v, _layers(k_scale), _layers(v_scale), src, dst, num_slots, status)
+        return
+    dev = k[0].device
     if status is None and _CHECK:
         status = status_word(dev)
     if BACKEND == "torch":
@@ -691,10 +694,12 @@ def reorder_beams(pool: PoolState, slots: torch.Tensor, parents: torch.Tensor, n
     last block is copied in every layer, blocks that no beam continues are freed; see block_pool_reorder.
     """
     k, v = _layers(k_cache), _layers(v_cache)
+    slots, parents, num_tokens = _i32(slots), _i32(parents), _i32(num_tokens)
     if not k:
         raise ValueError("as many K as V pools are needed, one at least (got none)")
+    if BACKEND == "torch" and not _CHECK:  # the op checks the rest
+        return _op("reorder_beams")(*pool, slots, parents, num_tokens, k, v, _layers(k_scale), _layers(v_scale), status)
     dev = k[0].device
-    slots, parents, num_tokens = _i32(slots), _i32(parents), _i32(num_tokens)
     if status is None and _CHECK:
         status = status_word(dev)
     if BACKEND == "torch":
