@@ -46,6 +46,7 @@ constexpr int kSpans = 8;              // a thread's units are remembered in so 
 constexpr int kHits = kRowWarps * kMaxBeamOut;  // logits at T that a split may have; with more its warps keep sorted lists
 constexpr int kMergeThreads = 512;
 constexpr int kMergeWarps = kMergeThreads / 32;
+constexpr int kNoGroup = static_cast<int>(0x80000000u);  // below every float in this order
 constexpr int kMergeKeys = 8192;        // candidates that the merge holds in shared memory (20 bytes each)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -115,18 +116,11 @@ struct RowShared {
   int count;                                  // of hit
 };
 
-// The n-th largest of groups' maxima: a group for each lane, of all warps, for
-// n <= 16, else two, of the even and the odd warps (the n-th of n groups would
-// be their smallest, and four times n logits reach it).  By lane, so that a part
-// which leaves warps without logits still has every group.  `top`: the largest.
-__device__ __forceinline__ float nth_peak(const float (*peak)[32], int n, float& top) {
+// The n-th largest of 64 groups' values, two (a, b) in each lane; for n <= 16 of
+// the 32 lanes' larger ones, which is enough (the n-th of n groups would be
+// their smallest, and four times n values reach it).  `top`: the largest.
+__device__ __forceinline__ float nth_group(float a, float b, int n, float& top) {
   const int lane = threadIdx.x & 31;
-  float a = peak[0][lane], b = peak[1][lane];
-#pragma unroll
-  for (int w = 2; w < kRowWarps; w += 2) {
-    a = fmaxf(a, peak[w][lane]);
-    b = fmaxf(b, peak[w + 1][lane]);
-  }
   float v;
   if (n <= 16) {
     v = sort_lanes(fmaxf(a, b));
@@ -337,8 +331,14 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) beam_rows_kernel(const 
   sh.peak[warp][lane] = m;
   __syncthreads();
   if (warp == 0) {
-    float top;
-    const float limit = nth_peak(sh.peak, n, top);
+    // a group for each lane, of the even and of the odd warps: a part that leaves warps without logits has every group
+    float a = sh.peak[0][lane], b = sh.peak[1][lane], top;
+#pragma unroll
+    for (int w = 2; w < kRowWarps; w += 2) {
+      a = fmaxf(a, sh.peak[w][lane]);
+      b = fmaxf(b, sh.peak[w + 1][lane]);
+    }
+    const float limit = nth_group(a, b, n, top);
     if (lane == 0) {
       sh.top = fminf(top, FLT_MAX);
       sh.limit = limit;
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) beam_rows_kernel(const 
 // One CTA per sequence: the n best of its beams' parts.  Scores are compared in
 // 64 bits: candidates of different beams lie as near as their logits' rounding,
 // and -50 + x - lse in 32 bits would swap them.  Only candidates that may be
-// among the n best get there: as in the rows, T is the n-th largest of 32 groups'
+// among the n best get there: as in the rows, T is the n-th largest of groups'
 // maxima, here of scores in fp32 and less their rounding.  A part's list is
 // sorted, so the groups mix ranks and lists.
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamParams p) {
@@ -442,15 +442,28 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
   int* which = reinterpret_cast<int*>(score + total);
   __shared__ double top[kMaxBeams], logsum[kMaxBeams];  // apart: beside a maximum of 1e30 the logarithm would vanish
   __shared__ float ftop[kMaxBeams], offset[kMaxBeams];
-  __shared__ int group[32], count;
+  __shared__ int group[64], count;
   __shared__ float limit_of_all;
   const int row0 = b * K;
-  if (tid < 32) group[tid] = static_cast<int>(0x80000000u);
+  if (tid < 64) group[tid] = kNoGroup;
   if (tid == 0) count = 0;
   pdl_enter();
   // rows and lists of candidate i, by multiplication (total < 2^14: exact)
   const unsigned per_inv = (1u << 28) / per + 1, n_inv = (1u << 28) / n + 1;
   auto over = [](int i, unsigned inv) { return static_cast<int>((static_cast<unsigned long long>(i) * inv) >> 28); };
+  auto load_key = [&](int i) -> unsigned long long {
+    const int k = over(i, per_inv), r = i - k * per;
+    if (!(p.finished && p.finished[row0 + k])) return p.part_key[static_cast<long long>(row0) * per + i];
+    if (r >= n || r >= p.vocab) return 0;
+    return make_key(r == 0 ? 0.f : -INFINITY, r == 0 ? p.eos : r - 1 + (r - 1 >= p.eos));  // eos, then the others at -inf
+  };
+  constexpr int kFirst = 4;  // keys on their way while the sums are joined
+  unsigned long long first[kFirst];
+#pragma unroll
+  for (int q = 0; q < kFirst; ++q) {
+    const int i = tid + q * kMergeThreads;
+    first[q] = i < total ? load_key(i) : 0;
+  }
   for (int k = warp; k < K; k += kMergeWarps) {
     const bool fin = p.finished && p.finished[row0 + k];
     const int parts = fin ? 0 : S, at = (row0 + k) * S;
@@ -479,17 +492,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
       offset[k] = static_cast<float>(base - log_sum);
     }
   }
-  for (int i = tid; i < total; i += kMergeThreads) {
-    const int k = over(i, per_inv), r = i - k * per;
-    unsigned long long key;
-    if (p.finished && p.finished[row0 + k]) {  // eos, then the other tokens at -inf
-      key = 0;
-      if (r < n && r < p.vocab) key = make_key(r == 0 ? 0.f : -INFINITY, r == 0 ? p.eos : r - 1 + (r - 1 >= p.eos));
-    } else {
-      key = p.part_key[static_cast<long long>(row0) * per + i];
-    }
-    keys[i] = key;
+#pragma unroll
+  for (int q = 0; q < kFirst; ++q) {
+    const int i = tid + q * kMergeThreads;
+    if (i < total) keys[i] = first[q];
   }
+  for (int i = tid + kFirst * kMergeThreads; i < total; i += kMergeThreads) keys[i] = load_key(i);
   __syncthreads();
   auto rough = [&](int i, int k) {
     const float v = (key_logit(keys[i]) - ftop[k]) + offset[k];
@@ -499,13 +507,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
     if (!keys[i]) continue;
     const int list = over(i, n_inv), r = i - list * n;
     const int f = __float_as_int(rough(i, over(i, per_inv)) + 0.f);
-    atomicMax(&group[(r + 11 * list) & 31], f >= 0 ? f : f ^ 0x7fffffff);  // floats in their order
+    atomicMax(&group[(r + 11 * list) & 63], f >= 0 ? f : f ^ 0x7fffffff);  // floats in their order
   }
   __syncthreads();
   if (warp == 0) {
-    const int g = group[lane];
-    const float v = sort_lanes(g == static_cast<int>(0x80000000u) ? -INFINITY : __int_as_float(g >= 0 ? g : g ^ 0x7fffffff));
-    if (lane == n - 1) limit_of_all = v;
+    auto value = [](int g) { return g == kNoGroup ? -INFINITY : __int_as_float(g >= 0 ? g : g ^ 0x7fffffff); };
+    float largest;
+    const float v = nth_group(value(group[lane]), value(group[32 + lane]), n, largest);
+    if (lane == 0) limit_of_all = v;
   }
   __syncthreads();
   const float limit = limit_of_all;
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
       const float v = rough(i, k);
       // x - top and the sum with the offset are rounded twice, the limit's too
       const float slack = 4.f * 1.2e-7f * (fabsf(limit) + fabsf(v) + fabsf(offset[k]));
-      hit = !(v < limit) || !(limit - v > slack);
+      hit = v >= limit || (v > -INFINITY && !(limit - v > slack));
     }
     if (!hit) continue;
     const int at = atomicAdd(&count, 1);
