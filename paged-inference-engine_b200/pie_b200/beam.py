@@ -21,11 +21,13 @@ import torch
 from . import ops
 from .block_pool import AllocStatus, DeviceBlockManager
 
+MAX_BEAMS = 32  # of ops.beam_select and ops.reorder_beams
+
 
 class BeamSearch:
     """``num_beams`` beams of each of ``seq_ids``, which hold ``num_tokens[i]`` prompt tokens in the cache.
 
-    ``logits`` [B, V] are those of each prompt's last token.  The beams' pool ids are ``beam_ids(i, k)``; the
+    ``logits`` [B, V] are those of each prompt's last token.  The beams' pool ids are ``beam_id(seq_id, k)``; the
     sequences must hold exactly the blocks that their tokens fill.  A beam that emits ``eos_id`` is finished: it keeps
     its score and competes with the others until ``finish``.
     """
@@ -35,14 +37,28 @@ class BeamSearch:
         B, K = len(seq_ids), int(num_beams)
         if logits.dim() != 2 or logits.shape[0] != B or len(num_tokens) != B:
             raise ValueError(f"logits must be [{B}, vocab] and num_tokens hold {B} lengths")
-        if not 1 <= K <= logits.shape[1]:
-            raise ValueError(f"num_beams {K} is outside 1..vocab ({logits.shape[1]})")
+        V = logits.shape[1]
+        if not 1 <= K <= min(V, MAX_BEAMS):
+            raise ValueError(f"num_beams {K} is outside 1..min(vocab, {MAX_BEAMS})")
+        if not 0 <= eos_id < V:
+            raise ValueError(f"eos_id {eos_id} is outside the vocabulary of {V}")
         if max_new_tokens < 1 or B < 1:
             raise ValueError("at least one sequence and one new token are needed")
         self.pool, self.B, self.K, self.eos = pool, B, K, int(eos_id)
         self.seq_ids = [int(s) for s in seq_ids]
         self.host_tokens = [int(n) for n in num_tokens]
         dev = pool.free_top.device
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.num_tokens = torch.tensor(self.host_tokens, dtype=torch.int32).to(dev)
+        self.max_new = int(max_new_tokens)
+        self.history = torch.empty(2, self.max_new, B, K, **i32)  # tokens and parents of every step
+        self.q_len = torch.ones(B * K, **i32)
+        self.cu = torch.arange(B * K + 1, **i32)
+        self.scores = torch.zeros(B, 1, device=dev)
+        self.finished = torch.zeros(B, 1, dtype=torch.bool, device=dev)
+        self.steps = 0
+        self._room = self._ended = False
+        self._choose(logits.unsqueeze(1))  # before the forks: a refused call leaves the pool as it was
         made = []
         try:
             for s, n in zip(self.seq_ids, self.host_tokens):
@@ -55,18 +71,7 @@ class BeamSearch:
                 pool.dissolve_beams(s)
             raise
         pool.flush()
-        i32 = dict(dtype=torch.int32, device=dev)
         self.slots = pool.beam_slots(self.seq_ids)
-        self.num_tokens = torch.tensor(self.host_tokens, dtype=torch.int32).to(dev)
-        self.max_new = int(max_new_tokens)
-        self.history = torch.empty(2, self.max_new, B, K, **i32)  # tokens and parents of every step
-        self.q_len = torch.ones(B * K, **i32)
-        self.cu = torch.arange(B * K + 1, **i32)
-        self.scores = torch.zeros(B, 1, device=dev)
-        self.finished = torch.zeros(B, 1, dtype=torch.bool, device=dev)
-        self.steps = 0
-        self._room = False
-        self._choose(logits.unsqueeze(1))
 
     @staticmethod
     def beam_id(seq_id: int, k: int) -> object:
@@ -91,13 +96,15 @@ class BeamSearch:
 
         The new token of a beam of sequence b goes to position ``num_tokens[b]`` and attends to one more key.
         """
-        if self.steps >= self.max_new:
-            raise RuntimeError(f"the search was made for {self.max_new} new tokens")
+        if self._ended or self.steps >= self.max_new:
+            raise RuntimeError(f"the search has ended or was made for {self.max_new} new tokens")
         pool, S = self.pool, self.B * self.K
         if not self._room:
-            need = [s for s, n in zip(self.seq_ids, self.host_tokens) if n % pool.block_size == 0]
+            need = [s for s, n in zip(self.seq_ids, self.host_tokens) if pool.blocks_of(s) * pool.block_size <= n]
             if pool.num_free_blocks() < len(need) * self.K:
                 raise RuntimeError(f"{len(need) * self.K} blocks are needed, {pool.num_free_blocks()} are free")
+            if any(pool.blocks_of(s) >= pool.max_blocks_per_seq for s in need):
+                raise RuntimeError(f"a beam would hold more than max_blocks_per_seq={pool.max_blocks_per_seq} blocks")
             for s in need:
                 pool.allocate_beams(s, 1)
             self._room = True
@@ -132,9 +139,11 @@ class BeamSearch:
         """End the search and free its blocks: each sequence's (score, new tokens), best first, without what follows eos."""
         tokens, parents = self.history[:, :self.steps].cpu().tolist()
         scores = self.scores.cpu().tolist()
-        for s in self.seq_ids:
-            self.pool.release_beams(s)
-        self.pool.flush()
+        if not self._ended:
+            for s in self.seq_ids:
+                self.pool.release_beams(s)
+            self.pool.flush()
+            self._ended = True
         found = []
         for b in range(self.B):
             beams = []

@@ -411,7 +411,8 @@ def test_beam_search_that_cannot_start_leaves_the_prompts():
     x = torch.zeros(2, 30, device="cuda")
     with pytest.raises(RuntimeError, match="INSUFFICIENT"):
         BeamSearch(dm, [0, 1], [7, 7], x, 4, 0, 5)  # three forks each, four free blocks
-    for bad in (dict(logits=x[:1]), dict(num_beams=0), dict(num_beams=31), dict(max_new_tokens=0)):
+    for bad in (dict(logits=x[:1]), dict(num_beams=0), dict(num_beams=31), dict(max_new_tokens=0), dict(eos_id=30),
+                dict(eos_id=-1), dict(logits=x.double()), dict(num_tokens=[7, 3]), dict(seq_ids=[1, 1])):
         with pytest.raises(ValueError):
             BeamSearch(**(dict(pool=dm, seq_ids=[0, 1], num_tokens=[7, 7], logits=x, num_beams=2, eos_id=0, max_new_tokens=5) | bad))
     dm.flush()
@@ -423,3 +424,36 @@ def test_beam_search_that_cannot_start_leaves_the_prompts():
     search.step_inputs()
     with pytest.raises(ValueError):
         search.advance(x[:1])
+    search.advance(x[:1].expand(1, 3, 30))
+    search.step_inputs()
+    search.step_inputs()  # again: nothing more is taken
+    assert dm.num_free_blocks() == 1  # one shared block, and two for each beam
+    search.finish()
+    search.finish()
+    with pytest.raises(RuntimeError, match="ended"):
+        search.step_inputs()
+    assert dm.num_free_blocks() == 8 == dm.free_top.item()
+
+
+def test_beam_search_at_the_ends_of_the_pool():
+    """A row without room, and a pool without blocks: step_inputs refuses, takes nothing, and goes on when there is room."""
+    from pie_b200.beam import BeamSearch
+
+    x = torch.randn(1, 30, device="cuda")
+    dm = manager(NB=8, seqs=12, cols=2)
+    dm.allocate(0, 2)
+    search = BeamSearch(dm, [0], [8], x, 2, 0, 9)
+    with pytest.raises(RuntimeError, match="max_blocks_per_seq"):
+        search.step_inputs()
+    assert dm.num_free_blocks() == 6
+    dm = manager(NB=6, seqs=12, cols=5)
+    dm.allocate("other", 3)
+    dm.allocate(0, 2)
+    search = BeamSearch(dm, [0], [8], x, 2, 0, 9)
+    with pytest.raises(RuntimeError, match="free"):
+        search.step_inputs()
+    dm.release_blocks("other")
+    inp = search.step_inputs()
+    assert inp["num_blocks_per_seq"].tolist() == [3, 3] and dm.num_free_blocks() == 2
+    search.finish()
+    assert dm.num_free_blocks() == 6 == dm.free_top.item()
