@@ -338,10 +338,11 @@ cudaError_t launch_block_pool_reorder(const PoolParams& p, const ShareParams& s,
                                       const PageParams& g, cudaStream_t stream, bool first) {
   const int chunks = !first ? 0 : p.max_blocks_per_seq > kColumns ? (p.max_blocks_per_seq + kColumns - 1) / kColumns : 1;
   // A fork's copies are shared by so many CTAs that all forks together, half of
-  // the beams perhaps, fill every SM several times: planning a group costs a CTA
-  // about 1 us, and partly filled blocks differ in size.
+  // the beams perhaps, fill every SM twice: planning a group costs a CTA more than
+  // 1 us, and partly filled blocks differ in size (64 groups of 8 beams, 4 layers
+  // of 64 KB pages: 34.8 us with 32 CTAs an SM, 30.8 with 16, 33 with 4 to 10).
   const long long items = g.layers * 2LL * g.parts, forks = static_cast<long long>(r.groups) * (r.beams - 1);
-  long long shares = forks ? (32LL * device_sm_count() + forks - 1) / forks : 1;
+  long long shares = forks ? (16LL * device_sm_count() + forks - 1) / forks : 1;
   shares = shares < items ? shares : items;
   const long long ctas = static_cast<long long>(r.groups) * chunks + forks * shares;
   if (ctas <= 0) return cudaSuccess;
