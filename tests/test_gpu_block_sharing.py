@@ -457,3 +457,60 @@ def test_beam_search_at_the_ends_of_the_pool():
     assert inp["num_blocks_per_seq"].tolist() == [3, 3] and dm.num_free_blocks() == 2
     search.finish()
     assert dm.num_free_blocks() == 6 == dm.free_top.item()
+
+
+def test_decode_graph_over_forked_sequences():
+    """The captured decode step over a sequence and its forks: each attends to its own continuation of the shared prompt."""
+    from pie_b200 import ops as o
+    from pie_b200.block_pool import DeviceBlockManager
+    from pie_b200.decode_step import DecodeStepGraph
+
+    BS, Hkv, D, Hq, NB, n = 16, 2, 64, 4, 40, 21
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k, v = (torch.zeros(NB, BS, Hkv, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    pool = DeviceBlockManager(NB, BS, 8, 6)
+    pool.attach_caches(k, v)
+    graph = DecodeStepGraph(pool, k, v, None, None, Hq, 4)
+    pool.allocate(0, 2)
+    inp = pool.step_inputs([0], [n], [n])
+    rows = [torch.randn(n, Hkv, D, device="cuda", generator=g).half() for _ in range(2)]
+    o.write_kv(*rows, inp["block_table"], inp["token_seq"], inp["positions"], k, v)
+    pool.fork(0, 1, n)
+    pool.fork(0, 2, 18)  # an earlier point
+    pool.fork(1, 3, n)   # a fork of a fresh fork
+    lens, have = [n, n, 18, n], [[r[:m] for r in rows] for m in (n, n, 18, n)]
+    for _ in range(15):
+        lens = [m + 1 for m in lens]
+        q, kn, vn = (torch.randn(4, h, D, device="cuda", generator=g).half() for h in (Hq, Hkv, Hkv))
+        out = graph.step([0, 1, 2, 3], lens, q, kn, vn).clone()
+        for i in range(4):
+            have[i] = [torch.cat([have[i][0], kn[i:i + 1]]), torch.cat([have[i][1], vn[i:i + 1]])]
+            rep = Hq // Hkv
+            kk, vv = (t.double().repeat_interleave(rep, 1) for t in have[i])
+            a = torch.softmax(torch.einsum("hd,thd->ht", q[i].double(), kk) / D**0.5, -1)
+            want = torch.einsum("ht,thd->hd", a, vv)
+            # fp16 probabilities and output: 2^-11 each of values up to 4, and the exponentials' 2^-11 of the logits
+            assert (out[i].double() - want).abs().max() < 8e-3
+    graph.check()
+    assert pool.status.item() == 0
+
+
+def test_checked_mode_raises_what_the_status_says(monkeypatch):
+    """PIE_B200_CHECK: the skipped pairs and groups become IndexErrors."""
+    from pie_b200 import ops as o
+
+    monkeypatch.setattr(o, "_CHECK", True)
+    caches = make_caches(8, 16, 1, 64, torch.float16)
+    o.copy_blocks(caches[0], caches[1], _i32([1]), _i32([2]))
+    with pytest.raises(IndexError, match="another copy"):
+        o.copy_blocks(caches[0], caches[1], _i32([1, 3]), _i32([2, 2]))
+    with pytest.raises(IndexError, match="block id"):
+        o.copy_blocks(caches[0], caches[1], _i32([1]), _i32([8]))
+    m, slots, lens = beam_state(5, 2, 3, 4, 6)
+    pool, caches = pool_arrays(o, m, m.max_blocks), make_caches(m.NB, 4, 1, 64, torch.float16)
+    o.reorder_beams(pool, _i32(slots), _i32([[0, 1, 2]] * 2), _i32(lens), *caches)
+    with pytest.raises(IndexError, match="sequence index"):
+        o.reorder_beams(pool, _i32(slots), _i32([[0, 1, 3]] * 2), _i32(lens), *caches)
+    with pytest.raises(IndexError, match="contradict"):
+        o.compact_blocks(pool, *caches, num_blocks=1)
+    o.compact_blocks(pool, *caches)
