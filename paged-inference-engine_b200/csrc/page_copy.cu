@@ -129,6 +129,9 @@ __device__ __forceinline__ int block_prefix(int mine, int* warp_sum, int* total)
   return before;
 }
 
+// One CTA: planning 8192 blocks takes 8 us of a compaction's 168.  A single launch
+// in which every resident CTA planned for itself (a bitmap of live blocks, moves
+// by rank) took 182 us: its copies have no later CTAs to even out the SMs.
 // Live pages are counted, then the holes below that count and the live pages
 // at or above it are listed in ascending order: page src[i] moves to dst[i].
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PoolParams p, const ShareParams s, int after,

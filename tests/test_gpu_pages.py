@@ -209,7 +209,7 @@ def random_model(seed, NB, BS=16, seqs=20, cols=12, share=True):
     return m
 
 
-@pytest.mark.parametrize("seed,NB", [(0, 40), (1, 100), (2, 5000), (3, 131), (4, 1), (5, 64), (6, 40000)])
+@pytest.mark.parametrize("seed,NB", [(0, 40), (1, 100), (2, 5000), (3, 131), (4, 1), (5, 64), (6, 40000), (7, 65536), (8, 70001)])
 @pytest.mark.parametrize("dtype,layers,layout", [(torch.int8, 2, "slots"), (torch.float16, 1, "heads"), (torch.float32, 66, "slots")])
 def test_compaction(ops, seed, NB, dtype, layers, layout):
     if NB > 1000 and layers > 2:
