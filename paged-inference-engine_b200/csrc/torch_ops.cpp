@@ -424,10 +424,22 @@ std::vector<pa_kv_cache_t> layer_descs(at::TensorList k, at::TensorList v, at::T
   TORCH_CHECK_VALUE(k[0].is_cuda(), "pie_b200: the pools must be CUDA tensors");
   std::vector<pa_kv_cache_t> d;
   d.reserve(k.size());
-  for (size_t i = 0; i < k.size(); ++i) {
-    check_device(k[0], k[i], "K");
-    if (i8) d.push_back(kv_desc(k[i], v[i], ks[i], vs[i]));
-    else d.push_back(kv_desc(k[i], v[i], std::nullopt, std::nullopt));
+  d.push_back(i8 ? kv_desc(k[0], v[0], ks[0], vs[0]) : kv_desc(k[0], v[0], std::nullopt, std::nullopt));
+  // further layers: like layer 0 but for their pointers
+  const auto like = [](const at::Tensor& a, const at::Tensor& b) {
+    return a.scalar_type() == b.scalar_type() && a.device() == b.device() && a.sizes() == b.sizes() &&
+           a.strides() == b.strides();
+  };
+  for (size_t i = 1; i < k.size(); ++i) {
+    TORCH_CHECK_VALUE(like(k[i], k[0]) && like(v[i], v[0]) && (!i8 || (like(ks[i], ks[0]) && like(vs[i], vs[0]))),
+                      "pie_b200: layer ", i, "'s pools or scales differ from layer 0's in type, device, shape or strides");
+    d.push_back(d[0]);
+    d[i].k = ptr(k[i]);
+    d[i].v = ptr(v[i]);
+    if (i8) {
+      d[i].k_scale = ptr(ks[i]);
+      d[i].v_scale = ptr(vs[i]);
+    }
   }
   return d;
 }

@@ -283,6 +283,7 @@ class DeviceBlockManager:
         self._share = _lib.PaBlockShare(self.ref_count.data_ptr(), self.scratch.data_ptr(), self.scratch.numel())
         self.ledger = BlockLedger(self.num_blocks, self.max_seqs, self.max_blocks_per_seq)
         self.caches: Optional[tuple] = None  # (K, V, K scales, V scales) of every layer
+        self._cache_descs = None             # and their descriptors
         self._copies: set = set()            # sequences whose queued forks copy a page
         self._results: Optional[torch.Tensor] = None
         lib = _lib.load()
@@ -326,7 +327,7 @@ class DeviceBlockManager:
         lists = [list(ops._layers(c)) for c in (k_cache, v_cache, k_scale, v_scale)]
         if lists[0][0].device.type != "cuda" or lists[0][0].device != self.free_top.device:
             raise ValueError(f"the caches are on {lists[0][0].device}, the pool on {self.free_top.device}")
-        self.caches = tuple(lists)
+        self.caches, self._cache_descs = tuple(lists), descs
 
     @property
     def state(self) -> ops.PoolState:
@@ -334,10 +335,14 @@ class DeviceBlockManager:
         return ops.PoolState(self.free_stack, self.free_top, self.table[:self.max_seqs, :self.max_blocks_per_seq],
                              self.count[:self.max_seqs], self.ref_count[:self.num_blocks], self.scratch)
 
-    def _need_caches(self) -> tuple:
-        if self.caches is None:
+    def _need_caches(self):
+        if self._cache_descs is None:
             raise ValueError("attach_caches() names the pools whose pages are to be moved")
-        return self.caches
+        return self._cache_descs
+
+    def _checked(self, fn: str) -> None:
+        if ops._CHECK:
+            ops._raise_status(fn, self.status)
 
     def _copies_first(self) -> None:
         """A released block may be handed out again: the copies queued so far read their pages before that."""
@@ -393,9 +398,12 @@ class DeviceBlockManager:
         Which blocks became free only the device knows; ``num_free_blocks`` counts them when the beams are
         released.  No host synchronisation: the call can be captured (with no queued calls).
         """
-        caches = self._need_caches()
+        descs = self._need_caches()
         self.flush()
-        return ops.reorder_beams(self.state, slots, parents, num_tokens, *caches, status=self.status)
+        out = ops._reorder_call(self._desc, self._share, descs, self.free_top.device, ops._i32(slots), ops._i32(parents),
+                                ops._i32(num_tokens), self.status)
+        self._checked("reorder_beams")
+        return out
 
     def release_beams(self, seq_id: int) -> AllocStatus:
         """Return the blocks of all beams of ``seq_id``'s search to the free list."""
@@ -409,13 +417,14 @@ class DeviceBlockManager:
         their memory can be given up (``attach_caches`` with smaller pools).  Raises ValueError when more blocks
         are in use.
         """
-        caches = self._need_caches()
+        descs = self._need_caches()
         n = self.num_blocks if num_blocks is None else int(num_blocks)
         used = self.num_blocks - self.ledger.free
         if not used <= n <= self.num_blocks:
             raise ValueError(f"{used} of {self.num_blocks} blocks are in use: the pool cannot have {n}")
         self.flush()
-        live = ops.compact_blocks(self.state, *caches, num_blocks=n, status=self.status)
+        live = ops._compact_call(self._desc, self._share, descs, self.free_top.device, n, self.status)
+        self._checked("compact")
         self.ledger.free -= self.num_blocks - n
         self.num_blocks = self.ledger.num_blocks = self._desc.num_blocks = n
         return live
@@ -442,9 +451,9 @@ class DeviceBlockManager:
                 ctypes.byref(self._desc), ctypes.byref(self._share), dev_ops.data_ptr(), n, self.block_size,
                 ops._ptr(res), ops._ptr(src), ops._ptr(dst), ops._ptr(slots), self._stream()))
         if copies is not None:
-            k, v, ks, vs = self._need_caches()
-            ops.copy_blocks(k, v, src, dst, ks, vs, num_slots=slots, status=self.status)
+            ops._copy_call(self._need_caches(), self.free_top.device, src, dst, slots, self.status)
             self._copies.clear()
+            self._checked("fork")
         self._results = res
 
     @property

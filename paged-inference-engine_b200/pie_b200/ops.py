@@ -628,6 +628,14 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _copy_call(descs, dev: torch.device, src: torch.Tensor, dst: torch.Tensor, num_slots: Optional[torch.Tensor],
+               status: Optional[torch.Tensor]) -> None:
+    _check_vectors(dev, src=src, dst=dst, num_slots=num_slots, status=status)
+    with torch.cuda.device(dev):
+        _lib.check("kv_copy_blocks", _lib.load().kv_copy_blocks(
+            descs, len(descs), src.data_ptr(), dst.data_ptr(), _ptr(num_slots), src.numel(), _ptr(status), _stream(dev)))
+
+
 def copy_blocks(k_cache: Caches, v_cache: Caches, src: torch.Tensor, dst: torch.Tensor,
                 k_scale: Optional[Caches] = None, v_scale: Optional[Caches] = None, *,
                 num_slots: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
@@ -654,12 +662,7 @@ def copy_blocks(k_cache: Caches, v_cache: Caches, src: torch.Tensor, dst: torch.
     if BACKEND == "torch":
         _op("copy_blocks")(k, v, _layers(k_scale), _layers(v_scale), src, dst, num_slots, status)
     else:
-        descs = layer_descs(k, v, k_scale, v_scale)
-        _check_vectors(dev, src=src, dst=dst, num_slots=num_slots, status=status)
-        with torch.cuda.device(dev):
-            _lib.check("kv_copy_blocks", _lib.load().kv_copy_blocks(
-                descs, len(descs), src.data_ptr(), dst.data_ptr(), _ptr(num_slots), src.numel(), _ptr(status),
-                _stream(dev)))
+        _copy_call(layer_descs(k_cache, v_cache, k_scale, v_scale), dev, src, dst, num_slots, status)
     if _CHECK and status is not None:
         _raise_status("copy_blocks", status)
 
@@ -684,6 +687,19 @@ def pool_descs(pool: PoolState):
             _lib.PaBlockShare(pool.ref_count.data_ptr(), pool.scratch.data_ptr(), pool.scratch.numel()))
 
 
+def _reorder_call(desc, share, descs, dev: torch.device, slots: torch.Tensor, parents: torch.Tensor,
+                  num_tokens: torch.Tensor, status: Optional[torch.Tensor]) -> torch.Tensor:
+    if slots.dim() != 2 or parents.shape != slots.shape or num_tokens.shape != slots.shape[:1]:
+        raise ValueError("slots and parents must be [num_groups, num_beams], num_tokens [num_groups]")
+    _check_vectors(dev, slots=slots, parents=parents, num_tokens=num_tokens, status=status)
+    out = torch.empty_like(slots)
+    with torch.cuda.device(dev):
+        _lib.check("block_pool_reorder", _lib.load().block_pool_reorder(
+            ctypes.byref(desc), ctypes.byref(share), slots.data_ptr(), parents.data_ptr(), num_tokens.data_ptr(),
+            slots.shape[0], slots.shape[1], out.data_ptr(), descs, len(descs), _ptr(status), _stream(dev)))
+    return out
+
+
 def reorder_beams(pool: PoolState, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor,
                   k_cache: Caches, v_cache: Caches, k_scale: Optional[Caches] = None,
                   v_scale: Optional[Caches] = None, *, status: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -705,19 +721,22 @@ def reorder_beams(pool: PoolState, slots: torch.Tensor, parents: torch.Tensor, n
     if BACKEND == "torch":
         out = _op("reorder_beams")(*pool, slots, parents, num_tokens, k, v, _layers(k_scale), _layers(v_scale), status)
     else:
-        descs = layer_descs(k, v, k_scale, v_scale)
-        desc, share = pool_descs(pool)
-        if slots.dim() != 2 or parents.shape != slots.shape or num_tokens.shape != slots.shape[:1]:
-            raise ValueError("slots and parents must be [num_groups, num_beams], num_tokens [num_groups]")
-        _check_vectors(dev, slots=slots, parents=parents, num_tokens=num_tokens, status=status, ref_count=pool.ref_count)
-        out = torch.empty_like(slots)
-        with torch.cuda.device(dev):
-            _lib.check("block_pool_reorder", _lib.load().block_pool_reorder(
-                ctypes.byref(desc), ctypes.byref(share), slots.data_ptr(), parents.data_ptr(), num_tokens.data_ptr(),
-                slots.shape[0], slots.shape[1], out.data_ptr(), descs, len(descs), _ptr(status), _stream(dev)))
+        _check_vectors(dev, ref_count=pool.ref_count)
+        out = _reorder_call(*pool_descs(pool), layer_descs(k_cache, v_cache, k_scale, v_scale), dev, slots, parents,
+                            num_tokens, status)
     if _CHECK and status is not None:
         _raise_status("reorder_beams", status)
     return out
+
+
+def _compact_call(desc, share, descs, dev: torch.device, num_blocks: int, status: Optional[torch.Tensor]) -> torch.Tensor:
+    _check_vectors(dev, status=status)
+    live = torch.empty(1, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check("block_pool_compact", _lib.load().block_pool_compact(
+            ctypes.byref(desc), ctypes.byref(share), num_blocks, live.data_ptr(), descs, len(descs), _ptr(status),
+            _stream(dev)))
+    return live
 
 
 def compact_blocks(pool: PoolState, k_cache: Caches, v_cache: Caches, k_scale: Optional[Caches] = None,
@@ -740,14 +759,10 @@ def compact_blocks(pool: PoolState, k_cache: Caches, v_cache: Caches, k_scale: O
         live = _op("compact_blocks")(*pool, -1 if num_blocks is None else num_blocks, k, v, _layers(k_scale),
                                      _layers(v_scale), status)
     else:
-        descs = layer_descs(k, v, k_scale, v_scale)
+        _check_vectors(dev, ref_count=pool.ref_count)
         desc, share = pool_descs(pool)
-        _check_vectors(dev, status=status, ref_count=pool.ref_count)
-        live = torch.empty(1, dtype=torch.int32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check("block_pool_compact", _lib.load().block_pool_compact(
-                ctypes.byref(desc), ctypes.byref(share), desc.num_blocks if num_blocks is None else num_blocks,
-                live.data_ptr(), descs, len(descs), _ptr(status), _stream(dev)))
+        live = _compact_call(desc, share, layer_descs(k_cache, v_cache, k_scale, v_scale), dev,
+                             desc.num_blocks if num_blocks is None else num_blocks, status)
     if _CHECK and status is not None:
         _raise_status("compact_blocks", status)
     return live
