@@ -7,7 +7,9 @@
 // (core/block_manager.py:19-68: every id belongs to one sequence).
 //
 // Integer work on a few kilobytes; the page copies of a reorder are the only
-// large traffic (both bytes of each copied token, once).
+// large traffic (both bytes of each copied token, once).  64 groups of 8 beams
+// with 4 forks each, 4 layers of 64 KB pages: 26 us for 130 MB (20 us of HBM);
+// one group: 7.5 us, a chain of dependent accesses.
 #include "page_copy.cuh"
 
 namespace pa {

@@ -1,7 +1,8 @@
 """Loader of _pie_b200_torch.so: the torch.library ops over the C ABI (csrc/torch_ops.cpp).
 
 Registers ``torch.ops.pie_b200.{paged_attention, paged_attention_out,
-paged_attention_varlen, paged_attention_varlen_out, write_kv}``.  Built in-tree
+paged_attention_varlen, paged_attention_varlen_out, write_kv, project_write_kv,
+copy_blocks, reorder_beams, compact_blocks, beam_select}``.  Built in-tree
 by ``paged-inference-engine_b200/build.py``; a missing build raises (there is no
 fallback).
 """
