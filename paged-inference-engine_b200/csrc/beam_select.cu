@@ -208,7 +208,7 @@ __device__ __forceinline__ float take_runs(const uint4 (&u)[N], float& m, float&
     b = word_max<DT>(word_max<DT>(b, u[i].z), u[i].w);
   }
   const float2 f = word_logits<DT>(word_max<DT>(a, b));
-  const float top = fminf(fmaxf(f.x, f.y), FLT_MAX);
+  const float top = clean(fmaxf(f.x, f.y));  // of NaN alone too
   if (top > m) {
     s *= ex2((m - top) * kLog2e);
     m = top;

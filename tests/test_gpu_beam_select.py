@@ -123,6 +123,21 @@ def test_masked_and_extreme_logits(ops, dtype):
     _check(ops.beam_select(x, s, n), x, s, n)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_runs_of_nan(ops, dtype):
+    """Stretches of NaN that fill whole threads, warps and parts beside ordinary logits."""
+    V = 40013
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = (torch.randn(4, 2, V, device="cuda", generator=g) * 2).to(dtype)
+    s = -torch.rand(4, 2, device="cuda", generator=g)
+    x[0, :, 100:9000] = float("nan")
+    x[1, :, 8:] = float("nan")
+    x[2, 0, :-3] = float("nan")
+    x[2, 1, 20000:] = float("nan")
+    x[3].view(2, -1)[:, 1024:2048] = float("nan")
+    _check(ops.beam_select(x, s, 9), x, s, 9)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_finished_beams(ops, dtype):
     B, K, V, n, eos = 6, 4, 10007, 8, 17
