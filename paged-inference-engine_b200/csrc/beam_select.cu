@@ -15,19 +15,19 @@
 // Bound: every logit is read once, so the floor is rows * vocab * size bytes
 // of HBM; next comes the one exponential per logit (16 a clock and SM: 0.77 of
 // the HBM time for 16-bit logits).  Two launches: `beam_rows_kernel` streams a
-// split of a row through registers, each thread with its own running maximum
-// and sum, and no barrier until the split's end; `beam_merge_kernel` joins the
-// splits and the beams of one sequence.
+// part of a row through registers, each thread with its own running maximum
+// and sum, and no barrier until the part's end; `beam_merge_kernel` joins the
+// parts and the beams of one sequence.
 //
 // The best logits come from the maxima that the softmax needs anyway.  The
 // threads' maxima are joined in groups; with T the num_out-th largest of the
 // groups' maxima, num_out logits are at least T, so the best are among the
 // logits that are, and only the threads whose maximum reaches T have their
 // logits looked at again (for 16 of 32768 independent logits: 22 threads of
-// 256; each remembers the maxima of 8 spans, so it reads one of them, from L2).  Selection compares (logit, token) as one 64-bit integer, so it
-// is exact whatever the order of the threads; the sum's order depends on the
-// logits' places in the row alone, not on its address, so equal rows have equal
-// sums.
+// 256; each remembers the maxima of 8 spans, so it reads one of them, from L2).
+// Selection compares (logit, token) as one 64-bit integer, so it is exact
+// whatever the order of the threads; the sum's order depends on the logits'
+// places in the row alone, not on its address, so equal rows have equal sums.
 #include "pa_common.cuh"
 
 #include <atomic>
@@ -39,15 +39,15 @@ namespace pa {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowCtas = 5;             // resident on an SM
+constexpr int kRowCtas = 5;            // resident on an SM
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kLaneRuns = 4;            // runs of 16 bytes of a lane per chunk
 constexpr int kLogLaneRuns = 2;
 constexpr int kChunkRuns = 32 * kLaneRuns;
 constexpr int kUnitRuns = kRowWarps * kChunkRuns;  // a chunk of every warp: the grain in which rows are split
-constexpr int kStages = 2;    // chunks of a warp in shared memory
+constexpr int kStages = 2;             // chunks of a warp in shared memory
 constexpr int kSpans = 8;              // a thread's units are remembered in so many spans, by their maxima
-constexpr int kHits = kRowWarps * kMaxBeamOut;  // logits at T that a split may have; with more its warps keep sorted lists
+constexpr int kHits = kRowWarps * kMaxBeamOut;  // logits at T that a part may have; with more its warps keep sorted lists
 constexpr int kMergeThreads = 512;
 constexpr int kMergeWarps = kMergeThreads / 32;
 constexpr int kNoGroup = static_cast<int>(0x80000000u);  // below every float in this order
@@ -208,7 +208,7 @@ __device__ __forceinline__ float take_runs(const uint4 (&u)[N], float& m, float&
     b = word_max<DT>(word_max<DT>(b, u[i].z), u[i].w);
   }
   const float2 f = word_logits<DT>(word_max<DT>(a, b));
-  const float top = clean(fmaxf(f.x, f.y));  // of NaN alone too
+  const float top = fminf(fmaxf(fmaxf(f.x, f.y), -INFINITY), FLT_MAX);  // both NaN: -inf
   if (top > m) {
     s *= ex2((m - top) * kLog2e);
     m = top;
@@ -234,10 +234,11 @@ __device__ __forceinline__ float take_runs(const uint4 (&u)[N], float& m, float&
     f2_unpack(f2_add(part[0], part[1]), a, b);
     return a + b;
   };
-  // exp(x - ref) = 2^(x L + c) 2^e with c = -ref L rounded and e what that left off
+  // exp(x - ref) = 2^(x L + c) 2^e with c = -ref L rounded and e what that left off: at most 2^-11 for these ref, so
+  // that 1 + e ln 2 is 2^e to 2^-24
   const float c = -ref * kLog2e, e = fmaf(-ref, kLog2e, -c);
   float sum = NAN;
-  if (fabsf(ref) < 1e30f) {
+  if (fabsf(ref) < 8192.f) {
     const uint64_t scale = f2_pack(kLog2e, kLog2e), shift = f2_pack(c, c);
     sum = all([&](float x, float y) {
       float a, b;
@@ -246,7 +247,7 @@ __device__ __forceinline__ float take_runs(const uint4 (&u)[N], float& m, float&
     });
     sum = fmaf(sum, e * 0.6931472f, sum);
   }
-  if (!(sum <= FLT_MAX)) {  // NaN, +inf, or a maximum that x L would pass the largest float for
+  if (!(sum <= FLT_MAX)) {  // NaN, +inf, or a larger maximum: the difference first
     sum = all([&](float x, float y) { return f2_pack(ex2((clean(x) - ref) * kLog2e), ex2((clean(y) - ref) * kLog2e)); });
   }
   s += sum;

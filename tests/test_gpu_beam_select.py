@@ -138,6 +138,18 @@ def test_runs_of_nan(ops, dtype):
     _check(ops.beam_select(x, s, 9), x, s, 9)
 
 
+@pytest.mark.parametrize("shift", [-3e4, 8000.25, 12345.625, 1e6, -1e30])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_logits_far_from_zero(ops, dtype, shift):
+    """Only differences of logits count: a common shift of any size leaves the sums as good."""
+    if dtype == torch.float16 and abs(shift) > 6e4:
+        pytest.skip("past fp16")
+    g = torch.Generator(device="cuda").manual_seed(14)
+    x = (torch.randn(2, 3, 9001, device="cuda", generator=g) * 2 + shift).to(dtype)
+    s = -torch.rand(2, 3, device="cuda", generator=g)
+    _check(ops.beam_select(x, s, 9), x, s, 9)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_finished_beams(ops, dtype):
     B, K, V, n, eos = 6, 4, 10007, 8, 17
