@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
   __shared__ double top[kMaxBeams], logsum[kMaxBeams];  // apart: beside a maximum of 1e30 the logarithm would vanish
   __shared__ float ftop[kMaxBeams], offset[kMaxBeams];
   __shared__ int group[64], count;
-  __shared__ float limit_of_all;
+  __shared__ float limit_of_all, largest_offset;
   const int row0 = b * K;
   if (tid < 64) group[tid] = kNoGroup;
   if (tid == 0) count = 0;
@@ -521,16 +521,22 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
     const float v = nth_group(value(group[lane]), value(group[32 + lane]), n, largest);
     if (lane == 0) limit_of_all = v;
   }
+  if (warp == 1) {  // the largest finite |offset|; floats of no sign lie in the order of their bits
+    const float o = lane < K ? fabsf(offset[lane]) : 0.f;
+    const unsigned most = __reduce_max_sync(0xffffffffu, o <= FLT_MAX ? __float_as_uint(o) : 0u);
+    if (lane == 0) largest_offset = __uint_as_float(most);
+  }
   __syncthreads();
-  const float limit = limit_of_all;
+  const float limit = limit_of_all, coarse = fabsf(limit) + largest_offset;
   for (int i = tid; i < total; i += kMergeThreads) {
     const unsigned long long key = keys[i];
     const int k = over(i, per_inv);
     bool hit = key != 0;
     if (hit) {
       const float v = rough(i, k);
-      // x - top and the sum with the offset are rounded twice, the limit's too
-      const float slack = 4.f * 1.2e-7f * (fabsf(limit) + fabsf(v) + fabsf(offset[k]));
+      // offset, x - top and their sum are rounded here, and in the n candidates at the limit, of any beam:
+      // each time by at most 2^-24 of |offset| + |sum|, and no sum is larger than its offset
+      const float slack = 4.f * 1.2e-7f * (coarse + fabsf(v));
       hit = v >= limit || (v > -INFINITY && !(limit - v > slack));
     }
     if (!hit) continue;

@@ -150,6 +150,31 @@ def test_logits_far_from_zero(ops, dtype, shift):
     _check(ops.beam_select(x, s, 9), x, s, 9)
 
 
+def test_beams_with_scores_of_very_different_size(ops):
+    """A beam at 1e6 whose candidates come back to ordinary scores: its fp32 sums are coarse, the others' must not suffer."""
+    V = 5000
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x = torch.randn(3, 3, V, device="cuda", generator=g)
+    x[:, 0, 77] = 1e6                       # log-sum-exp 1e6: token v scores 1e6 + (x - 1e6)
+    x[:, 2, 11] = -1e6
+    s = torch.tensor([1e6, 11.5, 11.0], device="cuda").expand(3, 3).contiguous()
+    for n in (1, 7, 16, 32):
+        _check(ops.beam_select(x, s, n), x, s, n)
+
+
+@pytest.mark.parametrize("n", [2, 16, 32])
+def test_coarse_sums_of_another_beam_do_not_hide_a_candidate(ops, n):
+    """Beam 0's scores pass 1e6, where fp32 steps by 1/16: 0.04 is 0.0625 there, above beam 1's 0.05."""
+    x = torch.full((1, 2, 4096), 0.04, device="cuda")
+    x[0, 0, 77] = 1e6
+    x[0, 1] = -100.0
+    x[0, 1, 5] = 0.0
+    s = torch.tensor([[1e6, 0.05]], device="cuda")
+    got = ops.beam_select(x, s, n)
+    _check(got, x, s, n, exact_order=True)
+    assert got[2][0, :2].tolist() == [0, 1] and got[1][0, :2].tolist() == [77, 5]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_finished_beams(ops, dtype):
     B, K, V, n, eos = 6, 4, 10007, 8, 17
