@@ -44,6 +44,7 @@ class BeamSearch:
             raise ValueError(f"eos_id {eos_id} is outside the vocabulary of {V}")
         if max_new_tokens < 1 or B < 1:
             raise ValueError("at least one sequence and one new token are needed")
+        pool._need_caches()  # not only when the first partly filled block is copied
         self.pool, self.B, self.K, self.eos = pool, B, K, int(eos_id)
         self.seq_ids = [int(s) for s in seq_ids]
         self.host_tokens = [int(n) for n in num_tokens]
@@ -121,7 +122,7 @@ class BeamSearch:
     def advance(self, logits: torch.Tensor) -> torch.Tensor:
         """Take the next tokens from ``logits`` [B, K, V], after the step's K/V rows were written; returns ``tokens``."""
         if not self._room:
-            raise RuntimeError("step_inputs() comes before advance()")
+            raise RuntimeError("the search has ended" if self._ended else "step_inputs() comes before advance()")
         if tuple(logits.shape[:2]) != (self.B, self.K):
             raise ValueError(f"logits must be [{self.B}, {self.K}, vocab]")
         parents = self._choose(logits)
@@ -143,7 +144,7 @@ class BeamSearch:
             for s in self.seq_ids:
                 self.pool.release_beams(s)
             self.pool.flush()
-            self._ended = True
+            self._ended, self._room = True, False
         found = []
         for b in range(self.B):
             beams = []

@@ -435,6 +435,36 @@ def test_beam_search_that_cannot_start_leaves_the_prompts():
     assert dm.num_free_blocks() == 8 == dm.free_top.item()
 
 
+def test_beam_search_that_has_ended_moves_no_blocks():
+    """advance() after finish(): its rows may belong to others by now."""
+    from pie_b200.beam import BeamSearch
+
+    x = torch.randn(1, 30, device="cuda")
+    dm = manager(NB=12, seqs=4, cols=4)
+    dm.allocate(0, 2)
+    search = BeamSearch(dm, [0], [7], x, 2, 0, 9)
+    search.step_inputs()
+    search.finish()
+    for s in (5, 6, 7, 8):  # all rows, with as many blocks each as a beam had
+        dm.allocate(s, 2)
+    dm.flush()
+    before = [t.cpu() for t in dm.state[:5]]
+    with pytest.raises(RuntimeError, match="ended"):
+        search.advance(x.expand(1, 2, 30))
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(before, dm.state))
+
+
+def test_beam_search_needs_the_caches_from_the_start():
+    from pie_b200.beam import BeamSearch
+    from pie_b200.block_pool import DeviceBlockManager
+
+    dm = DeviceBlockManager(8, 4, max_seqs=4, max_blocks_per_seq=4)
+    dm.allocate(0, 2)
+    with pytest.raises(ValueError, match="attach_caches"):
+        BeamSearch(dm, [0], [8], torch.zeros(1, 30, device="cuda"), 2, 0, 5)  # full blocks: no fork copies
+    assert dm.num_free_blocks() == 6
+
+
 def test_beam_search_at_the_ends_of_the_pool():
     """A row without room, and a pool without blocks: step_inputs refuses, takes nothing, and goes on when there is room."""
     from pie_b200.beam import BeamSearch
