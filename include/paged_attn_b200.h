@@ -526,7 +526,7 @@ int block_pool_compact(const pa_block_pool_t* pool, const pa_block_share_t* shar
  *   scores    fp32 [num_seqs, num_beams]; NaN counts as -inf
  *   finished  uint8 [num_seqs, num_beams] or NULL: a finished beam's logits are
  *             not read; its log-probabilities are 0 at eos_id and -inf elsewhere
- * Sums are held in fp32 per split and joined in 64 bits; scores are compared
+ * Sums are held in fp32 per part of a row and joined in 64 bits; scores are compared
  * in 64 bits and rounded once to fp32.
  * Limits: num_beams <= 32, num_out <= min(32, num_beams * vocab), vocab <= 2^30.
  */
