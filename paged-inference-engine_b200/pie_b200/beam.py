@@ -27,8 +27,9 @@ MAX_BEAMS = 32  # of ops.beam_select and ops.reorder_beams
 class BeamSearch:
     """``num_beams`` beams of each of ``seq_ids``, which hold ``num_tokens[i]`` prompt tokens in the cache.
 
-    ``logits`` [B, V] are those of each prompt's last token.  The beams' pool ids are ``beam_id(seq_id, k)``; the
-    sequences must hold exactly the blocks that their tokens fill.  A beam that emits ``eos_id`` is finished: it keeps
+    ``logits`` [B, V] are those of each prompt's last token.  The pool knows the search as the sequences ``beam_id(seq_id,
+    k)``, but which row beam k has only the device knows (``slots``, in the order of ``tokens``): the pool refuses these
+    ids until ``finish``.  The sequences must hold exactly the blocks that their tokens fill.  A beam that emits ``eos_id`` is finished: it keeps
     its score and competes with the others until ``finish``.
     """
 
@@ -76,7 +77,7 @@ class BeamSearch:
 
     @staticmethod
     def beam_id(seq_id: int, k: int) -> object:
-        """The pool's id of beam k: the sequence itself, or (sequence, k)."""
+        """The id under which the pool counts the blocks of the search's k-th row: the sequence itself, or (sequence, k)."""
         return seq_id if k == 0 else (seq_id, k)
 
     @property

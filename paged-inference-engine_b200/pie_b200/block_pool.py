@@ -99,10 +99,27 @@ class BlockLedger:
         self.prefix: dict[int, _Prefix] = {}  # seq_id -> its last shared columns
         self.beams: dict[int, tuple[int, ...]] = {}  # first beam -> all beams of a search
         self.member: dict[int, int] = {}      # beam -> first beam
+        self.moved: set = set()               # first beams of searches whose rows the device has permuted
+
+    def row(self, seq_id: int) -> int:
+        """The table row of ``seq_id``.  A reordering permutes a search's rows on the device: its beams have none here."""
+        if self.moved and self.member.get(seq_id, seq_id) in self.moved:
+            raise ValueError(f"sequence {seq_id} is a beam of {self.member[seq_id]}, whose beams were reordered: only the "
+                             "device knows their rows (reorder_beams returned them)")
+        return self.slot[seq_id]
+
+    def beams_moved(self) -> None:
+        """Beams were reordered, of which searches only the device knows."""
+        self.moved.update(self.beams)
 
     def _alone(self, seq_id: int) -> None:
         if seq_id in self.member:
             raise ValueError(f"sequence {seq_id} is a beam of {self.member[seq_id]}: beams are extended and released together")
+
+    def none_is_a_beam(self, seq_ids: Sequence[int]) -> None:
+        if self.member:
+            for s in seq_ids:
+                self._alone(s if s in self.slot else int(s))
 
     def allocate(self, seq_id: int, num_blocks: int) -> tuple[AllocStatus, int, int]:
         """Returns (status, slot, first new column); queues the operation on success."""
@@ -225,6 +242,7 @@ class BlockLedger:
     def dissolve_beams(self, seq_id: int) -> None:
         """Undo fork_beams before any reordering: the forks are released, ``seq_id`` keeps its blocks."""
         beams = self.beams.pop(seq_id)
+        self.moved.discard(seq_id)
         for b in beams:
             del self.member[b]
         for b in beams[1:]:
@@ -244,6 +262,7 @@ class BlockLedger:
         # the counts agree again when all beams are gone.
         if seq_id not in self.beams:
             return AllocStatus.FAILURE
+        self.moved.discard(seq_id)
         for b in self.beams.pop(seq_id):
             del self.member[b]
             self._release(b)
@@ -331,7 +350,10 @@ class DeviceBlockManager:
 
     @property
     def state(self) -> ops.PoolState:
-        """The pool's device arrays, for ``ops.reorder_beams`` and ``ops.compact_blocks``."""
+        """The pool's device arrays, for ``ops.reorder_beams`` and ``ops.compact_blocks``.
+
+        The manager does not see what those do: use its own methods where it goes on handing out blocks.
+        """
         return ops.PoolState(self.free_stack, self.free_top, self.table[:self.max_seqs, :self.max_blocks_per_seq],
                              self.count[:self.max_seqs], self.ref_count[:self.num_blocks], self.scratch)
 
@@ -389,17 +411,20 @@ class DeviceBlockManager:
 
     def beam_slots(self, seq_ids: Sequence[int]) -> torch.Tensor:
         """The rows of the beams as ``fork_beams`` made them, int32 [len(seq_ids), num_beams] on the device."""
-        rows = [[self.ledger.slot[b] for b in self.ledger.beams[s]] for s in seq_ids]
+        rows = [[self.ledger.row(b) for b in self.ledger.beams[s]] for s in seq_ids]
         return torch.tensor(rows, dtype=torch.int32).to(self.device)
 
     def reorder_beams(self, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor) -> torch.Tensor:
         """Beam j of group g continues beam ``parents[g, j]``: returns the beams' rows afterwards (``ops.reorder_beams``).
 
         Which blocks became free only the device knows; ``num_free_blocks`` counts them when the beams are
-        released.  No host synchronisation: the call can be captured (with no queued calls).
+        released.  From now on only the returned rows name the beams: their ids are refused by ``slot_of``,
+        ``step_inputs`` and ``block_table`` until the search is released.  No host synchronisation: the call can be
+        captured (with no queued calls).
         """
         descs = self._need_caches()
         self.flush()
+        self.ledger.beams_moved()
         out = ops._reorder_call(self._desc, self._share, descs, self.free_top.device, ops._i32(slots), ops._i32(parents),
                                 ops._i32(num_tokens), self.status)
         self._checked("reorder_beams")
@@ -462,7 +487,8 @@ class DeviceBlockManager:
         return self._results
 
     def slot_of(self, seq_id: int) -> int:
-        return self.ledger.slot[seq_id]
+        """The table row of ``seq_id``; ValueError for a beam once ``reorder_beams`` has permuted the beams' rows."""
+        return self.ledger.row(seq_id)
 
     def blocks_of(self, seq_id: int) -> int:
         return self.ledger.blocks.get(seq_id, 0)
@@ -480,11 +506,12 @@ class DeviceBlockManager:
         first.  One pinned host-to-device copy of the per-sequence values and
         one launch; no host synchronisation.
         """
+        ids = [s if s in self.ledger.slot else int(s) for s in sequence_ids]
+        slots = [self.ledger.row(s) for s in ids]
         self.flush()
-        S = len(sequence_ids)
-        slots = [self.ledger.slot[int(s)] for s in sequence_ids]
+        S = len(ids)
         if bt_cols is None:
-            bt_cols = max((self.ledger.blocks[int(s)] for s in sequence_ids), default=0)
+            bt_cols = max((self.ledger.blocks[s] for s in ids), default=0)
         cu = [0]
         for q in q_lens:
             cu.append(cu[-1] + int(q))
@@ -527,10 +554,14 @@ class DeviceBlockManager:
 
     @property
     def block_table(self) -> dict:
-        """The per-sequence block lists as a host dict (reads the device: synchronises; for checks)."""
+        """The per-sequence block lists as a host dict (reads the device: synchronises; for checks).
+
+        ValueError while a search whose beams were reordered holds blocks: its rows have no names here.
+        """
+        rows = {sid: self.ledger.row(sid) for sid in self.ledger.slot}
         self.flush()
         tab = self.table.cpu()
-        return {sid: tab[slot, :self.ledger.blocks[sid]].tolist() for sid, slot in self.ledger.slot.items()}
+        return {sid: tab[slot, :self.ledger.blocks[sid]].tolist() for sid, slot in rows.items()}
 
     def free_list(self) -> list[int]:
         """The free list bottom to top, as the reference's ``st`` (reads the device: synchronises)."""

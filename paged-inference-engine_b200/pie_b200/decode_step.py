@@ -122,6 +122,7 @@ class DecodeStepGraph:
         """Append one token to each of ``seq_ids`` and attend.
 
         ``seq_lens[i]``: tokens of sequence i including this step's;
+        Beams of a search are refused: they are extended together, by ``BeamSearch``.
         ``q`` [n, Hq, D], ``k_new`` / ``v_new`` [n, Hkv, D] on the device.
         Returns O [n, Hq, D] (float16), a view of the graph's output buffer:
         consume it before the next ``step``.
@@ -129,6 +130,7 @@ class DecodeStepGraph:
         n = len(seq_ids)
         if n > self.S:
             raise ValueError(f"{n} sequences, the graph holds {self.S}")
+        self.pool.ledger.none_is_a_beam(seq_ids)
         if self.graphs is None:
             self.capture()
         for sid, ln in zip(seq_ids, seq_lens):

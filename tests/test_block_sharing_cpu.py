@@ -300,3 +300,63 @@ def test_selection_oracle_on_known_values():
     s, t, p = obs.select(x, np.array([[0.0, np.log(0.5)]]), 5)
     assert t.tolist() == [[1, 0, 2, 0, 1]] and p.tolist() == [[0, 0, 0, 1, 1]]
     np.testing.assert_allclose(s, [np.log([0.5, 0.25, 0.25, 0.25, 0.25])])
+
+
+def _host_manager(ledger):
+    """A manager without its device half: what it refuses before it touches the device."""
+    from pie_b200.block_pool import DeviceBlockManager
+
+    dm = DeviceBlockManager.__new__(DeviceBlockManager)
+    dm.ledger, dm.block_size, dm.num_blocks, dm._copies = ledger, 4, ledger.num_blocks, set()
+    return dm
+
+
+def test_beams_have_no_rows_here_once_the_device_has_permuted_them():
+    """Rows [0, 1, 2] and parents [1, 1, 0] give the beams the rows [1, 2, 0]: a beam's id would name another's row."""
+    from pie_b200.block_pool import BlockLedger
+
+    led = BlockLedger(40, 8, 6)
+    model = SharedPool(40, 8, 6, 4)
+    for s in (7, 8, 9):
+        led.allocate(s, 2)
+    assert led.fork_beams(7, ["a", (7, 2)], 8, 4).value == 0 and led.fork_beams(8, ["c"], 8, 4).value == 0
+    _apply(model, led.take_ops())
+    before = [led.row(s) for s in (7, "a", (7, 2))]
+    assert model.reorder(before, [1, 1, 0], 8)[0] == [before[1], before[2], before[0]]
+    dm = _host_manager(led)
+    assert dm.slot_of("a") == before[1]  # as fork_beams made them
+    led.beams_moved()
+    for s in (7, "a", (7, 2), 8, "c"):
+        with pytest.raises(ValueError, match="beam of"):
+            dm.slot_of(s)
+        with pytest.raises(ValueError, match="beam of"):
+            dm.step_inputs([9, s], [1, 1], [8, 8])
+        with pytest.raises(ValueError, match="beam of"):
+            led.none_is_a_beam([9, s])
+    with pytest.raises(ValueError, match="beam of"):
+        dm.beam_slots([7])
+    with pytest.raises(ValueError, match="beam of"):
+        dm.block_table
+    assert dm.slot_of(9) == led.slot[9]
+    led.none_is_a_beam([9])
+    led.release_beams(7)
+    led.release_beams(8)
+    led.allocate(7, 1)  # the id is an ordinary one again
+    assert dm.slot_of(7) == led.slot[7] and not led.moved
+    led.none_is_a_beam([7, 9])
+
+
+def test_the_decode_step_takes_no_beam():
+    from pie_b200.block_pool import BlockLedger
+    from pie_b200.decode_step import DecodeStepGraph
+
+    led = BlockLedger(40, 8, 6)
+    led.allocate(0, 2)
+    led.allocate(1, 2)
+    led.fork_beams(0, [(0, 1)], 8, 4)
+    graph = DecodeStepGraph.__new__(DecodeStepGraph)
+    graph.pool, graph.S = _host_manager(led), 4
+    for ids in ([0], [(0, 1)], [1, 0], [np.int64(0)]):
+        with pytest.raises(ValueError, match="beam of"):
+            graph.step(ids, [9] * len(ids), None, None, None)
+    assert len(led.take_ops()) == 3  # nothing was queued

@@ -544,3 +544,39 @@ def test_checked_mode_raises_what_the_status_says(monkeypatch):
     with pytest.raises(IndexError, match="contradict"):
         o.compact_blocks(pool, *caches, num_blocks=1)
     o.compact_blocks(pool, *caches)
+
+
+def test_a_beam_id_never_names_another_beams_row():
+    """After a reordering the manager's older methods refuse the beams, and take the ids again once they are released."""
+    from pie_b200 import ops as o
+    from pie_b200.beam import BeamSearch
+    from pie_b200.block_pool import DeviceBlockManager
+    from pie_b200.decode_step import DecodeStepGraph
+
+    NB, BS = 40, 16
+    k, v = (torch.zeros(NB, BS, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    pool = DeviceBlockManager(NB, BS, 8, 6)
+    pool.attach_caches(k, v)
+    graph = DecodeStepGraph(pool, k, v, None, None, 2, 3)
+    pool.allocate(0, 2)
+    pool.allocate(5, 1)
+    search = BeamSearch(pool, [0], [20], torch.randn(1, 30, device="cuda"), 3, 0, 5)
+    assert set(pool.block_table) == {DecodeStepGraph.PAD_SEQ, 0, 5, (0, 1), (0, 2)}
+    inp = pool.step_inputs([0, 5, (0, 2)], [1, 1, 1], [20, 9, 20])
+    assert inp["block_table"][0, 0] == inp["block_table"][2, 0] != inp["block_table"][1, 0]
+    search.step_inputs()
+    search.advance(torch.randn(1, 3, 30, device="cuda"))
+    rows = torch.ones(1, 2, 64, dtype=torch.float16, device="cuda")
+    before = [t.cpu() for t in pool.state[:5]]
+    for s in (0, (0, 1), (0, 2)):
+        for call in (lambda: pool.slot_of(s), lambda: pool.step_inputs([s], [1], [21]), lambda: pool.beam_slots([0]),
+                     lambda: pool.block_table, lambda: graph.step([s], [22], rows, rows, rows)):
+            with pytest.raises(ValueError, match="beam of"):
+                call()
+    assert graph.step([5], [10], rows, rows, rows).shape == (1, 2, 64)
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(before, pool.state))
+    mine = {pool.table[pool.slot_of(s), 0].item() for s in (5, DecodeStepGraph.PAD_SEQ)}
+    assert set(k.flatten(1).any(1).nonzero().flatten().tolist()) <= mine  # no beam's page was written
+    search.finish()
+    pool.allocate(0, 1)
+    assert len(pool.block_table[0]) == 1 and pool.step_inputs([0], [1], [3])["num_blocks_per_seq"].tolist() == [1]
