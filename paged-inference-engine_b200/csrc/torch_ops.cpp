@@ -404,16 +404,6 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& dev)
   return at::Tensor(at::detail::empty_cuda(sizes, t, dev, std::nullopt));
 }
 
-// Piece i of a fresh int32 [n, rows, cols], as a contiguous [rows, cols] of a 4-byte type.
-at::Tensor piece(const at::Tensor& all, int64_t i, at::ScalarType t) {
-  const int64_t rows = all.size(1), cols = all.size(2);
-  at::Tensor p = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
-                                                          at::scalarTypeToTypeMeta(t));
-  p.unsafeGetTensorImpl()->set_sizes_contiguous({rows, cols});
-  p.unsafeGetTensorImpl()->set_storage_offset(i * rows * cols);
-  return p;
-}
-
 // One descriptor per layer; the scale lists are empty but for int8 pools.
 std::vector<pa_kv_cache_t> layer_descs(at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs) {
   TORCH_CHECK_VALUE(!k.empty() && k.size() == v.size(), "pie_b200: as many K as V pools are needed, one at least (got ",
@@ -576,9 +566,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_op(const at::Tensor& 
   check_rc(beam_select_workspace_size(&a, &bytes), "beam_select");
   // a workspace of this call's own: calls on other streams and captured graphs do not share it
   at::Tensor ws = fresh({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, at::kByte, logits.device());
-  const at::Tensor all = fresh({3, logits.size(0), num_out}, at::kInt, logits.device());  // one allocation for the outputs
-  std::tuple<at::Tensor, at::Tensor, at::Tensor> out{piece(all, 0, at::kFloat), piece(all, 1, at::kInt),
-                                                     piece(all, 2, at::kInt)};
+  // three tensors of their own, as the schema says: compiled code takes them to start on 16 bytes, and two types
+  // over one storage could not be saved together
+  std::tuple<at::Tensor, at::Tensor, at::Tensor> out{fresh({logits.size(0), num_out}, at::kFloat, logits.device()),
+                                                     fresh({logits.size(0), num_out}, at::kInt, logits.device()),
+                                                     fresh({logits.size(0), num_out}, at::kInt, logits.device())};
   a.out_scores = static_cast<float*>(std::get<0>(out).data_ptr());
   a.out_tokens = static_cast<int32_t*>(std::get<1>(out).data_ptr());
   a.out_parents = static_cast<int32_t*>(std::get<2>(out).data_ptr());

@@ -262,3 +262,30 @@ def test_refusals_on_the_gpu(ops):
         ops.beam_select(x, s, 33)
     with pytest.raises(RuntimeError, match="num_beams"):
         ops.beam_select(torch.zeros(1, 33, 50, device="cuda"), torch.zeros(1, 33, device="cuda"), 3)
+
+
+@pytest.mark.parametrize("B,n", [(1, 3), (3, 7), (5, 32)])
+def test_outputs_are_tensors_of_their_own(ops, tmp_path, B, n):
+    """As the schema says: each starts a storage (compiled code takes that for 16-byte alignment), and all can be saved."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    x, s = torch.randn(B, 4, 1000, device="cuda", generator=g), torch.zeros(B, 4, device="cuda")
+    got = ops.beam_select(x, s, n)
+    assert [t.storage_offset() for t in got] == [0] * 3 and all(t.data_ptr() % 16 == 0 for t in got)
+    assert len({t.untyped_storage().data_ptr() for t in got}) == 3
+    assert all(t.untyped_storage().nbytes() == 4 * B * n for t in got)
+    torch.save(got, tmp_path / "beams.pt")
+    assert all(torch.equal(a, b) for a, b in zip(torch.load(tmp_path / "beams.pt"), got))
+
+
+def test_compiled_call_with_odd_outputs():
+    """Through torch.compile, whose generated code asserts the outputs' alignment; 1 x 3 outputs of 4 bytes."""
+    from pie_b200 import _torch_ext
+
+    op = _torch_ext.ops().beam_select
+    x = torch.randn(1, 3, 500, device="cuda")
+    s = torch.zeros(1, 3, device="cuda")
+    want = op(x, s, 3, None, -1)
+    got = torch.compile(lambda x, s: op(x, s, 3, None, -1), fullgraph=True)(x, s)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    torch.library.opcheck(op.default if hasattr(op, "default") else op, (x, s, 3, None, -1),
+                          test_utils=("test_schema", "test_faketensor"))
