@@ -580,6 +580,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select_op(const at::Tensor& 
 }
 
 // ---- shapes only (fake / meta tensors) ------------------------------------
+// Of every op that writes into its arguments and returns nothing.
+void write_only_meta(const c10::OperatorHandle& op, c10::DispatchKeySet, torch::jit::Stack* stack) {
+  torch::jit::drop(*stack, op.schema().arguments().size());
+}
+
 at::Tensor reorder_beams_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                               const at::Tensor&, const at::Tensor&, const at::Tensor& slots, const at::Tensor&,
                               const at::Tensor&, at::TensorList, at::TensorList, at::TensorList, at::TensorList,
@@ -669,4 +674,6 @@ TORCH_LIBRARY_IMPL(pie_b200, Meta, m) {
   m.impl("reorder_beams", &reorder_beams_meta);
   m.impl("compact_blocks", &compact_blocks_meta);
   m.impl("beam_select", &beam_select_meta);
+  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "copy_blocks"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&write_only_meta>());
 }

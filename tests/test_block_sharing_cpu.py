@@ -360,3 +360,30 @@ def test_the_decode_step_takes_no_beam():
         with pytest.raises(ValueError, match="beam of"):
             graph.step(ids, [9] * len(ids), None, None, None)
     assert len(led.take_ops()) == 3  # nothing was queued
+
+
+def test_every_op_has_a_meta_kernel():
+    """On meta tensors: ops that return nothing leave their arguments alone, the others give their outputs' shapes."""
+    from pie_b200 import _torch_ext
+
+    ops = _torch_ext.ops()
+
+    def t(*shape, dtype=torch.int32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    half = torch.float16
+    kv = [t(10, 16, 2, 64, dtype=half)]
+    pool = (t(10), t(1), t(6, 5), t(6), t(10), t(60))
+    assert ops.copy_blocks(kv, kv, [], [], t(3), t(3), None, None) is None
+    assert ops.copy_blocks(kv * 2, kv * 2, [], [], t(3), t(3), t(3), t(1)) is None
+    assert ops.write_kv(t(4, 2, 64, dtype=half), t(4, 2, 64, dtype=half), t(2, 5), t(4), t(4), kv[0], kv[0], None, None,
+                        None) is None
+    assert ops.project_write_kv(t(4, 256, dtype=half), t(256, 256, dtype=half), None, t(2, 5), t(4), t(4), kv[0], kv[0],
+                                None, None, None) is None
+    q, lse = t(2, 4, 1, 64, dtype=half), t(2, 4, 1, dtype=half)
+    assert ops.paged_attention_out(q, kv[0], kv[0], t(2), t(2, 5), t(2), t(2), None, None, False, 0.0, 0, None, q, lse) is None
+    q, lse = t(7, 4, 64, dtype=half), t(7, 4, dtype=half)
+    assert ops.paged_attention_varlen_out(q, t(3), t(2), 5, kv[0], kv[0], t(2, 5), t(2), t(2), None, None, False, 0.0, None,
+                                          q, lse) is None
+    assert ops.reorder_beams(*pool, t(2, 3), t(2, 3), t(2), kv, kv, [], [], None).shape == (2, 3)
+    assert ops.compact_blocks(*pool, -1, kv, kv, [], [], None).shape == (1,)

@@ -269,3 +269,21 @@ def test_compaction_of_contradicting_arrays(ops):
     assert pool.table[row, :2].tolist() == [free_high, 100]
     pool.count[row] = -1
     pool_equals(pool, m)
+
+
+def test_compiled_copies():
+    """Through torch.compile, which traces the op on fake tensors."""
+    from pie_b200 import _torch_ext
+
+    op = _torch_ext.ops().copy_blocks
+    k, v, _, _ = make_caches(9, 16, 2, 64, torch.float16, 2)
+    want = moved(host((k, v)), [(1, 4, 16), (2, 7, 16)])
+    src, dst = _i32([1, 2]), _i32([4, 7])
+
+    def step(k0, k1, v0, v1, src, dst):
+        op([k0, k1], [v0, v1], [], [], src, dst, None, None)
+        return src
+
+    got = torch.compile(step, fullgraph=True)(*k, *v, src, dst)
+    assert got.tolist() == [1, 2]
+    same((k, v), want)
