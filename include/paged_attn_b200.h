@@ -496,7 +496,9 @@ int block_pool_apply_shared(const pa_block_pool_t* pool, const pa_block_share_t*
  * layers), nothing is read back; all arrays int32 on the device.  Every row
  * belongs to one beam of one group.  A group with a bad or repeated row, a bad
  * parent (PA_STATUS_BAD_SEQ_INDEX), or rows whose blocks do not hold its
- * tokens or are not equally many (PA_STATUS_BAD_POSITION) is left as it is.
+ * tokens or are not equally many (PA_STATUS_BAD_POSITION) is left as it is,
+ * and so is one whose num_tokens ends inside a block that another row holds
+ * too (PA_STATUS_BAD_POOL): that block cannot be written.
  * Limits: 1 <= num_beams <= 32.
  */
 int block_pool_reorder(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* slots,

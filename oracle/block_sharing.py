@@ -58,6 +58,11 @@ class SharedPool:
         self.rows[slot] = row
         return SUCCESS, copy
 
+    def may_reorder(self, slots, tokens) -> bool:
+        """Whether a partly filled last block, which copies and the next tokens write, belongs to its row alone."""
+        full, tail = divmod(tokens, self.BS)
+        return not tail or all(self.ref[self.rows[s][full]] == 1 for s in slots)
+
     def reorder(self, slots, parents, tokens):
         """One group: (new slots, page copies); freed blocks are returned, to be pushed in ascending order by ``push``."""
         K = len(slots)

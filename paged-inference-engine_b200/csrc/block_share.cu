@@ -163,8 +163,8 @@ struct Forks {
 };
 
 // By warp 0; lane j stands for beam j.  False: the group is left as it is.
-__device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderParams& r, int log2BS, int g, Forks& f,
-                                           bool write) {
+__device__ __forceinline__ bool plan_group(const PoolParams& p, const ShareParams& s, const ReorderParams& r, int log2BS,
+                                           int g, Forks& f, bool write) {
   const int lane = threadIdx.x & 31, K = r.beams;
   const bool on = lane < K;
   const int slot = on ? r.slots[g * K + lane] : -1 - lane;
@@ -185,11 +185,16 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
     if (!__all_sync(0xffffffffu, !on || c == c0) || need < 0 || need > c0 || c0 > p.max_blocks_per_seq)
       bad = ST_BAD_POSITION;
   }
-  if (bad) {
+  const auto refuse = [&](int why) {
     if (write && on) r.slots_out[g * K + lane] = slot;
-    if (write && lane == 0) set_status(r.status, bad);
+    if (write && lane == 0) set_status(r.status, why);
     return false;
-  }
+  };
+  if (bad) return refuse(bad);
+  // holders of the row's partly filled block: its copy and the next token write it, so there must be no other
+  const int tail = tokens & (bs - 1);
+  const bool counted = on && tail && last >= 0 && last < p.num_blocks;
+  const int holders = counted ? __ldcg(&s.ref[last]) : 1;
   const unsigned same = __match_any_sync(0xffffffffu, parent);
   const bool again = on && (same & ((1u << lane) - 1));
   const unsigned forks = __ballot_sync(0xffffffffu, again);
@@ -201,6 +206,7 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
   const int child = __shfl_sync(0xffffffffu, slot, taken & 31);
   const int src = __shfl_sync(0xffffffffu, last, on ? parent : 0);
   const int dst = __shfl_sync(0xffffffffu, last, taken & 31);
+  if (!__all_sync(0xffffffffu, holders == 1)) return refuse(ST_BAD_POOL);
   if (again) {
     f.child[nth] = child;
     f.donor[nth] = donor;
@@ -210,7 +216,7 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ReorderPar
   if (lane == 0) {
     f.n = __popc(forks);
     f.full = full;
-    f.tail = tokens & (bs - 1);
+    f.tail = tail;
   }
   if (write && on) r.slots_out[g * K + lane] = again ? child : donor;
   return true;
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolPara
     const int cta = blockIdx.x - tables, share = cta % shares, fork = cta / shares;
     const int nth = fork / r.groups, group = fork - nth * r.groups;  // groups' first forks first: few groups have K - 1
     if (threadIdx.x < 32) {
-      const bool good = plan_group(p, r, log2BS, group, f, false);
+      const bool good = plan_group(p, s, r, log2BS, group, f, false);
       if (threadIdx.x == 0) ok = good;
     }
     __syncthreads();
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolPara
   const int group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
   unsigned* bitmap = reinterpret_cast<unsigned*>(s.scratch + kShareHead);
   if (threadIdx.x < 32) {
-    const bool good = plan_group(p, r, log2BS, group, f, chunk == 0);
+    const bool good = plan_group(p, s, r, log2BS, group, f, chunk == 0);
     if (threadIdx.x == 0) ok = good;
   }
   __syncthreads();

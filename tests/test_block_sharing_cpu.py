@@ -387,3 +387,18 @@ def test_every_op_has_a_meta_kernel():
                                           q, lse) is None
     assert ops.reorder_beams(*pool, t(2, 3), t(2, 3), t(2), kv, kv, [], [], None).shape == (2, 3)
     assert ops.compact_blocks(*pool, -1, kv, kv, [], [], None).shape == (1,)
+
+
+def test_a_reordering_inside_a_shared_block_would_write_others_tokens():
+    """Tokens rolled back into a block that an earlier reordering shared: on the model, two copies have one target."""
+    m = SharedPool(20, 4, 4, 4)
+    m.allocate(0, 1)
+    for s in (1, 2):
+        m.fork(s, 4, 0)
+    for s in range(3):
+        m.allocate(s, 1)
+    assert m.may_reorder([0, 1, 2], 6)
+    m.push(m.reorder([0, 1, 2], [1, 1, 1], 8)[2])  # the second block is full: all three hold beam 1's
+    assert m.may_reorder([0, 1, 2], 8) and not m.may_reorder([0, 1, 2], 6)
+    copies = m.reorder([0, 1, 2], [0, 0, 0], 6)[1]
+    assert len({d for _, d, _ in copies}) == 1 < len(copies)

@@ -580,3 +580,40 @@ def test_a_beam_id_never_names_another_beams_row():
     search.finish()
     pool.allocate(0, 1)
     assert len(pool.block_table[0]) == 1 and pool.step_inputs([0], [1], [3])["num_blocks_per_seq"].tolist() == [1]
+
+
+def test_reorder_refuses_tokens_inside_a_shared_block(ops):  # noqa: F811
+    """Tokens rolled back below a shared block's end, in a group or to another sequence: left as they are, others go on."""
+    BS = 4
+    m = SharedPool(60, 12, 5, BS)
+    caches = make_caches(m.NB, BS, 2, 64, torch.float16, 2)
+    want = host(caches)
+    groups = [[0, 1, 2], [5, 4, 3], [6, 7, 8]]
+    for g in groups:
+        m.allocate(g[0], 1)
+        for s in g[1:]:
+            m.fork(s, BS, g[0])
+        for s in g:
+            m.allocate(s, 1)
+    m.push(m.reorder(groups[0], [1, 1, 2], 8)[2])   # beams 0 and 1 hold one second block
+    m.fork(9, 8, groups[1][2])                      # another sequence holds beam 2's second block
+    assert [m.may_reorder(g, 6) for g in groups] == [False, False, True]
+    pool, st = pool_arrays(ops, m, m.max_blocks), _i32([0])
+    parents = [[2, 2, 0], [1, 1, 0], [2, 0, 2]]
+    got = ops.reorder_beams(pool, _i32(groups), _i32(parents), _i32([6, 7, 5]), *caches, status=st)
+    new, copies, freed = m.reorder(groups[2], parents[2], 5)
+    m.push(freed)
+    m.check()
+    assert got.tolist() == groups[:2] + [new] and st.item() == 128
+    pool_equals(pool, m)
+    same(caches, moved(want, copies))
+    st.zero_()
+    got = ops.reorder_beams(pool, _i32(groups[:2]), _i32(parents[:2]), _i32([4, 8]), *caches, status=st)  # whole blocks
+    after = []
+    for g, p, n in zip(groups, parents, (4, 8)):
+        new, copies, freed = m.reorder(g, p, n)
+        after.append(new)
+        m.push(freed)
+        assert not copies
+    assert got.tolist() == after and st.item() == 0
+    pool_equals(pool, m)
