@@ -162,9 +162,12 @@ struct Forks {
   int n, full, tail;                       // full blocks and tokens of the last one
 };
 
-// By warp 0; lane j stands for beam j.  False: the group is left as it is.
-__device__ __forceinline__ bool plan_group(const PoolParams& p, const ShareParams& s, const ReorderParams& r, int log2BS,
-                                           int g, Forks& f, bool write) {
+// By warp 0; lane j stands for beam j: its row afterwards, and the holders of its row's partly filled block, which its
+// copy and the next token write, so that a group with any other than 1 is left as it is too (ST_BAD_POOL).  That count
+// is not waited for here: a CTA that copies has its first loads under way meanwhile.  Returns a status, 0 if the group's
+// arguments hold.
+__device__ __forceinline__ int plan_group(const PoolParams& p, const ShareParams& s, const ReorderParams& r, int log2BS,
+                                          int g, Forks& f, int& row, int& holders) {
   const int lane = threadIdx.x & 31, K = r.beams;
   const bool on = lane < K;
   const int slot = on ? r.slots[g * K + lane] : -1 - lane;
@@ -185,16 +188,10 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ShareParam
     if (!__all_sync(0xffffffffu, !on || c == c0) || need < 0 || need > c0 || c0 > p.max_blocks_per_seq)
       bad = ST_BAD_POSITION;
   }
-  const auto refuse = [&](int why) {
-    if (write && on) r.slots_out[g * K + lane] = slot;
-    if (write && lane == 0) set_status(r.status, why);
-    return false;
-  };
-  if (bad) return refuse(bad);
-  // holders of the row's partly filled block: its copy and the next token write it, so there must be no other
+  if (bad) return bad;
   const int tail = tokens & (bs - 1);
   const bool counted = on && tail && last >= 0 && last < p.num_blocks;
-  const int holders = counted ? __ldcg(&s.ref[last]) : 1;
+  holders = counted ? __ldcg(&s.ref[last]) : 1;
   const unsigned same = __match_any_sync(0xffffffffu, parent);
   const bool again = on && (same & ((1u << lane) - 1));
   const unsigned forks = __ballot_sync(0xffffffffu, again);
@@ -206,7 +203,6 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ShareParam
   const int child = __shfl_sync(0xffffffffu, slot, taken & 31);
   const int src = __shfl_sync(0xffffffffu, last, on ? parent : 0);
   const int dst = __shfl_sync(0xffffffffu, last, taken & 31);
-  if (!__all_sync(0xffffffffu, holders == 1)) return refuse(ST_BAD_POOL);
   if (again) {
     f.child[nth] = child;
     f.donor[nth] = donor;
@@ -218,8 +214,8 @@ __device__ __forceinline__ bool plan_group(const PoolParams& p, const ShareParam
     f.full = full;
     f.tail = tail;
   }
-  if (write && on) r.slots_out[g * K + lane] = again ? child : donor;
-  return true;
+  row = again ? child : donor;
+  return 0;
 }
 
 // The first groups * chunks CTAs share full blocks (a CTA for kColumns table
@@ -234,15 +230,16 @@ __global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolPara
                                                                int chunks, int shares) {
   pdl_enter();
   __shared__ Forks f;
-  __shared__ bool ok, last;
+  __shared__ bool ok, writable, last;
   __shared__ int warp_sum[kApplyThreads / 32];
   const int tables = r.groups * chunks;
+  int row, holders;
   if (static_cast<int>(blockIdx.x) >= tables) {
     const int cta = blockIdx.x - tables, share = cta % shares, fork = cta / shares;
     const int nth = fork / r.groups, group = fork - nth * r.groups;  // groups' first forks first: few groups have K - 1
     if (threadIdx.x < 32) {
-      const bool good = plan_group(p, s, r, log2BS, group, f, false);
-      if (threadIdx.x == 0) ok = good;
+      const int bad = plan_group(p, s, r, log2BS, group, f, row, holders);
+      if (threadIdx.x == 0) ok = bad == 0;
     }
     __syncthreads();
     if (!ok || nth >= f.n || f.tail == 0) return;
@@ -251,8 +248,15 @@ __global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolPara
       if (threadIdx.x == 0) set_status(r.status, ST_BAD_BLOCK_ID);
       return;
     }
-    const int items = g.layers * 2 * g.parts;
-    for (int i = items * share / shares; i < items * (share + 1) / shares; ++i)
+    const int items = g.layers * 2 * g.parts, begin = items * share / shares;
+    prefetch_page<4>(g, begin / g.parts >> 1, begin / g.parts & 1, src, f.tail, begin % g.parts);
+    if (threadIdx.x < 32) {
+      const bool sole = __all_sync(0xffffffffu, holders == 1);
+      if (threadIdx.x == 0) writable = sole;
+    }
+    __syncthreads();
+    if (!writable) return;
+    for (int i = begin; i < items * (share + 1) / shares; ++i)
       copy_page<4>(g, i / g.parts >> 1, i / g.parts & 1, src, dst, f.tail, i % g.parts);
     return;
   }
@@ -260,8 +264,12 @@ __global__ void __launch_bounds__(kCopyThreads, 5) reorder_kernel(const PoolPara
   const int group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
   unsigned* bitmap = reinterpret_cast<unsigned*>(s.scratch + kShareHead);
   if (threadIdx.x < 32) {
-    const bool good = plan_group(p, s, r, log2BS, group, f, chunk == 0);
-    if (threadIdx.x == 0) ok = good;
+    int bad = plan_group(p, s, r, log2BS, group, f, row, holders);
+    if (!bad && !__all_sync(0xffffffffu, holders == 1)) bad = ST_BAD_POOL;
+    const int at = group * r.beams + threadIdx.x;
+    if (chunk == 0 && static_cast<int>(threadIdx.x) < r.beams) r.slots_out[at] = bad ? r.slots[at] : row;
+    if (chunk == 0 && threadIdx.x == 0 && bad) set_status(r.status, bad);
+    if (threadIdx.x == 0) ok = bad == 0;
   }
   __syncthreads();
   if (ok) {

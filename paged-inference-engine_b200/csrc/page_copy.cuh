@@ -43,6 +43,22 @@ __device__ __forceinline__ void copy_vecs(const char* from, char* to, int v0, in
   }
 }
 
+// The first N vectors per thread that copy_page will read of page src, into L2.
+template <int N>
+__device__ __forceinline__ void prefetch_page(const PageParams& g, int layer, int kv, int src, int slots, int part) {
+  const PageSide& s = g.side[kv];
+  const char* from = g.page[kv][layer] + src * s.blk;
+  const int vecs = (slots * g.heads) << g.row_vecs_log2;
+  const int per = (vecs + g.parts - 1) / g.parts;
+  const int begin = part * per + threadIdx.x, end = min(vecs, (part + 1) * per);
+  const bool run = s.linear || (s.dense && slots == g.block_size);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int v = begin + i * kCopyThreads;
+    if (v < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + (run ? 16LL * v : page_vec(g, s, v, slots))));
+  }
+}
+
 // Part `part` of the copy of the first `slots` slots of page src to page dst,
 // of layer `layer`'s K (kv 0) or V (kv 1) pool, by all threads of the CTA.
 // Part 0 takes the page's scales too; a scale per block goes with any slot.
