@@ -187,6 +187,15 @@ class BlockLedger:
             node = node.up
         return node
 
+    def shared_columns(self, seq_id: int) -> int:
+        """The first columns of ``seq_id`` that other sequences hold too."""
+        n, node = 0, self.prefix.get(seq_id)
+        while node is not None:
+            if node.holders > 1:
+                n += node.n
+            node = node.up
+        return n
+
     def fork(self, parent_id: int, child_id: int, num_tokens: int, block_size: int) -> tuple[AllocStatus, int]:
         """The child gets the parent's first tokens: (status, the child's slot); queues the operation on success."""
         self._alone(parent_id)
@@ -229,6 +238,9 @@ class BlockLedger:
         if self.blocks[seq_id] != -(-num_tokens // block_size):
             raise ValueError(f"sequence {seq_id} holds {self.blocks[seq_id]} blocks: beams start with the "
                              f"{-(-num_tokens // block_size)} that {num_tokens} tokens fill")
+        if num_tokens % block_size and self.shared_columns(seq_id) > num_tokens // block_size:
+            raise ValueError(f"sequence {seq_id} ends inside a block that another sequence holds: its next token cannot be "
+                             f"written there (fork it at {num_tokens} tokens first)")
         if len(self.free_slots) < len(beam_ids):
             raise RuntimeError(f"more than max_seqs={self.max_seqs} sequences hold blocks")
         if self.free < (len(beam_ids) if num_tokens % block_size else 0):

@@ -402,3 +402,24 @@ def test_a_reordering_inside_a_shared_block_would_write_others_tokens():
     assert m.may_reorder([0, 1, 2], 8) and not m.may_reorder([0, 1, 2], 6)
     copies = m.reorder([0, 1, 2], [0, 0, 0], 6)[1]
     assert len({d for _, d, _ in copies}) == 1 < len(copies)
+
+
+def test_beams_do_not_start_inside_a_shared_block():
+    """A fork of a whole block, taken as holding fewer tokens: beam 0 would append into the block of its parent."""
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    led = BlockLedger(20, 8, 4)
+    led.allocate(0, 2)
+    led.fork(0, 1, 8, 4)
+    for tokens in (5, 7):
+        with pytest.raises(ValueError, match="another sequence holds"):
+            led.fork_beams(1, ["a"], tokens, 4)
+    with pytest.raises(ValueError, match="another sequence holds"):
+        led.fork_beams(0, ["a"], 6, 4)  # the parent neither
+    assert led.shared_columns(0) == led.shared_columns(1) == 2 and not led.beams and len(led.take_ops()) == 2
+    led.fork(1, 2, 6, 4)                # a copy of the last block is its own
+    assert led.shared_columns(2) == 1 and led.fork_beams(2, ["a"], 6, 4) is AllocStatus.SUCCESS
+    assert led.fork_beams(1, ["b"], 8, 4) is AllocStatus.SUCCESS  # whole blocks: the next token opens a new one
+    led.release_beams(1)
+    led.release_beams(2)
+    assert led.shared_columns(0) == 0 and led.fork_beams(0, ["a"], 6, 4) is AllocStatus.SUCCESS  # alone again
