@@ -52,6 +52,7 @@ class BeamSearch:
         dev = pool.free_top.device
         i32 = dict(dtype=torch.int32, device=dev)
         self.num_tokens = torch.tensor(self.host_tokens, dtype=torch.int32).to(dev)
+        self.status = torch.zeros(1, **i32)  # of the search's own launches, read by finish
         self.max_new = int(max_new_tokens)
         self.history = torch.empty(2, self.max_new, B, K, **i32)  # tokens and parents of every step
         self.q_len = torch.ones(B * K, **i32)
@@ -117,7 +118,7 @@ class BeamSearch:
                    kv_len=(self.num_tokens + 1).repeat_interleave(self.K), cu_seqlens=self.cu,
                    positions=torch.empty(S, **i32), token_seq=torch.empty(S, **i32))
         pool.step_rows(self.slots.view(-1), self.q_len, out["kv_len"], self.cu, S, out["block_table"],
-                       out["num_blocks_per_seq"], out["positions"], out["token_seq"], pool.status)
+                       out["num_blocks_per_seq"], out["positions"], out["token_seq"], self.status)
         return out
 
     def advance(self, logits: torch.Tensor) -> torch.Tensor:
@@ -129,7 +130,7 @@ class BeamSearch:
         parents = self._choose(logits)
         self.num_tokens += 1
         self.host_tokens = [n + 1 for n in self.host_tokens]
-        self.slots = self.pool.reorder_beams(self.slots, parents, self.num_tokens)
+        self.slots = self.pool.reorder_beams(self.slots, parents, self.num_tokens, self.status)
         self._room = False
         return self.tokens
 
@@ -138,7 +139,11 @@ class BeamSearch:
         return bool(self.finished.all().item())
 
     def finish(self) -> list[list[tuple[float, list[int]]]]:
-        """End the search and free its blocks: each sequence's (score, new tokens), best first, without what follows eos."""
+        """End the search and free its blocks: each sequence's (score, new tokens), best first, without what follows eos.
+
+        IndexError if a step did not fit the pool (a reordering that left a group as it was, a row without an entry): the
+        beams' cache and their tokens were out of step from there on, so there are no lines to return.
+        """
         tokens, parents = self.history[:, :self.steps].cpu().tolist()
         scores = self.scores.cpu().tolist()
         if not self._ended:
@@ -146,6 +151,7 @@ class BeamSearch:
                 self.pool.release_beams(s)
             self.pool.flush()
             self._ended, self._room = True, False
+        ops._raise_status_value("beam search", int(self.status.item()))
         found = []
         for b in range(self.B):
             beams = []

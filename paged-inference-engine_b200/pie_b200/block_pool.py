@@ -374,9 +374,9 @@ class DeviceBlockManager:
             raise ValueError("attach_caches() names the pools whose pages are to be moved")
         return self._cache_descs
 
-    def _checked(self, fn: str) -> None:
+    def _checked(self, fn: str, status: Optional[torch.Tensor] = None) -> None:
         if ops._CHECK:
-            ops._raise_status(fn, self.status)
+            ops._raise_status(fn, self.status if status is None else status)
 
     def _copies_first(self) -> None:
         """A released block may be handed out again: the copies queued so far read their pages before that."""
@@ -426,8 +426,11 @@ class DeviceBlockManager:
         rows = [[self.ledger.row(b) for b in self.ledger.beams[s]] for s in seq_ids]
         return torch.tensor(rows, dtype=torch.int32).to(self.device)
 
-    def reorder_beams(self, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor) -> torch.Tensor:
+    def reorder_beams(self, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor,
+                      status: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Beam j of group g continues beam ``parents[g, j]``: returns the beams' rows afterwards (``ops.reorder_beams``).
+
+        What does not fit is left as it is and reported in ``status`` (int32 [1] on the device; the manager's by default).
 
         Which blocks became free only the device knows; ``num_free_blocks`` counts them when the beams are
         released.  From now on only the returned rows name the beams: their ids are refused by ``slot_of``,
@@ -438,8 +441,8 @@ class DeviceBlockManager:
         self.flush()
         self.ledger.beams_moved()
         out = ops._reorder_call(self._desc, self._share, descs, self.free_top.device, ops._i32(slots), ops._i32(parents),
-                                ops._i32(num_tokens), self.status)
-        self._checked("reorder_beams")
+                                ops._i32(num_tokens), self.status if status is None else status)
+        self._checked("reorder_beams", status)
         return out
 
     def release_beams(self, seq_id: int) -> AllocStatus:

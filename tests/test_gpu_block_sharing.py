@@ -617,3 +617,33 @@ def test_reorder_refuses_tokens_inside_a_shared_block(ops):  # noqa: F811
         assert not copies
     assert got.tolist() == after and st.item() == 0
     pool_equals(pool, m)
+
+
+@pytest.mark.parametrize("wrong,refused", [(1000, True), (-5, True), (-3, False), (0, False)])
+def test_a_search_that_left_the_pool_behind_returns_no_lines(wrong, refused):
+    """A reordering that leaves a group as it is (the token count does not fit the rows): finish says so, and frees.
+
+    The second sequence is at 8 tokens then, in blocks of 4: 3 tokens end inside the first block, which its beams share,
+    5 inside the second, of which each has its own.
+    """
+    from pie_b200.beam import BeamSearch
+
+    dm = manager(NB=40, seqs=12, cols=6)
+    dm.allocate(0, 2)
+    dm.allocate(1, 2)
+    x = torch.randn(2, 30, device="cuda")
+    dm.status.fill_(2)  # of something else: not the search's
+    search = BeamSearch(dm, [0, 1], [7, 6], x, 3, 0, 9)
+    for step in range(3):
+        search.step_inputs()
+        if step == 1:
+            search.num_tokens[1] += wrong
+        search.advance(torch.randn(2, 3, 30, device="cuda"))
+    if refused:
+        for _ in range(2):
+            with pytest.raises(IndexError, match="beam search"):
+                search.finish()
+    else:
+        assert [len(b) for b in search.finish()] == [3, 3]
+    dm.flush()
+    assert dm.num_free_blocks() == 40 == dm.free_top.item() and dm.status.item() == 2
