@@ -529,8 +529,10 @@ int block_pool_compact(const pa_block_pool_t* pool, const pa_block_share_t* shar
  *   finished  uint8 [num_seqs, num_beams] or NULL: a finished beam's logits are
  *             not read; its log-probabilities are 0 at eos_id and -inf elsewhere
  * Sums are held in fp32 per part of a row and joined in 64 bits; scores are compared
- * in 64 bits and rounded once to fp32.
- * Limits: num_beams <= 32, num_out <= min(32, num_beams * vocab), vocab <= 2^30.
+ * in 64 bits and rounded once to fp32.  A row's log-sum is good to 2.2e-5, whatever
+ * its length: a part has at most 2^17 logits (fp32) or 2^18 (16 bits).
+ * Limits: num_beams <= 32, num_out <= min(32, num_beams * vocab), vocab <=
+ * floor(8192 / (num_beams * num_out)) parts (2^20 logits at 32 x 32 in fp32) and <= 2^30.
  */
 typedef struct {
   const void* logits;

@@ -46,6 +46,7 @@ constexpr int kLogLaneRuns = 2;
 constexpr int kChunkRuns = 32 * kLaneRuns;
 constexpr int kUnitRuns = kRowWarps * kChunkRuns;  // a chunk of every warp: the grain in which rows are split
 constexpr int kStages = 2;             // chunks of a warp in shared memory
+constexpr int kPartUnits = 32;         // units of a part at most: a thread's sum is rounded, and perhaps rescaled, once a unit
 constexpr int kSpans = 8;              // a thread's units are remembered in so many spans, by their maxima
 constexpr int kHits = kRowWarps * kMaxBeamOut;  // logits at T that a part may have; with more its warps keep sorted lists
 constexpr int kMergeThreads = 512;
@@ -577,7 +578,17 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPar
 
 // Parts of a row: the number that leaves the fewest SMs idle at the rows
 // kernel's end, with a unit's time added to each part for its selection; the
-// merge's shared memory bounds it.
+// merge's shared memory bounds it, and the sums' accuracy asks for enough.  With U
+// units a thread's sum is rounded U + 23 times (10 in a unit, 13 where threads
+// and warps are joined) by 2^-24 of its size and rescaled U + 1 times with 2^-22
+// more; exponentials and their arguments add 113 times 2^-24.  6 U + 141 of
+// those are 2e-5 for U = 32.
+long long beam_vocab_limit(int beams, int num_out, int dtype) {
+  const int per = dtype == PA_DTYPE_F32 ? 4 : 8;
+  const long long most = (kMergeKeys / (static_cast<long long>(beams) * num_out)) * kPartUnits * kUnitRuns * per;
+  return most < 1 << 30 ? most : 1 << 30;
+}
+
 void beam_plan(BeamParams& p, int dtype) {
   const int per = dtype == PA_DTYPE_F32 ? 4 : 8;
   const long long rows = static_cast<long long>(p.seqs) * p.beams;
@@ -586,10 +597,11 @@ void beam_plan(BeamParams& p, int dtype) {
   const long long slots = static_cast<long long>(kRowCtas) * device_sm_count();
   const long long fit = kMergeKeys / (static_cast<long long>(p.beams) * p.num_out);
   long long least = 0;
-  for (long long parts = 1; parts <= units && parts <= fit; ++parts) {
+  const long long fewest = (units + kPartUnits - 1) / kPartUnits;
+  for (long long parts = fewest; parts <= units && parts <= fit; ++parts) {
     const long long share = (units + parts - 1) / parts, used = (units + share - 1) / share;
     const long long cost = (rows * used + slots - 1) / slots * (share + 1);
-    if (parts == 1 || cost < least) {
+    if (parts == fewest || cost < least) {
       least = cost;
       p.part_units = static_cast<int>(share);
       p.parts = static_cast<int>(used);

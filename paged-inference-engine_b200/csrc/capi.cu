@@ -1201,7 +1201,10 @@ static int beam_params(const pa_beam_select_t* a, pa::BeamParams& p, size_t& byt
   if (a->finished && (a->eos_id < 0 || a->eos_id >= a->vocab))
     return fail(PA_ERR_INVALID, "eos_id %d is outside the vocabulary", a->eos_id);
   if (a->stride_seq < 0 || a->stride_beam < 0) return fail(PA_ERR_INVALID, "beam_select: negative strides");
-  if (a->vocab > 1 << 30) return fail(PA_ERR_UNSUPPORTED, "vocab %d exceeds 2^30", a->vocab);
+  const long long most = pa::beam_vocab_limit(a->num_beams, a->num_out, a->dtype);
+  if (a->vocab > most)
+    return fail(PA_ERR_UNSUPPORTED, "vocab %d exceeds %lld, the limit for %d beams and %d outputs", a->vocab, most,
+                a->num_beams, a->num_out);
   const long long rows = static_cast<long long>(a->num_seqs) * a->num_beams;
   if (rows > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "beam_select: too many rows");
   p = pa::BeamParams{};

@@ -213,6 +213,7 @@ struct BeamParams {
   int* out_tokens;
   int* out_parents;
 };
+long long beam_vocab_limit(int beams, int num_out, int dtype);
 void beam_plan(BeamParams& p, int dtype);  // sets row_units, part_units, parts and log_span
 cudaError_t launch_beam_select(const BeamParams& p, int dtype, cudaStream_t stream);
 

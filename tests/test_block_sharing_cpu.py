@@ -423,3 +423,26 @@ def test_beams_do_not_start_inside_a_shared_block():
     led.release_beams(1)
     led.release_beams(2)
     assert led.shared_columns(0) == 0 and led.fork_beams(0, ["a"], 6, 4) is AllocStatus.SUCCESS  # alone again
+
+
+@pytest.mark.parametrize("dtype,part", [(3, 2**17), (0, 2**18), (1, 2**18)])
+@pytest.mark.parametrize("beams,out", [(32, 32), (4, 8), (1, 1), (8, 16), (3, 7)])
+def test_parts_are_short_enough_for_the_sums(dtype, part, beams, out):
+    """A thread's fp32 sum takes one addition, and perhaps one rescaling, for each unit of its part: 32 at most."""
+    from pie_b200 import _lib
+
+    lib, n = _lib.load(), ctypes.c_size_t(0)
+    most = min(2**30, 8192 // (beams * out) * part)
+    for seqs in (1, 700):
+        for vocab in (out, 50257, 131072, 262144, part + 1, 5 * part, most - 1, most):
+            if vocab > most:
+                continue
+            a = _lib.PaBeamSelect(dtype=dtype, num_seqs=seqs, num_beams=beams, vocab=vocab, num_out=out, eos_id=-1)
+            assert lib.beam_select_workspace_size(a, ctypes.byref(n)) == _lib.PA_OK
+            parts, rest = divmod(n.value, seqs * beams * (8 * out + 8))
+            assert rest == 0 and -(-vocab // part) <= parts <= 8192 // (beams * out), (vocab, parts)
+    if most < 2**30:
+        for vocab in (most + 1, 2**30):
+            a = _lib.PaBeamSelect(dtype=dtype, num_seqs=1, num_beams=beams, vocab=vocab, num_out=out, eos_id=-1)
+            assert lib.beam_select_workspace_size(a, ctypes.byref(n)) == _lib.PA_ERR_UNSUPPORTED
+            assert str(most).encode() in lib.paged_attn_error_string()
