@@ -289,3 +289,110 @@ def test_compiled_call_with_odd_outputs():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     torch.library.opcheck(op.default if hasattr(op, "default") else op, (x, s, 3, None, -1),
                           test_utils=("test_schema", "test_faketensor"))
+
+
+# ---- parts of several units ------------------------------------------------------------
+# With many rows a row has few parts, and a part several units (a unit: 4096 logits in fp32, 8192 in 16 bits).
+LONG = [  # seqs, beams, vocab, out, units of a part in fp32 and in 16 bits at least
+    (6, 16, 65536, 32, 2, 2), (760, 1, 33001, 4, 3, 2), (33, 16, 113435, 26, 7, 7), (32, 32, 152064, 16, 10, 10),
+    (1, 32, 2**20, 32, 32, 16), (1, 32, 2**20 - 5, 32, 32, 16)]
+
+
+def _part_units(dtype, B, K, V, n):
+    import ctypes
+
+    from pie_b200 import _lib
+
+    lib, size = _lib.load(), ctypes.c_size_t(0)
+    a = _lib.PaBeamSelect(dtype={torch.float32: 3, torch.float16: 0, torch.bfloat16: 1}[dtype], num_seqs=B, num_beams=K,
+                          vocab=V, num_out=n, eos_id=-1)
+    assert lib.beam_select_workspace_size(a, ctypes.byref(size)) == 0
+    unit = 4096 if dtype == torch.float32 else 8192
+    return -(-(-(-V // unit)) // (size.value // (B * K * (8 * n + 8))))
+
+
+def _check_each(got, x, s, n, seqs=None, finished=None, eos=-1):
+    """Every output scored again in 64 bits: its own score and the column's best must both be the returned one."""
+    B, K, V = x.shape
+    score, token, parent = got
+    assert score.shape == token.shape == parent.shape == (B, n)
+    assert (0 <= token).all() and (token < V).all() and (0 <= parent).all() and (parent < K).all()
+    for b in range(B) if seqs is None else seqs:
+        y = x[b].double().nan_to_num(nan=-np.inf, posinf=torch.finfo(torch.float32).max, neginf=-np.inf)
+        top = y.amax(-1, keepdim=True)
+        lp = y - torch.where(top.isinf(), 0.0, top)
+        lp = torch.where(top.isinf(), -np.inf, lp - lp.exp().sum(-1, keepdim=True).log())
+        if finished is not None:
+            one = torch.full((V,), -np.inf, dtype=torch.float64, device=x.device)
+            one[eos] = 0
+            lp = torch.where(finished[b].bool()[:, None], one, lp)
+        total = (s[b].double()[:, None] + lp).nan_to_num(nan=-np.inf, posinf=np.inf, neginf=-np.inf).flatten()
+        want = total.topk(n).values
+        at = parent[b].long() * V + token[b].long()
+        assert at.unique().numel() == n
+        mine, have = total[at], score[b].double()
+        assert torch.equal(have.isinf(), want.isinf()) and torch.equal(mine.isinf(), want.isinf())
+        some = ~want.isinf()
+        tol = LSE + 2.0**-24 * want.abs()
+        assert ((have - mine).abs()[some] <= tol[some]).all()
+        assert ((have - want).abs()[some] <= tol[some]).all()
+        assert ((want - mine)[some] <= 2 * tol[some]).all()  # no better candidate was left out
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,K,V,n,u32,u16", LONG)
+def test_parts_of_several_units(ops, B, K, V, n, u32, u16, dtype):
+    """Independent logits, rows off 16-byte boundaries, then rising, flat and tied rows and runs of NaN."""
+    assert _part_units(dtype, B, K, V, n) >= (u32 if dtype == torch.float32 else u16)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    few = sorted({0, B // 2, B - 1})
+    s = -torch.rand(B, K, device="cuda", generator=g) * 3
+    R = min(B * K, 48)  # rows that differ; the others repeat them
+    rows = (torch.randn(R, V + 3, device="cuda", generator=g) * 2.5).to(dtype)
+    pick = torch.arange(B * K, device="cuda") % R
+    x = rows[pick].view(B, K, V + 3)
+    _check_each(ops.beam_select(x[..., :V], s, n), x[..., :V], s, n, few)
+    _check_each(ops.beam_select(x[..., 3:], s, n), x[..., 3:], s, n, few)
+    ramp = torch.arange(V, device="cuda", dtype=torch.float64) / V
+    for y in (ramp * 0.5, ramp * 40 - 20, -ramp * 40, torch.zeros_like(ramp), (ramp * 7 * V).long() % 3 * 1.0):
+        y = y.to(dtype).expand(B, K, V)
+        got = _check_each(ops.beam_select(y, s, n), y, s, n, few)
+        if not y[0, 0].any():  # flat: the best beam's lowest tokens
+            best = s.argmax(1, keepdim=True).expand(B, n)
+            assert torch.equal(got[2].long(), best) and torch.equal(got[1], torch.arange(n, device="cuda").int().expand(B, n))
+    z = rows[:1, :V].clone()
+    z[0, 9000:30000] = float("nan")
+    z[0, V - 4000:] = float("nan")
+    z[0, 2:4] = -float("inf")
+    z = z.expand(B, K, V)
+    _check_each(ops.beam_select(z, s, n), z, s, n, few)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_parts_with_finished_beams_and_masks(ops, dtype):
+    """Rows of which a few tokens are allowed, spread over units and parts, beside finished beams."""
+    B, K, V, n, eos = 40, 16, 100003, 20, 77
+    assert _part_units(dtype, B, K, V, n) >= 5
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = (torch.randn(B, K, V, device="cuda", generator=g) * 2).to(dtype)
+    s = -torch.rand(B, K, device="cuda", generator=g) * 3
+    keep = torch.zeros(4, V, dtype=torch.bool, device="cuda")
+    keep[0, torch.randperm(V, device="cuda", generator=g)[:50]] = True
+    keep[1, [5, 60000, V - 1]] = True
+    keep[2] = True
+    keep[3, 70000:70100] = True
+    x.masked_fill_(~keep[torch.arange(B, device="cuda") % 4][:, None], -float("inf"))
+    fin = torch.rand(B, K, device="cuda", generator=g) < 0.3
+    x[3].masked_fill_(x[3].isinf(), torch.finfo(dtype).min)
+    _check_each(ops.beam_select(x, s, n, finished=fin, eos_id=eos), x, s, n, None, fin, eos)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,K,V,n", CASES)
+def test_each_output_is_the_one_it_says(ops, B, K, V, n, dtype):
+    """The identity of every output, the last one's too, by its score from the definition."""
+    g = torch.Generator(device="cuda").manual_seed(B + 17 * V)
+    x = (torch.randn(B, K, V, device="cuda", generator=g) * 3).to(dtype)
+    s = -torch.rand(B, K, device="cuda", generator=g) * 30
+    _check_each(ops.beam_select(x, s, n), x, s, n)
