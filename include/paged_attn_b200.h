@@ -399,7 +399,9 @@ int block_pool_init(const pa_block_pool_t* pool, void* stream);
  *                     entry, or FAILURE when the slot has none
  *                     (BlockManager.release_blocks, :47-57)
  * results (int32 [n_ops], device, may be NULL) receives each status.  One
- * launch; ops and results are device pointers.
+ * launch; ops and results are device pointers.  A pool whose blocks have holder
+ * counts (pa_block_share_t) takes block_pool_apply_sole or _shared instead: this
+ * call leaves the counts as they are.
  */
 int block_pool_apply(const pa_block_pool_t* pool, const int32_t* ops, int32_t n_ops, int32_t* results, void* stream);
 
@@ -464,6 +466,14 @@ int64_t block_pool_scratch_words(int32_t num_blocks);
 
 /* block_pool_init, with no holders and zeroed scratch. */
 int block_pool_init_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, void* stream);
+
+/*
+ * block_pool_apply with the counts kept, for operations on slots none of whose
+ * blocks has another holder, which is the caller's to know: an allocated block
+ * has one holder and a released one none, and no count is read.
+ */
+int block_pool_apply_sole(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* ops, int32_t n_ops,
+                          int32_t* results, void* stream);
 
 /*
  * block_pool_apply with holders counted, ops int32 [n_ops][4] = (kind, slot, n,

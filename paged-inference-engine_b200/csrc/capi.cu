@@ -944,7 +944,7 @@ int block_pool_apply(const pa_block_pool_t* pool, const int32_t* ops, int32_t n_
   if (rc) return rc;
   if (n_ops < 0) return fail(PA_ERR_INVALID, "n_ops < 0");
   if (n_ops > 0 && !ops) return fail(PA_ERR_INVALID, "ops is NULL");
-  cudaError_t e = pa::launch_block_pool_apply(p, ops, n_ops, results, static_cast<cudaStream_t>(stream));
+  cudaError_t e = pa::launch_block_pool_apply(p, ops, n_ops, results, nullptr, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_apply launch");
 }
 
@@ -1103,6 +1103,19 @@ int block_pool_init_shared(const pa_block_pool_t* pool, const pa_block_share_t* 
   if (rc) return rc;
   cudaError_t e = pa::launch_block_pool_init_shared(p, s, share->scratch_words, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_init_shared launch");
+}
+
+int block_pool_apply_sole(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* ops, int32_t n_ops,
+                          int32_t* results, void* stream) {
+  g_err[0] = 0;
+  pa::PoolParams p;
+  pa::ShareParams s;
+  int rc = block_share_check(pool, share, p, s);
+  if (rc) return rc;
+  if (n_ops < 0) return fail(PA_ERR_INVALID, "n_ops < 0");
+  if (n_ops > 0 && !ops) return fail(PA_ERR_INVALID, "ops is NULL");
+  cudaError_t e = pa::launch_block_pool_apply(p, ops, n_ops, results, s.ref, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PA_OK : cuda_fail(e, "block_pool_apply_sole launch");
 }
 
 int block_pool_apply_shared(const pa_block_pool_t* pool, const pa_block_share_t* share, const int32_t* ops,

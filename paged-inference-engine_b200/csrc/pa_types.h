@@ -143,7 +143,7 @@ struct StepParams {
   int* status;
 };
 cudaError_t launch_block_pool_init(const PoolParams& p, cudaStream_t stream);
-cudaError_t launch_block_pool_apply(const PoolParams& p, const int* ops, int n_ops, int* results,
+cudaError_t launch_block_pool_apply(const PoolParams& p, const int* ops, int n_ops, int* results, int* ref,
                                     cudaStream_t stream);
 cudaError_t launch_block_pool_step(const PoolParams& p, const StepParams& s, cudaStream_t stream);
 

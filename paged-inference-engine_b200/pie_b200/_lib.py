@@ -150,6 +150,7 @@ SIGNATURES = {
     "kv_copy_blocks": (ctypes.c_int, [ctypes.POINTER(PaKvCache), _i32, _vp, _vp, _vp, _i32, _vp, _vp]),
     "block_pool_scratch_words": (_i64, [_i32]),
     "block_pool_init_shared": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp]),
+    "block_pool_apply_sole": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp, _i32, _vp, _vp]),
     "block_pool_apply_shared": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp, _i32, _i32, _vp, _vp, _vp, _vp,
                                                _vp]),
     "block_pool_reorder": (ctypes.c_int, [_vp, ctypes.POINTER(PaBlockShare), _vp, _vp, _vp, _i32, _i32, _vp,

@@ -96,6 +96,7 @@ class BlockLedger:
         self.slot: dict[int, int] = {}        # seq_id -> table row
         self.free_slots = list(range(self.max_seqs - 1, -1, -1))
         self.ops: list[tuple[int, ...]] = []
+        self.counted = False                  # a queued operation meets blocks that several sequences hold or held
         self.prefix: dict[int, _Prefix] = {}  # seq_id -> its last shared columns
         self.beams: dict[int, tuple[int, ...]] = {}  # first beam -> all beams of a search
         self.member: dict[int, int] = {}      # beam -> first beam
@@ -123,7 +124,8 @@ class BlockLedger:
 
     def allocate(self, seq_id: int, num_blocks: int) -> tuple[AllocStatus, int, int]:
         """Returns (status, slot, first new column); queues the operation on success."""
-        self._alone(seq_id)
+        if self.member:
+            self._alone(seq_id)
         return self._allocate(seq_id, num_blocks)
 
     def _allocate(self, seq_id: int, num_blocks: int) -> tuple[AllocStatus, int, int]:
@@ -148,7 +150,8 @@ class BlockLedger:
         return AllocStatus.SUCCESS, slot, base
 
     def release(self, seq_id: int) -> AllocStatus:
-        self._alone(seq_id)
+        if self.member:
+            self._alone(seq_id)
         return self._release(seq_id)
 
     def _release(self, seq_id: int) -> AllocStatus:
@@ -157,11 +160,12 @@ class BlockLedger:
         slot = self.slot.pop(seq_id)
         self.ops.append((POOL_RELEASE, slot, 0))
         self.free += self.blocks.pop(seq_id)
-        node = self.prefix.pop(seq_id, None)
+        node = self.prefix.pop(seq_id, None) if self.prefix else None
         while node is not None:  # columns that others hold are not free
             node.holders -= 1
             if node.holders:
                 self.free -= node.n
+                self.counted = True
             node = node.up
         self.free_slots.append(slot)
         return AllocStatus.SUCCESS
@@ -216,6 +220,7 @@ class BlockLedger:
             raise RuntimeError(f"more than max_seqs={self.max_seqs} sequences hold blocks")
         slot = self.slot[child_id] = self.free_slots.pop()
         self.ops.append((POOL_FORK, slot, num_tokens, self.slot[parent_id]))
+        self.counted = True
         self.blocks[child_id] = full + (tail > 0)
         self.free -= tail > 0
         node = self._shared(parent_id, full)
@@ -257,6 +262,7 @@ class BlockLedger:
         self.moved.discard(seq_id)
         for b in beams:
             del self.member[b]
+        self.counted = True
         for b in beams[1:]:
             self._release(b)
 
@@ -275,13 +281,14 @@ class BlockLedger:
         if seq_id not in self.beams:
             return AllocStatus.FAILURE
         self.moved.discard(seq_id)
+        self.counted = True  # a reordering may have given one block to several
         for b in self.beams.pop(seq_id):
             del self.member[b]
             self._release(b)
         return AllocStatus.SUCCESS
 
     def take_ops(self) -> list[tuple[int, ...]]:
-        ops, self.ops = self.ops, []
+        ops, self.ops, self.counted = self.ops, [], False
         return ops
 
 
@@ -335,7 +342,8 @@ class DeviceBlockManager:
 
     def release_blocks(self, seq_id: int) -> AllocStatus:
         """core/block_manager.py:47-57: return ``seq_id``'s blocks (that no other sequence holds) to the free list."""
-        self._copies_first()
+        if self._copies:
+            self._copies_first()
         return self.ledger.release(seq_id)
 
     def num_free_blocks(self) -> int:
@@ -476,16 +484,23 @@ class DeviceBlockManager:
         ``keep_results``: keep the per-call device statuses (``last_results``)
         for checking against the host's decisions.
         """
+        sole = not self.ledger.counted
         ops_list = self.ledger.take_ops()
         if not ops_list:
             return
         n = len(ops_list)
-        host = torch.tensor([(*o, 0)[:4] for o in ops_list], dtype=torch.int32).pin_memory()
+        host = torch.tensor(ops_list if sole else [(*o, 0)[:4] for o in ops_list], dtype=torch.int32).pin_memory()
         dev_ops = host.to(self.device, non_blocking=True)
         res = torch.empty(n, dtype=torch.int32, device=self.device) if keep_results else None
+        lib = _lib.load()
+        if sole:
+            with torch.cuda.device(self.device):
+                _lib.check("block_pool_apply_sole", lib.block_pool_apply_sole(
+                    ctypes.byref(self._desc), ctypes.byref(self._share), dev_ops.data_ptr(), n, ops._ptr(res), self._stream()))
+            self._results = res
+            return
         copies = torch.empty(3, n, dtype=torch.int32, device=self.device) if self._copies else None
         src, dst, slots = (None, None, None) if copies is None else copies
-        lib = _lib.load()
         with torch.cuda.device(self.device):
             _lib.check("block_pool_apply_shared", lib.block_pool_apply_shared(
                 ctypes.byref(self._desc), ctypes.byref(self._share), dev_ops.data_ptr(), n, self.block_size,

@@ -446,3 +446,54 @@ def test_parts_are_short_enough_for_the_sums(dtype, part, beams, out):
             a = _lib.PaBeamSelect(dtype=dtype, num_seqs=1, num_beams=beams, vocab=vocab, num_out=out, eos_id=-1)
             assert lib.beam_select_workspace_size(a, ctypes.byref(n)) == _lib.PA_ERR_UNSUPPORTED
             assert str(most).encode() in lib.paged_attn_error_string()
+
+
+def test_only_batches_that_meet_shared_blocks_are_counted():
+    """A scheduler that shares nothing keeps the plain pool's launch: the ledger says which batches need the counts."""
+    from pie_b200.block_pool import BlockLedger
+
+    led = BlockLedger(60, 12, 6)
+
+    def counted():
+        flag, _ = led.counted, led.take_ops()
+        return flag
+
+    for s in range(4):
+        led.allocate(s, 2)
+    led.release(3)
+    assert not counted()
+    led.fork(0, 10, 8, 4)
+    assert counted()
+    led.allocate(10, 1)           # a block of its own
+    led.release(2)
+    assert not counted()
+    led.release(0)                # the fork still holds its blocks
+    assert counted()
+    led.release(10)               # nobody else does any more
+    assert not counted()
+    led.fork_beams(1, ["b"], 8, 4)
+    assert counted()
+    led.allocate_beams(1, 1)
+    assert not counted()
+    led.release_beams(1)
+    assert counted()
+    led.allocate(1, 2)
+    led.fork_beams(1, ["b"], 8, 4)
+    led.take_ops()
+    led.dissolve_beams(1)
+    assert counted()
+    led.release(1)
+    assert not counted() and led.free == 60
+
+
+def test_sole_batches_validate_without_gpu():
+    from pie_b200 import _lib
+    from pie_b200.block_pool import PaBlockPool
+
+    lib, p, B = _lib.load(), 1 << 21, ctypes.byref
+    d = PaBlockPool(p, p, p, p, 8, 16, 8, 8, 0)
+    s = _lib.PaBlockShare(p, p, lib.block_pool_scratch_words(16))
+    assert lib.block_pool_apply_sole(B(d), B(_lib.PaBlockShare(None, p, 999)), p, 1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_sole(B(d), B(s), None, 1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_sole(B(d), B(s), p, -1, None, None) == _lib.PA_ERR_INVALID
+    assert lib.block_pool_apply_sole(B(d), B(s), p, 0, None, None) == _lib.PA_OK

@@ -647,3 +647,27 @@ def test_a_search_that_left_the_pool_behind_returns_no_lines(wrong, refused):
         assert [len(b) for b in search.finish()] == [3, 3]
     dm.flush()
     assert dm.num_free_blocks() == 40 == dm.free_top.item() and dm.status.item() == 2
+
+
+@pytest.mark.parametrize("NB", [60, 20])
+def test_sole_batches_keep_the_counts(NB):
+    """More operations than a launch stages at once, refused ones among them: statuses, rows and counts as the general call's."""
+    from pie_b200 import _lib
+
+    r, lib = np.random.default_rng(3), _lib.load()
+    rows = [(int(k), int(s), int(n)) for k, s, n in zip(r.choice([0, 0, 1, 5], 700), r.integers(-1, 13, 700), r.integers(-1, 5, 700))]
+    a, b = manager(NB, seqs=12, cols=9), manager(NB, seqs=12, cols=9)
+    res = torch.full((2, len(rows)), -9, dtype=torch.int32, device="cuda")
+    t3, t4 = _i32(rows), _i32([(*x, 0) for x in rows])
+    _lib.check("sole", lib.block_pool_apply_sole(ctypes.byref(a._desc), ctypes.byref(a._share), t3.data_ptr(), len(rows),
+                                                 res[0].data_ptr(), None))
+    _lib.check("shared", lib.block_pool_apply_shared(ctypes.byref(b._desc), ctypes.byref(b._share), t4.data_ptr(), len(rows), 4,
+                                                     res[1].data_ptr(), None, None, None, None))
+    torch.cuda.synchronize()
+    model, want = SharedPool(NB, 12, 9, 4), []
+    for kind, slot, n in rows:
+        ok = kind in (0, 1) and 0 <= slot < 12 and n >= 0
+        want.append(4 if not ok else model.allocate(slot, n) if kind == 0 else model.release(slot))
+    assert res[0].tolist() == res[1].tolist() == want and (1 in want) == (NB == 20)
+    pool_equals(a.state, model)
+    pool_equals(b.state, model)
