@@ -7,7 +7,8 @@ caller's model over them (``write_kv`` and ``paged_attention`` as in any
 decode step), and ``advance(logits)``: ``ops.beam_select`` picks the best
 continuations and ``reorder_beams`` makes the cache follow them: beams share
 their parents' full blocks, partly filled ones are copied.  Nothing is read
-back before ``finish()``.
+back before ``finish()``, unless the pool seems to have no block left for a
+step.
 
 The reference decodes one sampled continuation per sequence
 (core/model_runner.py:28-159) and has no beams.
@@ -97,14 +98,15 @@ class BeamSearch:
     def step_inputs(self) -> dict:
         """Attention inputs of the next token of every beam (row ``b * K + k``), as ``DeviceBlockManager.step_inputs``.
 
-        The new token of a beam of sequence b goes to position ``num_tokens[b]`` and attends to one more key.
+        The new token of a beam of sequence b goes to position ``num_tokens[b]`` and attends to one more key.  Reads
+        nothing back, unless the pool counts too few free blocks: then it looks what the reorderings have freed.
         """
         if self._ended or self.steps >= self.max_new:
             raise RuntimeError(f"the search has ended or was made for {self.max_new} new tokens")
         pool, S = self.pool, self.B * self.K
         if not self._room:
             need = [s for s, n in zip(self.seq_ids, self.host_tokens) if pool.blocks_of(s) * pool.block_size <= n]
-            if pool.num_free_blocks() < len(need) * self.K:
+            if pool.num_free_blocks() < len(need) * self.K and pool.recount() < len(need) * self.K:
                 raise RuntimeError(f"{len(need) * self.K} blocks are needed, {pool.num_free_blocks()} are free")
             if any(pool.blocks_of(s) >= pool.max_blocks_per_seq for s in need):
                 raise RuntimeError(f"a beam would hold more than max_blocks_per_seq={pool.max_blocks_per_seq} blocks")

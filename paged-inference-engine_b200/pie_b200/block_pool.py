@@ -100,6 +100,7 @@ class BlockLedger:
         self.prefix: dict[int, _Prefix] = {}  # seq_id -> its last shared columns
         self.beams: dict[int, tuple[int, ...]] = {}  # first beam -> all beams of a search
         self.member: dict[int, int] = {}      # beam -> first beam
+        self.regained: dict[int, int] = {}    # first beam -> blocks that reorderings freed, as last counted
         self.moved: set = set()               # first beams of searches whose rows the device has permuted
 
     def row(self, seq_id: int) -> int:
@@ -263,6 +264,7 @@ class BlockLedger:
         for b in beams:
             del self.member[b]
         self.counted = True
+        self.free -= self.regained.pop(seq_id, 0)
         for b in beams[1:]:
             self._release(b)
 
@@ -274,6 +276,23 @@ class BlockLedger:
             self._allocate(b, num_blocks)
         return AllocStatus.SUCCESS
 
+    def private_columns(self, seq_id: int) -> tuple[int, int]:
+        """The columns [first, last) in which each beam of the search began with blocks of its own."""
+        first, node = 0, self.prefix.get(self.beams[seq_id][-1])
+        while node is not None:
+            first, node = first + node.n, node.up
+        return first, self.blocks[seq_id]
+
+    def count_beams(self, seq_id: int, held: int) -> None:
+        """The search's beams hold ``held`` different blocks in their private columns: the others count as free.
+
+        Later reorderings only free more of them, and an allocation adds as many blocks here as on the device.
+        """
+        first, last = self.private_columns(seq_id)
+        freed = len(self.beams[seq_id]) * (last - first) - held
+        self.free += freed - self.regained.get(seq_id, 0)
+        self.regained[seq_id] = freed
+
     def release_beams(self, seq_id: int) -> AllocStatus:
         # Reordering keeps each column's blocks within those that the beams
         # held before, so the device never uses more than is counted here, and
@@ -282,6 +301,7 @@ class BlockLedger:
             return AllocStatus.FAILURE
         self.moved.discard(seq_id)
         self.counted = True  # a reordering may have given one block to several
+        self.free -= self.regained.pop(seq_id, 0)
         for b in self.beams.pop(seq_id):
             del self.member[b]
             self._release(b)
@@ -351,6 +371,23 @@ class DeviceBlockManager:
 
     def can_allocate(self, num_blocks: int) -> bool:
         return self.ledger.free >= num_blocks
+
+    def recount(self) -> int:
+        """Count as free what reorderings of beams have freed so far; returns ``num_free_blocks()``.
+
+        Reads the beams' rows (synchronises).  Without it a search's blocks count as its beams held them at their
+        widest, until they are released.
+        """
+        searches = list(self.ledger.beams)
+        if searches:
+            self.flush()
+            rows = [self.ledger.slot[b] for s in searches for b in self.ledger.beams[s]]
+            table = self.table[torch.tensor(rows).to(self.device)].cpu()
+            for s in searches:
+                mine, table = table.split([len(self.ledger.beams[s]), len(table) - len(self.ledger.beams[s])])
+                first, last = self.ledger.private_columns(s)
+                self.ledger.count_beams(s, mine[:, first:last].unique().numel())
+        return self.ledger.free
 
     # ---- shared blocks ------------------------------------------------------
     def attach_caches(self, k_cache: ops.Caches, v_cache: ops.Caches, k_scale: Optional[ops.Caches] = None,
@@ -440,8 +477,8 @@ class DeviceBlockManager:
 
         What does not fit is left as it is and reported in ``status`` (int32 [1] on the device; the manager's by default).
 
-        Which blocks became free only the device knows; ``num_free_blocks`` counts them when the beams are
-        released.  From now on only the returned rows name the beams: their ids are refused by ``slot_of``,
+        Which blocks became free only the device knows; ``num_free_blocks`` counts them at ``recount`` or when the beams
+        are released.  From now on only the returned rows name the beams: their ids are refused by ``slot_of``,
         ``step_inputs`` and ``block_table`` until the search is released.  No host synchronisation: the call can be
         captured (with no queued calls).
         """
@@ -467,6 +504,8 @@ class DeviceBlockManager:
         """
         descs = self._need_caches()
         n = self.num_blocks if num_blocks is None else int(num_blocks)
+        if n < self.num_blocks - self.ledger.free:
+            self.recount()
         used = self.num_blocks - self.ledger.free
         if not used <= n <= self.num_blocks:
             raise ValueError(f"{used} of {self.num_blocks} blocks are in use: the pool cannot have {n}")

@@ -497,3 +497,94 @@ def test_sole_batches_validate_without_gpu():
     assert lib.block_pool_apply_sole(B(d), B(s), None, 1, None, None) == _lib.PA_ERR_INVALID
     assert lib.block_pool_apply_sole(B(d), B(s), p, -1, None, None) == _lib.PA_ERR_INVALID
     assert lib.block_pool_apply_sole(B(d), B(s), p, 0, None, None) == _lib.PA_OK
+
+
+def _recount(led, model):
+    for s in led.beams:
+        first, last = led.private_columns(s)
+        rows = [model.rows[led.slot[b]] for b in led.beams[s]]
+        assert all(len(r) == last for r in rows) and len({tuple(r[:first]) for r in rows}) == 1
+        led.count_beams(s, len({b for r in rows for b in r[first:last]}))
+
+
+def test_ledger_learns_what_reorderings_freed():
+    """One search of 4 beams over 512 new tokens that follow one line: 34 blocks in use, 129 counted before."""
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    NB, BS = 160, 16
+    led, model = BlockLedger(NB, 8, 64), SharedPool(NB, 8, 64, BS)
+    led.allocate(0, 1)
+    led.fork_beams(0, [1, 2, 3], 16, BS)
+    _apply(model, led.take_ops())
+    slots = [led.slot[b] for b in led.beams[0]]
+    for n in range(16, 16 + 512):
+        if n % BS == 0:
+            assert led.allocate_beams(0, 1) is AllocStatus.SUCCESS
+            _apply(model, led.take_ops())
+        slots, _, freed = model.reorder(slots, [0, 0, 0, 0], n + 1)
+        model.push(freed)
+    assert NB - led.free == 129
+    assert led.allocate("other", 60)[0] is AllocStatus.INSUFFICIENT_SPACE
+    _recount(led, model)
+    assert NB - led.free == NB - len(model.stack) == 33
+    assert led.allocate("other", 60)[0] is AllocStatus.SUCCESS
+    led.release_beams(0)
+    _apply(model, led.take_ops())
+    model.check()
+    assert led.free == len(model.stack) == NB - 60 and not led.regained
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_recounted_ledger_is_the_model_and_never_above_it(seed):
+    """Searches that start, share prompts, grow, reorder, are recounted and end at any time, beside plain sequences."""
+    from pie_b200.block_pool import AllocStatus, BlockLedger
+
+    r = random.Random(500 + seed)
+    NB, BS, seqs, cols = 120, 4, 20, 12
+    led, model = BlockLedger(NB, seqs, cols), SharedPool(NB, seqs, cols, BS)
+    groups, plain, nxt = {}, {}, 0
+    for _ in range(400):
+        what = r.random()
+        if what < 0.15 and len(led.blocks) < seqs:
+            n = r.randint(0, 14)
+            if led.allocate(nxt, -(-n // BS))[0] is AllocStatus.SUCCESS:
+                plain[nxt] = n
+            nxt += 1
+        elif what < 0.3 and plain and len(led.blocks) < seqs:
+            s = r.choice(list(plain))
+            n = r.randint(0, plain[s])
+            if led.fork(s, nxt, n, BS)[0] is AllocStatus.SUCCESS:
+                plain[nxt] = n
+            nxt += 1
+        elif what < 0.4 and plain:
+            s, k = r.choice(list(plain)), r.randint(1, 5)
+            if len(led.blocks) + k - 1 <= seqs and (plain[s] % BS == 0 or led.shared_columns(s) <= plain[s] // BS):
+                ids = [(s, j) for j in range(1, k)]
+                if led.fork_beams(s, ids, plain[s], BS) is AllocStatus.SUCCESS:
+                    groups[s] = [[led.slot[b] for b in (s, *ids)], plain.pop(s)]
+        elif what < 0.8 and groups:
+            s = r.choice(list(groups))
+            slots, n = groups[s]
+            if n % BS == 0:
+                if n // BS >= cols or led.allocate_beams(s, 1) is not AllocStatus.SUCCESS:
+                    continue
+                _apply(model, led.take_ops())
+            new, _, freed = model.reorder(slots, [r.randrange(len(slots)) for _ in slots], n + 1)
+            model.push(freed)
+            groups[s] = [new, n + 1]
+        elif what < 0.85 and groups:
+            s = r.choice(list(groups))
+            del groups[s]
+            led.release_beams(s)
+        elif what < 0.92:
+            _apply(model, led.take_ops())
+            _recount(led, model)
+            assert led.free == len(model.stack)
+        elif plain:
+            s = r.choice(list(plain))
+            del plain[s]
+            led.release(s)
+        _apply(model, led.take_ops())
+        model.check()
+        assert 0 <= led.free <= len(model.stack)
+        assert groups or led.free == len(model.stack)

@@ -671,3 +671,43 @@ def test_sole_batches_keep_the_counts(NB):
     assert res[0].tolist() == res[1].tolist() == want and (1 in want) == (NB == 20)
     pool_equals(a.state, model)
     pool_equals(b.state, model)
+
+
+def test_blocks_that_reorderings_freed_can_be_had():
+    """Beams that follow one line hold few blocks: the next step, other sequences and a smaller pool get the others."""
+    from pie_b200.beam import BeamSearch
+    from pie_b200.block_pool import AllocStatus
+
+    dm = manager(NB=24, seqs=12, cols=9)
+    dm.allocate(0, 2)
+    dm.allocate(1, 1)
+    x = torch.full((1, 30), -9.0, device="cuda")
+    x[0, 1:5] = torch.tensor([5.0, 1.0, 0.5, 0.0], device="cuda")
+    pull = x.expand(1, 4, 30).clone()
+    search = BeamSearch(dm, [0], [6], x, 4, 0, 40)
+    other = BeamSearch(dm, [1], [4], x, 2, 0, 40)
+    for step in range(24):  # 6 columns of 4 blocks, were they private: more than there are
+        search.step_inputs()
+        search.scores[:, 1:] -= 1000.0  # the best beam has all children
+        search.advance(pull)
+    other.step_inputs()
+    other.advance(pull[:, :2])
+    assert dm.status.item() == 0 == search.status.item()
+    before = dm.num_free_blocks()
+    assert dm.recount() == dm.free_top.item() == dm.num_free_blocks() >= before
+    assert dm.recount() == dm.free_top.item()  # again: the same
+    spare = dm.num_free_blocks()
+    assert spare >= 8 and dm.allocate("late", spare - 6).status is AllocStatus.SUCCESS
+    for _ in range(2):
+        search.step_inputs()
+        search.scores[:, 1:] -= 1000.0
+        search.advance(pull)
+    with pytest.raises(ValueError, match="in use"):
+        dm.compact(3)
+    used = 24 - dm.recount()
+    assert dm.compact(used + 1).item() == used and dm.num_free_blocks() == dm.free_top.item() == 1
+    search.finish()
+    assert dm.num_free_blocks() <= dm.free_top.item()
+    other.finish()
+    dm.release_blocks("late")
+    assert dm.num_free_blocks() == used + 1 == len(dm.free_list()) and not dm.ref_count.any() and not dm.block_table
