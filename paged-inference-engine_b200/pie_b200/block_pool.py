@@ -400,6 +400,8 @@ class DeviceBlockManager:
         if descs[0].block_size != self.block_size or descs[0].num_blocks < self.num_blocks:
             raise ValueError(f"the caches hold {descs[0].num_blocks} blocks of {descs[0].block_size} tokens, "
                              f"the manager hands out {self.num_blocks} of {self.block_size}")
+        # what the page copies cannot move is refused here, not by the flush that has already applied a fork
+        _lib.check("attach_caches", _lib.load().kv_copy_blocks(descs, len(descs), None, None, None, 0, None, None))
         lists = [list(ops._layers(c)) for c in (k_cache, v_cache, k_scale, v_scale)]
         if lists[0][0].device.type != "cuda" or lists[0][0].device != self.free_top.device:
             raise ValueError(f"the caches are on {lists[0][0].device}, the pool on {self.free_top.device}")

@@ -588,3 +588,27 @@ def test_recounted_ledger_is_the_model_and_never_above_it(seed):
         model.check()
         assert 0 <= led.free <= len(model.stack)
         assert groups or led.free == len(model.stack)
+
+
+@pytest.mark.parametrize("shape,layers,why", [
+    ((20, 12, 2, 64), None, "power of two"), ((20, 4, 2, 96), None, "head_dim"), ((20, 4, 2, 64), (20, 4, 4, 64), "layer 1"),
+    ((20, 4, 2, 64), (20, 4, 2, 128), "layer 1"), ((20, 4, 2, 67), None, "strides")])
+def test_caches_that_cannot_be_copied_are_refused_when_attached(shape, layers, why):
+    """Not at the flush, which had applied the fork on the device and then could not copy its page."""
+    from pie_b200 import _lib
+    from pie_b200.block_pool import BlockLedger
+
+    dm = _host_manager(BlockLedger(20, 8, 4))
+    dm.block_size, dm.caches, dm._cache_descs = shape[1], None, None
+    dm.free_top = torch.zeros(1, dtype=torch.int32)
+
+    def pool(s):
+        t = torch.zeros(s, dtype=torch.float16)
+        return t[..., :64] if s[-1] == 67 else t
+
+    k = [pool(shape)] + ([pool(layers)] if layers else [])
+    with pytest.raises((_lib.PagedAttnError, ValueError), match=why):
+        dm.attach_caches(k, [t.clone() if t.is_contiguous() else t for t in k])
+    assert dm.caches is None and dm._cache_descs is None
+    with pytest.raises(ValueError, match="attach_caches"):
+        dm.fork(0, 1, 5)
