@@ -122,7 +122,8 @@ class DecodeStepGraph:
         """Append one token to each of ``seq_ids`` and attend.
 
         ``seq_lens[i]``: tokens of sequence i including this step's;
-        Beams of a search are refused: they are extended together, by ``BeamSearch``.
+        Beams of a search are refused (they are extended together, by ``BeamSearch``), and so is a position inside a
+        block that a fork shares: it would overwrite the other sequence's token.
         ``q`` [n, Hq, D], ``k_new`` / ``v_new`` [n, Hkv, D] on the device.
         Returns O [n, Hq, D] (float16), a view of the graph's output buffer:
         consume it before the next ``step``.
@@ -130,7 +131,12 @@ class DecodeStepGraph:
         n = len(seq_ids)
         if n > self.S:
             raise ValueError(f"{n} sequences, the graph holds {self.S}")
-        self.pool.ledger.none_is_a_beam(seq_ids)
+        ledger = self.pool.ledger
+        ledger.none_is_a_beam(seq_ids)
+        if ledger.prefix:
+            for sid, ln in zip(seq_ids, seq_lens):
+                if (int(ln) - 1) // self.BS < ledger.shared_columns(int(sid)):
+                    raise ValueError(f"token {int(ln) - 1} of sequence {sid} lies in a block that another sequence holds")
         if self.graphs is None:
             self.capture()
         for sid, ln in zip(seq_ids, seq_lens):

@@ -612,3 +612,27 @@ def test_caches_that_cannot_be_copied_are_refused_when_attached(shape, layers, w
     assert dm.caches is None and dm._cache_descs is None
     with pytest.raises(ValueError, match="attach_caches"):
         dm.fork(0, 1, 5)
+
+
+def test_the_decode_step_writes_no_shared_block():
+    """A sequence rolled back below the point at which it was forked: its next token would be its fork's too."""
+    from pie_b200.block_pool import BlockLedger
+    from pie_b200.decode_step import DecodeStepGraph
+
+    led = BlockLedger(40, 8, 6)
+    led.allocate(0, 3)
+    led.allocate(1, 1)
+    led.fork(0, 5, 9, 4)  # two whole blocks shared, the third copied
+    graph = DecodeStepGraph.__new__(DecodeStepGraph)
+    graph.pool, graph.S, graph.BS = _host_manager(led), 4, 4
+    graph.pool.flush = lambda: (_ for _ in ()).throw(KeyError("the device"))  # what the host lets pass ends here
+    graph.graphs, graph.pool.max_blocks_per_seq = (), 6
+    for ids, lens in (([0], [8]), ([5], [1]), ([1, 5], [4, 7]), ([1, 0], [3, 5])):
+        with pytest.raises(ValueError, match="another sequence holds"):
+            graph.step(ids, lens, None, None, None)
+    for ids, lens in (([0], [9]), ([5], [10]), ([1], [1]), ([0, 5, 1], [12, 9, 2])):
+        with pytest.raises(KeyError, match="the device"):
+            graph.step(ids, lens, None, None, None)
+    led.release(0)
+    with pytest.raises(KeyError, match="the device"):
+        graph.step([5], [3], None, None, None)  # alone again
