@@ -132,7 +132,7 @@ class BeamSearch:
         parents = self._choose(logits)
         self.num_tokens += 1
         self.host_tokens = [n + 1 for n in self.host_tokens]
-        self.slots = self.pool.reorder_beams(self.slots, parents, self.num_tokens, self.status)
+        self.slots = self.pool.reorder_beams(self.slots, parents, self.num_tokens, self.status, self.seq_ids)
         self._room = False
         return self.tokens
 

@@ -110,9 +110,9 @@ class BlockLedger:
                              "device knows their rows (reorder_beams returned them)")
         return self.slot[seq_id]
 
-    def beams_moved(self) -> None:
-        """Beams were reordered, of which searches only the device knows."""
-        self.moved.update(self.beams)
+    def beams_moved(self, seq_ids: Optional[Sequence[int]] = None) -> None:
+        """The beams of these searches were reordered (None: of which ones only the device knows)."""
+        self.moved.update(self.beams if seq_ids is None else [s for s in seq_ids if s in self.beams])
 
     def _alone(self, seq_id: int) -> None:
         if seq_id in self.member:
@@ -474,19 +474,20 @@ class DeviceBlockManager:
         return torch.tensor(rows, dtype=torch.int32).to(self.device)
 
     def reorder_beams(self, slots: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor,
-                      status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      status: Optional[torch.Tensor] = None, seq_ids: Optional[Sequence[int]] = None) -> torch.Tensor:
         """Beam j of group g continues beam ``parents[g, j]``: returns the beams' rows afterwards (``ops.reorder_beams``).
 
         What does not fit is left as it is and reported in ``status`` (int32 [1] on the device; the manager's by default).
 
         Which blocks became free only the device knows; ``num_free_blocks`` counts them at ``recount`` or when the beams
         are released.  From now on only the returned rows name the beams: their ids are refused by ``slot_of``,
-        ``step_inputs`` and ``block_table`` until the search is released.  No host synchronisation: the call can be
+        ``beam_slots``, ``step_inputs`` and ``block_table`` until the search is released.  ``seq_ids`` names the searches
+        whose rows ``slots`` holds; without it that counts for every search of the pool.  No host synchronisation: the call can be
         captured (with no queued calls).
         """
         descs = self._need_caches()
         self.flush()
-        self.ledger.beams_moved()
+        self.ledger.beams_moved(seq_ids)
         out = ops._reorder_call(self._desc, self._share, descs, self.free_top.device, ops._i32(slots), ops._i32(parents),
                                 ops._i32(num_tokens), self.status if status is None else status)
         self._checked("reorder_beams", status)

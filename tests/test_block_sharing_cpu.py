@@ -636,3 +636,20 @@ def test_the_decode_step_writes_no_shared_block():
     led.release(0)
     with pytest.raises(KeyError, match="the device"):
         graph.step([5], [3], None, None, None)  # alone again
+
+
+def test_only_the_searches_that_moved_lose_their_rows():
+    from pie_b200.block_pool import BlockLedger
+
+    led = BlockLedger(40, 8, 6)
+    for s in (0, 1):
+        led.allocate(s, 2)
+        led.fork_beams(s, [(s, 1)], 8, 4)
+    led.beams_moved([0, 77])
+    dm = _host_manager(led)
+    assert dm.slot_of(1) == led.slot[1] and dm.slot_of((1, 1)) == led.slot[(1, 1)]
+    for s in (0, (0, 1)):
+        with pytest.raises(ValueError, match="beam of"):
+            dm.slot_of(s)
+    led.release_beams(0)
+    assert not led.moved
