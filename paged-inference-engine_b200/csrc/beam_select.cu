@@ -8,9 +8,11 @@
 // log-probability 0 at eos_id and -inf elsewhere and is not read.  NaN logits
 // count as -inf, +inf as the largest float.
 //
-// Measured (B200, through the op): 64 x 8 rows of 131072 bf16 logits in 36.0 us
-// (134 MB, 20.6 us of HBM), 6 x 16 rows of 65536 fp16 in 14.8, one sequence of 4
-// rows in 11 (the kernels 5.6 + 5.4).
+// Measured (B200): 64 x 8 rows of 131072 bf16 logits in 36 us (134 MB, 20.6 us of
+// HBM), 6 x 16 rows of 65536 fp16 in 14.7, one sequence of 4 rows of 32000 in 7.3
+// in a captured graph and 12 through the op.  Rows with fewer finite logits than
+// T needs in a part (masks) take a second, slower look: 294 us for the first of
+// these with 50 tokens a row allowed.
 //
 // Bound: every logit is read once, so the floor is rows * vocab * size bytes
 // of HBM; next comes the one exponential per logit (16 a clock and SM: 0.77 of

@@ -8,8 +8,8 @@
 //
 // Integer work on a few kilobytes; the page copies of a reorder are the only
 // large traffic (both bytes of each copied token, once).  64 groups of 8 beams
-// with 4 forks each, 4 layers of 64 KB pages: 26 us for 130 MB (20 us of HBM);
-// one group: 7.5 us, a chain of dependent accesses.
+// with 4 forks each, 4 layers of 64 KB pages: 28 us for 130 MB (20 us of HBM);
+// one group: 6 us, a chain of seven dependent accesses.
 #include "page_copy.cuh"
 
 namespace pa {
@@ -355,8 +355,10 @@ cudaError_t launch_block_pool_reorder(const PoolParams& p, const ShareParams& s,
   const int chunks = !first ? 0 : p.max_blocks_per_seq > kColumns ? (p.max_blocks_per_seq + kColumns - 1) / kColumns : 1;
   // A fork's copies are shared by so many CTAs that all forks together, half of
   // the beams perhaps, fill every SM twice: planning a group costs a CTA more than
-  // 1 us, and partly filled blocks differ in size (64 groups of 8 beams, 4 layers
-  // of 64 KB pages: 34.8 us with 32 CTAs an SM, 30.8 with 16, 33 with 4 to 10).
+  // 1 us, and partly filled blocks differ in size.  With 4, 8, 16 and 32 CTAs an SM:
+  // 64 groups of 8 beams, 4 layers of 64 KB pages 32.0, 30.5, 29.9 and 33.7 us; 16
+  // layers of 32 KB 55.9, 49.5, 49.3 and 50.4; 16 x 6, 4 x 4, 64 x 4 and 1 x 4
+  // within 0.1 us of one another.
   const long long items = g.layers * 2LL * g.parts, forks = static_cast<long long>(r.groups) * (r.beams - 1);
   long long shares = forks ? (16LL * device_sm_count() + forks - 1) / forks : 1;
   shares = shares < items ? shares : items;
