@@ -711,3 +711,97 @@ def test_blocks_that_reorderings_freed_can_be_had():
     other.finish()
     dm.release_blocks("late")
     assert dm.num_free_blocks() == used + 1 == len(dm.free_list()) and not dm.ref_count.any() and not dm.block_table
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_manager_with_searches_follows_the_model(seed):
+    """Plain sequences, forks, searches, recounts and compactions in any order: tables, counts, stack, pages and free blocks."""
+    from pie_b200.block_pool import AllocStatus
+
+    r = random.Random(40 + seed)
+    NB, BS, seqs, cols = 110, 4, 18, 9
+    dm, model = manager(NB, BS, seqs, cols, layers=2), SharedPool(NB, seqs, cols, BS)
+    want = host(dm.caches)
+    plain, groups, nxt, queue = {}, {}, 0, []
+
+    def applied():  # the list model follows the queued calls, in order
+        for op in queue:
+            op()
+        queue.clear()
+
+    def forked(slot, n, parent):
+        st, copy = model.fork(slot, n, parent)
+        assert st == SUCCESS
+        moved(want, [copy] if copy else [])
+
+    for _ in range(220):
+        what = r.random()
+        if what < 0.2 and len(dm.ledger.blocks) < seqs:
+            n = r.randint(0, 14)
+            if dm.allocate(nxt, -(-n // BS)).status is AllocStatus.SUCCESS:
+                plain[nxt] = n
+                queue.append(lambda s=dm.slot_of(nxt), k=-(-n // BS): model.allocate(s, k))
+            nxt += 1
+        elif what < 0.35 and plain and len(dm.ledger.blocks) < seqs:
+            p = r.choice(list(plain))
+            n = r.randint(0, plain[p])
+            if dm.fork(p, nxt, n).status is AllocStatus.SUCCESS:
+                plain[nxt] = n
+                queue.append(lambda s=dm.slot_of(nxt), n=n, p=dm.slot_of(p): forked(s, n, p))
+            nxt += 1
+        elif what < 0.45 and plain:
+            p, k = r.choice(list(plain)), r.randint(1, 4)
+            if len(dm.ledger.blocks) + k - 1 <= seqs and (plain[p] % BS == 0 or dm.ledger.shared_columns(p) <= plain[p] // BS):
+                if dm.fork_beams(p, [(p, j) for j in range(1, k)], plain[p]) is AllocStatus.SUCCESS:
+                    slots = [dm.slot_of(b) for b in dm.ledger.beams[p]]
+                    groups[p] = [slots, plain.pop(p)]
+                    for s in slots[1:]:
+                        queue.append(lambda s=s, n=groups[p][1], q=slots[0]: forked(s, n, q))
+        elif what < 0.75 and groups:  # a step of one search
+            g = r.choice(list(groups))
+            slots, n = groups[g]
+            if n % BS == 0:
+                if n // BS >= cols or dm.allocate_beams(g, 1) is not AllocStatus.SUCCESS:
+                    continue
+                queue += [lambda s=dm.ledger.slot[b]: model.allocate(s, 1) for b in dm.ledger.beams[g]]
+            applied()
+            parents = [r.randrange(len(slots)) for _ in slots]
+            out = dm.reorder_beams(_i32([slots]), _i32([parents]), _i32([n + 1]))
+            new, copies, freed = model.reorder(slots, parents, n + 1)
+            model.push(freed)
+            moved(want, copies)
+            assert out.tolist() == [new]
+            groups[g] = [new, n + 1]
+        elif what < 0.82 and groups:
+            g = r.choice(list(groups))
+            rows = [dm.ledger.slot[b] for b in dm.ledger.beams[g]]
+            del groups[g]
+            assert dm.release_beams(g) is AllocStatus.SUCCESS
+            queue += [lambda s=s: model.release(s) for s in rows]
+        elif what < 0.9 and plain:
+            p = r.choice(list(plain))
+            del plain[p]
+            queue.append(lambda s=dm.slot_of(p): model.release(s))
+            assert dm.release_blocks(p) is AllocStatus.SUCCESS
+        elif what < 0.95:
+            dm.recount()
+            dm.flush()
+            applied()
+            assert dm.num_free_blocks() == len(model.stack) == dm.free_top.item()
+        else:
+            dm.compact()
+            applied()
+            moved(want, [(s, d, BS) for s, d in model.compact()[1]])
+        if r.random() < 0.2:
+            dm.flush()
+            applied()
+            model.check()
+            pool_equals(dm.state, model)
+            same(dm.caches, want)
+            assert dm.num_free_blocks() <= len(model.stack)
+    for g in list(groups):
+        dm.release_beams(g)
+    for p in plain:
+        dm.release_blocks(p)
+    dm.flush()
+    assert dm.num_free_blocks() == NB == dm.free_top.item() and not dm.ref_count.any() and dm.status.item() == 0
