@@ -13,7 +13,8 @@ the padded table live in device memory:
   which sequences hold blocks (the decisions the reference makes,
   core/block_manager.py:32-33,49-50); the block ids themselves exist only on
   the device.  Calls are queued and applied in order by one launch at
-  ``flush()`` (``block_pool_apply``), so a scheduler step costs one launch and
+  ``flush()`` (``block_pool_apply_sole``, or ``_shared`` where a call meets
+  shared blocks), so a scheduler step costs one launch and
   one small host-to-device copy, whatever the number of calls.
 * ``step_inputs(...)`` builds a step's attention inputs on the device
   (``block_pool_step``): the zero-padded block table and ``num_blocks_per_seq``
@@ -29,7 +30,8 @@ holders (``ref_count``); a block is written only while one sequence holds it:
   the full blocks are shared, a partly filled last one is copied in every layer
   of the caches named by ``attach_caches``;
 * ``fork_beams`` / ``allocate_beams`` / ``reorder_beams`` / ``release_beams``
-  keep the beams of a beam search, whose parents only the device knows;
+  keep the beams of a beam search, whose parents only the device knows, and
+  ``recount`` learns which blocks its reorderings have freed;
 * ``compact`` moves the blocks in use to the lowest ids.
 """
 from __future__ import annotations
