@@ -346,6 +346,41 @@ int kv_write_copy(const pa_kv_new_t* nw, const pa_kv_cache_t* kv, const pa_pagin
                   void* stream);
 
 /*
+ * Rotary position embedding of new query and key rows, with the write of the
+ * K/V rows into the pool: for the pair (a, b) of a row's dims and the row
+ * cos_sin[position] = (cos of the rot_dim / 2 pairs, then their sin)
+ *   a' = a * cos - b * sin,  b' = b * cos + a * sin
+ * each product and sum rounded to fp32 by itself.  Pairs are the dims i and
+ * i + rot_dim / 2, or with interleaved != 0 the dims 2i and 2i + 1; dims from
+ * rot_dim on stay as they are.  K rows (rotated) and V rows (not) are then
+ * written as kv_write_quant / kv_write_copy write them, in one launch.  The
+ * token's position is both its row of cos_sin and its place in the cache.
+ *   q        [num_tokens, num_q_heads, head_dim] in nw->dtype, written rotated
+ *            to q_out (which may be q); num_q_heads 0: no queries
+ *   cos_sin  fp32 [num_positions, rot_dim], row stride cs_stride
+ * A token whose position is outside cos_sin is left out (PA_STATUS_BAD_POSITION);
+ * one whose K/V rows have no place has its query rows rotated all the same.
+ * Limits: rot_dim a multiple of 16 up to head_dim; rows 16-byte aligned; an INT8
+ * pool needs per-token scales.  The reference has no position embedding in its
+ * attention layer (transformer/model.py:69-122 writes k as projected).
+ */
+typedef struct {
+  const void* q;
+  void* q_out;
+  int64_t q_stride_token, q_stride_head;
+  int64_t qo_stride_token, qo_stride_head;
+  const float* cos_sin;
+  int64_t cs_stride;
+  int32_t num_q_heads;
+  int32_t rot_dim;
+  int32_t num_positions;
+  int32_t interleaved;
+} pa_rotate_t;
+
+int kv_rotate_write(const pa_kv_new_t* nw, const pa_rotate_t* rot, const pa_kv_cache_t* kv, const pa_paging_t* pg,
+                    int32_t* status, void* stream);
+
+/*
  * Device-resident block pool: the free list and every sequence's block list
  * kept in device memory and updated in place, replacing the host allocator
  * and the per-step block-table rebuild of the reference:
@@ -562,6 +597,52 @@ typedef struct {
 
 int beam_select_workspace_size(const pa_beam_select_t* args, size_t* bytes);
 int beam_select(const pa_beam_select_t* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Penalties for repeated tokens, biases and grammar masks on logits: for logit x
+ * of token v in row r, with n the times v stands among the row's generated tokens,
+ *   x = seen(v) ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x = (x - frequency * n) - (n > 0 ? presence : 0)
+ *   x = x + bias[bias_row[r]][v]
+ *   x = -inf where bit v % 32 of mask[mask_row[r]][v / 32] is 0
+ * in fp32, each operation rounded by itself, and rounded once to out_dtype.  The
+ * reference samples from plain logits (core/model_runner.py:28-159).
+ *   logits      [rows, vocab], PA_DTYPE_F32, F16 or BF16, any alignment; NaN stays NaN
+ *               unless it is masked
+ *   out         [rows, vocab], the same type or fp32; may be logits (same strides and type)
+ *   tokens      int32 [rows, max_tokens] or NULL (max_tokens 0): what each row has seen; the
+ *               first prompt_len[r] (NULL: none) are its prompt, which counts as seen but not as
+ *               generated, and those from num_tokens[r] (NULL: max_tokens) on do not count.
+ *               Ids outside 0..vocab-1 do not count.
+ *   repetition, presence, frequency   fp32 [rows], or NULL for the value beside it
+ *   bias        fp32 [bias_rows, vocab] or NULL;  mask  int32 [mask_rows, ceil(vocab / 32)] or NULL
+ *   bias_row, mask_row   int32 [rows], -1: none for this row; NULL: row r, or the only one.
+ *               Another value outside the rows counts as -1 and sets PA_STATUS_BAD_SEQ_INDEX.
+ */
+typedef struct {
+  const void* logits;
+  void* out;
+  int64_t stride_row, out_stride_row;
+  int32_t dtype, out_dtype;
+  int32_t rows, vocab;
+  const int32_t* tokens;
+  int64_t tokens_stride;
+  const int32_t* num_tokens;
+  const int32_t* prompt_len;
+  int32_t max_tokens;
+  float repetition_value, presence_value, frequency_value;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const float* bias;
+  const int32_t* bias_row;
+  const int32_t* mask;
+  const int32_t* mask_row;
+  int64_t bias_stride, mask_stride;
+  int32_t bias_rows, mask_rows;
+} pa_logits_t;
+
+int logits_adjust(const pa_logits_t* args, int32_t* status, void* stream);
 
 /* Message for the last failing call on this thread ("" if none). */
 const char* paged_attn_error_string(void);

@@ -779,6 +779,102 @@ int kv_write_copy(const pa_kv_new_t* nw, const pa_kv_cache_t* kv, const pa_pagin
   return PA_OK;
 }
 
+int kv_rotate_write(const pa_kv_new_t* nw, const pa_rotate_t* rot, const pa_kv_cache_t* kv, const pa_paging_t* pg,
+                    int32_t* status, void* stream) {
+  g_err[0] = 0;
+  pa::WriteParams w;
+  int rc = build_write(nw, kv, pg, status, w);
+  if (rc) return rc;
+  if (!rot) return fail(PA_ERR_INVALID, "rotation descriptor is NULL");
+  if (kv->dtype == PA_DTYPE_I8 && kv->block_size > 1 && (kv->ks_stride_slot == 0 || kv->vs_stride_slot == 0))
+    return fail(PA_ERR_INVALID, "an int8 pool written per token needs per-token scales");
+  if (rot->rot_dim < 16 || rot->rot_dim > kv->head_dim || rot->rot_dim % 16)
+    return fail(PA_ERR_UNSUPPORTED, "rot_dim %d must be a multiple of 16 up to head_dim %d", rot->rot_dim, kv->head_dim);
+  if (rot->num_positions < 0 || rot->num_q_heads < 0) return fail(PA_ERR_INVALID, "kv_rotate_write: negative sizes");
+  if (static_cast<long long>(nw->num_tokens) * (kv->num_kv_heads + static_cast<long long>(rot->num_q_heads)) > (1LL << 26))
+    return fail(PA_ERR_UNSUPPORTED, "rotation of more than 2^26 (token, head) rows in one call");
+  const int e = elt_size(nw->dtype);
+  if (nw->num_tokens > 0) {
+    if (rot->num_positions > 0 && !rot->cos_sin) return fail(PA_ERR_INVALID, "kv_rotate_write: cos_sin is NULL");
+    if (!al(rot->cos_sin, 16) || !row_al(rot->cs_stride, 4, 16) || rot->cs_stride < 0)
+      return fail(PA_ERR_INVALID, "cos_sin rows must be 16-byte aligned");
+    if (rot->num_q_heads > 0) {
+      if (!rot->q || !rot->q_out) return fail(PA_ERR_INVALID, "kv_rotate_write: q or q_out is NULL");
+      if (!al(rot->q, 16) || !al(rot->q_out, 16) || !row_al(rot->q_stride_token, e, 16) ||
+          !row_al(rot->q_stride_head, e, 16) || !row_al(rot->qo_stride_token, e, 16) || !row_al(rot->qo_stride_head, e, 16))
+        return fail(PA_ERR_INVALID, "q rows must be 16-byte aligned (contiguous head_dim)");
+    }
+  }
+  pa::RotateParams r{};
+  r.q = rot->q;
+  r.q_out = rot->q_out;
+  r.q_st = rot->q_stride_token;
+  r.q_sh = rot->q_stride_head;
+  r.qo_st = rot->qo_stride_token;
+  r.qo_sh = rot->qo_stride_head;
+  r.Hq = rot->num_q_heads;
+  r.rot = rot->rot_dim;
+  r.table = rot->cos_sin;
+  r.table_stride = rot->cs_stride;
+  r.num_pos = rot->num_positions;
+  r.pairs = rot->interleaved != 0;
+  cudaError_t ce = pa::launch_kv_rotate(w, r, static_cast<cudaStream_t>(stream));
+  return ce == cudaSuccess ? PA_OK : cuda_fail(ce, "kv_rotate_write launch");
+}
+
+int logits_adjust(const pa_logits_t* a, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  if (!a) return fail(PA_ERR_INVALID, "logits_adjust: NULL descriptor");
+  const int e = a->dtype == PA_DTYPE_I8 ? 0 : elt_size(a->dtype);
+  const int oe = a->out_dtype == PA_DTYPE_F32 || a->out_dtype == a->dtype ? elt_size(a->out_dtype) : 0;
+  if (!e) return fail(PA_ERR_INVALID, "logits dtype must be fp32, fp16 or bf16");
+  if (!oe) return fail(PA_ERR_INVALID, "out dtype must be the logits' or fp32");
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > (1 << 30) || a->max_tokens < 0 || a->bias_rows < 0 || a->mask_rows < 0)
+    return fail(PA_ERR_INVALID, "logits_adjust: sizes out of range");
+  if (a->stride_row < 0 || a->out_stride_row < 0 || a->tokens_stride < 0 || a->bias_stride < 0 || a->mask_stride < 0)
+    return fail(PA_ERR_INVALID, "logits_adjust: negative strides");
+  if (a->rows == 0) return PA_OK;
+  if (!a->logits || !a->out || (a->max_tokens > 0 && !a->tokens)) return fail(PA_ERR_INVALID, "logits_adjust: NULL pointer");
+  if (!al(a->logits, e) || !al(a->out, oe)) return fail(PA_ERR_INVALID, "logits or out misaligned");
+  if (a->out == a->logits && (a->dtype != a->out_dtype || (a->stride_row != a->out_stride_row && a->rows > 1)))
+    return fail(PA_ERR_INVALID, "out over the logits must have their strides and type");
+  if (a->rows > 1 && a->out_stride_row < a->vocab) return fail(PA_ERR_INVALID, "rows of out overlap");
+  if (!a->repetition && !(a->repetition_value > 0.f)) return fail(PA_ERR_INVALID, "repetition penalty must be positive");
+  if (a->bias && !a->bias_row && a->bias_rows != 1 && a->bias_rows != a->rows)
+    return fail(PA_ERR_INVALID, "bias has %d rows for %d rows of logits", a->bias_rows, a->rows);
+  if (a->mask && !a->mask_row && a->mask_rows != 1 && a->mask_rows != a->rows)
+    return fail(PA_ERR_INVALID, "mask has %d rows for %d rows of logits", a->mask_rows, a->rows);
+  pa::LogitsParams p{};
+  p.x = a->logits;
+  p.out = a->out;
+  p.x_stride = a->stride_row;
+  p.out_stride = a->out_stride_row;
+  p.rows = a->rows;
+  p.vocab = a->vocab;
+  p.tokens = a->tokens;
+  p.tokens_stride = a->tokens_stride;
+  p.max_tokens = a->max_tokens;
+  p.num_tokens = a->num_tokens;
+  p.prompt_len = a->prompt_len;
+  p.rep = a->repetition;
+  p.pres = a->presence;
+  p.freq = a->frequency;
+  p.rep_v = a->repetition_value;
+  p.pres_v = a->presence_value;
+  p.freq_v = a->frequency_value;
+  p.bias = a->bias;
+  p.bias_stride = a->bias_stride;
+  p.bias_rows = a->bias_rows;
+  p.bias_row = a->bias_row;
+  p.mask = a->mask;
+  p.mask_stride = a->mask_stride;
+  p.mask_rows = a->mask_rows;
+  p.mask_row = a->mask_row;
+  p.status = status;
+  cudaError_t ce = pa::launch_logits_adjust(p, a->dtype, a->out_dtype, static_cast<cudaStream_t>(stream));
+  return ce == cudaSuccess ? PA_OK : cuda_fail(ce, "logits_adjust launch");
+}
+
 // Decode with the split-K scratch taken from the library's own static device
 // array (see paged_attn_b200.h).  The persistent grid keeps every SM but may use
 // fewer warps per CTA so that the partials fit the fixed scratch.

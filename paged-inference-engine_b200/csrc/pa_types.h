@@ -110,6 +110,47 @@ struct WriteParams {
   int* status;
 };
 
+// Rotation of query and key rows beside the write (csrc/kv_rotate.cu).
+struct RotateParams {
+  const void* q;  // [T, Hq, D], the type of the new rows
+  void* q_out;
+  long long q_st, q_sh, qo_st, qo_sh;
+  int Hq;  // 0: no queries
+  int rot;
+  const float* table;  // [num_pos, rot]: cos of the rot / 2 pairs, then sin
+  long long table_stride;
+  int num_pos;
+  int pairs;  // neighbouring dims make a pair, else dims rot / 2 apart
+};
+cudaError_t launch_kv_rotate(const WriteParams& p, const RotateParams& r, cudaStream_t stream);
+
+// Penalties, biases and masks on logits (csrc/logits_adjust.cu).
+struct LogitsParams {
+  const void* x;
+  void* out;
+  long long x_stride, out_stride;  // elements between rows
+  int rows, vocab;
+  const int* tokens;  // [rows, max_tokens]: what each row has seen, prompt first
+  long long tokens_stride;
+  int max_tokens;
+  const int* num_tokens;  // [rows] or NULL: max_tokens
+  const int* prompt_len;  // [rows] or NULL: 0
+  const float* rep;       // [rows] or NULL: the value beside it
+  const float* pres;
+  const float* freq;
+  float rep_v, pres_v, freq_v;
+  const float* bias;  // [bias_rows, vocab]
+  long long bias_stride;
+  int bias_rows;
+  const int* bias_row;  // [rows] or NULL
+  const int* mask;      // [mask_rows, ceil(vocab / 32)]
+  long long mask_stride;
+  int mask_rows;
+  const int* mask_row;
+  int* status;
+};
+cudaError_t launch_logits_adjust(const LogitsParams& p, int dtype, int out_dtype, cudaStream_t stream);
+
 // Device-resident block pool (csrc/block_pool.cu).
 enum : int { POOL_ALLOC = 0, POOL_RELEASE = 1 };
 enum : int {

@@ -8,6 +8,9 @@
 //                                           K/V rows (transformer/model.py:85-122)
 //   pie_b200::project_write_kv              the K/V projection with that write in
 //                                           its epilogue (transformer/model.py:75-122)
+//   pie_b200::rotate_write_kv               new query and key rows rotated by their
+//                                           positions, K/V rows written
+//   pie_b200::adjust_logits                 penalties, biases and masks on logits
 //   pie_b200::copy_blocks                   page copies inside the pools of all layers
 //   pie_b200::reorder_beams                 beams take over their parents' pool rows
 //   pie_b200::compact_blocks                the blocks in use move to the lowest ids
@@ -75,6 +78,18 @@ void check_i32(const at::Tensor& ref, const at::Tensor& t, const char* name, int
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(), "pie_b200: ", name,
               " must be a contiguous int32 vector");
   TORCH_CHECK_VALUE(t.numel() == n, "pie_b200: ", name, " has ", t.numel(), " entries, expected ", n);
+}
+
+void check_vec(const at::Tensor& ref, const at::Tensor& t, const char* name) {
+  check_device(ref, t, name);
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous(), "pie_b200: ", name, " must be contiguous int32");
+}
+
+void check_status(const at::Tensor& ref, const std::optional<at::Tensor>& status) {
+  if (status.has_value()) {
+    check_vec(ref, *status, "status");
+    TORCH_CHECK_VALUE(status->numel() >= 1, "pie_b200: status holds no word");
+  }
 }
 
 pa_kv_cache_t kv_desc(const at::Tensor& K, const at::Tensor& V, const std::optional<at::Tensor>& ks,
@@ -386,19 +401,165 @@ void project_write_kv(const at::Tensor& x, const at::Tensor& w, const std::optio
   check_rc(kv_project_write(&pj, &kv, &pg, opt_ptr<int32_t>(status), stream), "kv_project_write");
 }
 
-// ---- shared blocks, page copies, beams ---------------------------------------
-void check_vec(const at::Tensor& ref, const at::Tensor& t, const char* name) {
-  check_device(ref, t, name);
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous(), "pie_b200: ", name, " must be contiguous int32");
+pa_kv_new_t new_rows(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& seq_index,
+                     const at::Tensor& positions) {
+  pa_kv_new_t nw{};
+  nw.k_new = ptr(k_new);
+  nw.v_new = ptr(v_new);
+  nw.dtype = pa_dtype(k_new.scalar_type());
+  nw.num_tokens = static_cast<int32_t>(k_new.size(0));
+  nw.k_stride_token = k_new.stride(0);
+  nw.k_stride_head = k_new.stride(1);
+  nw.v_stride_token = v_new.stride(0);
+  nw.v_stride_head = v_new.stride(1);
+  nw.seq_index = static_cast<const int32_t*>(seq_index.data_ptr());
+  nw.positions = static_cast<const int32_t*>(positions.data_ptr());
+  return nw;
 }
 
-void check_status(const at::Tensor& ref, const std::optional<at::Tensor>& status) {
-  if (status.has_value()) {
-    check_vec(ref, *status, "status");
-    TORCH_CHECK_VALUE(status->numel() >= 1, "pie_b200: status holds no word");
+void rotate_write_kv(const std::optional<at::Tensor>& q, const at::Tensor& k_new, const at::Tensor& v_new,
+                     const at::Tensor& cos_sin, bool interleaved, const at::Tensor& block_table,
+                     const at::Tensor& seq_index, const at::Tensor& positions, at::Tensor& k_cache, at::Tensor& v_cache,
+                     const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                     const std::optional<at::Tensor>& status, const std::optional<at::Tensor>& q_out) {
+  TORCH_CHECK_VALUE(k_new.dim() == 3 && v_new.sizes() == k_new.sizes() && v_new.scalar_type() == k_new.scalar_type(),
+                    "pie_b200: k_new / v_new must be [num_tokens, num_kv_heads, head_dim] of equal shape and dtype");
+  TORCH_CHECK_VALUE(k_new.stride(2) == 1 && v_new.stride(2) == 1, "pie_b200: new rows need a contiguous head_dim");
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && k_new.size(1) == k_cache.size(2) && k_new.size(2) == k_cache.size(3),
+                    "pie_b200: new rows do not match the pool's heads");
+  check_device(k_cache, k_new, "k_new");
+  check_device(k_cache, v_new, "v_new");
+  check_device(k_cache, cos_sin, "cos_sin");
+  check_device(k_cache, block_table, "block_table");
+  TORCH_CHECK_VALUE(block_table.scalar_type() == at::kInt && block_table.dim() == 2, "pie_b200: block_table must be int32 2-D");
+  TORCH_CHECK_VALUE(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.stride(1) == 1,
+                    "pie_b200: cos_sin must be float32 [num_positions, rot_dim] with contiguous rows");
+  const int64_t T = k_new.size(0);
+  check_i32(k_cache, seq_index, "seq_index", T);
+  check_i32(k_cache, positions, "positions", T);
+  check_status(k_cache, status);
+  TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "pie_b200: q and q_out come together");
+  pa_rotate_t r{};
+  if (q.has_value()) {
+    check_device(k_cache, *q, "q");
+    check_device(k_cache, *q_out, "q_out");
+    TORCH_CHECK_VALUE(q->dim() == 3 && q->size(0) == T && q->size(2) == k_new.size(2) &&
+                          q->scalar_type() == k_new.scalar_type() && q->stride(2) == 1,
+                      "pie_b200: q must be [num_tokens, num_q_heads, head_dim] in the new rows' dtype");
+    TORCH_CHECK_VALUE(q_out->sizes() == q->sizes() && q_out->scalar_type() == q->scalar_type() && q_out->stride(2) == 1,
+                      "pie_b200: q_out must be shaped and typed like q");
+    r.q = ptr(*q);
+    r.q_out = ptr(*q_out);
+    r.q_stride_token = q->stride(0);
+    r.q_stride_head = q->stride(1);
+    r.qo_stride_token = q_out->stride(0);
+    r.qo_stride_head = q_out->stride(1);
+    r.num_q_heads = static_cast<int32_t>(q->size(1));
   }
+  r.cos_sin = static_cast<const float*>(cos_sin.data_ptr());
+  r.cs_stride = cos_sin.size(0) > 1 ? cos_sin.stride(0) : cos_sin.size(1);
+  r.rot_dim = static_cast<int32_t>(cos_sin.size(1));
+  r.num_positions = static_cast<int32_t>(cos_sin.size(0));
+  r.interleaved = interleaved ? 1 : 0;
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  pa_kv_cache_t kv = kv_desc(k_cache, v_cache, k_scale, v_scale);
+  TORCH_CHECK_VALUE(kv.dtype != PA_DTYPE_I8 || (k_scale->dim() == 3 && v_scale->dim() == 3),
+                    "pie_b200: an int8 pool written per token needs per-token scales [NB, BS, H]");
+  pa_paging_t pg{};
+  pg.block_table = static_cast<const int32_t*>(block_table.data_ptr());
+  pg.bt_stride_seq = block_table.stride(0);
+  pg.bt_stride_col = block_table.stride(1);
+  pg.bt_cols = static_cast<int32_t>(block_table.size(1));
+  pg.num_seqs = static_cast<int32_t>(block_table.size(0));
+  const pa_kv_new_t nw = new_rows(k_new, v_new, seq_index, positions);
+  void* stream = c10::cuda::getCurrentCUDAStream(k_cache.device().index()).stream();
+  check_rc(kv_rotate_write(&nw, &r, &kv, &pg, opt_ptr<int32_t>(status), stream), "kv_rotate_write");
 }
 
+void check_rows(const at::Tensor& ref, const std::optional<at::Tensor>& t, const char* name, at::ScalarType type,
+                int64_t rows) {
+  if (!t.has_value()) return;
+  check_device(ref, *t, name);
+  TORCH_CHECK_VALUE(t->scalar_type() == type && t->dim() == 1 && t->is_contiguous() && t->size(0) == rows, "pie_b200: ",
+                    name, " must be a contiguous vector of ", rows, type == at::kInt ? " int32" : " float32", " values");
+}
+
+void adjust_logits(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                   const std::optional<at::Tensor>& num_tokens, const std::optional<at::Tensor>& prompt_len,
+                   const std::optional<at::Tensor>& repetition, double repetition_value,
+                   const std::optional<at::Tensor>& presence, double presence_value,
+                   const std::optional<at::Tensor>& frequency, double frequency_value,
+                   const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& bias_row,
+                   const std::optional<at::Tensor>& mask, const std::optional<at::Tensor>& mask_row,
+                   const std::optional<at::Tensor>& status, at::Tensor& out) {
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1),
+                    "pie_b200: logits must be a CUDA tensor [rows, vocab] with a contiguous vocabulary");
+  check_device(logits, out, "out");
+  TORCH_CHECK_VALUE(out.sizes() == logits.sizes() && (out.size(1) < 2 || out.stride(1) == 1),
+                    "pie_b200: out must be shaped like logits, with a contiguous vocabulary");
+  const int64_t R = logits.size(0), V = logits.size(1);
+  constexpr int64_t kMost = int64_t{1} << 31;
+  TORCH_CHECK_VALUE(R < kMost && V >= 1 && V <= (int64_t{1} << 30), "pie_b200: logits sizes out of range");
+  check_rows(logits, num_tokens, "num_tokens", at::kInt, R);
+  check_rows(logits, prompt_len, "prompt_len", at::kInt, R);
+  check_rows(logits, repetition, "repetition_penalty", at::kFloat, R);
+  check_rows(logits, presence, "presence_penalty", at::kFloat, R);
+  check_rows(logits, frequency, "frequency_penalty", at::kFloat, R);
+  check_rows(logits, bias_row, "bias_row", at::kInt, R);
+  check_rows(logits, mask_row, "mask_row", at::kInt, R);
+  check_status(logits, status);
+  pa_logits_t a{};
+  a.logits = logits.data_ptr();
+  a.out = out.data_ptr();
+  a.stride_row = logits.stride(0);
+  a.out_stride_row = out.stride(0);
+  a.dtype = pa_dtype(logits.scalar_type());
+  a.out_dtype = pa_dtype(out.scalar_type());
+  a.rows = static_cast<int32_t>(R);
+  a.vocab = static_cast<int32_t>(V);
+  if (tokens.has_value()) {
+    check_device(logits, *tokens, "tokens");
+    TORCH_CHECK_VALUE(tokens->scalar_type() == at::kInt && tokens->dim() == 2 && tokens->size(0) == R &&
+                          tokens->size(1) < kMost && (tokens->size(1) < 2 || tokens->stride(1) == 1),
+                      "pie_b200: tokens must be int32 [", R, ", max_tokens] with contiguous rows");
+    a.tokens = static_cast<const int32_t*>(tokens->data_ptr());
+    a.tokens_stride = tokens->stride(0);
+    a.max_tokens = static_cast<int32_t>(tokens->size(1));
+  }
+  a.num_tokens = opt_ptr<const int32_t>(num_tokens);
+  a.prompt_len = opt_ptr<const int32_t>(prompt_len);
+  a.repetition = opt_ptr<const float>(repetition);
+  a.presence = opt_ptr<const float>(presence);
+  a.frequency = opt_ptr<const float>(frequency);
+  a.repetition_value = static_cast<float>(repetition_value);
+  a.presence_value = static_cast<float>(presence_value);
+  a.frequency_value = static_cast<float>(frequency_value);
+  if (bias.has_value()) {
+    check_device(logits, *bias, "bias");
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->dim() == 2 && bias->size(1) == V && bias->size(0) < kMost &&
+                          (V < 2 || bias->stride(1) == 1),
+                      "pie_b200: bias must be float32 [bias rows, ", V, "] with contiguous rows");
+    a.bias = static_cast<const float*>(bias->data_ptr());
+    a.bias_stride = bias->stride(0);
+    a.bias_rows = static_cast<int32_t>(bias->size(0));
+    a.bias_row = opt_ptr<const int32_t>(bias_row);
+  }
+  if (mask.has_value()) {
+    check_device(logits, *mask, "mask");
+    TORCH_CHECK_VALUE(mask->scalar_type() == at::kInt && mask->dim() == 2 && mask->size(1) == (V + 31) / 32 &&
+                          mask->size(0) < kMost && (mask->size(1) < 2 || mask->stride(1) == 1),
+                      "pie_b200: mask must be int32 [mask rows, ", (V + 31) / 32, "] with contiguous rows");
+    a.mask = static_cast<const int32_t*>(mask->data_ptr());
+    a.mask_stride = mask->stride(0);
+    a.mask_rows = static_cast<int32_t>(mask->size(0));
+    a.mask_row = opt_ptr<const int32_t>(mask_row);
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  void* stream = c10::cuda::getCurrentCUDAStream(logits.device().index()).stream();
+  check_rc(logits_adjust(&a, opt_ptr<int32_t>(status), stream), "logits_adjust");
+}
+
+// ---- shared blocks, page copies, beams ---------------------------------------
 // An uninitialised tensor on the current device's allocator, without a dispatch.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& dev) {
   return at::Tensor(at::detail::empty_cuda(sizes, t, dev, std::nullopt));
@@ -642,6 +803,12 @@ TORCH_LIBRARY(pie_b200, m) {
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
   m.def("project_write_kv(Tensor x, Tensor w, Tensor? bias, Tensor block_table, Tensor seq_index, Tensor positions, "
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
+  m.def("rotate_write_kv(Tensor? q, Tensor k_new, Tensor v_new, Tensor cos_sin, bool interleaved, Tensor block_table, "
+        "Tensor seq_index, Tensor positions, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, "
+        "Tensor(d!)? v_scale, Tensor(s!)? status, Tensor(e!)? q_out) -> ()");
+  m.def("adjust_logits(Tensor logits, Tensor? tokens, Tensor? num_tokens, Tensor? prompt_len, Tensor? repetition, "
+        "float repetition_value, Tensor? presence, float presence_value, Tensor? frequency, float frequency_value, "
+        "Tensor? bias, Tensor? bias_row, Tensor? mask, Tensor? mask_row, Tensor(s!)? status, Tensor(a!) out) -> ()");
   m.def("copy_blocks(Tensor(a!)[] k_caches, Tensor(b!)[] v_caches, Tensor(c!)[] k_scales, Tensor(d!)[] v_scales, "
         "Tensor src, Tensor dst, Tensor? num_slots, Tensor(s!)? status) -> ()");
   m.def("reorder_beams(Tensor(a!) free_stack, Tensor(b!) free_top, Tensor(c!) table, Tensor(d!) count, "
@@ -662,6 +829,8 @@ TORCH_LIBRARY_IMPL(pie_b200, CUDA, m) {
   m.impl("paged_attention_varlen_out", &paged_attention_varlen_out);
   m.impl("write_kv", &write_kv);
   m.impl("project_write_kv", &project_write_kv);
+  m.impl("rotate_write_kv", &rotate_write_kv);
+  m.impl("adjust_logits", &adjust_logits);
   m.impl("copy_blocks", &copy_blocks);
   m.impl("reorder_beams", &reorder_beams);
   m.impl("compact_blocks", &compact_blocks);
@@ -674,6 +843,7 @@ TORCH_LIBRARY_IMPL(pie_b200, Meta, m) {
   m.impl("reorder_beams", &reorder_beams_meta);
   m.impl("compact_blocks", &compact_blocks_meta);
   m.impl("beam_select", &beam_select_meta);
-  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "copy_blocks"})
+  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "rotate_write_kv",
+                         "adjust_logits", "copy_blocks"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&write_only_meta>());
 }

@@ -93,6 +93,29 @@ class PaKvProj(ctypes.Structure):
     ]
 
 
+class PaRotate(ctypes.Structure):
+    """Mirror of pa_rotate_t."""
+
+    _fields_ = [
+        ("q", _vp), ("q_out", _vp), ("q_stride_token", _i64), ("q_stride_head", _i64), ("qo_stride_token", _i64),
+        ("qo_stride_head", _i64), ("cos_sin", _vp), ("cs_stride", _i64), ("num_q_heads", _i32), ("rot_dim", _i32),
+        ("num_positions", _i32), ("interleaved", _i32),
+    ]
+
+
+class PaLogits(ctypes.Structure):
+    """Mirror of pa_logits_t."""
+
+    _fields_ = [
+        ("logits", _vp), ("out", _vp), ("stride_row", _i64), ("out_stride_row", _i64), ("dtype", _i32),
+        ("out_dtype", _i32), ("rows", _i32), ("vocab", _i32), ("tokens", _vp), ("tokens_stride", _i64),
+        ("num_tokens", _vp), ("prompt_len", _vp), ("max_tokens", _i32), ("repetition_value", ctypes.c_float),
+        ("presence_value", ctypes.c_float), ("frequency_value", ctypes.c_float), ("repetition", _vp),
+        ("presence", _vp), ("frequency", _vp), ("bias", _vp), ("bias_row", _vp), ("mask", _vp), ("mask_row", _vp),
+        ("bias_stride", _i64), ("mask_stride", _i64), ("bias_rows", _i32), ("mask_rows", _i32),
+    ]
+
+
 class PaBlockShare(ctypes.Structure):
     """Mirror of pa_block_share_t."""
 
@@ -143,6 +166,9 @@ SIGNATURES = {
                                      _vp, _vp]),
     "kv_project_write": (ctypes.c_int, [ctypes.POINTER(PaKvProj), ctypes.POINTER(PaKvCache),
                                         ctypes.POINTER(PaPaging), _vp, _vp]),
+    "kv_rotate_write": (ctypes.c_int, [ctypes.POINTER(PaKvNew), ctypes.POINTER(PaRotate), ctypes.POINTER(PaKvCache),
+                                       ctypes.POINTER(PaPaging), _vp, _vp]),
+    "logits_adjust": (ctypes.c_int, [ctypes.POINTER(PaLogits), _vp, _vp]),
     "block_pool_init": (ctypes.c_int, [_vp, _vp]),
     "block_pool_apply": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, _vp, _vp]),
     "block_pool_step": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_int64, ctypes.c_int32,

@@ -567,6 +567,106 @@ def project_write_kv(x: torch.Tensor, w_kv: torch.Tensor, bias: Optional[torch.T
         _raise_status("project_write_kv", status)
 
 
+def rope_table(num_positions: int, rot_dim: int, base: float = 10000.0, *, scaling: float = 1.0,
+               device: torch.device | str = "cuda") -> torch.Tensor:
+    """cos and sin of every position's angles, float32 [num_positions, rot_dim], for ``rotate_write_kv``.
+
+    Pair i of position p turns by ``p / scaling * base ** (-2 i / rot_dim)`` (cos of the pairs, then sin; computed
+    in 64 bits).  Any table of this layout will do: other schemes fill it themselves.
+    """
+    if rot_dim < 2 or rot_dim % 2 or num_positions < 0:
+        raise ValueError(f"rot_dim {rot_dim} must be even and positive, num_positions {num_positions} >= 0")
+    freq = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    angle = (torch.arange(num_positions, dtype=torch.float64) / scaling)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+def rotate_write_kv(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch.Tensor, cos_sin: torch.Tensor,
+                    block_table: torch.Tensor, seq_index: torch.Tensor, positions: torch.Tensor,
+                    k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                    v_scale: Optional[torch.Tensor] = None, *, interleaved: bool = False,
+                    q_out: Optional[torch.Tensor] = None,
+                    status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``write_kv`` of keys rotated by their positions; returns ``q`` [T, Hq, D] rotated (None without q).
+
+    ``cos_sin`` float32 [num_positions, rot_dim]: cos of each position's rot_dim / 2 pairs, then sin
+    (``rope_table``).  Pairs are the dims i and i + rot_dim / 2, or with ``interleaved`` 2i and 2i + 1; dims from
+    rot_dim on stay.  ``q``, ``k_new`` and ``v_new`` share a dtype; ``q_out`` may be ``q``.  A token whose position is
+    outside ``cos_sin`` is left out (its row of the result too); see kv_rotate_write in the C header.
+    """
+    if k_new.dim() != 3 or v_new.shape != k_new.shape:
+        raise ValueError("k_new / v_new must be [num_tokens, num_kv_heads, head_dim] of equal shape")
+    T, H, D = k_new.shape
+    if k_cache.dim() != 4 or (H, D) != (k_cache.shape[2], k_cache.shape[3]):
+        raise ValueError(f"new rows [*, {H}, {D}] do not match the pool {tuple(k_cache.shape)}")
+    if k_new.dtype not in (torch.float16, torch.bfloat16, torch.float32) or v_new.dtype != k_new.dtype:
+        raise ValueError("k_new / v_new must share a float16, bfloat16 or float32 dtype")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32:
+        raise ValueError("cos_sin must be float32 [num_positions, rot_dim]")
+    if not 16 <= cos_sin.shape[1] <= D or cos_sin.shape[1] % 16:
+        raise ValueError(f"rot_dim {cos_sin.shape[1]} must be a multiple of 16 up to head_dim {D}")
+    if k_cache.dtype == torch.int8 and (k_scale is None or v_scale is None or k_scale.dim() != 3 or v_scale.dim() != 3):
+        raise ValueError("quantise-on-write stores one scale per (token, head): scales must be [NB, BS, H]")
+    if k_new.stride(2) != 1:
+        k_new = k_new.contiguous()
+    if v_new.stride(2) != 1:
+        v_new = v_new.contiguous()
+    if cos_sin.stride(1) != 1:
+        cos_sin = cos_sin.contiguous()
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    else:
+        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != k_new.dtype:
+            raise ValueError(f"q must be [{T}, num_q_heads, {D}] in {k_new.dtype}")
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+            raise ValueError("q_out must be shaped and typed like q, with a contiguous head_dim")
+    bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    si, ps = _i32(seq_index), _i32(positions)
+    if bt.dim() != 2 or si.numel() != T or ps.numel() != T:
+        raise ValueError("block_table must be 2-D [num_seqs, max_blocks]; seq_index / positions need one entry per token")
+    if status is None and _CHECK:
+        status = status_word(k_cache.device)
+    int8 = k_cache.dtype == torch.int8
+    if BACKEND == "torch":
+        _op("rotate_write_kv")(q, k_new, v_new, cos_sin, bool(interleaved), bt, si.view(-1), ps.view(-1), k_cache, v_cache,
+                               k_scale if int8 else None, v_scale if int8 else None, status, q_out)
+    else:
+        dev = k_cache.device
+        for name, t in (("q", q), ("q_out", q_out), ("k_new", k_new), ("v_new", v_new), ("v_cache", v_cache),
+                        ("cos_sin", cos_sin), ("block_table", bt), ("seq_index", si), ("positions", ps)):
+            if t is not None and t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, the pool on {dev}")
+        kc = kv_cache_desc(k_cache, v_cache, k_scale, v_scale)
+        pg = _lib.PaPaging()
+        pg.block_table = bt.data_ptr()
+        pg.bt_stride_seq, pg.bt_stride_col = bt.stride(0), bt.stride(1)
+        pg.bt_cols, pg.num_seqs = bt.shape[1], bt.shape[0]
+        nw = PaKvNew()
+        nw.k_new, nw.v_new = k_new.data_ptr(), v_new.data_ptr()
+        nw.dtype, nw.num_tokens = _TORCH2PA[k_new.dtype], T
+        nw.k_stride_token, nw.k_stride_head = k_new.stride(0), k_new.stride(1)
+        nw.v_stride_token, nw.v_stride_head = v_new.stride(0), v_new.stride(1)
+        nw.seq_index, nw.positions = si.data_ptr(), ps.data_ptr()
+        r = _lib.PaRotate()
+        if q is not None:
+            r.q, r.q_out, r.num_q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            r.q_stride_token, r.q_stride_head = q.stride(0), q.stride(1)
+            r.qo_stride_token, r.qo_stride_head = q_out.stride(0), q_out.stride(1)
+        r.cos_sin, r.num_positions, r.rot_dim = cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1]
+        r.cs_stride = cos_sin.stride(0) if cos_sin.shape[0] > 1 else cos_sin.shape[1]
+        r.interleaved = int(bool(interleaved))
+        with torch.cuda.device(dev):
+            _lib.check("kv_rotate_write", _lib.load().kv_rotate_write(nw, r, kc, pg, _ptr(status), _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("rotate_write_kv", status)
+    return q_out
+
+
 class PoolState(NamedTuple):
     """The device arrays of a block pool whose blocks sequences share (all int32, see pa_block_share_t).
 
@@ -821,3 +921,116 @@ def beam_select(logits: torch.Tensor, beam_scores: torch.Tensor, num_out: Option
         a.out_scores, a.out_tokens, a.out_parents = scores.data_ptr(), tokens.data_ptr(), parents.data_ptr()
         _lib.check("beam_select", lib.beam_select(a, ws.data_ptr(), nbytes.value, _stream(dev)))
     return scores, tokens, parents
+
+
+Penalty = Union[float, torch.Tensor]
+
+
+def _per_row(name: str, v: Penalty, rows: int, dev: torch.device) -> tuple[Optional[torch.Tensor], float]:
+    if not isinstance(v, torch.Tensor):
+        return None, float(v)
+    if v.numel() != rows or v.device != dev:
+        raise ValueError(f"{name} must be a number or {rows} values on {dev}")
+    return v.to(torch.float32).reshape(rows).contiguous(), 0.0
+
+
+def adjust_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None,
+                  num_tokens: Optional[torch.Tensor] = None, prompt_len: Optional[torch.Tensor] = None,
+                  repetition_penalty: Penalty = 1.0, presence_penalty: Penalty = 0.0, frequency_penalty: Penalty = 0.0,
+                  bias: Optional[torch.Tensor] = None, bias_row: Optional[torch.Tensor] = None,
+                  mask: Optional[torch.Tensor] = None, mask_row: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and grammar masks on ``logits`` [..., V]; returns the new logits.
+
+    Of a row, with n the times that token v was generated: ``x / repetition`` (``x * repetition`` below 0) where v was
+    seen, then ``- frequency * n``, then ``- presence`` where n > 0, then ``+ bias``, then -inf where the mask's bit is
+    clear, in float32 and rounded once to the dtype of ``out`` (by default the logits' own; float32 or ``logits``
+    itself will do).
+
+    ``tokens`` [..., L] (int32) are what each row has seen: the first ``prompt_len`` of them its prompt, which
+    counts as seen but not as generated, those from ``num_tokens`` on nothing, ids outside the vocabulary nothing.
+    A penalty is a number or one value per row.  ``bias`` float32 [N, V] (or [V]) and ``mask`` int32 [M, ceil(V / 32)]
+    (token v: bit v % 32 of word v // 32, 1 = allowed) are one per row, one for all, or chosen by ``bias_row`` /
+    ``mask_row`` (-1: none).  See logits_adjust in the C header.
+    """
+    if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"logits must be float32, float16 or bfloat16 [..., vocab], got {logits.dtype} {tuple(logits.shape)}")
+    V = logits.shape[-1]
+    if V < 1:
+        raise ValueError("logits need a vocabulary")
+    if not isinstance(repetition_penalty, torch.Tensor) and not repetition_penalty > 0:
+        raise ValueError(f"repetition_penalty {repetition_penalty} must be positive")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1:
+        x = x.contiguous()
+    R, dev = x.shape[0], logits.device
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype not in (logits.dtype, torch.float32):
+        raise ValueError("out must be shaped like logits, in their dtype or float32")
+    o = out if out.dim() == 2 else out.view(-1, V)
+    if o.stride(1) != 1 and V > 1:
+        raise ValueError("out needs a contiguous vocabulary")
+    if tokens is not None:
+        if tokens.dim() != logits.dim() or tokens.shape[:-1] != logits.shape[:-1]:
+            raise ValueError(f"tokens must be [{', '.join(map(str, logits.shape[:-1]))}, max_tokens]")
+        tokens = tokens if tokens.dtype == torch.int32 else tokens.to(torch.int32)
+        tokens = tokens if tokens.dim() == 2 else tokens.reshape(R, tokens.shape[-1])
+        if tokens.stride(1) != 1 and tokens.shape[1] > 1:
+            tokens = tokens.contiguous()
+    elif num_tokens is not None or prompt_len is not None:
+        raise ValueError("num_tokens and prompt_len come with tokens")
+    num_tokens, prompt_len, bias_row, mask_row = (t if t is None else _i32(t).view(-1) for t in
+                                                  (num_tokens, prompt_len, bias_row, mask_row))
+    rep, rep_v = _per_row("repetition_penalty", repetition_penalty, R, dev)
+    pres, pres_v = _per_row("presence_penalty", presence_penalty, R, dev)
+    freq, freq_v = _per_row("frequency_penalty", frequency_penalty, R, dev)
+    if bias is not None:
+        bias = (bias if bias.dtype == torch.float32 else bias.float()).view(-1, V) if bias.dim() == 1 else bias.float()
+        if bias.dim() != 2 or bias.shape[1] != V:
+            raise ValueError(f"bias must be [N, {V}] or [{V}]")
+        if bias.stride(1) != 1 and V > 1:
+            bias = bias.contiguous()
+    if mask is not None:
+        mask = mask.view(1, -1) if mask.dim() == 1 else mask
+        if mask.dim() != 2 or mask.dtype != torch.int32 or mask.shape[1] != (V + 31) // 32:
+            raise ValueError(f"mask must be int32 [M, {(V + 31) // 32}] or [{(V + 31) // 32}]")
+        if mask.stride(1) != 1 and mask.shape[1] > 1:
+            mask = mask.contiguous()
+    for name, t, by in (("bias", bias, bias_row), ("mask", mask, mask_row)):
+        if t is None and by is not None:
+            raise ValueError(f"{name}_row without {name}")
+        if t is not None and by is None and t.shape[0] not in (1, R):
+            raise ValueError(f"{name} has {t.shape[0]} rows for {R} rows of logits: pass {name}_row")
+    if status is None and _CHECK:
+        status = status_word(dev)
+    if BACKEND == "torch":
+        _op("adjust_logits")(x, tokens, num_tokens, prompt_len, rep, rep_v, pres, pres_v, freq, freq_v, bias, bias_row, mask,
+                             mask_row, status, o)
+    else:
+        for name, t in (("tokens", tokens), ("num_tokens", num_tokens), ("prompt_len", prompt_len), ("bias", bias),
+                        ("bias_row", bias_row), ("mask", mask), ("mask_row", mask_row), ("out", o), ("status", status)):
+            if t is not None and t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, logits on {dev}")
+        if dev.type != "cuda":
+            raise ValueError("logits must be a CUDA tensor")
+        for name, t in (("num_tokens", num_tokens), ("prompt_len", prompt_len), ("bias_row", bias_row), ("mask_row", mask_row)):
+            if t is not None and t.numel() != R:
+                raise ValueError(f"{name} must hold {R} values")
+        a = _lib.PaLogits()
+        a.logits, a.out, a.stride_row, a.out_stride_row = x.data_ptr(), o.data_ptr(), x.stride(0), o.stride(0)
+        a.dtype, a.out_dtype, a.rows, a.vocab = _TORCH2PA[x.dtype], _TORCH2PA[o.dtype], R, V
+        if tokens is not None:
+            a.tokens, a.tokens_stride, a.max_tokens = tokens.data_ptr(), tokens.stride(0), tokens.shape[1]
+        a.num_tokens, a.prompt_len = _ptr(num_tokens), _ptr(prompt_len)
+        a.repetition, a.presence, a.frequency = _ptr(rep), _ptr(pres), _ptr(freq)
+        a.repetition_value, a.presence_value, a.frequency_value = rep_v, pres_v, freq_v
+        if bias is not None:
+            a.bias, a.bias_stride, a.bias_rows, a.bias_row = bias.data_ptr(), bias.stride(0), bias.shape[0], _ptr(bias_row)
+        if mask is not None:
+            a.mask, a.mask_stride, a.mask_rows, a.mask_row = mask.data_ptr(), mask.stride(0), mask.shape[0], _ptr(mask_row)
+        with torch.cuda.device(dev):
+            _lib.check("logits_adjust", _lib.load().logits_adjust(a, _ptr(status), _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("adjust_logits", status)
+    return out
