@@ -250,6 +250,39 @@ int paged_attn_varlen(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_
                       int32_t total_q_rows, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /*
+ * Decode attention of a batch whose groups share a prefix, which is read once
+ * for a group instead of once for a sequence (the reference attends for every
+ * sequence by itself, kernels/flash_attention.py:38-123).  The sequences
+ * group_start[g] .. group_start[g + 1] - 1 of the batch are group g, and the
+ * first prefix_len[g] keys of all of them are the same: their block tables name
+ * the same blocks there, as block_pool_apply_shared's forks do.  The result is
+ * that of paged_attn_forward up to the order of sums.
+ *   group_start   int32 [num_groups + 1] on the device, rising, within 0..num_seqs
+ *                 (else nothing is shared and PA_STATUS_BAD_SEQ_INDEX is set);
+ *                 sequences outside every group share nothing
+ *   prefix_len    int32 [num_groups] on the device
+ * What a group shares is cut on the device to whole blocks, and to the keys that
+ * every query row of its members sees (members without rows or keys aside); it is read through
+ * the block table of the first member with keys.  A group with fewer than two such members shares nothing.
+ * Rows are masked as in paged_attn_forward with causal_top_left 0.  The keys and values of a block outside
+ * the pool count as zeros (PA_STATUS_BAD_BLOCK_ID).
+ * Limits: max_q_len * (num_q_heads / num_kv_heads) <= 16, num_seqs and num_groups
+ * <= 4096, F16, BF16 or I8 pools.  workspace: >= shared_prefix_workspace_size()
+ * bytes, 256-byte aligned, of this call's own until it has run.
+ */
+typedef struct {
+  const int32_t* group_start;
+  const int32_t* prefix_len;
+  int32_t num_groups;
+  int32_t _reserved;
+} pa_groups_t;
+
+int shared_prefix_workspace_size(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg,
+                                 const pa_groups_t* groups, size_t* bytes);
+int shared_prefix_attn(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg, const pa_groups_t* groups,
+                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
  * Head-sharded decode with the output exchange fused into the attention
  * kernels (the NCCL all-gather of head outputs that follows per-GPU decode in
  * a KV-head-sharded engine; the reference runs on one GPU and has none).

@@ -779,6 +779,127 @@ int kv_write_copy(const pa_kv_new_t* nw, const pa_kv_cache_t* kv, const pa_pagin
   return PA_OK;
 }
 
+// The checks, launch plan and workspace layout of a shared-prefix call.
+namespace {
+struct SharedCall {
+  pa::SharedParams p;
+  pa::KvMaps maps;
+  bool tma;
+  int kvk, nt;
+  pa::DecodeLaunch plan;
+  size_t rec, tile, unit, grp, ml, o, total;
+};
+
+int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg, const pa_groups_t* gr,
+                int32_t* status, SharedCall& c) {
+  pa::AttnParams a;
+  int rc = build_attn(io, kv, pg, status, a);
+  if (rc) return rc;
+  if (!gr) return fail(PA_ERR_INVALID, "groups descriptor is NULL");
+  if (gr->num_groups < 0) return fail(PA_ERR_INVALID, "num_groups < 0");
+  if (a.top_left) return fail(PA_ERR_INVALID, "shared prefixes need the bottom-right mask (causal_top_left 0)");
+  if (kv->dtype == PA_DTYPE_F32) return fail(PA_ERR_UNSUPPORTED, "shared prefixes are read from fp16, bf16 or int8 pools");
+  if (a.maxq * static_cast<long long>(a.G) > kNcMax)
+    return fail(PA_ERR_UNSUPPORTED, "shared prefixes: max_q_len * (num_q_heads / num_kv_heads) must be <= %d", kNcMax);
+  if (a.B > pa::kMaxSharedSeqs || gr->num_groups > pa::kMaxSharedSeqs)
+    return fail(PA_ERR_UNSUPPORTED, "shared prefixes: at most %d sequences and groups", pa::kMaxSharedSeqs);
+  c.total = 0;
+  c.p = pa::SharedParams{};
+  static_cast<pa::AttnParams&>(c.p) = a;
+  if (a.B == 0 || a.maxq == 0) return PA_OK;
+  if (!gr->group_start || (gr->num_groups > 0 && !gr->prefix_len)) return fail(PA_ERR_INVALID, "groups: NULL pointer");
+  // work list indexes are 32-bit: entries of 16 keys, twice a sequence and kv head
+  if (2LL * a.B * a.Hkv * ((static_cast<long long>(a.bt_cols) << a.log2BS) / 16 + 1) > 0x7fffffffLL)
+    return fail(PA_ERR_UNSUPPORTED, "shared prefixes: %d sequences of up to %lld keys on %d kv heads", a.B,
+                static_cast<long long>(a.bt_cols) << a.log2BS, a.Hkv);
+  c.p.group_start = gr->group_start;
+  c.p.prefix_len = gr->prefix_len;
+  c.p.groups = gr->num_groups;
+  const int per = a.maxq * a.G;
+  c.p.cpm = kNcMax / per;
+  c.kvk = kv_kind(kv->dtype);
+  c.p.decode_tile = kv->dtype == PA_DTYPE_I8 ? 32 : 16;
+  c.tma = make_kv_maps(kv, &c.maps);
+  c.p.wide = c.tma && a.B * per > kNcMax && pa::prefix_wide_supported(c.kvk, kv->head_dim, kv->block_size) &&
+             !std::getenv("PIE_B200_NO_TCGEN05");
+  c.p.wide_ctas = pa::device_sm_count();
+  c.nt = c.p.wide ? (per <= 8 ? 1 : 2) : (c.p.cpm * per <= 8 || a.B * per <= 8 ? 1 : 2);
+  {
+    static std::mutex mu;
+    static std::map<std::tuple<int, int, int, int, int, int, int>, pa::DecodeLaunch> cache;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(PA_ERR_CUDA, "no CUDA device");
+    const auto key = std::make_tuple(dev, c.kvk, a.q_bf16, kv->head_dim, c.nt, a.B, static_cast<int>(c.tma));
+    std::lock_guard<std::mutex> lk(mu);
+    auto it = cache.find(key);
+    if (it == cache.end()) {
+      if (pa::prefix_decode_plan(c.kvk, a.q_bf16, kv->head_dim, c.nt, a.B, c.tma, &c.plan) != 0)
+        return fail(PA_ERR_CUDA, "could not plan the shared-prefix launch (no CUDA device?)");
+      cache[key] = c.plan;
+    } else {
+      c.plan = it->second;
+    }
+  }
+  c.p.num_warps_total = c.plan.ctas * c.plan.warps_per_cta;
+  const long long base_rows = static_cast<long long>(a.B) * a.Hkv * per;
+  c.p.prefix_row0 = base_rows + static_cast<long long>(c.p.num_warps_total) * per;
+  const long long rows = c.p.prefix_row0 + base_rows +
+                         (c.p.wide ? static_cast<long long>(c.p.wide_ctas) * pa::kWideRows
+                                   : static_cast<long long>(c.p.num_warps_total) * pa::kChunkCols);
+  c.rec = 0;
+  c.tile = align256(static_cast<size_t>(2) * a.B * sizeof(int4));
+  c.unit = c.tile + align256((static_cast<size_t>(2) * a.B + 1) * sizeof(int));
+  c.grp = c.unit + align256((static_cast<size_t>(gr->num_groups) + 1) * sizeof(int));
+  c.ml = c.grp + align256(static_cast<size_t>(gr->num_groups) * sizeof(int4));
+  c.o = c.ml + align256(static_cast<size_t>(rows) * 2 * sizeof(float));
+  c.total = c.o + align256(static_cast<size_t>(rows) * kv->head_dim * sizeof(float));
+  return PA_OK;
+}
+}  // namespace
+
+int shared_prefix_workspace_size(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg,
+                                 const pa_groups_t* groups, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(PA_ERR_INVALID, "bytes is NULL");
+  *bytes = 0;
+  SharedCall c;
+  const int rc = shared_call(io, kv, pg, groups, nullptr, c);
+  if (rc) return rc;
+  *bytes = c.total;
+  return PA_OK;
+}
+
+int shared_prefix_attn(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg, const pa_groups_t* groups,
+                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  g_err[0] = 0;
+  SharedCall c;
+  const int rc = shared_call(io, kv, pg, groups, status, c);
+  if (rc) return rc;
+  if (c.total == 0) return PA_OK;
+  if (!workspace || workspace_bytes < c.total)
+    return fail(PA_ERR_WORKSPACE, "shared-prefix workspace needs %zu bytes, got %zu", c.total, workspace_bytes);
+  if (!al(workspace, 256)) return fail(PA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  pa::SharedParams& p = c.p;
+  p.rec = reinterpret_cast<int4*>(ws + c.rec);
+  p.tstart = reinterpret_cast<int*>(ws + c.tile);
+  p.unit0 = reinterpret_cast<int*>(ws + c.unit);
+  p.grp = reinterpret_cast<int4*>(ws + c.grp);
+  p.part_ml = reinterpret_cast<float*>(ws + c.ml);
+  p.part_o = reinterpret_cast<float*>(ws + c.o);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = pa::launch_prefix_plan(p, st);
+  if (e != cudaSuccess) return cuda_fail(e, "shared-prefix plan launch");
+  if (p.wide) {
+    e = pa::launch_prefix_wide(p, c.maps, c.kvk, kv->head_dim, st);
+    if (e != cudaSuccess) return cuda_fail(e, "shared-prefix tensor-core launch");
+  }
+  e = pa::launch_prefix_decode(p, c.tma ? &c.maps : nullptr, c.kvk, kv->head_dim, c.nt, c.plan, st);
+  if (e != cudaSuccess) return cuda_fail(e, "shared-prefix split-K launch");
+  e = pa::launch_prefix_merge(p, kv->head_dim, st);
+  return e == cudaSuccess ? PA_OK : cuda_fail(e, "shared-prefix merge launch");
+}
+
 int kv_rotate_write(const pa_kv_new_t* nw, const pa_rotate_t* rot, const pa_kv_cache_t* kv, const pa_paging_t* pg,
                     int32_t* status, void* stream) {
   g_err[0] = 0;

@@ -85,6 +85,40 @@ struct AttnParams {
   unsigned int abort_gen;  // launch generation used by bounded waits to stop together
 };
 
+// Attention of a batch whose groups share a prefix (csrc/prefix_plan.cu).  The partial results of a piece (a work
+// list entry's part that one worker covered) are rows of D + 2 floats: first those of what sequences have to
+// themselves, then those of the shared prefixes.  A piece of entry e by worker w starts at (rows of the entries before e) + w *
+// (most rows of an entry): both grow along the work list, so no two pieces overlap, however the list is cut.
+struct SharedParams : AttnParams {
+  int4* rec;              // [2 B], see decode_kernel.cuh
+  const int* group_start; // [groups + 1]
+  const int* prefix_len;  // [groups]
+  int groups;
+  int cpm;                // sequences of a chunk (split-K form)
+  int decode_tile;        // keys of a split-K tile
+  int wide;               // the prefixes go to the tensor-core kernel (csrc/prefix_sm100.cu)
+  int wide_ctas;
+  int* unit0;             // [groups + 1] first work unit of a group (wide)
+  int4* grp;              // [groups] shared keys, first sequence, sequences, leader
+  long long prefix_row0;  // first partial row of the shared prefixes
+};
+constexpr int kMaxSharedSeqs = 4096;
+constexpr int kChunkCols = 16;  // most columns of a chunk
+constexpr int kWideRows = 128;  // query rows of a tensor-core tile
+constexpr int kWideKeys = 128;  // and its keys
+// First partial row of worker w's piece of a chunk, of a sequence's own keys, of a tensor-core segment.
+__host__ __device__ inline long long shared_chunk_row(const SharedParams& p, int b0, int n, int kvh, int w) {
+  return p.prefix_row0 + (static_cast<long long>(b0) * p.Hkv + static_cast<long long>(kvh) * n) * p.maxq * p.G +
+         static_cast<long long>(w) * kChunkCols;
+}
+__host__ __device__ inline long long shared_own_row(const SharedParams& p, int b, int kvh, int w) {
+  return (static_cast<long long>(b) * p.Hkv + kvh + w) * p.maxq * p.G;
+}
+__host__ __device__ inline long long shared_wide_row(const SharedParams& p, int first, int rows, int kvh, int tile, int cta) {
+  return p.prefix_row0 + static_cast<long long>(first) * p.Hkv * p.maxq * p.G + static_cast<long long>(kvh) * rows +
+         static_cast<long long>(tile) * kWideRows + static_cast<long long>(cta) * kWideRows;
+}
+
 struct WriteParams {
   const void* k_new;
   const void* v_new;
@@ -295,6 +329,14 @@ cudaError_t launch_peer_barrier(int* local_flags, const PeerFlags& peers, int n,
                                 cudaStream_t stream);
 cudaError_t launch_decode(const AttnParams& p, const KvMaps* maps, int kv_kind, int q_bf16, int D, int nt,
                           const DecodeLaunch& plan, cudaStream_t stream, int phase = DECODE_BOTH);
+// Shared prefixes: the plan, the split-K pass over p.rec, the tensor-core pass over the prefixes, the merge.
+cudaError_t launch_prefix_plan(const SharedParams& p, cudaStream_t stream);
+cudaError_t launch_prefix_merge(const SharedParams& p, int D, cudaStream_t stream);
+int prefix_decode_plan(int kv_kind, int q_bf16, int D, int nt, int B, int use_tma, DecodeLaunch* out);
+cudaError_t launch_prefix_decode(const SharedParams& p, const KvMaps* maps, int kv_kind, int D, int nt,
+                                 const DecodeLaunch& plan, cudaStream_t stream);
+bool prefix_wide_supported(int kv_kind, int D, int BS);
+cudaError_t launch_prefix_wide(const SharedParams& p, const KvMaps& maps, int kv_kind, int D, cudaStream_t stream);
 cudaError_t launch_prefill(const AttnParams& p, int kv_kind, int D, int mma_bf16, cudaStream_t stream);
 // INT8 blocks of a prefill call -> fp16 scratch pool (gather: block (b, j) to b * bt_cols + j with the
 // matching table written to dbt; mirror: block x to x).

@@ -8,6 +8,7 @@
 //                                           K/V rows (transformer/model.py:85-122)
 //   pie_b200::project_write_kv              the K/V projection with that write in
 //                                           its epilogue (transformer/model.py:75-122)
+//   pie_b200::shared_prefix_attention       decode attention over groups that share a prefix
 //   pie_b200::rotate_write_kv               new query and key rows rotated by their
 //                                           positions, K/V rows written
 //   pie_b200::adjust_logits                 penalties, biases and masks on logits
@@ -186,6 +187,11 @@ at::Tensor workspace(const at::Device& dev, size_t bytes) {
   return ws;
 }
 
+// An uninitialised tensor on the current device's allocator, without a dispatch.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, t, dev, std::nullopt));
+}
+
 pa_attn_io_t io_desc(const at::Tensor& Q, const at::Tensor& O, const at::Tensor& L, bool ragged, int64_t max_q_len,
                      bool causal_top_left, double softmax_scale) {
   pa_attn_io_t io{};
@@ -315,6 +321,41 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_varlen(
   paged_attention_varlen_out(Q, q_start, q_len, max_q_len, K, V, block_table, num_blocks, kv_len, k_scale, v_scale,
                              causal_top_left, softmax_scale, status, out, lse);
   return {out, lse};
+}
+
+void shared_prefix_attention(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const at::Tensor& q_len,
+                             const at::Tensor& block_table, const at::Tensor& num_blocks, const at::Tensor& kv_len,
+                             const at::Tensor& group_start, const at::Tensor& prefix_len,
+                             const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                             double softmax_scale, const std::optional<at::Tensor>& status, at::Tensor& out,
+                             at::Tensor& lse) {
+  check_q(Q, 4);
+  check_out(Q, out, lse);
+  TORCH_CHECK_VALUE(Q.size(3) < 2 || out.stride(3) == 1, "pie_b200: out needs a contiguous head_dim");
+  check_device(Q, K, "K");
+  TORCH_CHECK_VALUE(K.dim() == 4 && K.size(3) == Q.size(3), "pie_b200: head_dim of Q and of the pool differ");
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && block_table.size(0) == Q.size(0), "pie_b200: block_table needs ", Q.size(0),
+                    " rows");
+  TORCH_CHECK_VALUE(group_start.numel() >= 1, "pie_b200: group_start holds num_groups + 1 entries");
+  const int64_t G = group_start.numel() - 1;
+  check_i32(Q, group_start, "group_start", G + 1);
+  check_i32(Q, prefix_len, "prefix_len", G);
+  check_status(Q, status);
+  const c10::cuda::CUDAGuard guard(Q.device());
+  pa_kv_cache_t kv = kv_desc(K, V, k_scale, v_scale);
+  pa_paging_t pg = paging(Q, block_table, num_blocks, q_len, kv_len);
+  pa_attn_io_t io = io_desc(Q, out, lse, false, Q.size(2), false, softmax_scale);
+  pa_groups_t gr{};
+  gr.group_start = static_cast<const int32_t*>(group_start.data_ptr());
+  gr.prefix_len = static_cast<const int32_t*>(prefix_len.data_ptr());
+  gr.num_groups = static_cast<int32_t>(G);
+  size_t bytes = 0;
+  check_rc(shared_prefix_workspace_size(&io, &kv, &pg, &gr, &bytes), "shared_prefix_attn");
+  // a workspace of this call's own: calls on other streams and captured graphs do not share it
+  at::Tensor ws = fresh({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, at::kByte, Q.device());
+  void* stream = c10::cuda::getCurrentCUDAStream(Q.device().index()).stream();
+  check_rc(shared_prefix_attn(&io, &kv, &pg, &gr, ws.data_ptr(), bytes, opt_ptr<int32_t>(status), stream),
+           "shared_prefix_attn");
 }
 
 void write_kv(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& block_table,
@@ -560,11 +601,6 @@ void adjust_logits(const at::Tensor& logits, const std::optional<at::Tensor>& to
 }
 
 // ---- shared blocks, page copies, beams ---------------------------------------
-// An uninitialised tensor on the current device's allocator, without a dispatch.
-at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const at::Device& dev) {
-  return at::Tensor(at::detail::empty_cuda(sizes, t, dev, std::nullopt));
-}
-
 // One descriptor per layer; the scale lists are empty but for int8 pools.
 std::vector<pa_kv_cache_t> layer_descs(at::TensorList k, at::TensorList v, at::TensorList ks, at::TensorList vs) {
   TORCH_CHECK_VALUE(!k.empty() && k.size() == v.size(), "pie_b200: as many K as V pools are needed, one at least (got ",
@@ -803,6 +839,9 @@ TORCH_LIBRARY(pie_b200, m) {
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
   m.def("project_write_kv(Tensor x, Tensor w, Tensor? bias, Tensor block_table, Tensor seq_index, Tensor positions, "
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
+  m.def("shared_prefix_attention(Tensor Q, Tensor K, Tensor V, Tensor q_len, Tensor block_table, Tensor num_blocks, "
+        "Tensor kv_len, Tensor group_start, Tensor prefix_len, Tensor? k_scale, Tensor? v_scale, float softmax_scale, "
+        "Tensor(s!)? status, Tensor(a!) out, Tensor(b!) lse) -> ()");
   m.def("rotate_write_kv(Tensor? q, Tensor k_new, Tensor v_new, Tensor cos_sin, bool interleaved, Tensor block_table, "
         "Tensor seq_index, Tensor positions, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, "
         "Tensor(d!)? v_scale, Tensor(s!)? status, Tensor(e!)? q_out) -> ()");
@@ -829,6 +868,7 @@ TORCH_LIBRARY_IMPL(pie_b200, CUDA, m) {
   m.impl("paged_attention_varlen_out", &paged_attention_varlen_out);
   m.impl("write_kv", &write_kv);
   m.impl("project_write_kv", &project_write_kv);
+  m.impl("shared_prefix_attention", &shared_prefix_attention);
   m.impl("rotate_write_kv", &rotate_write_kv);
   m.impl("adjust_logits", &adjust_logits);
   m.impl("copy_blocks", &copy_blocks);
@@ -843,7 +883,7 @@ TORCH_LIBRARY_IMPL(pie_b200, Meta, m) {
   m.impl("reorder_beams", &reorder_beams_meta);
   m.impl("compact_blocks", &compact_blocks_meta);
   m.impl("beam_select", &beam_select_meta);
-  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "rotate_write_kv",
+  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "shared_prefix_attention", "rotate_write_kv",
                          "adjust_logits", "copy_blocks"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&write_only_meta>());
 }

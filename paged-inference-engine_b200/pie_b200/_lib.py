@@ -93,6 +93,12 @@ class PaKvProj(ctypes.Structure):
     ]
 
 
+class PaGroups(ctypes.Structure):
+    """Mirror of pa_groups_t."""
+
+    _fields_ = [("group_start", _vp), ("prefix_len", _vp), ("num_groups", _i32), ("_reserved", _i32)]
+
+
 class PaRotate(ctypes.Structure):
     """Mirror of pa_rotate_t."""
 
@@ -166,6 +172,11 @@ SIGNATURES = {
                                      _vp, _vp]),
     "kv_project_write": (ctypes.c_int, [ctypes.POINTER(PaKvProj), ctypes.POINTER(PaKvCache),
                                         ctypes.POINTER(PaPaging), _vp, _vp]),
+    "shared_prefix_workspace_size": (ctypes.c_int, [ctypes.POINTER(PaAttnIO), ctypes.POINTER(PaKvCache),
+                                                    ctypes.POINTER(PaPaging), ctypes.POINTER(PaGroups),
+                                                    ctypes.POINTER(ctypes.c_size_t)]),
+    "shared_prefix_attn": (ctypes.c_int, [ctypes.POINTER(PaAttnIO), ctypes.POINTER(PaKvCache), ctypes.POINTER(PaPaging),
+                                          ctypes.POINTER(PaGroups), _vp, ctypes.c_size_t, _vp, _vp]),
     "kv_rotate_write": (ctypes.c_int, [ctypes.POINTER(PaKvNew), ctypes.POINTER(PaRotate), ctypes.POINTER(PaKvCache),
                                        ctypes.POINTER(PaPaging), _vp, _vp]),
     "logits_adjust": (ctypes.c_int, [ctypes.POINTER(PaLogits), _vp, _vp]),

@@ -403,6 +403,85 @@ def paged_attention_varlen(Q: torch.Tensor, cu_seqlens_q: torch.Tensor, K: torch
     return out, lse
 
 
+def shared_prefix_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, q_len_per_seq: torch.Tensor,
+                            block_table: torch.Tensor, num_blocks_per_seq: torch.Tensor, block_size: int,
+                            kv_len_per_seq: torch.Tensor, group_start: torch.Tensor, prefix_len: torch.Tensor,
+                            k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, *,
+                            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                            softmax_scale: Optional[float] = None,
+                            status: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``paged_attention`` of decode rows where groups of sequences share a prefix, read once a group; (O, L) fp16.
+
+    Sequences ``group_start[g] .. group_start[g + 1] - 1`` (int32 [G + 1], on the device, rising) form group g; their
+    block tables name the same blocks for the first ``prefix_len[g]`` tokens (int32 [G]; cut to whole blocks, and to
+    what every row sees).  ``DeviceBlockManager.shared_prefixes`` and ``BeamSearch.step_inputs`` give both.  At most
+    16 query rows times heads of a KV head (``max_q_len * Hq / Hkv``); fp16, bf16 and int8 pools.
+    """
+    if Q.dim() != 4:
+        raise ValueError("Q must be [num_seqs, num_q_heads, max_q_len, head_dim]")
+    B, Hq, maxq, D = Q.shape
+    K, V = pool_layout(K, V, block_size)
+    if K.dim() != 4 or K.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} does not match the pool {tuple(K.shape)}")
+    if K.shape[3] != D:
+        raise ValueError(f"head_dim of Q ({D}) and of the pool ({K.shape[3]}) differ")
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"block_table must be [{B}, max_blocks]")
+    if group_start.dim() != 1 or group_start.numel() < 1 or tuple(prefix_len.shape) != (group_start.numel() - 1,):
+        raise ValueError("group_start must hold num_groups + 1 offsets, prefix_len num_groups lengths")
+    dev = Q.device
+    if Q.dtype not in (torch.float16, torch.bfloat16):
+        Q = Q.to(K.dtype if K.dtype in (torch.float16, torch.bfloat16) else torch.float16)
+    if Q.stride(3) != 1:
+        Q = Q.contiguous()
+    if out is None and lse is None:
+        out, lse = _out_and_lse((B, Hq, maxq, D), dev)
+    if out is None:
+        out = torch.empty((B, Hq, maxq, D), dtype=torch.float16, device=dev)
+    elif out.dtype != torch.float16 or tuple(out.shape) != (B, Hq, maxq, D) or (D > 1 and out.stride(3) != 1):
+        raise ValueError("out must be float16 with Q's shape and a contiguous head_dim")
+    if lse is None:
+        lse = torch.empty((B, Hq, maxq), dtype=torch.float16, device=dev)
+    elif lse.dtype != torch.float16 or tuple(lse.shape) != (B, Hq, maxq):
+        raise ValueError("lse must be float16 with Q's shape without head_dim")
+    if status is None and _CHECK:
+        status = status_word(dev)
+    gs, pl = _i32(group_start), _i32(prefix_len)
+    scale = float(softmax_scale) if softmax_scale else 0.0
+    if BACKEND == "torch":
+        bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+        _op("shared_prefix_attention")(Q, K, V, _i32(q_len_per_seq), bt, _i32(num_blocks_per_seq), _i32(kv_len_per_seq), gs,
+                                       pl, k_scale, v_scale, scale, status, out, lse)
+    else:
+        for name, t in (("K", K), ("V", V), ("block_table", block_table), ("q_len_per_seq", q_len_per_seq),
+                        ("kv_len_per_seq", kv_len_per_seq), ("num_blocks_per_seq", num_blocks_per_seq),
+                        ("group_start", gs), ("prefix_len", pl), ("out", out), ("lse", lse)):
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, Q on {dev}")
+        keep: list = []
+        kc = kv_cache_desc(K, V, k_scale, v_scale)
+        pg = paging_desc(block_table, num_blocks_per_seq, q_len_per_seq, kv_len_per_seq, keep)
+        io = PaAttnIO()
+        io.q, io.q_dtype, io.num_q_heads, io.max_q_len = Q.data_ptr(), _TORCH2PA[Q.dtype], Hq, maxq
+        io.q_stride_seq, io.q_stride_head, io.q_stride_row = Q.stride(0), Q.stride(1), Q.stride(2)
+        io.o = out.data_ptr()
+        io.o_stride_seq, io.o_stride_head, io.o_stride_row = out.stride(0), out.stride(1), out.stride(2)
+        io.lse = lse.data_ptr()
+        io.l_stride_seq, io.l_stride_head, io.l_stride_row = lse.stride(0), lse.stride(1), lse.stride(2)
+        io.softmax_scale = scale
+        gr = _lib.PaGroups(gs.data_ptr(), pl.data_ptr(), pl.numel(), 0)
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            nbytes = ctypes.c_size_t(0)
+            _lib.check("shared_prefix_attn", lib.shared_prefix_workspace_size(io, kc, pg, gr, ctypes.byref(nbytes)))
+            ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=dev)
+            _lib.check("shared_prefix_attn", lib.shared_prefix_attn(io, kc, pg, gr, ws.data_ptr(), nbytes.value, _ptr(status),
+                                                                    _stream(dev)))
+    if _CHECK and status is not None:
+        _raise_status("shared_prefix_attention", status)
+    return out, lse
+
+
 def paged_attention_peers(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, q_len_per_seq: torch.Tensor,
                           block_table: torch.Tensor, num_blocks_per_seq: torch.Tensor, block_size: int,
                           kv_len_per_seq: torch.Tensor, k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor],
