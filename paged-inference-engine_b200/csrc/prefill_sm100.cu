@@ -99,31 +99,6 @@ __device__ unsigned int g_tc_abort_gen = 0;
 // are 256 apart.
 __device__ unsigned int g_pf_sched[256][2];
 
-// 8 x 8 transpose of 16-byte pieces across the eight lanes of a group (lane
-// index i = lane & 7): on return lane i holds piece i of lanes 0..7's rows.
-// Three butterfly stages; in stage m a lane swaps, with lane i ^ m, the four
-// pieces whose index differs from i in bit m (selects on compile-time
-// indices, 16 shuffles a stage).
-__device__ __forceinline__ void transpose8_u4(uint4 (&v)[8], int i) {
-#pragma unroll
-  for (int m = 1; m < 8; m <<= 1) {
-    const bool hi = (i & m) != 0;
-#pragma unroll
-    for (int j0 = 0; j0 < 8; ++j0) {
-      if (j0 & m) continue;
-      const int j1 = j0 | m;
-      const uint4 t = hi ? v[j0] : v[j1];
-      uint4 u;
-      u.x = __shfl_xor_sync(0xffffffffu, t.x, m);
-      u.y = __shfl_xor_sync(0xffffffffu, t.y, m);
-      u.z = __shfl_xor_sync(0xffffffffu, t.z, m);
-      u.w = __shfl_xor_sync(0xffffffffu, t.w, m);
-      if (hi) v[j0] = u;
-      else v[j1] = u;
-    }
-  }
-}
-
 // Bounded mbarrier wait; false (and a status bit) on time-out or abort.  The
 // first poll is inlined: a wait on a phase that has already completed costs
 // ~55 cycles this way against ~240 through the out-of-line loop.
