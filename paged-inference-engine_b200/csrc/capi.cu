@@ -787,7 +787,7 @@ struct SharedCall {
   bool tma;
   int kvk, nt;
   pa::DecodeLaunch plan;
-  size_t rec, tile, unit, grp, ml, o, total;
+  size_t rec, tile, unit, grp, head, ml, o, total;
 };
 
 int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg, const pa_groups_t* gr,
@@ -819,6 +819,7 @@ int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging
   c.p.cpm = kNcMax / per;
   c.kvk = kv_kind(kv->dtype);
   c.p.decode_tile = kv->dtype == PA_DTYPE_I8 ? 32 : 16;
+  c.p.min_chunk = 1;
   c.tma = make_kv_maps(kv, &c.maps);
   c.p.wide = c.tma && a.B * per > kNcMax && pa::prefix_wide_supported(c.kvk, kv->head_dim, kv->block_size) &&
              !std::getenv("PIE_B200_NO_TCGEN05");
@@ -843,14 +844,15 @@ int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging
   c.p.num_warps_total = c.plan.ctas * c.plan.warps_per_cta;
   const long long base_rows = static_cast<long long>(a.B) * a.Hkv * per;
   c.p.prefix_row0 = base_rows + static_cast<long long>(c.p.num_warps_total) * per;
-  const long long rows = c.p.prefix_row0 + base_rows +
-                         (c.p.wide ? static_cast<long long>(c.p.wide_ctas) * pa::kWideRows
-                                   : static_cast<long long>(c.p.num_warps_total) * pa::kChunkCols);
+  const long long rows = c.p.prefix_row0 +
+                         (c.p.wide ? pa::kWideRoom * base_rows + 2LL * c.p.wide_ctas * pa::kWideRows
+                                   : base_rows + static_cast<long long>(c.p.num_warps_total) * pa::kChunkCols);
   c.rec = 0;
   c.tile = align256(static_cast<size_t>(2) * a.B * sizeof(int4));
   c.unit = c.tile + align256((static_cast<size_t>(2) * a.B + 1) * sizeof(int));
   c.grp = c.unit + align256((static_cast<size_t>(gr->num_groups) + 1) * sizeof(int));
-  c.ml = c.grp + align256(static_cast<size_t>(gr->num_groups) * sizeof(int4));
+  c.head = c.grp + align256(static_cast<size_t>(gr->num_groups) * sizeof(int4));
+  c.ml = c.head + align256(sizeof(int4));
   c.o = c.ml + align256(static_cast<size_t>(rows) * 2 * sizeof(float));
   c.total = c.o + align256(static_cast<size_t>(rows) * kv->head_dim * sizeof(float));
   return PA_OK;
@@ -883,7 +885,8 @@ int shared_prefix_attn(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa
   pa::SharedParams& p = c.p;
   p.rec = reinterpret_cast<int4*>(ws + c.rec);
   p.tstart = reinterpret_cast<int*>(ws + c.tile);
-  p.unit0 = reinterpret_cast<int*>(ws + c.unit);
+  p.step0 = reinterpret_cast<int*>(ws + c.unit);
+  p.head = reinterpret_cast<int4*>(ws + c.head);
   p.grp = reinterpret_cast<int4*>(ws + c.grp);
   p.part_ml = reinterpret_cast<float*>(ws + c.ml);
   p.part_o = reinterpret_cast<float*>(ws + c.o);

@@ -150,7 +150,8 @@ __device__ __forceinline__ int seq_keys(const AttnParams& p, int b) {
 // Keys of a shared-prefix problem: virtual sequence v < B is a chunk of up to `cpm` neighbouring sequences, led
 // by sequence v, over the prefix that they share (rec[v] = keys, 0, row of the block table, sequences; keys 0 where v leads none), and
 // B + b is what sequence b has to itself (rec[B + b] = keys, first key, leader and sequences of its chunk).
-__device__ __forceinline__ int4 shared_rec(const SharedParams& p, int v) { return p.rec[v]; }
+// (past the L1 cache: this kernel may start while the plan's reader is still running)
+__device__ __forceinline__ int4 shared_rec(const SharedParams& p, int v) { return __ldcg(p.rec + v); }
 
 struct Cursor {
   int b, kvh, tile, nt;
@@ -336,7 +337,15 @@ __device__ __forceinline__ float scale_from_word(uint32_t w, bool hi, int is_f32
 template <int D, int KVT, int QT, int NT, bool TMA, bool SHARED = false>
 __global__ void __launch_bounds__(max_warps<NT>() * 32, 1)
     pa_decode_kernel(const std::conditional_t<SHARED, SharedParams, AttnParams> p, const __grid_constant__ KvMaps maps) {
-  pdl_enter();
+  if constexpr (SHARED) {
+    // Behind the tensor-core kernel this one needs nothing of it, only the plan, which has run when
+    // that kernel let this one start: it fills the SMs as they come free and waits at its end, so that what
+    // follows finds both complete.
+    if (p.wide) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    else pdl_enter();
+  } else {
+    pdl_enter();
+  }
   using C = DecCfg<D, KVT>;
   using Lay = DecLayout<D, KVT, NT>;
   constexpr int STAGES = C::STAGES;
@@ -366,7 +375,7 @@ __global__ void __launch_bounds__(max_warps<NT>() * 32, 1)
 
   // ---- prologue: tiles per sequence and their exclusive scan -------------
   if constexpr (SHARED) {
-    for (int i = tid; i <= NV; i += NW * 32) s_ts[i] = p.tstart[i];
+    for (int i = tid; i <= NV; i += NW * 32) s_ts[i] = __ldcg(p.tstart + i);
   } else {
     for (int i = tid; i < p.B; i += NW * 32) {
       const int nk = seq_keys(p, i);
@@ -406,11 +415,15 @@ __global__ void __launch_bounds__(max_warps<NT>() * 32, 1)
 
   const int total = s_ts[NV] * p.Hkv;
   const int W = p.num_warps_total;
-  const int chunk = (total + W - 1) / W;
+  int chunk = (total + W - 1) / W;
+  if constexpr (SHARED) chunk = max(chunk, p.min_chunk);
   const int gw = blockIdx.x * NW + warp;
   const int g0 = gw * chunk;
   const int g1 = min(g0 + chunk, total);
-  if (total == 0 || g0 >= g1) return;
+  if (total == 0 || g0 >= g1) {
+    if constexpr (SHARED) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    return;
+  }
 
   const int r = lane >> 2;  // fragment row group
   const int q4 = lane & 3;  // thread in group
@@ -1044,6 +1057,7 @@ __global__ void __launch_bounds__(max_warps<NT>() * 32, 1)
   }
   if constexpr (USE_CPASYNC) cp_async_wait<0>();
   peer_store_fence(p);
+  if constexpr (SHARED) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 

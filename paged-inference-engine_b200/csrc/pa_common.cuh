@@ -236,6 +236,15 @@ __device__ __forceinline__ float warp_sum_xor(float v, int first_mask) {
   return v;
 }
 
+// Key tiles of CTA part `part` of a team's steps [s0, s1) of a (pass, kv head): the first of them, n their number.
+__device__ __forceinline__ int wide_tiles(const WideShape& s, int s0, int s1, int part, int& n) {
+  const int up = (1 << s.lweight) - 1;
+  const int b0 = (s0 + up) >> s.lweight, b1 = (s1 + up) >> s.lweight;
+  const int t = (b0 << s.lparts) + part * (b1 - b0);
+  n = min(t + (b1 - b0), min(b1 << s.lparts, s.KT)) - t;
+  return t;
+}
+
 __device__ __forceinline__ void set_status(int* status, int bit) {
   if (status) atomicOr(status, bit);
 }
@@ -428,6 +437,71 @@ __device__ __forceinline__ void tc_mma_ts_seq(uint32_t d_tmem, uint32_t a_tmem, 
         "r"(a_tmem), "l"(b0), "r"(idesc), "r"(accumulate)
         : "memory");
   }
+}
+
+// ---------------------------------------------------------------------------
+// The same products issued by a whole converged warp, one elected lane of which
+// executes the tcgen05 instructions.  The descriptors then stay warp-uniform: issued by one
+// lane inside a divergent branch, each product pays for moving its operands to
+// uniform registers.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void tc_elect_commit(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred pe;\n elect.sync _|pe, 0xffffffff;\n"
+      " @pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
+      : "memory");
+}
+// D (tmem) = A B, NK K16 steps of two K-major SW128 operands; steps past a 64-column half start AH / BH (16-byte units)
+// further on.
+template <int NK, int AH, int BH>
+__device__ __forceinline__ void tc_elect_mma_ss(uint32_t d_tmem, uint64_t a0, uint64_t b0, uint32_t idesc) {
+  static_assert(NK == 4 || NK == 8, "4 or 8 steps");
+  asm volatile(
+      "{\n .reg .pred pe, p0, p1;\n .reg .b64 a1, a2, a3, b1, b2, b3;\n elect.sync _|pe, 0xffffffff;\n"
+      " setp.ne.b32 p0, %3, %3;\n setp.eq.b32 p1, %3, %3;\n"
+      " add.s64 a1, %1, 2;\n add.s64 a2, %1, 4;\n add.s64 a3, %1, 6;\n"
+      " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p0;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, p1;\n}\n" ::"r"(d_tmem),
+      "l"(a0), "l"(b0), "r"(idesc)
+      : "memory");
+  if constexpr (NK == 8) {
+    asm volatile(
+        "{\n .reg .pred pe, p1;\n .reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n elect.sync _|pe, 0xffffffff;\n"
+        " setp.eq.b32 p1, %3, %3;\n"
+        " add.s64 a0, %1, %4;\n add.s64 a1, a0, 2;\n add.s64 a2, a0, 4;\n add.s64 a3, a0, 6;\n"
+        " add.s64 b0, %2, %5;\n add.s64 b1, b0, 2;\n add.s64 b2, b0, 4;\n add.s64 b3, b0, 6;\n"
+        " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a0, b0, %3, p1;\n"
+        " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, p1;\n"
+        " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, p1;\n"
+        " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, p1;\n}\n" ::"r"(d_tmem),
+        "l"(a0), "l"(b0), "r"(idesc), "n"(AH), "n"(BH)
+        : "memory");
+  }
+}
+// D (tmem) (+)= A B, 8 K16 steps with A in TMEM and B MN-major (see tc_mma_ts_seq).
+__device__ __forceinline__ void tc_elect_mma_ts8(uint32_t d_tmem, uint32_t a_tmem, uint64_t b0, uint32_t idesc,
+                                                 uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred pe, p0, p1;\n .reg .b32 t1, t2, t3, t4, t5, t6, t7;\n"
+      " .reg .b64 b1, b2, b3, b4, b5, b6, b7;\n elect.sync _|pe, 0xffffffff;\n"
+      " setp.ne.b32 p0, %4, 0;\n setp.eq.b32 p1, %3, %3;\n"
+      " add.u32 t1, %1, 8;\n add.u32 t2, %1, 16;\n add.u32 t3, %1, 24;\n add.u32 t4, %1, 32;\n"
+      " add.u32 t5, %1, 40;\n add.u32 t6, %1, 48;\n add.u32 t7, %1, 56;\n"
+      " add.s64 b1, %2, 128;\n add.s64 b2, %2, 256;\n add.s64 b3, %2, 384;\n add.s64 b4, %2, 512;\n"
+      " add.s64 b5, %2, 640;\n add.s64 b6, %2, 768;\n add.s64 b7, %2, 896;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p0;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t1], b1, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t2], b2, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t3], b3, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t4], b4, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t5], b5, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t6], b6, %3, p1;\n"
+      " @pe tcgen05.mma.cta_group::1.kind::f16 [%0], [t7], b7, %3, p1;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b0), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 // 8 x 8 transpose of 16-byte pieces across the eight lanes of a group (lane

@@ -87,8 +87,8 @@ struct AttnParams {
 
 // Attention of a batch whose groups share a prefix (csrc/prefix_plan.cu).  The partial results of a piece (a work
 // list entry's part that one worker covered) are rows of D + 2 floats: first those of what sequences have to
-// themselves, then those of the shared prefixes.  A piece of entry e by worker w starts at (rows of the entries before e) + w *
-// (most rows of an entry): both grow along the work list, so no two pieces overlap, however the list is cut.
+// themselves, then those of the shared prefixes.  A piece of entry e by worker w starts at (room of the entries before e) + w *
+// (most room of an entry): both grow along the work list, so no two pieces overlap, however the list is cut.
 struct SharedParams : AttnParams {
   int4* rec;              // [2 B], see decode_kernel.cuh
   const int* group_start; // [groups + 1]
@@ -96,17 +96,54 @@ struct SharedParams : AttnParams {
   int groups;
   int cpm;                // sequences of a chunk (split-K form)
   int decode_tile;        // keys of a split-K tile
+  int min_chunk;          // fewest split-K tiles of a worker
   int wide;               // the prefixes go to the tensor-core kernel (csrc/prefix_sm100.cu)
   int wide_ctas;
-  int* unit0;             // [groups + 1] first work unit of a group (wide)
+  int* step0;             // [groups + 1] first step of a group (wide)
   int4* grp;              // [groups] shared keys, first sequence, sequences, leader
+  int4* head;             // [1] CTAs of a team, teams, steps of a team (wide)
   long long prefix_row0;  // first partial row of the shared prefixes
 };
 constexpr int kMaxSharedSeqs = 4096;
 constexpr int kChunkCols = 16;  // most columns of a chunk
 constexpr int kWideRows = 128;  // query rows of a tensor-core tile
 constexpr int kWideKeys = 128;  // and its keys
-// First partial row of worker w's piece of a chunk, of a sequence's own keys, of a tensor-core segment.
+constexpr int kWideRoom = 4;    // partial rows that a group's prefix may take, for each of its rows; most parts
+
+// How the tensor-core kernel works on a group.  Its row tiles go to CTAs in pairs (or the only one alone, whose two streams then
+// take the key tiles in turn), the pairs' CTAs form a team that walks the same keys at the same time, so that
+// K and V come from HBM once; a team with CTAs to spare also cuts its keys into `parts`.
+struct WideShape {
+  int rows, RT, KT;  // query rows (a kv head), row tiles, key tiles
+  int RP;            // row pairs
+  int lanes;         // of a pass: min(RP, team)
+  int passes;
+  int lparts;        // log2 of the parts
+  int room;          // partial rows of a CTA's piece
+  int bundles;       // of a (pass, kv head): a key tile for every part each
+  int lweight;       // log2 of the steps of a bundle: row tiles that a CTA multiplies with a key tile
+
+  __host__ __device__ WideShape() {}
+  // n > 0 sequences of `per` rows
+  __host__ __device__ WideShape(int keys, int n, int per, int team) {
+    rows = n * per;
+    RT = (rows + kWideRows - 1) / kWideRows;
+    KT = (keys + kWideKeys - 1) / kWideKeys;
+    RP = (RT + 1) / 2;
+    lanes = RP < team ? RP : team;
+    passes = RP <= team ? 1 : (RP + team - 1) / team;
+    room = rows < 2 * kWideRows ? rows : 2 * kWideRows;
+    lparts = 0;
+    while (passes == 1 && lparts < 2 && (lanes << (lparts + 1)) <= team &&
+           (lanes * room << (lparts + 1)) <= kWideRoom * rows)
+      ++lparts;
+    bundles = (KT + (1 << lparts) - 1) >> lparts;
+    lweight = RT > 1 ? 1 : 0;
+  }
+  __host__ __device__ int steps() const { return bundles << lweight; }  // of a (pass, kv head)
+};
+
+// First partial row of worker w's piece of a chunk, of a sequence's own keys, of a team's piece.
 __host__ __device__ inline long long shared_chunk_row(const SharedParams& p, int b0, int n, int kvh, int w) {
   return p.prefix_row0 + (static_cast<long long>(b0) * p.Hkv + static_cast<long long>(kvh) * n) * p.maxq * p.G +
          static_cast<long long>(w) * kChunkCols;
@@ -114,9 +151,11 @@ __host__ __device__ inline long long shared_chunk_row(const SharedParams& p, int
 __host__ __device__ inline long long shared_own_row(const SharedParams& p, int b, int kvh, int w) {
   return (static_cast<long long>(b) * p.Hkv + kvh + w) * p.maxq * p.G;
 }
-__host__ __device__ inline long long shared_wide_row(const SharedParams& p, int first, int rows, int kvh, int tile, int cta) {
-  return p.prefix_row0 + static_cast<long long>(first) * p.Hkv * p.maxq * p.G + static_cast<long long>(kvh) * rows +
-         static_cast<long long>(tile) * kWideRows + static_cast<long long>(cta) * kWideRows;
+__host__ __device__ inline long long shared_wide_row(const SharedParams& p, const WideShape& s, int first, int seg, int team,
+                                                     int team_size, int part, int lane) {
+  return p.prefix_row0 + static_cast<long long>(kWideRoom) * first * p.Hkv * p.maxq * p.G +
+         (static_cast<long long>(seg) * s.lanes * s.room << s.lparts) + static_cast<long long>(team) * team_size * 2 * kWideRows +
+         (part * s.lanes + lane) * s.room;
 }
 
 struct WriteParams {

@@ -20,8 +20,6 @@
 namespace pa {
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
-
 // Visible keys of sequence b's last row (0 for a sequence without rows).
 __device__ __forceinline__ int plan_keys(const SharedParams& p, int b, int rows) {
   if (rows <= 0) return 0;
@@ -43,8 +41,8 @@ __device__ __forceinline__ int group_of(const int* s_start, int G, int b) {
 
 // Exclusive scan of at[0..n) in place by the whole CTA, the sum to at[n].
 __device__ void scan_cta(int* at, int n, int* s_warp) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (n + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, T = blockDim.x;
+  const int per = (n + T - 1) / T;
   const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
   int sum = 0;
   for (int i = i0; i < i1; ++i) sum += at[i];
@@ -57,7 +55,7 @@ __device__ void scan_cta(int* at, int n, int* s_warp) {
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int v = s_warp[lane];
+    int v = lane < (T >> 5) ? s_warp[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, v, o);
@@ -72,14 +70,14 @@ __device__ void scan_cta(int* at, int n, int* s_warp) {
     at[i] = run;
     run += v;
   }
-  if (tid == PLAN_THREADS - 1) at[n] = run;
+  if (tid == T - 1) at[n] = run;
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const SharedParams p) {
+__global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p) {
   pdl_enter();
   extern __shared__ int s_plan[];
-  const int tid = threadIdx.x, G = p.groups, B = p.B;
+  const int tid = threadIdx.x, T = blockDim.x, G = p.groups, B = p.B;
   int* s_start = s_plan;            // [G + 1]
   int* s_keys = s_start + G + 1;    // [G] shared keys
   int* s_lead = s_keys + G;         // [G]
@@ -87,9 +85,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const SharedP
   int* s_unit = s_count + G;        // [G + 1]
   int* s_tile = s_unit + G + 1;     // [2 B + 1]
   __shared__ int s_warp[32];
+  __shared__ int s_team;
 
   int bad = 0;
-  for (int i = tid; i <= G; i += PLAN_THREADS) {
+  for (int i = tid; i <= G; i += T) {
     const int s = p.group_start[i];
     s_start[i] = s;
     bad |= s < 0 || s > B || (i > 0 && p.group_start[i - 1] > s);
@@ -99,10 +98,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const SharedP
       s_count[i] = 0;
     }
   }
+  if (tid == 0) s_team = 1;
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) set_status(p.status, ST_BAD_SEQ_INDEX);
 
-  for (int b = tid; b < B; b += PLAN_THREADS) {
+  for (int b = tid; b < B; b += T) {
     const int rows = seq_rows(p, b);
     const int keys = plan_keys(p, b, rows);
     if (rows > 0 && p.nblk[b] > p.bt_cols) set_status(p.status, ST_BAD_NUM_BLOCKS);
@@ -114,31 +114,41 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const SharedP
   }
   __syncthreads();
   const int per = p.maxq * p.G;
-  for (int g = tid; g < G; g += PLAN_THREADS) {
+  for (int g = tid; g < G; g += T) {
     const int keys = s_count[g] < 2 ? 0 : s_keys[g] & ~(p.BS - 1);
     s_keys[g] = keys;
-    int units = 0;
-    if (p.wide && keys > 0) {
-      const int n = s_start[g + 1] - s_start[g];
-      units = p.Hkv * ((n * per + kWideRows - 1) / kWideRows) * ((keys + kWideKeys - 1) / kWideKeys);
-    }
-    s_unit[g] = units;
-    p.grp[g] = make_int4(keys, s_start[g], keys > 0 ? s_start[g + 1] - s_start[g] : 0, s_lead[g]);
+    const int n = keys > 0 ? s_start[g + 1] - s_start[g] : 0;
+    p.grp[g] = make_int4(keys, s_start[g], n, s_lead[g]);
+    if (p.wide && n > 0) atomicMax(&s_team, min(p.wide_ctas, (n * per + 2 * kWideRows - 1) / (2 * kWideRows)));
   }
   __syncthreads();
   if (p.wide) {
+    const int team = s_team;
+    for (int g = tid; g < G; g += T) {
+      int steps = 0;
+      if (s_keys[g] > 0) {
+        const WideShape s(s_keys[g], s_start[g + 1] - s_start[g], per, team);
+        steps = s.passes * p.Hkv * s.steps();
+      }
+      s_unit[g] = steps;
+    }
+    __syncthreads();
     scan_cta(s_unit, G, s_warp);
-    for (int g = tid; g <= G; g += PLAN_THREADS) p.unit0[g] = s_unit[g];
+    for (int g = tid; g <= G; g += T) p.step0[g] = s_unit[g];
+    if (tid == 0) {
+      const int teams = p.wide_ctas / team;
+      p.head[0] = make_int4(team, teams, (s_unit[G] + teams - 1) / teams, s_unit[G]);
+    }
   }
 
-  for (int b = tid; b < B; b += PLAN_THREADS) {
+  for (int b = tid; b < B; b += T) {
     const int keys = plan_keys(p, b, seq_rows(p, b));
     const int g = bad ? -1 : group_of(s_start, G, b);
     int4 chunk = make_int4(0, 0, 0, 0), own = make_int4(keys, 0, 0, 0);
     if (g >= 0 && s_keys[g] > 0) {
       const int first = s_start[g], last = s_start[g + 1];
       if (p.wide) {
-        chunk.y = s_unit[g];
+        chunk.y = g;  // where prefix_merge_kernel finds the group (no keys: not a work list entry)
         own.z = first;
         own.w = last - first;
       } else {
@@ -160,95 +170,135 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const SharedP
   }
   __syncthreads();
   scan_cta(s_tile, 2 * B, s_warp);
-  for (int i = tid; i <= 2 * B; i += PLAN_THREADS) p.tstart[i] = s_tile[i];
+  for (int i = tid; i <= 2 * B; i += T) p.tstart[i] = s_tile[i];
 }
 
-// Joins the pieces of every output row.  Grid (Hkv, B), a warp per (row, head) column: lane i reads the statistics of piece
-// i, 32 at a time; the rows of the pieces are then added up with their weights.
+constexpr int MERGE_WARPS = 4;
+
+// Joins the pieces of every output row.  Grid (Hkv, B), a warp per column (query row and head): lane i reads the
+// statistics of piece i, 32 at a time; then all lanes add up the pieces' rows with their weights, 16 bytes a lane and
+// eight rows in flight.
 template <int D>
-__global__ void __launch_bounds__(128) prefix_merge_kernel(const SharedParams p) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) prefix_merge_kernel(const SharedParams p) {
   pdl_enter();
   const int kvh = blockIdx.x, b = blockIdx.y;
-  const int rows = seq_rows(p, b);
-  if (rows <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = p.maxq * p.G;
+  const int rows = seq_rows(p, b);
   const int4 own = p.rec[p.B + b];
-  const int W = p.num_warps_total;
-  const int total = p.tstart[2 * p.B] * p.Hkv;
-  const int chunk = max(1, (total + W - 1) / W);
-  // pieces of the list entries [s0, s0 + n)
-  int o0 = 0, on = 0;
-  {
-    const int t0 = p.tstart[p.B + b], n = p.tstart[p.B + b + 1] - t0;
-    if (n > 0) {
-      const int s0 = t0 * p.Hkv + kvh * n;
-      o0 = s0 / chunk;
-      on = (s0 + n - 1) / chunk - o0 + 1;
-    }
+  const int g = p.rec[b].y;
+  const int t_own = p.tstart[p.B + b], n_own = p.tstart[p.B + b + 1] - t_own;
+  const int tiles = p.tstart[2 * p.B];
+  const int4 head = p.wide ? p.head[0] : make_int4(1, 0, 1, 0);
+  const int cols = rows * p.G;
+  if (warp >= cols) return;
+  const int chunk = max(p.min_chunk, (tiles * p.Hkv + p.num_warps_total - 1) / p.num_warps_total);
+  int o0 = 0, on = 0;  // first piece of the sequence's own keys, pieces
+  if (n_own > 0) {
+    const int s0 = t_own * p.Hkv + kvh * n_own;
+    o0 = s0 / chunk;
+    on = (s0 + n_own - 1) / chunk - o0 + 1;
   }
   if (own.y == 0 && on == 1) return;  // written by the split-K kernel
-  const int head0 = kvh * p.G;
-  for (int col = warp; col < rows * p.G; col += 4) {
-    const int qi = col / p.G, hq = col - qi * p.G;
-    int c0 = 0, cn = 0;
-    long long crow = 0;  // partial row of piece 0
-    int cstep = 0;
-    if (own.y > 0) {
-      if (p.wide) {
-        const int R = (b - own.z) * per + col, rows_g = own.w * per;
-        const int KT = (own.y + kWideKeys - 1) / kWideKeys, RT = (rows_g + kWideRows - 1) / kWideRows;
-        const int units = p.unit0[p.groups];
-        const int wchunk = (units + p.wide_ctas - 1) / p.wide_ctas;
-        const int s0 = p.rec[b].y + (kvh * RT + R / kWideRows) * KT;
-        c0 = s0 / wchunk;
-        cn = (s0 + KT - 1) / wchunk - c0 + 1;
-        crow = shared_wide_row(p, own.z, rows_g, kvh, R / kWideRows, c0) + R % kWideRows;
-        cstep = kWideRows;
-      } else {
-        const int t0 = p.tstart[own.z], n = p.tstart[own.z + 1] - t0;
-        const int s0 = t0 * p.Hkv + kvh * n;
-        c0 = s0 / chunk;
-        cn = (s0 + n - 1) / chunk - c0 + 1;
-        crow = shared_chunk_row(p, own.z, own.w, kvh, c0) + (b - own.z) * per + col;
-        cstep = kChunkCols;
+  const bool wide = p.wide && own.y > 0;
+  WideShape shape;
+  int step0 = 0;
+  if (wide) {
+    shape = WideShape(own.y, own.w, per, head.x);
+    step0 = p.step0[g];
+  }
+  constexpr int LPR = D / 4;     // lanes of a row (16 bytes each)
+  constexpr int RPI = 32 / LPR;  // rows of a load instruction
+  const int sub = lane / LPR, at = lane % LPR;
+  for (int col = warp; col < cols; col += MERGE_WARPS) {
+    // pieces of the shared part: `cn`, the first of worker or team f0
+    int f0 = 0, cn = 0, s0 = 0;
+    long long crow = 0;
+    if (wide) {
+      const int R = (b - own.z) * per + col;
+      int rp = R / (2 * kWideRows), seg = kvh;
+      const int in_pair = R - rp * 2 * kWideRows;
+      if (shape.passes > 1) {
+        seg += rp / shape.lanes * p.Hkv;
+        rp %= shape.lanes;
       }
+      s0 = step0 + seg * shape.steps();
+      f0 = s0 / head.z;
+      cn = ((s0 + shape.steps() - 1) / head.z - f0 + 1) << shape.lparts;
+      crow = shared_wide_row(p, shape, own.z, seg, f0, head.x, 0, rp) + in_pair;
+    } else if (own.y > 0) {
+      const int t0 = p.tstart[own.z], n = p.tstart[own.z + 1] - t0;
+      s0 = t0 * p.Hkv + kvh * n;
+      f0 = s0 / chunk;
+      cn = (s0 + n - 1) / chunk - f0 + 1;
+      crow = shared_chunk_row(p, own.z, own.w, kvh, f0) + (b - own.z) * per + col;
     }
-    const long long orow0 = shared_own_row(p, b, kvh, o0) + col;
-    auto piece = [&](int i) { return i < on ? orow0 + static_cast<long long>(i) * per : crow + static_cast<long long>(i - on) * cstep; };
+    const long long orow = shared_own_row(p, b, kvh, o0) + col;
+    // the partial row of piece i, or -1 where a team's part is empty
+    auto piece = [&](int i) -> long long {
+      if (i < on) return orow + static_cast<long long>(i) * per;
+      i -= on;
+      if (!wide) return crow + static_cast<long long>(i) * kChunkCols;
+      const int t = i >> shape.lparts, q = i - (t << shape.lparts);
+      const int a = (f0 + t) * head.z - s0;
+      int n;
+      wide_tiles(shape, max(0, a), min(shape.steps(), a + head.z), q, n);
+      return n > 0 ? crow + static_cast<long long>(t) * head.x * 2 * kWideRows + q * shape.lanes * shape.room : -1;
+    };
     const int np = on + cn;
-    float M = -INFINITY;
-    for (int i = lane; i < np; i += 32) M = fmaxf(M, p.part_ml[piece(i) * 2]);
-    M = warp_max_xor(M, 1);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float l = 0.f, o[D / 32];
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+    float M = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int base = 0; base < np; base += 32) {
-      float f = 0.f;
-      if (base + lane < np) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + piece(base + lane) * 2);
-        f = ex2(ml.x - Mu);
-        l += ml.y * f;
-      }
+      long long r = -1;
+      if (base + lane < np) r = piece(base + lane);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (r >= 0) ml = *reinterpret_cast<const float2*>(p.part_ml + r * 2);
+      // join with what the pieces before gave
+      const float Mn = fmaxf(M, warp_max_xor(ml.x, 1));
+      const float Mu = Mn == -INFINITY ? 0.f : Mn;
+      const float old = ex2(M - Mu), f = ex2(ml.x - Mu);
+      M = Mn;
+      l = l * old + ml.y * f;
+      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
       const int n = min(32, np - base);
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        const float* po = p.part_o + piece(base + j) * D;
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += 8 * RPI) {
+        float4 v[8];
+        float w[8];
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) o[k] += po[lane + 32 * k] * fj;
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + k * RPI + sub;
+          const long long rj = __shfl_sync(0xffffffffu, r, j & 31);
+          w[k] = __shfl_sync(0xffffffffu, f, j & 31);
+          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (j < n && rj >= 0) v[k] = *reinterpret_cast<const float4*>(p.part_o + rj * D + 4 * at);
+          else w[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          acc.x += v[k].x * w[k], acc.y += v[k].y * w[k], acc.z += v[k].z * w[k], acc.w += v[k].w * w[k];
+        }
       }
     }
     l = warp_sum_xor(l, 1);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const long long orow = o_seq_base(p, b) + (head0 + hq) * p.o_sh + static_cast<long long>(qi) * p.o_sm;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) static_cast<__half*>(p.o)[orow + lane + 32 * k] = __float2half_rn(o[k] * inv);
+    for (int o = LPR; o < 32; o <<= 1) {
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int qi = col / p.G, hq = col - qi * p.G + kvh * p.G;
+    if (sub == 0) {
+      __half2* out = reinterpret_cast<__half2*>(static_cast<__half*>(p.o) + o_seq_base(p, b) + hq * p.o_sh +
+                                                static_cast<long long>(qi) * p.o_sm + 4 * at);
+      out[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
+      out[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+    }
     if (lane == 0 && p.lse) {
       const float L = l > 0.f ? (M + lg2(l)) * 0.6931471805599453f : -INFINITY;
-      static_cast<__half*>(p.lse)[l_seq_base(p, b) + (head0 + hq) * p.l_sh + static_cast<long long>(qi) * p.l_sm] =
-          __float2half_rn(L);
+      static_cast<__half*>(p.lse)[l_seq_base(p, b) + hq * p.l_sh + static_cast<long long>(qi) * p.l_sm] = __float2half_rn(L);
     }
   }
 }
@@ -261,11 +311,15 @@ cudaError_t launch_prefix_plan(const SharedParams& p, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(prefix_plan_kernel, dim3(1), dim3(PLAN_THREADS), smem, stream, p);
+  // a thread for each work list entry: barriers cost more the more threads meet at them
+  const int most = 2 * p.B > p.groups ? 2 * p.B : p.groups;
+  const int threads = most >= 1024 ? 1024 : most <= 128 ? 128 : (most + 31) / 32 * 32;
+  return launch_pdl(prefix_plan_kernel, dim3(1), dim3(threads), smem, stream, p);
 }
 
 cudaError_t launch_prefix_merge(const SharedParams& p, int D, cudaStream_t stream) {
-  return launch_pdl(D == 64 ? prefix_merge_kernel<64> : prefix_merge_kernel<128>, dim3(p.Hkv, p.B), dim3(128), 0, stream, p);
+  return launch_pdl(D == 64 ? prefix_merge_kernel<64> : prefix_merge_kernel<128>, dim3(p.Hkv, p.B), dim3(32 * MERGE_WARPS), 0,
+                    stream, p);
 }
 
 }  // namespace pa

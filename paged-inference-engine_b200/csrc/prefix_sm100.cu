@@ -2,18 +2,19 @@
 // tensor cores (tcgen05 + TMEM).
 //
 // A group's rows over one kv head (sequences x query rows x group heads) are cut into tiles of
-// 128, its shared keys into tiles of 128.  A work unit is one of each; units lie in the
-// order (group, kv head, row tile, key tile), and every CTA of a persistent grid takes an equal
-// run of them.  A run's part within one (group, kv head, row tile) is a piece: its 128 rows'
-// statistics and unnormalised sums go to the workspace, where prefix_merge_kernel
-// joins them (csrc/prefix_plan.cu).  Every row sees every shared key (the plan sees to it), so
-// the only mask is the end of the last tile.
+// 128, its shared keys into tiles of 128.  The CTAs of a persistent grid form teams that walk the list
+// of (group, kv head, key tiles), an equal run of it each; inside a team, every CTA has two row tiles of
+// the group (WideShape).  So the row tiles of a group pass over the same keys at about the same time, and
+// K and V come from HBM once: with the row tiles one after the other along the list, 128 sequences of 4 heads over 65536 bf16 keys
+// read their 268 MB four times (231 us).  What a CTA makes of its part of a run within one (group, kv
+// head) is a piece: its rows' statistics and unnormalised sums go to the workspace, where
+// prefix_merge_kernel joins them (csrc/prefix_plan.cu).  Every row sees every shared key (the plan
+// sees to it), so the only mask is the end of the last tile.
 //
-// The two softmax groups of a CTA take the key tiles of a piece in turn, each with its own logits,
-// maximum and sum in TMEM (S0 S1 O0 O1): while one turns its logits into
-// probabilities, the tensor core works for the other, as with the two heads of
-// csrc/prefill_sm100.cu, but with one row tile, so that few rows do not leave half of the CTA idle.
-// At the end of a piece the two results are joined in registers and written once.
+// A CTA runs two streams, each with its own logits, maximum and sum in TMEM (S0 S1 O0 O1): while one
+// turns its logits into probabilities, the tensor core works for the other.  The streams are its two
+// row tiles, which share each K/V tile; or, where there is one row tile, its even and odd key tiles, whose
+// results are joined in registers at the end of the piece, so that few rows do not leave half of the CTA idle.
 //
 //   warps 0-7    softmax: a thread per row (TMEM lane) and stream (w >> 2); they also load and convert Q
 //   warp 8       producer: K and V boxes gathered through the block table by TMA
@@ -24,6 +25,7 @@
 //
 // Bound by HBM up to about 256 rows a kv head (16-bit pools), by the softmax chain beyond.
 #include <atomic>
+#include <type_traits>
 
 #include "pa_common.cuh"
 
@@ -39,18 +41,19 @@ constexpr int W_PRODUCER = 8, W_MMA = 9, W_CONVERT = 10;
 
 template <int D, bool I8>
 struct WideCfg {
-  static constexpr int TILE = (D / 64) * W_HALF;      // fp16 / bf16 operand tile of 128 rows
-  static constexpr int RAW = 128 * D;                 // int8 tile
-  static constexpr int ST = I8 ? 2 : (D == 128 ? 3 : 6);  // K stages, and V stages
+  static constexpr int TILE = (D / 64) * W_HALF;   // fp16 / bf16 operand tile of 128 rows
+  static constexpr int RAW = 128 * D;              // int8 tile
+  static constexpr int KST = D == 128 ? (I8 ? 2 : 3) : (I8 ? 3 : 5);  // K stages
+  static constexpr int VST = D == 128 ? (I8 ? 1 : 2) : (I8 ? 3 : 5);  // V stages
   static constexpr int RST = I8 ? (D == 128 ? 4 : 8) : 0;  // raw tiles in flight, K and V alternating
-  static constexpr int K0 = TILE;
-  static constexpr int V0 = K0 + ST * TILE;
-  static constexpr int R0 = V0 + ST * TILE;
+  static constexpr int K0 = 2 * TILE;
+  static constexpr int V0 = K0 + KST * TILE;
+  static constexpr int R0 = V0 + VST * TILE;
   static constexpr int BAR = R0 + RST * RAW;
   static constexpr int B_QREADY = 0, B_QEMPTY = 1, B_SFULL = 2, B_PFULL = 4, B_ODONE = 6, B_SLOT = 8, B_PLACE = 9,
-                       B_KFULL = 11, B_KEMPTY = B_KFULL + ST, B_VFULL = B_KEMPTY + ST, B_VEMPTY = B_VFULL + ST,
-                       B_RFULL = B_VEMPTY + ST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
-  static constexpr int XCH = BAR + 512 / (D == 128 ? 2 : 1);
+                       B_KFULL = 10, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
+                       B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
+  static constexpr int XCH = BAR + (D == 128 ? 256 : 512);
   static constexpr int SMEM = XCH + 1024 + 1024;  // exchange of the two streams, alignment
   static constexpr int THREADS = 32 * (I8 ? W_CONVERT + 4 : W_CONVERT);
   static_assert(B_END * 8 <= XCH - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
@@ -71,80 +74,81 @@ __device__ __forceinline__ void wide_wait(const SharedParams& p, uint32_t bar, u
 }
 __device__ __forceinline__ void wide_barrier(int id, int n) { asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(n) : "memory"); }
 
-// The pieces of a CTA's run of units, walked alike by every role.
+// The pieces of a CTA, walked alike by every role.
 struct Pieces {
-  int left;                  // units of the run not walked yet
-  int g, kvh, rt, t;         // group, kv head, row tile, first key tile
-  int keys, first, n, lead;  // of the group
-  int rows, RT, KT;
+  int s, s1;          // steps of the team's run not walked yet
+  int team, q, size;  // team, the CTA's place in it, CTAs of a team
+  int g, base;        // group and its first step
+  int4 grp;           // shared keys, first sequence, sequences, leader
+  WideShape sh;
+  // the piece
+  int seg, kvh, t, n;  // (pass, kv head), key tiles [t, t + n)
+  int row0, live;      // first row of the CTA's row tiles in the group, rows of them
+  bool two;            // two row tiles (else one, whose key tiles alternate between the streams)
+  int part, lane;
 
-  __device__ __forceinline__ void group(const SharedParams& p) {
-    const int4 v = p.grp[g];
-    keys = v.x, first = v.y, n = v.z, lead = v.w;
-    rows = n * p.maxq * p.G;
-    RT = (rows + kWideRows - 1) / kWideRows;
-    KT = (keys + kWideKeys - 1) / kWideKeys;
-  }
-  __device__ __forceinline__ void begin(const SharedParams& p, int u0, int u1, int g0) {
-    left = u1 - u0;
-    g = g0;
-    if (left <= 0) return;
-    group(p);
-    const int u = u0 - p.unit0[g];
-    t = u % KT;
-    rt = u / KT % RT;
-    kvh = u / KT / RT;
-  }
-  __device__ __forceinline__ int tiles() const { return min(KT - t, left); }  // of this piece
-  __device__ __forceinline__ void next(const SharedParams& p) {
-    left -= tiles();
-    t = 0;
-    if (++rt == RT) {
-      rt = 0;
-      if (++kvh == p.Hkv) {
-        kvh = 0;
-        if (left > 0) {
-          do {
-            ++g;
-          } while (p.grp[g].x == 0);  // a group with units is still ahead
-          group(p);
-        }
-      }
+  __device__ __forceinline__ Pieces(const SharedParams& p, const int4& head, int cta, int g0) {
+    size = head.x;
+    team = cta / size;
+    q = cta - team * size;
+    s = min(team * head.z, head.w);
+    s1 = min(s + head.z, head.w);
+    g = g0 - 1;
+    base = -1;
+    if (s < s1) {
+      g = g0;
+      group(p);
     }
   }
+  __device__ __forceinline__ void group(const SharedParams& p) {
+    grp = p.grp[g];
+    base = p.step0[g];
+    sh = WideShape(grp.x, grp.z, p.maxq * p.G, size);
+  }
+  __device__ __forceinline__ bool next(const SharedParams& p) {
+    while (s < s1) {
+      const int len = sh.steps();
+      if (s - base >= sh.passes * p.Hkv * len) {  // a group with steps is still ahead
+        do {
+          ++g;
+        } while (p.grp[g].x == 0);
+        group(p);
+        continue;
+      }
+      const int off = s - base;
+      seg = off / len;
+      const int a = off - seg * len, b = min(len, a + s1 - s);
+      s += b - a;
+      const int pass = seg / p.Hkv;
+      kvh = seg - pass * p.Hkv;
+      const int lanes = min(sh.lanes, sh.RP - pass * sh.lanes);  // the last pass may have fewer pairs
+      part = q / sh.lanes;
+      lane = q - part * sh.lanes;
+      if (part >> sh.lparts || lane >= lanes) continue;
+      t = wide_tiles(sh, a, b, part, n);
+      if (n <= 0) continue;
+      row0 = (pass * sh.lanes + lane) * 2 * kWideRows;
+      live = min(2 * kWideRows, sh.rows - row0);
+      two = live > kWideRows;
+      return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ int units() const { return two ? 2 * n : n; }  // products of a row tile and a key tile
+  __device__ __forceinline__ int tile(int u) const { return two ? u >> 1 : u; }
 };
 
 template <int D, bool MMA_BF16, bool QBF16, bool I8>
 __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
     prefix_wide_kernel(const SharedParams p, const __grid_constant__ KvMaps maps) {
-  pdl_enter();
   using C = WideCfg<D, I8>;
-  constexpr int ST = C::ST, TILE = C::TILE;
+  constexpr int KST = C::KST, VST = C::VST, TILE = C::TILE;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   unsigned char* sm = smem_raw + (base - raw);
   auto bar = [&](int i) { return base + C::BAR + 8u * i; };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  const int units = p.unit0[p.groups];
-  const int chunk = (units + p.wide_ctas - 1) / p.wide_ctas;
-  const int u0 = static_cast<int>(blockIdx.x) * chunk, u1 = min(u0 + chunk, units);
-  if (u0 >= u1) return;
-
-  if (warp == 0) {
-    // the group of unit u0: the last with unit0[g] <= u0, found 32 at a time
-    int lo = 0, hi = p.groups;  // unit0[lo] <= u0 < unit0[hi]
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32;
-      const int at = lo + lane * step;
-      const unsigned le = __ballot_sync(0xffffffffu, at < hi && p.unit0[min(at, hi)] <= u0);
-      const int last = 31 - __clz(le);  // lane 0 always holds
-      lo += last * step;
-      hi = min(hi, lo + step);
-    }
-    if (lane == 0) *reinterpret_cast<volatile int*>(sm + C::BAR + 8 * C::B_PLACE) = lo;
-  }
   if (tid == 32) {
     mbar_init(bar(C::B_QREADY), 32 * W_SOFTMAX);
     mbar_init(bar(C::B_QEMPTY), 1);
@@ -153,9 +157,11 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       mbar_init(bar(C::B_PFULL + x), 16 * W_SOFTMAX);
       mbar_init(bar(C::B_ODONE + x), 1);
     }
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < KST; ++s) {
       mbar_init(bar(C::B_KFULL + s), I8 ? 128 : 1);
       mbar_init(bar(C::B_KEMPTY + s), 1);
+    }
+    for (int s = 0; s < VST; ++s) {
       mbar_init(bar(C::B_VFULL + s), I8 ? 128 : 1);
       mbar_init(bar(C::B_VEMPTY + s), 1);
     }
@@ -165,6 +171,23 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
     }
     fence_mbar_init();
   }
+  pdl_enter();
+  const int4 head = p.head[0];
+  const int s_first = static_cast<int>(blockIdx.x) / head.x * head.z;
+  if (static_cast<int>(blockIdx.x) / head.x >= head.y || s_first >= head.w) return;  // no team, or no steps for it
+  if (warp == 0) {
+    // the group of step s_first: the last with step0[g] <= s_first, found 32 at a time
+    int lo = 0, hi = p.groups;  // step0[lo] <= s_first < step0[hi]
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32;
+      const int at = lo + lane * step;
+      const unsigned le = __ballot_sync(0xffffffffu, at < hi && p.step0[min(at, hi)] <= s_first);
+      const int last = 31 - __clz(le);  // lane 0 always holds
+      lo += last * step;
+      hi = min(hi, lo + step);
+    }
+    if (lane == 0) *reinterpret_cast<volatile int*>(sm + C::BAR + 8 * C::B_PLACE) = lo;
+  }
   if (warp == W_MMA) {
     tmem_alloc(bar(C::B_SLOT), W_TMEM);
     tmem_relinquish();
@@ -173,121 +196,128 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + C::BAR + 8 * C::B_SLOT);
-  Pieces it;
-  it.begin(p, u0, u1, *reinterpret_cast<volatile int*>(sm + C::BAR + 8 * C::B_PLACE));
+  Pieces it(p, head, blockIdx.x, *reinterpret_cast<volatile int*>(sm + C::BAR + 8 * C::B_PLACE));
 
   if (warp == W_PRODUCER) {
     // ------------------------------------------------------------ producer
     // Lane i owns box i of every tile; the block ids of a tile are fetched one tile ahead.
     const int boxs = p.BS < 16 ? p.BS : 16;
     const int nbox = kWideKeys / boxs;  // <= 16 (block_size >= 8)
-    int gt = 0;
-    for (; it.left > 0; it.next(p)) {
-      const int* bt_row = p.bt + static_cast<long long>(it.lead) * p.bt_ss;
+    int gt = 0, gr = 0;  // tiles, and raw tiles, so far
+    while (it.next(p)) {
+      const int* bt_row = p.bt + static_cast<long long>(it.grp.w) * p.bt_ss;
       auto fetch = [&](int j) {
         const int key = (it.t + j) * kWideKeys + lane * boxs;
         int blk = p.NB;  // out of range: TMA fills the box with zeros
-        if (lane < nbox && key < it.keys) {
+        if (lane < nbox && key < it.grp.x) {
           const int x = bt_row[static_cast<long long>(key >> p.log2BS) * p.bt_sc];
           if (x >= 0 && x < p.NB) blk = x;
           else set_status(p.status, ST_BAD_BLOCK_ID);
         }
         return blk;
       };
-      const int n = it.tiles();
-      int blk = fetch(0);
-      for (int j = 0; j < n; ++j, ++gt) {
-        const int blk_next = j + 1 < n ? fetch(j + 1) : p.NB;
-        const int slot = blk < p.NB ? (it.t * kWideKeys + j * kWideKeys + lane * boxs) & (p.BS - 1) : 0;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          uint32_t dst, full;
-          if constexpr (I8) {
-            const int i = 2 * gt + v, s = i % C::RST;
-            full = bar(C::B_RFULL + s);
-            dst = base + C::R0 + s * C::RAW + lane * boxs * D;
-            if (lane == 0) {
-              if (i >= C::RST) wide_wait(p, bar(C::B_REMPTY + s), (i / C::RST - 1) & 1);
-              mbar_arrive_expect_tx(full, C::RAW);
-            }
-          } else {
-            const int s = gt % ST;
-            full = bar((v ? C::B_VFULL : C::B_KFULL) + s);
-            dst = base + (v ? C::V0 : C::K0) + s * TILE + lane * boxs * 128;
-            if (lane == 0) {
-              if (gt >= ST) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (gt / ST - 1) & 1);
-              mbar_arrive_expect_tx(full, TILE);
-            }
+      // The order of the loads is K0, K1 V0, K2 V1, ...: a key tile's K is wanted a product before its V, and a
+      // V stage comes free late.
+      auto load = [&](int v, int j, int blk) {
+        const int slot = blk < p.NB ? ((it.t + j) * kWideKeys + lane * boxs) & (p.BS - 1) : 0;
+        uint32_t dst, full;
+        if constexpr (I8) {
+          const int s = gr % C::RST;
+          full = bar(C::B_RFULL + s);
+          dst = base + C::R0 + s * C::RAW + lane * boxs * D;
+          if (lane == 0) {
+            if (gr >= C::RST) wide_wait(p, bar(C::B_REMPTY + s), (gr / C::RST - 1) & 1);
+            mbar_arrive_expect_tx(full, C::RAW);
           }
-          __syncwarp();
-          if (lane < nbox) {
-            const CUtensorMap* m = v ? &maps.v : &maps.k;
-            tma_load_4d(dst, m, full, 0, it.kvh, slot, blk);
-            if constexpr (!I8 && D == 128) tma_load_4d(dst + W_HALF, m, full, 64, it.kvh, slot, blk);
+          ++gr;
+        } else {
+          const int st = v ? VST : KST, g = gt + j, s = g % st;
+          full = bar((v ? C::B_VFULL : C::B_KFULL) + s);
+          dst = base + (v ? C::V0 : C::K0) + s * TILE + lane * boxs * 128;
+          if (lane == 0) {
+            if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
+            mbar_arrive_expect_tx(full, TILE);
           }
         }
-        blk = blk_next;
+        __syncwarp();
+        if (lane < nbox) {
+          const CUtensorMap* m = v ? &maps.v : &maps.k;
+          tma_load_4d(dst, m, full, 0, it.kvh, slot, blk);
+          if constexpr (!I8 && D == 128) tma_load_4d(dst + W_HALF, m, full, 64, it.kvh, slot, blk);
+        }
+      };
+      const int n = it.n;
+      int b0 = fetch(0), b1 = n > 1 ? fetch(1) : p.NB;
+      load(0, 0, b0);
+      for (int j = 0; j < n; ++j) {
+        const int b2 = j + 2 < n ? fetch(j + 2) : p.NB;
+        if (j + 1 < n) load(0, j + 1, b1);
+        load(1, j, b0);
+        b0 = b1;
+        b1 = b2;
       }
+      gt += n;
     }
   } else if (warp == W_MMA) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t IDESC_QK = instr_desc_f16(MMA_BF16, false, false, kWideRows, kWideKeys);
-      constexpr uint32_t IDESC_PV = instr_desc_f16(MMA_BF16, false, true, kWideRows, D);
-      int gt = 0, piece = 0;
-      int px[2] = {0, 0};  // probabilities taken of each stream
-      for (; it.left > 0; it.next(p), ++piece) {
-        const int n = it.tiles();
-        auto qk = [&](int j) {
-          const int x = j & 1, s = (gt + j) % ST;
-          wide_wait(p, bar(C::B_KFULL + s), ((gt + j) / ST) & 1);
-          tc_fence_after();
-          const uint64_t a = smem_desc(base, 16, 1024), b = smem_desc(base + C::K0 + s * TILE, 16, 1024);
-          const uint32_t d = tmem + 128u * x;
-          if constexpr (D == 128) {
-            tc_mma_ss_k128<W_HALF / 16, W_HALF / 16>(d, a, b, IDESC_QK);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tc_mma_ss(d, a + 2 * k, b + 2 * k, IDESC_QK, k > 0);
-          }
-          tc_commit(bar(C::B_SFULL + x));
-          tc_commit(bar(C::B_KEMPTY + s));
-          if (j == n - 1) tc_commit(bar(C::B_QEMPTY));
-        };
-        wide_wait(p, bar(C::B_QREADY), piece & 1);
+    // The whole warp walks along, one elected lane issues.
+    constexpr uint32_t IDESC_QK = instr_desc_f16(MMA_BF16, false, false, kWideRows, kWideKeys);
+    constexpr uint32_t IDESC_PV = instr_desc_f16(MMA_BF16, false, true, kWideRows, D);
+    int gt = 0, piece = 0;
+    int px0 = 0, px1 = 0;  // probabilities taken of each stream
+    for (; it.next(p); ++piece) {
+      // unit u: stream u & 1; both streams of a pair of row tiles take the same key tile
+      const int nu = it.units();
+      const bool two = it.two;
+      auto qk = [&](int u) {
+        const int x = u & 1, tile = gt + it.tile(u), s = tile % KST;
+        wide_wait(p, bar(C::B_KFULL + s), (tile / KST) & 1);
         tc_fence_after();
-        qk(0);
-        if (n > 1) qk(1);
-        for (int j = 0; j < n; ++j) {
-          const int x = j & 1, s = (gt + j) % ST;
-          wide_wait(p, bar(C::B_VFULL + s), ((gt + j) / ST) & 1);
-          wide_wait(p, bar(C::B_PFULL + x), px[x] & 1);
-          ++px[x];
-          tc_fence_after();
-          tc_mma_ts_seq<8>(tmem + W_OCOL + 128u * x, tmem + 128u * x, smem_desc(base + C::V0 + s * TILE, W_HALF, 1024),
-                           IDESC_PV, j >= 2 ? 1u : 0u);
-          tc_commit(bar(C::B_VEMPTY + s));
-          tc_commit(bar(C::B_ODONE + x));
-          if (j + 2 < n) qk(j + 2);
-        }
-        gt += n;
+        tc_elect_mma_ss<D / 16, W_HALF / 16, W_HALF / 16>(tmem + 128u * x, smem_desc(base + (two ? x * TILE : 0), 16, 1024),
+                                                          smem_desc(base + C::K0 + s * TILE, 16, 1024), IDESC_QK);
+        tc_elect_commit(bar(C::B_SFULL + x));
+        if (!two || x) tc_elect_commit(bar(C::B_KEMPTY + s));
+        if (u == nu - 1) tc_elect_commit(bar(C::B_QEMPTY));
+      };
+      wide_wait(p, bar(C::B_QREADY), piece & 1);
+      tc_fence_after();
+      qk(0);
+      if (nu > 1) qk(1);
+      for (int u = 0; u < nu; ++u) {
+        const int x = u & 1, tile = gt + it.tile(u), s = tile % VST;
+        wide_wait(p, bar(C::B_VFULL + s), (tile / VST) & 1);
+        wide_wait(p, bar(C::B_PFULL + x), (x ? px1 : px0) & 1);
+        px0 += x ^ 1;
+        px1 += x;
+        tc_fence_after();
+        tc_elect_mma_ts8(tmem + W_OCOL + 128u * x, tmem + 128u * x, smem_desc(base + C::V0 + s * TILE, W_HALF, 1024), IDESC_PV,
+                         u >= 2 ? 1u : 0u);
+        if (!two || x) tc_elect_commit(bar(C::B_VEMPTY + s));
+        tc_elect_commit(bar(C::B_ODONE + x));
+        if (u + 2 < nu) qk(u + 2);
       }
+      gt += it.n;
     }
   } else if (warp >= W_CONVERT) {
     // ------------------------------------------------------------ INT8 -> fp16 tiles
     if constexpr (I8) {
-      // Warp c converts rows 32 c .. 32 c + 31 of every tile; lane l holds the scales of row 32 c + l.
-      constexpr int CH = D / 16;        // 16-byte pieces of a raw row
-      constexpr int RPI = 32 / CH;      // rows an iteration of a warp
+      // Warp c converts rows 32 c .. 32 c + 31 of every tile; lane l holds the scales of row 32 c + l.  A lane takes 16
+      // dims of a row at a time.  The eight lanes that a shared-memory access serves at once are four pieces of rows a
+      // and a ^ 5: swizzled, those lie in different banks, in the raw tile (16 bytes a piece) as in the operand tile (twice
+      // 16 bytes, two apart).
+      constexpr int RPI = 32 / (D / 16);  // rows an iteration of a warp
       const int c = warp - W_CONVERT;
-      const int ch = lane % CH;
-      int gt = 0;
-      for (; it.left > 0; it.next(p)) {
-        const int* bt_row = p.bt + static_cast<long long>(it.lead) * p.bt_ss;
-        const int n = it.tiles();
+      const int half = D == 128 ? (lane >> 3) & 1 : 0;
+      const int ch = 4 * half + (lane & 3);                    // 16-byte piece of the raw row
+      const int pair = D == 128 ? lane >> 4 : lane >> 3;       // row pairs 0 5, 1 4, 2 7, 3 6 of eight rows
+      const int flip = (lane >> 2) & 1 ? 5 : 0;
+      int gt = 0, gr = 0;
+      while (it.next(p)) {
+        const int* bt_row = p.bt + static_cast<long long>(it.grp.w) * p.bt_ss;
+        const int n = it.n;
         auto block = [&](int j) {
           const int key = (it.t + j) * kWideKeys + 32 * c + lane;
-          return j < n && key < it.keys ? bt_row[static_cast<long long>(key >> p.log2BS) * p.bt_sc] : -1;
+          return j < n && key < it.grp.x ? bt_row[static_cast<long long>(key >> p.log2BS) * p.bt_sc] : -1;
         };
         auto scales = [&](int j, int blk, float& k, float& v) {
           k = v = 0.f;  // keys past the end, and of blocks outside the pool, are zeros
@@ -296,54 +326,71 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           k = load_scale(p.ks, blk * p.ks_sblk + slot * p.ks_sslot + it.kvh * p.ks_shead, p.scale_f32);
           v = load_scale(p.vs, blk * p.vs_sblk + slot * p.vs_sslot + it.kvh * p.vs_shead, p.scale_f32);
         };
-        float sk, sv, sk1, sv1;
-        scales(0, block(0), sk, sv);
-        int blk1 = block(1);
-        for (int j = 0; j < n; ++j, ++gt) {
-          const int blk2 = block(j + 2);
-          scales(j + 1, blk1, sk1, sv1);
-          const int s = gt % ST;
+        auto convert = [&](int v, int j, float mine) {
+          const int st = v ? VST : KST, g = gt + j, s = g % st, rs = gr % C::RST;
+          const unsigned char* src = sm + C::R0 + rs * C::RAW;
+          unsigned char* dst = sm + (v ? C::V0 : C::K0) + s * TILE;
+          wide_wait(p, bar(C::B_RFULL + rs), (gr / C::RST) & 1);
+          if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
+          ++gr;
+          auto rows = [&](auto fp32_scale) {
 #pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            const int i = 2 * gt + v, rs = i % C::RST;
-            const unsigned char* src = sm + C::R0 + rs * C::RAW;
-            unsigned char* dst = sm + (v ? C::V0 : C::K0) + s * TILE;
-            const float mine = v ? sv : sk;
-            wide_wait(p, bar(C::B_RFULL + rs), (i / C::RST) & 1);
-            if (gt >= ST) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (gt / ST - 1) & 1);
-#pragma unroll 4
             for (int k = 0; k < 32 / RPI; ++k) {
-              const int lr = k * RPI + lane / CH;  // row within the warp's 32
-              const int r = 32 * c + lr;
-              const float f = __shfl_sync(0xffffffffu, mine, lr);
+              const int lr = (D == 128 ? 8 * (k >> 1) + 2 * (k & 1) : 8 * k) + pair;  // row within the warp's 32
+              const int row = lr ^ flip;
+              const int r = 32 * c + row;
+              const float f = __shfl_sync(0xffffffffu, mine, row);
               const int at = D == 128 ? r * 128 + ((ch ^ (r & 7)) << 4) : r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
               const uint4 w = *reinterpret_cast<const uint4*>(src + at);
               const uint32_t x[4] = {w.x, w.y, w.z, w.w};
               uint32_t o[8];
+              if constexpr (decltype(fp32_scale)::value) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t a, b;
-                i8x4_to_f16x4(x[q], a, b);
-                const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a));
-                const float2 fb = __half22float2(*reinterpret_cast<__half2*>(&b));
-                o[2 * q] = pack_f16(fa.x * f, fa.y * f);
-                o[2 * q + 1] = pack_f16(fb.x * f, fb.y * f);
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t a, b;
+                  i8x4_to_f16x4(x[q], a, b);
+                  const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a));
+                  const float2 fb = __half22float2(*reinterpret_cast<__half2*>(&b));
+                  o[2 * q] = pack_f16(fa.x * f, fa.y * f);
+                  o[2 * q + 1] = pack_f16(fb.x * f, fb.y * f);
+                }
+              } else {
+                // an fp16 scale times a code has at most 18 significant bits: one rounding either way
+                const __half2 h = __float2half2_rn(f);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  i8x4_to_f16x4(x[q], o[2 * q], o[2 * q + 1]);
+                  __half2* y = reinterpret_cast<__half2*>(o + 2 * q);
+                  y[0] = __hmul2(y[0], h);
+                  y[1] = __hmul2(y[1], h);
+                }
               }
-              // dims 16 ch .. 16 ch + 15: two pieces of 64-column half ch / 4; the upper half's lanes store them the
-              // other way round, so that a row's lanes meet every bank once
-              const int half = ch >> 2, odd = half & 1;
-              unsigned char* row = dst + half * W_HALF + r * 128;
+              unsigned char* d = dst + half * W_HALF + r * 128;
               const int p0 = 2 * (ch & 3);
-              const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-              *reinterpret_cast<uint4*>(row + (((p0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-              *reinterpret_cast<uint4*>(row + (((p0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+              *reinterpret_cast<uint4*>(d + ((p0 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(d + (((p0 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
             }
-            fence_proxy_async_smem();
-            mbar_arrive(bar((v ? C::B_VFULL : C::B_KFULL) + s));
-            mbar_arrive(bar(C::B_REMPTY + rs));
-          }
-          sk = sk1, sv = sv1, blk1 = blk2;
+          };
+          if (p.scale_f32) rows(std::true_type{});
+          else rows(std::false_type{});
+          fence_proxy_async_smem();
+          mbar_arrive(bar((v ? C::B_VFULL : C::B_KFULL) + s));
+          mbar_arrive(bar(C::B_REMPTY + rs));
+        };
+        // in the order of the loads; the scales are fetched a tile ahead, the block ids two
+        float k0, v0, k1, v1, k2, v2;
+        scales(0, block(0), k0, v0);
+        scales(1, block(1), k1, v1);
+        int blk2 = block(2);
+        convert(0, 0, k0);
+        for (int j = 0; j < n; ++j) {
+          scales(j + 2, blk2, k2, v2);
+          blk2 = block(j + 3);
+          if (j + 1 < n) convert(0, j + 1, k1);
+          convert(1, j, v0);
+          v0 = v1, k1 = k2, v1 = v2;
         }
+        gt += n;
       }
     }
   } else {
@@ -354,42 +401,53 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
     const uint32_t scol = trow + 128u * x, ocol = trow + W_OCOL + 128u * x;
     float* xch = reinterpret_cast<float*>(sm + C::XCH);  // [2 streams][128 rows]
     const int per = p.maxq * p.G;
-    int done[2] = {0, 0};  // tiles of each stream
-    for (int piece = 0; it.left > 0; it.next(p), ++piece) {
-      const int n = it.tiles();
-      const int live = min(kWideRows, it.rows - it.rt * kWideRows);  // rows of this tile
-      const bool busy = 32 * (warp & 3) < live;                      // this warp holds one
-      // ---- Q: 16-byte pieces of the 128 rows, converted to the operand type, swizzled
-      if (piece > 0) wide_wait(p, bar(C::B_QEMPTY), (piece - 1) & 1);
-#pragma unroll 4
-      for (int i = 0; i < 128 * (D / 8) / 256; ++i) {
-        const int idx = i * 256 + tid;
-        const int row = idx / (D / 8), c = idx % (D / 8);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (row < live) {
-          const int R = it.rt * kWideRows + row;
+    int done[2] = {0, 0};  // units of each stream
+    int q_done = 0;
+    for (; it.next(p);) {
+      const int nu = it.units();
+      const bool two = it.two;
+      const int mine0 = two ? x * kWideRows : 0;                  // first row of this stream's tile
+      const int live = min(kWideRows, it.live - mine0);           // rows of it
+      const bool busy = 32 * (warp & 3) < live;                   // this warp holds one
+      // ---- Q: half a row a thread, converted to the operand type, swizzled
+      if (done[0] > 0) wide_wait(p, bar(C::B_QEMPTY), q_done & 1), ++q_done;
+#pragma unroll 1
+      for (int y = 0; y < (two ? 2 : 1); ++y) {
+        const int row = tid >> 1, c0 = (tid & 1) * (D / 16);
+        const int R = it.row0 + y * kWideRows + row;
+        uint4 w[D / 16];
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) w[c] = make_uint4(0, 0, 0, 0);
+        if (y * kWideRows + row < it.live) {
           const int m = R / per, rem = R - m * per;
-          const int qi = rem / p.G, b = it.first + m;
+          const int qi = rem / p.G, b = it.grp.y + m;
           if (qi < seq_rows(p, b)) {
-            w = *(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p.q) + q_seq_base(p, b) +
-                                                 (it.kvh * p.G + rem - qi * p.G) * p.q_sh + static_cast<long long>(qi) * p.q_sm) + c);
-            w.x = cvt_pair<QBF16, MMA_BF16>(w.x);
-            w.y = cvt_pair<QBF16, MMA_BF16>(w.y);
-            w.z = cvt_pair<QBF16, MMA_BF16>(w.z);
-            w.w = cvt_pair<QBF16, MMA_BF16>(w.w);
+            const uint4* src = reinterpret_cast<const uint4*>(
+                static_cast<const unsigned short*>(p.q) + q_seq_base(p, b) + (it.kvh * p.G + rem - qi * p.G) * p.q_sh +
+                static_cast<long long>(qi) * p.q_sm) + c0;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) w[c] = src[c];
           }
         }
-        *reinterpret_cast<uint4*>(sm + (c >> 3) * W_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          w[c].x = cvt_pair<QBF16, MMA_BF16>(w[c].x);
+          w[c].y = cvt_pair<QBF16, MMA_BF16>(w[c].y);
+          w[c].z = cvt_pair<QBF16, MMA_BF16>(w[c].z);
+          w[c].w = cvt_pair<QBF16, MMA_BF16>(w[c].w);
+          const int k = c0 + c;
+          *reinterpret_cast<uint4*>(sm + y * TILE + (k >> 3) * W_HALF + row * 128 + (((k & 7) ^ (row & 7)) << 4)) = w[c];
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(bar(C::B_QREADY));
 
       float m_ref = -INFINITY, l = 0.f;
-      for (int j = x; j < n; j += 2) {
-        wide_wait(p, bar(C::B_SFULL + x), (done[x] + (j >> 1)) & 1);
+      for (int u = x; u < nu; u += 2) {
+        wide_wait(p, bar(C::B_SFULL + x), (done[x] + (u >> 1)) & 1);
         tc_fence_after();
         if (busy) {
-          const int left = it.keys - (it.t + j) * kWideKeys;  // keys of this tile, maybe more than 128
+          const int left = it.grp.x - (it.t + it.tile(u)) * kWideKeys;  // keys of this tile, maybe more than 128
           // first look: the row's maximum.  The logits are read again below: 128 of them do not fit the registers
           // beside the rest, and a second read of TMEM is cheap
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -414,7 +472,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           bool resc = false;
           if (mx > m_ref + W_THRESHOLD) {  // also the first finite maximum
             alpha = ex2(m_ref - mx);
-            resc = j >= 2;  // O holds this stream's earlier tiles
+            resc = u >= 2;  // O holds this stream's earlier tiles
             m_ref = mx;
           }
           const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
@@ -468,10 +526,39 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         tc_fence_before();
         mbar_arrive(bar(C::B_PFULL + x));
       }
-      done[0] += (n + 1) / 2;
-      done[1] += n / 2;
-      // ---- end of the piece: the two streams' results joined and written ----------
-      const bool two = n > 1;
+      done[0] += (nu + 1) / 2;
+      done[1] += nu / 2;
+      // ---- end of the piece: its rows go to the workspace ---------------------------
+      const long long prow = shared_wide_row(p, it.sh, it.grp.y, it.seg, it.team, it.size, it.part, it.lane) + mine0;
+      const int rb = (warp & 3) * 32 + (lane & ~7);
+      // coalesced: the eight lanes of a group exchange their pieces, store k writes row 8 g + k
+      auto store = [&](uint4 (&ov)[8], int col) {
+        transpose8_u4(ov, lane & 7);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (rb + k < live) *reinterpret_cast<uint4*>(p.part_o + (prow + rb + k) * D + col + 4 * (lane & 7)) = ov[k];
+      };
+      if (two) {
+        wide_wait(p, bar(C::B_ODONE + x), (done[x] - 1) & 1);  // the stream's last P*V
+        tc_fence_after();
+        if (busy) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t a[32];
+            tmem_ld32(ocol + 32 * c, a);
+            tmem_wait_ld();
+            uint4 ov[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ov[i] = make_uint4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
+            store(ov, 32 * c);
+          }
+          if (r < live) *reinterpret_cast<float2*>(p.part_ml + (prow + r) * 2) = make_float2(m_ref, l);
+        }
+        tc_fence_before();
+        continue;
+      }
+      // one row tile: the two streams' results joined first
+      const bool both = nu > 1;
       float* mine = xch + x * 128 + r;
       const float* other = xch + (x ^ 1) * 128 + r;
       *mine = m_ref;
@@ -485,10 +572,11 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       const float Mu = M == -INFINITY ? 0.f : M;
       const float fm = ex2(m_ref - Mu), fo = ex2(m_o - Mu);
       const float f0 = x ? fo : fm, f1 = x ? fm : fo;
-      wide_wait(p, bar(C::B_ODONE), (done[0] - 1) & 1);  // every stream's last P*V
-      if (two) wide_wait(p, bar(C::B_ODONE + 1), (done[1] - 1) & 1);
+      // every stream's last P*V; past the exchange both have seen the S of their last unit, so that neither
+      // barrier is more than one phase behind
+      wide_wait(p, bar(C::B_ODONE), (done[0] - 1) & 1);
+      if (both) wide_wait(p, bar(C::B_ODONE + 1), (done[1] - 1) & 1);
       tc_fence_after();
-      const long long row0 = shared_wide_row(p, it.first, it.rows, it.kvh, it.rt, blockIdx.x);
       if (busy) {
         // this thread's stream names its half of the columns
 #pragma unroll 1
@@ -496,24 +584,19 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           const int col = (D / 2) * x + 32 * c;
           uint32_t a[32], b[32];
           tmem_ld32(trow + W_OCOL + col, a);
-          if (two) tmem_ld32(trow + W_OCOL + 128 + col, b);
+          if (both) tmem_ld32(trow + W_OCOL + 128 + col, b);
           tmem_wait_ld();
           uint4 ov[8];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             float v = __uint_as_float(a[i]) * f0;
-            if (two) v += __uint_as_float(b[i]) * f1;
+            if (both) v += __uint_as_float(b[i]) * f1;
             (&ov[i >> 2].x)[i & 3] = __float_as_uint(v);
           }
-          // coalesced: the eight lanes of a group exchange their pieces, store k writes row 8 g + k
-          transpose8_u4(ov, lane & 7);
-          const int rb = (warp & 3) * 32 + (lane & ~7);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (rb + k < live) *reinterpret_cast<uint4*>(p.part_o + (row0 + rb + k) * D + col + 4 * (lane & 7)) = ov[k];
+          store(ov, col);
         }
         if (x == 0 && r < live)
-          *reinterpret_cast<float2*>(p.part_ml + (row0 + r) * 2) = make_float2(M, l * fm + (two ? l_o * fo : 0.f));
+          *reinterpret_cast<float2*>(p.part_ml + (prow + r) * 2) = make_float2(M, l * fm + (both ? l_o * fo : 0.f));
       }
       // both streams' sums are read by all before the next piece's products overwrite them
       tc_fence_before();
