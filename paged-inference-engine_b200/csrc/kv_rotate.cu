@@ -12,13 +12,13 @@
 // multiply-add), so that the rows, and with them the INT8 codes, are those that
 // the same four elementary fp32 operations give anywhere else.
 //
-// Bound by HBM for prompts (each row is read and written once), by latency for a
-// decode step's few rows.  One warp per (token, unit): a unit is the K and V rows of HG
-// kv heads, or NL * RPI query rows, all loaded before the first is used; the
-// table row is loaded once a warp and serves all of the unit's rows, which is
-// why a unit does not cross tokens.  The partner dims of the halves form lie
-// R/2 dims away in the same row, that is in another lane of the same warp: they come by
-// shuffles of packed words instead of a second load.
+// Bound by the issue of instructions for prompts, by latency for a decode step's few rows.  One warp per (token, unit): a
+// unit is up to ROWS query rows, key rows or value rows of one token, all loaded before the first is
+// used; the table row is loaded once a warp and serves all of the unit's rows, which is why a unit does not cross tokens.
+// Where whole heads are rotated by halves (FULL), a lane takes the same few dims of both halves, so both of a pair are
+// its own and a cos and a sin serve two dims.  With fewer dims rotated, the partner lies
+// in another lane of the same warp and comes by shuffles of packed words.  16384 tokens of 32 + 8 + 8 heads, INT8
+// pool: 120 us with shuffles for all, K and V rows in one warp and arithmetic a value at a time.
 #include "pa_common.cuh"
 #include "quant.cuh"
 
@@ -26,17 +26,17 @@ namespace pa {
 namespace {
 
 constexpr int ROT_THREADS = 256;
+enum : int { ROT_HALVES = 0, ROT_PAIRS = 1, ROT_FULL = 2 };
 
 template <int IN, int D>
 struct RCfg {
   static constexpr int ESZ = IN == PA_DTYPE_F32 ? 4 : 2;
-  static constexpr int EPL = 16 / ESZ;  // elements per lane and load
+  static constexpr int EPL = 16 / ESZ;  // elements of a lane
   static constexpr int LPR = D / EPL;   // lanes per row
   static constexpr int RPI = 32 / LPR;  // rows per load instruction
-  static constexpr int NL = 4;          // loads per lane in flight
+  static constexpr int NL = 4;          // rows of a lane, in flight together
   static constexpr int ROWS = NL * RPI;
-  static constexpr int HG = ROWS / 2;   // kv heads of a unit (K and V rows)
-  static_assert(LPR <= 32 && 32 % LPR == 0 && ROWS % 2 == 0, "a row maps onto whole lanes");
+  static_assert(LPR <= 32 && 32 % LPR == 0, "a row maps onto whole lanes");
 };
 
 template <int IN, int EPL>
@@ -67,30 +67,68 @@ __device__ __forceinline__ uint4 pack_words(const float (&f)[EPL]) {
   }
 }
 
-// This lane's part of a table row: its dims' cos and sin.  HALVES: one each per
-// dim, the sin with the sign that the partner's product carries; pairs: one per pair.
-template <bool PAIRS, int EPL>
+// A lane's elements of a row: EPL neighbours, or (SPLIT) EPL / 2 neighbours of either half of the row.
+template <int D, int EPL, bool SPLIT>
+__device__ __forceinline__ int run_start(int part, int run) {
+  return SPLIT ? run * (D / 2) + part * (EPL / 2) : part * EPL + run * (EPL / 2);
+}
+template <int ESZ, int D, int EPL, bool SPLIT>
+__device__ __forceinline__ uint4 load_row(const char* row, int part) {
+  if constexpr (SPLIT) {
+    const uint2 a = *reinterpret_cast<const uint2*>(row + run_start<D, EPL, true>(part, 0) * ESZ);
+    const uint2 b = *reinterpret_cast<const uint2*>(row + run_start<D, EPL, true>(part, 1) * ESZ);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    return *reinterpret_cast<const uint4*>(row + part * EPL * ESZ);
+  }
+}
+// N bytes (2, 4, 8 or 16) of packed words.
+template <int N>
+__device__ __forceinline__ void store_bytes(char* at, const uint32_t* w) {
+  if constexpr (N == 2) *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w[0]);
+  else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(at) = w[0];
+  else if constexpr (N == 8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The lane's EPL elements as OSZ-byte values in the words w, to its one or two places in `row`.
+template <int OSZ, int D, int EPL, bool SPLIT>
+__device__ __forceinline__ void store_row(char* row, int part, const uint32_t* w) {
+  constexpr int RUN = EPL / 2 * OSZ;  // bytes of a run
+  if constexpr (SPLIT || RUN * 2 > 16) {
+    store_bytes<RUN>(row + run_start<D, EPL, SPLIT>(part, 0) * OSZ, w);
+    const uint32_t half = w[0] >> 16;  // (runs of two bytes: both in the first word)
+    store_bytes<RUN>(row + run_start<D, EPL, SPLIT>(part, 1) * OSZ, RUN == 2 ? &half : w + RUN / 4);
+  } else {
+    store_bytes<2 * RUN>(row + part * EPL * OSZ, w);
+  }
+}
+
+// This lane's part of a table row.  HALVES: a cos and a sin per dim, the sin with the sign that the partner's
+// product carries; PAIRS and FULL: one of each per pair.  (Scalar arithmetic: packed products, .rn or not, were found
+// contracted with the additions behind them.)
+template <int MODE, int EPL>
 struct Turn {
-  static constexpr int N = PAIRS ? EPL / 2 : EPL;
+  static constexpr int N = MODE == ROT_HALVES ? EPL : EPL / 2;
   float c[N], s[N];
-  int src;   // lane that holds the partner dims
+  int src;   // HALVES: lane that holds the partner dims
   bool on;   // dims below rot_dim
 
   __device__ __forceinline__ void load(const float* row, int rot, int part, int lane) {
-    const int d = part * EPL, half = rot >> 1;
-    on = d < rot;
+    const int half = rot >> 1;
+    const int d = part * EPL;
+    on = MODE == ROT_FULL || d < rot;
     src = lane;
     if (!on) return;
     float sign = 1.f;
-    int at = d >> 1;
-    if constexpr (!PAIRS) {
+    int at = part * (EPL / 2);
+    if constexpr (MODE == ROT_HALVES) {
       const bool low = d < half;  // half is a multiple of EPL: a lane's dims lie on one side
       sign = low ? -1.f : 1.f;
       src = low ? lane + half / EPL : lane - half / EPL;
       at = low ? d : d - half;
     }
 #pragma unroll
-    for (int i = 0; i < N; i += N < 4 ? N : 4) {
+    for (int i = 0; i < N; i += N < 4 ? 2 : 4) {
       if constexpr (N >= 4) {
         const float4 a = __ldg(reinterpret_cast<const float4*>(row + at + i));
         const float4 b = __ldg(reinterpret_cast<const float4*>(row + half + at + i));
@@ -100,25 +138,16 @@ struct Turn {
         const float2 a = __ldg(reinterpret_cast<const float2*>(row + at));
         const float2 b = __ldg(reinterpret_cast<const float2*>(row + half + at));
         c[0] = a.x, c[1] = a.y;
-        s[0] = b.x, s[1] = b.y;
+        s[0] = b.x * sign, s[1] = b.y * sign;
       }
     }
   }
 
-  // f: this lane's dims of a row, raw: the same as loaded (for the partner).  Every lane of the warp calls it.
+  // f: the rotated elements of a row, from those loaded.  Every lane of the warp calls it.
   template <int IN>
   __device__ __forceinline__ void apply(const uint4& raw, float (&f)[EPL]) const {
     unpack_words<IN, EPL>(raw, f);
-    if constexpr (PAIRS) {
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float a = f[2 * i], b = f[2 * i + 1];
-          f[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
-          f[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
-        }
-      }
-    } else {
+    if constexpr (MODE == ROT_HALVES) {
       uint4 o;
       o.x = __shfl_sync(0xffffffffu, raw.x, src);
       o.y = __shfl_sync(0xffffffffu, raw.y, src);
@@ -130,162 +159,181 @@ struct Turn {
 #pragma unroll
         for (int i = 0; i < EPL; ++i) f[i] = __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(g[i], s[i]));
       }
+    } else if (on) {
+#pragma unroll
+      for (int i = 0; i < EPL / 2; ++i) {
+        const int x = MODE == ROT_FULL ? i : 2 * i, y = MODE == ROT_FULL ? i + EPL / 2 : 2 * i + 1;
+        const float a = f[x], b = f[y];
+        f[x] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+        f[y] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+      }
     }
   }
 };
 
-template <int IN, int D, bool PAIRS>
-__global__ void __launch_bounds__(ROT_THREADS) kv_rotate_kernel(const WriteParams p, const RotateParams r) {
+// quant_row_fast on pairs of values: the codes' words, and whether a quotient lies near a rounding boundary.
+template <int EPL>
+__device__ __forceinline__ bool quant_pairs(const float (&f)[EPL], float inv, uint32_t* w) {
+  const uint64_t k = f2_pack(inv, inv), up = f2_pack(RNE_MAGIC, RNE_MAGIC), down = f2_pack(-RNE_MAGIC, -RNE_MAGIC);
+  const uint64_t minus = f2_pack(-1.f, -1.f);
+  float far = 0.f;
+  uint32_t b[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; i += 2) {
+    const uint64_t y = f2_fma(f2_pack(f[i], f[i + 1]), k, f2_pack(-0.f, -0.f));  // the product (near checks cover its rounding)
+    const uint64_t t = f2_add(y, up);
+    float d0, d1, t0, t1;
+    f2_unpack(f2_fma(f2_add(t, down), minus, y), d0, d1);  // y - rint(y)
+    f2_unpack(t, t0, t1);
+    far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+    b[i] = __float_as_uint(t0);
+    b[i + 1] = __float_as_uint(t1);
+  }
+#pragma unroll
+  for (int i = 0; i < EPL / 4; ++i) w[i] = pack_bytes(b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]);
+  return far > NEAR_HALF;
+}
+
+// One row of K or V into the pool: this lane's elements f (raw: as loaded), its row at element offset `at`, scale at `so`.
+template <int IN, int D, bool SPLIT>
+__device__ __forceinline__ void write_row(const WriteParams& p, const float (&f)[RCfg<IN, D>::EPL], const uint4& raw, bool same,
+                                          bool live, void* base, long long at, void* sbase, long long so, int part) {
+  using C = RCfg<IN, D>;
+  constexpr int EPL = C::EPL;
+  if (p.cache_dtype == PA_DTYPE_I8) {
+    float am = fmaxf(fabsf(f[0]), fabsf(f[1]));
+#pragma unroll
+    for (int i = 2; i < EPL; i += 2) am = fmax3f(am, fabsf(f[i]), fabsf(f[i + 1]));
+#pragma unroll
+    for (int o = C::LPR / 2; o >= 1; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+    const float sc = am == 0.f ? 1.0f : div127_rn(am);
+    uint32_t w[EPL / 4];
+    // the reciprocal of a scale below 2^-126 is not finite: such rows, too, take the division
+    const bool near = quant_pairs<EPL>(f, rcp_approx(sc), w) || sc < 1.2e-38f;
+    if (__any_sync(0xffffffffu, near)) quant_row_exact<EPL>(f, sc, w);
+    if (!live) return;
+    store_row<1, D, EPL, SPLIT>(static_cast<char*>(base) + at, part, w);
+    if (part == 0) {
+      if (p.scale_f32) static_cast<float*>(sbase)[so] = sc;
+      else static_cast<__half*>(sbase)[so] = __float2half_rn(sc);
+    }
+    return;
+  }
+  if (!live) return;
+  if (p.cache_dtype == PA_DTYPE_F32) {
+    store_row<4, D, EPL, SPLIT>(static_cast<char*>(base) + at * 4, part, reinterpret_cast<const uint32_t*>(f));
+    return;
+  }
+  const bool bf = p.cache_dtype == PA_DTYPE_BF16;
+  uint32_t w[EPL / 2];
+#pragma unroll
+  for (int i = 0; i < EPL / 2; ++i) w[i] = bf ? pack2<true>(f[2 * i], f[2 * i + 1]) : pack2<false>(f[2 * i], f[2 * i + 1]);
+  if constexpr (IN != PA_DTYPE_F32) {
+    if (same) {  // values of the pool's own type: the bits as they are
+      w[0] = raw.x, w[1] = raw.y, w[2] = raw.z, w[3] = raw.w;
+    }
+  }
+  store_row<2, D, EPL, SPLIT>(static_cast<char*>(base) + at * 2, part, w);
+}
+
+template <int IN, int D, int MODE>
+__global__ void __launch_bounds__(ROT_THREADS, 4) kv_rotate_kernel(const WriteParams p, const RotateParams r) {
   pdl_enter();
   using C = RCfg<IN, D>;
   constexpr int EPL = C::EPL;
+  constexpr bool SPLIT = MODE == ROT_FULL;
   const int lane = threadIdx.x & 31;
-  const int kv_units = (p.Hkv + C::HG - 1) / C::HG;
-  const int units = kv_units + (r.Hq + C::ROWS - 1) / C::ROWS;
+  const int kv_units = (p.Hkv + C::ROWS - 1) / C::ROWS;
+  const int q_units = (r.Hq + C::ROWS - 1) / C::ROWS;
+  const int units = q_units + 2 * kv_units;
   const long long wid = (static_cast<long long>(blockIdx.x) * ROT_THREADS + threadIdx.x) >> 5;
   if (wid >= static_cast<long long>(p.T) * units) return;
   const int t = static_cast<int>(wid / units);
-  const int u = static_cast<int>(wid - static_cast<long long>(t) * units);
+  int u = static_cast<int>(wid - static_cast<long long>(t) * units);
   const int part = lane % C::LPR;
   const int sub = lane / C::LPR;
-  const bool isq = u >= kv_units;
-  const int h0 = isq ? (u - kv_units) * C::ROWS : u * C::HG;
+  const int kind = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;  // queries, keys, values
+  u -= kind == 0 ? 0 : kind == 1 ? q_units : q_units + kv_units;
+  const int h0 = u * C::ROWS;
+  const int H = kind == 0 ? r.Hq : p.Hkv;
+  const char* src = static_cast<const char*>(kind == 0 ? r.q : kind == 1 ? p.k_new : p.v_new);
+  const long long src_t = kind == 0 ? r.q_st : kind == 1 ? p.kn_st : p.vn_st;
+  const long long src_h = kind == 0 ? r.q_sh : kind == 1 ? p.kn_sh : p.vn_sh;
 
-  // ---- source rows: row j of a kv unit is head h0 + j / 2, K for even j -------
   uint4 raw[C::NL];
 #pragma unroll
   for (int it = 0; it < C::NL; ++it) {
-    const int j = it * C::RPI + sub;
+    const int h = h0 + it * C::RPI + sub;
     raw[it] = make_uint4(0, 0, 0, 0);
-    if (isq) {
-      if (h0 + j < r.Hq)
-        raw[it] = *(reinterpret_cast<const uint4*>(static_cast<const char*>(r.q) +
-                                                   (t * r.q_st + (h0 + j) * r.q_sh) * C::ESZ) + part);
-    } else if (h0 + (j >> 1) < p.Hkv) {
-      const int h = h0 + (j >> 1);
-      const char* src = (j & 1) ? static_cast<const char*>(p.v_new) + (t * p.vn_st + h * p.vn_sh) * C::ESZ
-                                : static_cast<const char*>(p.k_new) + (t * p.kn_st + h * p.kn_sh) * C::ESZ;
-      raw[it] = __ldg(reinterpret_cast<const uint4*>(src) + part);
+    if (h < H) {
+      const char* row = src + (t * src_t + h * src_h) * C::ESZ;
+      raw[it] = kind < 2 ? load_row<C::ESZ, D, EPL, SPLIT>(row, part) : load_row<C::ESZ, D, EPL, false>(row, part);
     }
   }
   const int pos = p.pos[t];
+  const int s = kind == 0 ? 0 : p.seq_idx[t];
   if (pos < 0 || pos >= r.num_pos) {
     if (lane == 0) set_status(p.status, ST_BAD_POSITION);
     return;
   }
-  Turn<PAIRS, EPL> turn;
-  turn.load(r.table + pos * r.table_stride, r.rot, part, lane);
+  // the block and the angles at once: one more round of latency, not two
+  const int bi = pos >> p.log2BS;
+  const bool placed = s >= 0 && s < p.num_seqs && bi < p.bt_cols;
+  int blk = -1;
+  if (kind > 0 && placed) blk = p.bt[s * p.bt_ss + bi * p.bt_sc];
+  Turn<MODE, EPL> turn;
+  if (kind < 2) turn.load(r.table + pos * r.table_stride, r.rot, part, lane);
 
-  if (isq) {
+  if (kind == 0) {
 #pragma unroll
     for (int it = 0; it < C::NL; ++it) {
       const int h = h0 + it * C::RPI + sub;
       float f[EPL];
       turn.template apply<IN>(raw[it], f);
-      if (h < r.Hq)
-        *(reinterpret_cast<uint4*>(static_cast<char*>(r.q_out) + (t * r.qo_st + h * r.qo_sh) * C::ESZ) + part) =
-            pack_words<IN, EPL>(f);
+      if (h < H) {
+        const uint4 w = pack_words<IN, EPL>(f);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+        store_row<C::ESZ, D, EPL, SPLIT>(static_cast<char*>(r.q_out) + (t * r.qo_st + h * r.qo_sh) * C::ESZ, part, x);
+      }
     }
     return;
   }
-
-  // ---- destination block / slot (as kv_write_kernel) --------------------------
-  const int s = p.seq_idx[t];
-  if (s < 0 || s >= p.num_seqs) {
-    if (lane == 0) set_status(p.status, ST_BAD_SEQ_INDEX);
-    return;
-  }
-  const int bi = pos >> p.log2BS;
-  if (bi >= p.bt_cols) {
-    if (lane == 0) set_status(p.status, ST_BAD_POSITION);
-    return;
-  }
-  const int blk = p.bt[s * p.bt_ss + bi * p.bt_sc];
+  // ---- K and V rows, where kv_write_kernel puts them --------------------------
   if (blk < 0 || blk >= p.NB) {
-    if (lane == 0) set_status(p.status, ST_BAD_BLOCK_ID);
+    if (lane == 0)
+      set_status(p.status, placed ? ST_BAD_BLOCK_ID : (s < 0 || s >= p.num_seqs) ? ST_BAD_SEQ_INDEX : ST_BAD_POSITION);
     return;
   }
   const int slot = pos & (p.BS - 1);
-  const long long kb = blk * p.k_sblk + slot * p.k_sslot, vb = blk * p.v_sblk + slot * p.v_sslot;
-  const long long ksb = blk * p.ks_sblk + slot * p.ks_sslot, vsb = blk * p.vs_sblk + slot * p.vs_sslot;
-  const bool i8 = p.cache_dtype == PA_DTYPE_I8;
-  const bool f32 = p.cache_dtype == PA_DTYPE_F32;
-  const bool bf = p.cache_dtype == PA_DTYPE_BF16;
-
-  // rows stay in registers; the phases of an INT8 pool run over all of them, so that their shuffles overlap
-  float f[C::NL][EPL], am[C::NL];
-#pragma unroll
-  for (int it = 0; it < C::NL; ++it) {
-    const int j = it * C::RPI + sub;
-    turn.template apply<IN>(raw[it], f[it]);
-    if (j & 1) unpack_words<IN, EPL>(raw[it], f[it]);  // values are not rotated
-  }
-  if (i8) {
+  const bool same = kind == 2 && IN == p.cache_dtype;
+  const long long at0 = kind == 1 ? blk * p.k_sblk + slot * p.k_sslot : blk * p.v_sblk + slot * p.v_sslot;
+  const long long so0 = kind == 1 ? blk * p.ks_sblk + slot * p.ks_sslot : blk * p.vs_sblk + slot * p.vs_sslot;
+  if (kind == 1) {
 #pragma unroll
     for (int it = 0; it < C::NL; ++it) {
-      am[it] = fabsf(f[it][0]);
-#pragma unroll
-      for (int i = 1; i < EPL; ++i) am[it] = fmaxf(am[it], fabsf(f[it][i]));
+      const int h = h0 + it * C::RPI + sub;
+      float f[EPL];
+      turn.template apply<IN>(raw[it], f);
+      write_row<IN, D, SPLIT>(p, f, raw[it], false, h < H, p.k, at0 + h * p.k_shead, p.ks, so0 + h * p.ks_shead, part);
     }
+  } else {
 #pragma unroll
-    for (int o = C::LPR / 2; o >= 1; o >>= 1)
-#pragma unroll
-      for (int it = 0; it < C::NL; ++it) am[it] = fmaxf(am[it], __shfl_xor_sync(0xffffffffu, am[it], o));
-  }
-#pragma unroll
-  for (int it = 0; it < C::NL; ++it) {
-    const int j = it * C::RPI + sub;
-    const int h = h0 + (j >> 1);
-    const bool isv = j & 1;
-    const long long at = (isv ? vb + h * p.v_shead : kb + h * p.k_shead) + part * EPL;
-    void* base = isv ? p.v : p.k;
-    if (i8) {
-      const float sc = am[it] == 0.f ? 1.0f : div127_rn(am[it]);
-      uint32_t w[EPL / 4];
-      // the reciprocal of a scale below 2^-126 is not finite: such rows, too, take the division
-      const bool near = quant_row_fast<EPL>(f[it], rcp_approx(sc), w) || sc < 1.2e-38f;
-      if (__any_sync(0xffffffffu, near)) quant_row_exact<EPL>(f[it], sc, w);
-      if (h >= p.Hkv) continue;
-      int8_t* dst = static_cast<int8_t*>(base) + at;
-      if constexpr (EPL == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(dst) = w[0];
-      if (part == 0) {
-        const long long so = isv ? vsb + h * p.vs_shead : ksb + h * p.ks_shead;
-        void* sp = isv ? p.vs : p.ks;
-        if (p.scale_f32) static_cast<float*>(sp)[so] = sc;
-        else static_cast<__half*>(sp)[so] = __float2half_rn(sc);
-      }
-      continue;
+    for (int it = 0; it < C::NL; ++it) {
+      const int h = h0 + it * C::RPI + sub;
+      float f[EPL];
+      unpack_words<IN, EPL>(raw[it], f);
+      write_row<IN, D, false>(p, f, raw[it], same, h < H, p.v, at0 + h * p.v_shead, p.vs, so0 + h * p.vs_shead, part);
     }
-    if (h >= p.Hkv) continue;
-    if (f32) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
-#pragma unroll
-      for (int i = 0; i < EPL / 4; ++i) dst[i] = make_float4(f[it][4 * i], f[it][4 * i + 1], f[it][4 * i + 2], f[it][4 * i + 3]);
-      continue;
-    }
-    uint16_t* dst = static_cast<uint16_t*>(base) + at;
-    if constexpr (IN != PA_DTYPE_F32) {
-      if (isv && (IN == PA_DTYPE_BF16) == bf) {  // the same 16-bit type: the bits as they are
-        *reinterpret_cast<uint4*>(dst) = raw[it];
-        continue;
-      }
-    }
-    uint32_t w[EPL / 2];
-#pragma unroll
-    for (int i = 0; i < EPL / 2; ++i)
-      w[i] = bf ? pack2<true>(f[it][2 * i], f[it][2 * i + 1]) : pack2<false>(f[it][2 * i], f[it][2 * i + 1]);
-    if constexpr (EPL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
   }
 }
 
 template <int IN, int D>
 cudaError_t launch_rot(const WriteParams& p, const RotateParams& r, cudaStream_t stream) {
   using C = RCfg<IN, D>;
-  const long long units = (p.Hkv + C::HG - 1) / C::HG + (r.Hq + C::ROWS - 1) / C::ROWS;
+  const long long units = 2 * ((p.Hkv + C::ROWS - 1) / C::ROWS) + (r.Hq + C::ROWS - 1) / C::ROWS;
   const long long blocks = (p.T * units * 32 + ROT_THREADS - 1) / ROT_THREADS;
-  auto kern = r.pairs ? kv_rotate_kernel<IN, D, true> : kv_rotate_kernel<IN, D, false>;
+  auto kern = r.pairs ? kv_rotate_kernel<IN, D, ROT_PAIRS>
+              : r.rot == D ? kv_rotate_kernel<IN, D, ROT_FULL> : kv_rotate_kernel<IN, D, ROT_HALVES>;
   return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(ROT_THREADS), 0, stream, p, r);
 }
 
