@@ -787,7 +787,7 @@ struct SharedCall {
   bool tma;
   int kvk, nt;
   pa::DecodeLaunch plan;
-  size_t rec, tile, unit, grp, head, ml, o, total;
+  size_t rec, tile, unit, grp, head, info, ml, o, total;
 };
 
 int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging_t* pg, const pa_groups_t* gr,
@@ -847,12 +847,14 @@ int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging
   const long long rows = c.p.prefix_row0 +
                          (c.p.wide ? pa::kWideRoom * base_rows + 2LL * c.p.wide_ctas * pa::kWideRows
                                    : base_rows + static_cast<long long>(c.p.num_warps_total) * pa::kChunkCols);
+  if (rows > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "shared prefixes: %lld partial rows", rows);
   c.rec = 0;
   c.tile = align256(static_cast<size_t>(2) * a.B * sizeof(int4));
   c.unit = c.tile + align256((static_cast<size_t>(2) * a.B + 1) * sizeof(int));
   c.grp = c.unit + align256((static_cast<size_t>(gr->num_groups) + 1) * sizeof(int));
   c.head = c.grp + align256(static_cast<size_t>(gr->num_groups) * sizeof(int4));
-  c.ml = c.head + align256(sizeof(int4));
+  c.info = c.head + align256(sizeof(int4));
+  c.ml = c.info + align256(static_cast<size_t>(a.B) * sizeof(int4));
   c.o = c.ml + align256(static_cast<size_t>(rows) * 2 * sizeof(float));
   c.total = c.o + align256(static_cast<size_t>(rows) * kv->head_dim * sizeof(float));
   return PA_OK;
@@ -887,6 +889,7 @@ int shared_prefix_attn(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa
   p.tstart = reinterpret_cast<int*>(ws + c.tile);
   p.step0 = reinterpret_cast<int*>(ws + c.unit);
   p.head = reinterpret_cast<int4*>(ws + c.head);
+  p.info = reinterpret_cast<int4*>(ws + c.info);
   p.grp = reinterpret_cast<int4*>(ws + c.grp);
   p.part_ml = reinterpret_cast<float*>(ws + c.ml);
   p.part_o = reinterpret_cast<float*>(ws + c.o);

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   int* s_unit = s_count + G;        // [G + 1]
   int* s_tile = s_unit + G + 1;     // [2 B + 1]
   __shared__ int s_warp[32];
-  __shared__ int s_team;
+  __shared__ int s_team, s_total, s_run;
 
   int bad = 0;
   for (int i = tid; i <= G; i += T) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
       s_count[i] = 0;
     }
   }
-  if (tid == 0) s_team = 1;
+  if (tid == 0) s_team = 1, s_total = 0, s_run = INT_MAX;
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) set_status(p.status, ST_BAD_SEQ_INDEX);
 
@@ -123,22 +123,38 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   }
   __syncthreads();
   if (p.wide) {
-    const int team = s_team;
+    const int team = s_team, teams = p.wide_ctas / team;
     for (int g = tid; g < G; g += T) {
       int steps = 0;
       if (s_keys[g] > 0) {
         const WideShape s(s_keys[g], s_start[g + 1] - s_start[g], per, team);
-        steps = s.passes * p.Hkv * s.steps();
+        steps = s.steps();
+        s_lead[g] = s.passes;  // (the leader is in p.grp by now)
       }
       s_unit[g] = steps;
+      atomicAdd(&s_total, steps > 0 ? s_lead[g] * p.Hkv * steps : 0);
     }
+    __syncthreads();
+    // A run that crosses from one list entry into the next pays for two beginnings and ends (7 us against 1 us a
+    // step).  So, for few groups, the shortest run of which every entry takes whole ones, if no more of them than teams
+    // come together and it is not much longer than an equal share.
+    const int share = (s_total + teams - 1) / teams;
+    const int run = share + tid;
+    if (G <= 32 && share > 0 && tid <= 8 + share / 16) {
+      int runs = 0;
+      for (int g = 0; g < G; ++g)
+        if (s_unit[g] > 0) runs += s_lead[g] * p.Hkv * ((s_unit[g] + run - 1) / run);
+      if (runs <= teams) atomicMin(&s_run, run);
+    }
+    __syncthreads();
+    const bool pad = s_run != INT_MAX;
+    const int length = pad ? s_run : share;
+    for (int g = tid; g < G; g += T)
+      if (s_unit[g] > 0) s_unit[g] = s_lead[g] * p.Hkv * (pad ? (s_unit[g] + length - 1) / length * length : s_unit[g]);
     __syncthreads();
     scan_cta(s_unit, G, s_warp);
     for (int g = tid; g <= G; g += T) p.step0[g] = s_unit[g];
-    if (tid == 0) {
-      const int teams = p.wide_ctas / team;
-      p.head[0] = make_int4(team, teams, (s_unit[G] + teams - 1) / teams, s_unit[G]);
-    }
+    if (tid == 0) p.head[0] = make_int4(team, length, s_unit[G], pad);
   }
 
   for (int b = tid; b < B; b += T) {
@@ -148,13 +164,13 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
     if (g >= 0 && s_keys[g] > 0) {
       const int first = s_start[g], last = s_start[g + 1];
       if (p.wide) {
-        chunk.y = g;  // where prefix_merge_kernel finds the group (no keys: not a work list entry)
+        p.info[b] = make_int4(s_unit[g], 0, 0, 0);
         own.z = first;
         own.w = last - first;
       } else {
         const int lead = first + (b - first) / p.cpm * p.cpm;
         const int n = min(p.cpm, last - lead);
-        if (b == lead) chunk = make_int4(s_keys[g], 0, s_lead[g], n);
+        if (b == lead) chunk = make_int4(s_keys[g], 0, s_lead[g], n);  // (split-K form: the leader is still there)
         own.z = lead;
         own.w = n;
       }
@@ -171,27 +187,42 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   __syncthreads();
   scan_cta(s_tile, 2 * B, s_warp);
   for (int i = tid; i <= 2 * B; i += T) p.tstart[i] = s_tile[i];
+  if (!p.wide) {
+    for (int b = tid; b < B; b += T) {
+      const int g = bad ? -1 : group_of(s_start, G, b);
+      if (g < 0 || s_keys[g] == 0) continue;
+      const int lead = s_start[g] + (b - s_start[g]) / p.cpm * p.cpm;
+      p.info[b] = make_int4(s_tile[lead], s_tile[lead + 1] - s_tile[lead], 0, 0);
+    }
+  }
 }
 
-constexpr int MERGE_WARPS = 4;
+constexpr int MERGE_WARPS = 8;
 
-// Joins the pieces of every output row.  Grid (Hkv, B), a warp per column (query row and head): lane i reads the
-// statistics of piece i, 32 at a time; then all lanes add up the pieces' rows with their weights, 16 bytes a lane and
-// eight rows in flight.
-template <int D>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) prefix_merge_kernel(const SharedParams p) {
+// Joins the pieces of every output row.  Grid (Hkv * column sets, B); a column (query row and head) is taken by SHARE
+// warps, warp w having every SHARE-th piece: lane i reads the statistics of its i-th, then all lanes add up the pieces' rows with
+// their weights, 16 bytes a lane and eight rows in flight; the warps' results meet in shared memory.  Few rows are bound by
+// the latency of dependent loads: four warps a column, 5.7 us for one request of four beams against 9.8 with one.  Many
+// are bound by how many warps there is room for: one a column, 10 us for 128 sequences of 32 heads against 24 with four.
+template <int D, int SHARE>
+__global__ void __launch_bounds__(32 * MERGE_WARPS, 3) prefix_merge_kernel(const SharedParams p) {
   pdl_enter();
-  const int kvh = blockIdx.x, b = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float s_o[SHARE > 1 ? MERGE_WARPS : 1][D];
+  __shared__ float2 s_ml[MERGE_WARPS];
+  constexpr int COLS = MERGE_WARPS / SHARE;
+  const int b = blockIdx.y;
   const int per = p.maxq * p.G;
+  const int sets = (per + COLS - 1) / COLS;
+  const int kvh = blockIdx.x / sets;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = (blockIdx.x - kvh * sets) * COLS + warp / SHARE;
+  const int share = warp % SHARE;
   const int rows = seq_rows(p, b);
   const int4 own = p.rec[p.B + b];
-  const int g = p.rec[b].y;
+  const int4 info = p.info[b];
   const int t_own = p.tstart[p.B + b], n_own = p.tstart[p.B + b + 1] - t_own;
   const int tiles = p.tstart[2 * p.B];
-  const int4 head = p.wide ? p.head[0] : make_int4(1, 0, 1, 0);
-  const int cols = rows * p.G;
-  if (warp >= cols) return;
+  const int4 head = p.wide ? p.head[0] : make_int4(1, 1, 0, 0);
   const int chunk = max(p.min_chunk, (tiles * p.Hkv + p.num_warps_total - 1) / p.num_warps_total);
   int o0 = 0, on = 0;  // first piece of the sequence's own keys, pieces
   if (n_own > 0) {
@@ -200,106 +231,126 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) prefix_merge_kernel(const Sh
     on = (s0 + n_own - 1) / chunk - o0 + 1;
   }
   if (own.y == 0 && on == 1) return;  // written by the split-K kernel
+  const bool mine = col < rows * p.G;
+  if (SHARE == 1 && !mine) return;
   const bool wide = p.wide && own.y > 0;
+  // pieces of the shared part: `cn`, the first of worker or team f0
   WideShape shape;
-  int step0 = 0;
+  int f0 = 0, cn = 0, s0 = 0;
+  int crow = 0;  // (partial rows fit 32 bits: checked on the host)
   if (wide) {
     shape = WideShape(own.y, own.w, per, head.x);
-    step0 = p.step0[g];
+    const int R = (b - own.z) * per + col;
+    int rp = R / (2 * kWideRows), seg = kvh;
+    const int in_pair = R - rp * 2 * kWideRows;
+    if (shape.passes > 1) {
+      seg += rp / shape.lanes * p.Hkv;
+      rp %= shape.lanes;
+    }
+    s0 = info.x + seg * shape.padded(head.y, head.w);
+    f0 = s0 / head.y;
+    cn = ((s0 + shape.steps() - 1) / head.y - f0 + 1) << shape.lparts;
+    crow = static_cast<int>(shared_wide_row(p, shape, own.z, seg, f0, head.x, 0, rp)) + in_pair;
+  } else if (own.y > 0) {
+    s0 = info.x * p.Hkv + kvh * info.y;
+    f0 = s0 / chunk;
+    cn = (s0 + info.y - 1) / chunk - f0 + 1;
+    crow = static_cast<int>(shared_chunk_row(p, own.z, own.w, kvh, f0)) + (b - own.z) * per + col;
   }
+  const int orow = static_cast<int>(shared_own_row(p, b, kvh, o0)) + col;
+  // the partial row of piece i, or -1 where a team's part is empty
+  auto piece = [&](int i) -> int {
+    if (i < on) return orow + i * per;
+    i -= on;
+    if (!wide) return crow + i * kChunkCols;
+    const int t = i >> shape.lparts, q = i - (t << shape.lparts);
+    const int a = (f0 + t) * head.y - s0;
+    int n;
+    wide_tiles(shape, max(0, a), min(shape.steps(), a + head.y), q, n);
+    return n > 0 ? crow + t * head.x * 2 * kWideRows + q * shape.lanes * shape.room : -1;
+  };
+  const int np = mine ? on + cn : 0;
   constexpr int LPR = D / 4;     // lanes of a row (16 bytes each)
   constexpr int RPI = 32 / LPR;  // rows of a load instruction
   const int sub = lane / LPR, at = lane % LPR;
-  for (int col = warp; col < cols; col += MERGE_WARPS) {
-    // pieces of the shared part: `cn`, the first of worker or team f0
-    int f0 = 0, cn = 0, s0 = 0;
-    long long crow = 0;
-    if (wide) {
-      const int R = (b - own.z) * per + col;
-      int rp = R / (2 * kWideRows), seg = kvh;
-      const int in_pair = R - rp * 2 * kWideRows;
-      if (shape.passes > 1) {
-        seg += rp / shape.lanes * p.Hkv;
-        rp %= shape.lanes;
-      }
-      s0 = step0 + seg * shape.steps();
-      f0 = s0 / head.z;
-      cn = ((s0 + shape.steps() - 1) / head.z - f0 + 1) << shape.lparts;
-      crow = shared_wide_row(p, shape, own.z, seg, f0, head.x, 0, rp) + in_pair;
-    } else if (own.y > 0) {
-      const int t0 = p.tstart[own.z], n = p.tstart[own.z + 1] - t0;
-      s0 = t0 * p.Hkv + kvh * n;
-      f0 = s0 / chunk;
-      cn = (s0 + n - 1) / chunk - f0 + 1;
-      crow = shared_chunk_row(p, own.z, own.w, kvh, f0) + (b - own.z) * per + col;
-    }
-    const long long orow = shared_own_row(p, b, kvh, o0) + col;
-    // the partial row of piece i, or -1 where a team's part is empty
-    auto piece = [&](int i) -> long long {
-      if (i < on) return orow + static_cast<long long>(i) * per;
-      i -= on;
-      if (!wide) return crow + static_cast<long long>(i) * kChunkCols;
-      const int t = i >> shape.lparts, q = i - (t << shape.lparts);
-      const int a = (f0 + t) * head.z - s0;
-      int n;
-      wide_tiles(shape, max(0, a), min(shape.steps(), a + head.z), q, n);
-      return n > 0 ? crow + static_cast<long long>(t) * head.x * 2 * kWideRows + q * shape.lanes * shape.room : -1;
-    };
-    const int np = on + cn;
-    float M = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int base = 0; base < np; base += 32) {
-      long long r = -1;
-      if (base + lane < np) r = piece(base + lane);
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (r >= 0) ml = *reinterpret_cast<const float2*>(p.part_ml + r * 2);
-      // join with what the pieces before gave
-      const float Mn = fmaxf(M, warp_max_xor(ml.x, 1));
-      const float Mu = Mn == -INFINITY ? 0.f : Mn;
-      const float old = ex2(M - Mu), f = ex2(ml.x - Mu);
-      M = Mn;
-      l = l * old + ml.y * f;
-      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-      const int n = min(32, np - base);
+  float M = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = share; base < np; base += 32 * SHARE) {
+    const int i = base + lane * SHARE;
+    const int r = i < np ? piece(i) : -1;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (r >= 0) ml = reinterpret_cast<const float2*>(p.part_ml)[r];
+    // joined with what the pieces before gave
+    const float Mn = fmaxf(M, warp_max_xor(ml.x, 1));
+    const float Mu = Mn == -INFINITY ? 0.f : Mn;
+    const float old = ex2(M - Mu), f = ex2(ml.x - Mu);
+    M = Mn;
+    l = l * old + ml.y * f;
+    acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+    const int n = min(32, (np - base + SHARE - 1) / SHARE);
 #pragma unroll 1
-      for (int j0 = 0; j0 < n; j0 += 8 * RPI) {
-        float4 v[8];
-        float w[8];
+    for (int j0 = 0; j0 < n; j0 += 8 * RPI) {
+      float4 v[8];
+      float w[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int j = j0 + k * RPI + sub;
-          const long long rj = __shfl_sync(0xffffffffu, r, j & 31);
-          w[k] = __shfl_sync(0xffffffffu, f, j & 31);
-          v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (j < n && rj >= 0) v[k] = *reinterpret_cast<const float4*>(p.part_o + rj * D + 4 * at);
-          else w[k] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          acc.x += v[k].x * w[k], acc.y += v[k].y * w[k], acc.z += v[k].z * w[k], acc.w += v[k].w * w[k];
-        }
+      for (int k = 0; k < 8; ++k) {
+        const int j = j0 + k * RPI + sub;
+        const int rj = __shfl_sync(0xffffffffu, r, j & 31);
+        w[k] = __shfl_sync(0xffffffffu, f, j & 31);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < n && rj >= 0) v[k] = *reinterpret_cast<const float4*>(p.part_o + static_cast<long long>(rj) * D + 4 * at);
+        else w[k] = 0.f;
       }
-    }
-    l = warp_sum_xor(l, 1);
 #pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
-      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
-      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
-      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+      for (int k = 0; k < 8; ++k) acc.x += v[k].x * w[k], acc.y += v[k].y * w[k], acc.z += v[k].z * w[k], acc.w += v[k].w * w[k];
     }
+  }
+  l = warp_sum_xor(l, 1);
+#pragma unroll
+  for (int o = LPR; o < 32; o <<= 1) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+  }
+  const int qi = col / p.G, hq = col - qi * p.G + kvh * p.G;
+  __half* out = static_cast<__half*>(p.o) + o_seq_base(p, b) + hq * p.o_sh + static_cast<long long>(qi) * p.o_sm;
+  auto store_lse = [&](float m, float sum) {
+    const float L = sum > 0.f ? (m + lg2(sum)) * 0.6931471805599453f : -INFINITY;
+    static_cast<__half*>(p.lse)[l_seq_base(p, b) + hq * p.l_sh + static_cast<long long>(qi) * p.l_sm] = __float2half_rn(L);
+  };
+  if constexpr (SHARE == 1) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int qi = col / p.G, hq = col - qi * p.G + kvh * p.G;
     if (sub == 0) {
-      __half2* out = reinterpret_cast<__half2*>(static_cast<__half*>(p.o) + o_seq_base(p, b) + hq * p.o_sh +
-                                                static_cast<long long>(qi) * p.o_sm + 4 * at);
-      out[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
-      out[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+      reinterpret_cast<__half2*>(out + 4 * at)[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
+      reinterpret_cast<__half2*>(out + 4 * at)[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
     }
-    if (lane == 0 && p.lse) {
-      const float L = l > 0.f ? (M + lg2(l)) * 0.6931471805599453f : -INFINITY;
-      static_cast<__half*>(p.lse)[l_seq_base(p, b) + hq * p.l_sh + static_cast<long long>(qi) * p.l_sm] = __float2half_rn(L);
+    if (lane == 0 && p.lse) store_lse(M, l);
+  } else {
+    if (sub == 0) *reinterpret_cast<float4*>(&s_o[warp][4 * at]) = acc;
+    if (lane == 0) s_ml[warp] = make_float2(M, l);
+    __syncthreads();
+    if (!mine || share != 0) return;
+    float Mt = M;
+#pragma unroll
+    for (int k = 1; k < SHARE; ++k) Mt = fmaxf(Mt, s_ml[warp + k].x);
+    const float Mu = Mt == -INFINITY ? 0.f : Mt;
+    float lt = 0.f;
+    float o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < SHARE; ++k) {
+      const float f = ex2(s_ml[warp + k].x - Mu);
+      lt += s_ml[warp + k].y * f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] += s_o[warp + k][lane * (D / 32) + i] * f;
     }
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+      reinterpret_cast<__half2*>(out + lane * (D / 32))[i] = __floats2half2_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
+    if (lane == 0 && p.lse) store_lse(Mt, lt);
   }
 }
 
@@ -318,8 +369,14 @@ cudaError_t launch_prefix_plan(const SharedParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_prefix_merge(const SharedParams& p, int D, cudaStream_t stream) {
-  return launch_pdl(D == 64 ? prefix_merge_kernel<64> : prefix_merge_kernel<128>, dim3(p.Hkv, p.B), dim3(32 * MERGE_WARPS), 0,
-                    stream, p);
+  const int per = p.maxq * p.G;
+  auto go = [&](auto kern, int share) {
+    const int cols = MERGE_WARPS / share;
+    return launch_pdl(kern, dim3(p.Hkv * ((per + cols - 1) / cols), p.B), dim3(32 * MERGE_WARPS), 0, stream, p);
+  };
+  if (static_cast<long long>(p.B) * p.Hkv * per <= 8 * device_sm_count())
+    return D == 64 ? go(prefix_merge_kernel<64, 4>, 4) : go(prefix_merge_kernel<128, 4>, 4);
+  return D == 64 ? go(prefix_merge_kernel<64, 1>, 1) : go(prefix_merge_kernel<128, 1>, 1);
 }
 
 }  // namespace pa

@@ -78,6 +78,8 @@ __device__ __forceinline__ void wide_barrier(int id, int n) { asm volatile("bar.
 struct Pieces {
   int s, s1;          // steps of the team's run not walked yet
   int team, q, size;  // team, the CTA's place in it, CTAs of a team
+  int run;
+  bool pad;
   int g, base;        // group and its first step
   int4 grp;           // shared keys, first sequence, sequences, leader
   WideShape sh;
@@ -91,8 +93,10 @@ struct Pieces {
     size = head.x;
     team = cta / size;
     q = cta - team * size;
-    s = min(team * head.z, head.w);
-    s1 = min(s + head.z, head.w);
+    run = head.y;
+    pad = head.w != 0;
+    s = min(team * run, head.z);
+    s1 = min(s + run, head.z);
     g = g0 - 1;
     base = -1;
     if (s < s1) {
@@ -107,7 +111,7 @@ struct Pieces {
   }
   __device__ __forceinline__ bool next(const SharedParams& p) {
     while (s < s1) {
-      const int len = sh.steps();
+      const int len = sh.padded(run, pad);
       if (s - base >= sh.passes * p.Hkv * len) {  // a group with steps is still ahead
         do {
           ++g;
@@ -125,7 +129,8 @@ struct Pieces {
       part = q / sh.lanes;
       lane = q - part * sh.lanes;
       if (part >> sh.lparts || lane >= lanes) continue;
-      t = wide_tiles(sh, a, b, part, n);
+      if (a >= sh.steps()) continue;
+      t = wide_tiles(sh, a, min(b, sh.steps()), part, n);
       if (n <= 0) continue;
       row0 = (pass * sh.lanes + lane) * 2 * kWideRows;
       live = min(2 * kWideRows, sh.rows - row0);
@@ -173,8 +178,9 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
   }
   pdl_enter();
   const int4 head = p.head[0];
-  const int s_first = static_cast<int>(blockIdx.x) / head.x * head.z;
-  if (static_cast<int>(blockIdx.x) / head.x >= head.y || s_first >= head.w) return;  // no team, or no steps for it
+  const int team = static_cast<int>(blockIdx.x) / head.x;
+  const int s_first = team * head.y;
+  if (team >= p.wide_ctas / head.x || s_first >= head.z) return;  // no whole team, or no steps for it
   if (warp == 0) {
     // the group of step s_first: the last with step0[g] <= s_first, found 32 at a time
     int lo = 0, hi = p.groups;  // step0[lo] <= s_first < step0[hi]
