@@ -53,8 +53,8 @@ if _PKG_ROOT not in sys.path:
 
 from pie_b200 import ops as _ops  # noqa: E402
 
-__all__ = ["flash_attention_forward", "flash_attention_varlen", "FlashAttentionFunction", "write_kv_cache",
-           "project_write_kv_cache"]
+__all__ = ["flash_attention_forward", "flash_attention_varlen", "flash_attention_shared_prefix", "FlashAttentionFunction",
+           "write_kv_cache", "rotate_write_kv_cache", "project_write_kv_cache"]
 
 
 def flash_attention_forward(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, q_len_per_seq, block_table,
@@ -91,6 +91,21 @@ def flash_attention_varlen(q, cu_seqlens_q, K, V, block_table, num_blocks_per_se
                                        lse=lse, causal_top_left=causal_top_left, softmax_scale=softmax_scale)
 
 
+def flash_attention_shared_prefix(Q, K, V, q_len_per_seq, block_table, num_blocks_per_seq, block_size, kv_len_per_seq,
+                                  group_start, prefix_len, k_scale_ptr=None, v_scale_ptr=None, *, out=None, lse=None,
+                                  softmax_scale=None):
+    """flash_attention_forward of decode rows whose sequences share prefixes; returns (O, L) float16.
+
+    Sequences ``group_start[g] : group_start[g + 1]`` (int32 on the device) have the same blocks in the first
+    ``prefix_len[g]`` tokens of their tables, as forks of one prompt have; a group reads those once instead of once
+    per sequence.  At most 16 query rows times heads per KV head.
+    """
+    assert Q.is_cuda and K.is_cuda and V.is_cuda, "Not CUDA Tensors -_-"
+    return _ops.shared_prefix_attention(Q, K, V, q_len_per_seq, block_table, num_blocks_per_seq, int(block_size),
+                                        kv_len_per_seq, group_start, prefix_len, k_scale_ptr, v_scale_ptr, out=out, lse=lse,
+                                        softmax_scale=softmax_scale)
+
+
 class FlashAttentionFunction(torch.autograd.Function):
     """Autograd wrapper (forward only), as kernels/flash_attention.py:175-180."""
 
@@ -118,6 +133,19 @@ def write_kv_cache(k_new, v_new, block_table, seq_index, positions, k_cache, v_c
     """
     assert k_new.is_cuda and k_cache.is_cuda, "Not CUDA Tensors -_-"
     _ops.write_kv(k_new, v_new, block_table, seq_index, positions, k_cache, v_cache, k_scale, v_scale)
+
+
+def rotate_write_kv_cache(q, k_new, v_new, cos_sin, block_table, seq_index, positions, k_cache, v_cache, k_scale=None,
+                          v_scale=None, *, interleaved=False, q_out=None):
+    """write_kv_cache of keys rotated by their positions; returns the queries ``q`` [T, H, D] rotated alike.
+
+    ``cos_sin`` [num_positions, rot_dim] float32 holds each position's cosines, then its sines (``ops.rope_table``).  The
+    reference model rotates neither (transformer/model.py:75-82); models that do would otherwise read and write the rows
+    once more before the append.
+    """
+    assert k_new.is_cuda and k_cache.is_cuda, "Not CUDA Tensors -_-"
+    return _ops.rotate_write_kv(q, k_new, v_new, cos_sin, block_table, seq_index, positions, k_cache, v_cache, k_scale,
+                                v_scale, interleaved=interleaved, q_out=q_out)
 
 
 def project_write_kv_cache(x, w_kv, bias, block_table, seq_index, positions, k_cache, v_cache, k_scale=None,

@@ -203,6 +203,35 @@ class BlockLedger:
             node = node.up
         return n
 
+    def shared_runs(self, seq_ids: Sequence[int]) -> tuple[list[int], list[int]]:
+        """Neighbours in ``seq_ids`` whose first columns are the same: (where each run begins, and the end; its columns).
+
+        A sequence joins the run before it where the run's sequences then read no fewer columns together than without it.
+        """
+        starts, columns = [0], []
+        run: list[_Prefix] = []
+        width = 0
+        for i, s in enumerate(seq_ids):
+            path, node = [], self.prefix.get(s)
+            while node is not None:
+                path.append(node)
+                node = node.up
+            path.reverse()
+            n = i - starts[-1]
+            if n:
+                both = [a for a, b in zip(run, path) if a is b]
+                shared = sum(a.n for a in both)
+                if shared and shared * n >= width * (n - 1):
+                    run, width = both, shared
+                    continue
+                starts.append(i)
+                columns.append(width if n > 1 else 0)
+            run, width = path, sum(a.n for a in path)
+        if seq_ids:
+            columns.append(width if len(seq_ids) - starts[-1] > 1 else 0)
+            starts.append(len(seq_ids))
+        return starts, columns
+
     def fork(self, parent_id: int, child_id: int, num_tokens: int, block_size: int) -> tuple[AllocStatus, int]:
         """The child gets the parent's first tokens: (status, the child's slot); queues the operation on success."""
         self._alone(parent_id)
@@ -608,6 +637,25 @@ class DeviceBlockManager:
                 self._stream()))
         return dict(block_table=bt, num_blocks_per_seq=nb, q_len=ql, kv_len=kl, cu_seqlens=cus, positions=pos,
                     token_seq=tseq)
+
+    def shared_prefixes(self, sequence_ids: Sequence[int]) -> dict:
+        """Which neighbours of ``sequence_ids`` share their first blocks, for ``ops.shared_prefix_attention``.
+
+        Returns ``group_start`` [G + 1] and ``prefix_len`` [G] (tokens in whole blocks; 0 for a sequence that shares none
+        with its neighbours), int32 on the device.  Forks of one sequence should stand side by side in the step's order.
+        From the host's ledger: one host-to-device copy, nothing is read back.
+        """
+        starts, columns = self.shared_runs(sequence_ids)
+        host = torch.tensor(starts + [c * self.block_size for c in columns], dtype=torch.int32).pin_memory()
+        dev = host.to(self.device, non_blocking=True)
+        return dict(group_start=dev[:len(starts)], prefix_len=dev[len(starts):])
+
+    def shared_runs(self, sequence_ids: Sequence[int]) -> tuple[list[int], list[int]]:
+        """``shared_prefixes`` as host lists: where each group begins (and the end), and the blocks that it shares."""
+        ids = [s if s in self.ledger.slot else int(s) for s in sequence_ids]
+        for s in ids:
+            self.ledger.row(s)
+        return self.ledger.shared_runs(ids)
 
     def step_rows(self, seq_slot: torch.Tensor, q_len: torch.Tensor, kv_len: torch.Tensor, cu_seqlens: torch.Tensor,
                   total_tokens: int, block_table: torch.Tensor, num_blocks: torch.Tensor, positions: torch.Tensor,

@@ -12,8 +12,11 @@ step with one graph replay:
   2. ``block_pool_step``: padded block table, block counts and each new
      token's position and row, from the device-resident block pool;
   3. ``write_kv``: the new K/V rows into the paged cache (quantise-on-write for
-     INT8 pools);
-  4. paged attention of every sequence's new query over its whole cache.
+     INT8 pools), or with a ``rope`` table ``rotate_write_kv``, which also turns
+     the new queries by their positions;
+  4. paged attention of every sequence's new query over its whole cache, or with
+     ``share_prefixes`` ``shared_prefix_attention``: sequences forked from one
+     another that stand side by side in a step read their common blocks once.
 
 Decode positions follow the sequence: a sequence holding ``n`` tokens after
 this step's append writes its new token at position ``n - 1`` and attends to
@@ -44,8 +47,10 @@ class DecodeStepGraph:
 
     def __init__(self, pool: DeviceBlockManager, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], num_q_heads: int, max_seqs: int,
-                 q_dtype: torch.dtype = torch.float16):
+                 q_dtype: torch.dtype = torch.float16, *, rope: Optional[torch.Tensor] = None, interleaved: bool = False,
+                 share_prefixes: bool = False):
         self.pool = pool
+        self.rope, self.interleaved, self.share = rope, bool(interleaved), bool(share_prefixes)
         self.K, self.V, self.ks, self.vs = k_cache, v_cache, k_scale, v_scale
         self.dev = k_cache.device
         NB, BS, Hkv, D = k_cache.shape
@@ -64,9 +69,10 @@ class DecodeStepGraph:
         # two pinned staging buffers and two graphs, used by alternate steps: a
         # step fills the buffer the replay two steps back read, after that
         # replay's event, so the host never waits for the step just enqueued
-        self.staging = [torch.zeros(2 * S, dtype=torch.int32).pin_memory() for _ in range(2)]
+        words = 4 * S + 1 if self.share else 2 * S
+        self.staging = [torch.zeros(words, dtype=torch.int32).pin_memory() for _ in range(2)]
         self.events: list = [None, None]
-        self.meta = torch.zeros(2 * S, **i32)               # [slots | kv_len]
+        self.meta = torch.zeros(words, **i32)               # [slots | kv_len | group_start | prefix_len]
         self.q_len = torch.ones(S, **i32)
         self.cu = torch.arange(S + 1, **i32)
         self.block_table = torch.zeros(S, self.cols, **i32)
@@ -85,11 +91,22 @@ class DecodeStepGraph:
     def _body(self, k: int) -> None:
         S = self.S
         self.meta.copy_(self.staging[k], non_blocking=True)
-        slots, kv_len = self.meta[:S], self.meta[S:]
+        slots, kv_len = self.meta[:S], self.meta[S:2 * S]
         self.pool.step_rows(slots, self.q_len, kv_len, self.cu, S, self.block_table, self.num_blocks, self.positions,
                             self.token_seq, self.status)
-        ops.write_kv(self.k_new, self.v_new, self.block_table, self.token_seq, self.positions, self.K, self.V, self.ks,
-                     self.vs, status=self.status)
+        if self.rope is not None:
+            q = self.q[:, :, 0]
+            ops.rotate_write_kv(q, self.k_new, self.v_new, self.rope, self.block_table, self.token_seq, self.positions,
+                                self.K, self.V, self.ks, self.vs, interleaved=self.interleaved, q_out=q,
+                                status=self.status)
+        else:
+            ops.write_kv(self.k_new, self.v_new, self.block_table, self.token_seq, self.positions, self.K, self.V, self.ks,
+                         self.vs, status=self.status)
+        if self.share:
+            ops.shared_prefix_attention(self.q, self.K, self.V, self.q_len, self.block_table, self.num_blocks, self.BS,
+                                        kv_len, self.meta[2 * S:3 * S + 1], self.meta[3 * S + 1:], self.ks, self.vs,
+                                        out=self.out, lse=self.lse, status=self.status)
+            return
         ops.paged_attention(self.q, self.K, self.V, self.q_len, self.block_table, self.num_blocks, self.BS, kv_len,
                             self.ks, self.vs, out=self.out, lse=self.lse, mode="decode", status=self.status)
 
@@ -115,7 +132,13 @@ class DecodeStepGraph:
         st[:n] = [self.pool.slot_of(int(x)) for x in seq_ids]
         st[n:S] = self.pool.slot_of(self.PAD_SEQ)
         st[S:S + n] = [int(x) for x in seq_lens]
-        st[S + n:] = 1
+        st[S + n:2 * S] = 1
+        if self.share:  # groups behind the step's are empty, padding rows belong to none
+            starts, columns = self.pool.shared_runs(seq_ids)
+            st[2 * S:3 * S + 1] = n
+            st[2 * S:2 * S + len(starts)] = starts
+            st[3 * S + 1:] = 0
+            st[3 * S + 1:3 * S + 1 + len(columns)] = [c * self.BS for c in columns]
 
     def step(self, seq_ids: Sequence[int], seq_lens: Sequence[int], q: torch.Tensor, k_new: torch.Tensor,
              v_new: torch.Tensor) -> torch.Tensor:
