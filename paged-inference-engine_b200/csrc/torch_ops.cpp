@@ -8,10 +8,10 @@
 //                                           K/V rows (transformer/model.py:85-122)
 //   pie_b200::project_write_kv              the K/V projection with that write in
 //                                           its epilogue (transformer/model.py:75-122)
-//   pie_b200::shared_prefix_attention       decode attention over groups that share a prefix
-//   pie_b200::rotate_write_kv               new query and key rows rotated by their
+//   pie_b200::shared_prefix_attention(_out)       decode attention over groups that share a prefix
+//   pie_b200::rotate_write_kv(_out)               new query and key rows rotated by their
 //                                           positions, K/V rows written
-//   pie_b200::adjust_logits                 penalties, biases and masks on logits
+//   pie_b200::adjust_logits(_out)                 penalties, biases and masks on logits
 //   pie_b200::copy_blocks                   page copies inside the pools of all layers
 //   pie_b200::reorder_beams                 beams take over their parents' pool rows
 //   pie_b200::compact_blocks                the blocks in use move to the lowest ids
@@ -323,12 +323,21 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_varlen(
   return {out, lse};
 }
 
-void shared_prefix_attention(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const at::Tensor& q_len,
-                             const at::Tensor& block_table, const at::Tensor& num_blocks, const at::Tensor& kv_len,
-                             const at::Tensor& group_start, const at::Tensor& prefix_len,
-                             const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
-                             double softmax_scale, const std::optional<at::Tensor>& status, at::Tensor& out,
-                             at::Tensor& lse) {
+// As the Python front end hands them on: int32, contiguous.
+at::Tensor as_i32(const at::Tensor& t) {
+  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+}
+at::Tensor flat_i32(const at::Tensor& t) {
+  at::Tensor v = as_i32(t);
+  return v.dim() == 1 ? v : v.view({-1});
+}
+
+void shared_prefix_attention_out(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const at::Tensor& q_len,
+                                 const at::Tensor& block_table, const at::Tensor& num_blocks, const at::Tensor& kv_len,
+                                 const at::Tensor& group_start, const at::Tensor& prefix_len,
+                                 const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                                 double softmax_scale, const std::optional<at::Tensor>& status, at::Tensor& out,
+                                 at::Tensor& lse) {
   check_q(Q, 4);
   check_out(Q, out, lse);
   TORCH_CHECK_VALUE(Q.size(3) < 2 || out.stride(3) == 1, "pie_b200: out needs a contiguous head_dim");
@@ -356,6 +365,32 @@ void shared_prefix_attention(const at::Tensor& Q, const at::Tensor& K, const at:
   void* stream = c10::cuda::getCurrentCUDAStream(Q.device().index()).stream();
   check_rc(shared_prefix_attn(&io, &kv, &pg, &gr, ws.data_ptr(), bytes, opt_ptr<int32_t>(status), stream),
            "shared_prefix_attn");
+}
+
+// Makes O and L, and takes what the Python front end would convert: the whole call without Python's checks (a small
+// call is bound by the host: 26 us with them, 14 without).
+std::tuple<at::Tensor, at::Tensor> shared_prefix_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_len, const at::Tensor& block_table,
+    const at::Tensor& num_blocks, int64_t block_size, const at::Tensor& kv_len, const at::Tensor& group_start,
+    const at::Tensor& prefix_len, const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+    double softmax_scale, const std::optional<at::Tensor>& status) {
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
+                    "pie_b200: Q must be [num_seqs, num_q_heads, max_q_len, head_dim], K and V 4-D pools");
+  const bool swapped = k.size(1) != block_size && k.size(2) == block_size;
+  const at::Tensor K = swapped ? k.transpose(1, 2) : k, V = swapped ? v.transpose(1, 2) : v;
+  TORCH_CHECK_VALUE(K.size(1) == block_size, "pie_b200: block_size ", block_size, " does not match the pool");
+  const auto small = [](const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; };
+  at::Tensor Q = small(q) ? q : q.to(small(K) ? K.scalar_type() : at::kHalf);
+  if (Q.stride(3) != 1) Q = Q.contiguous();
+  TORCH_CHECK_VALUE(group_start.dim() == 1 && group_start.numel() >= 1 && prefix_len.dim() == 1,
+                    "pie_b200: group_start must hold num_groups + 1 offsets, prefix_len num_groups lengths");
+  check_q(Q, 4);
+  at::Tensor out = fresh(Q.sizes(), at::kHalf, Q.device()), lse = fresh(Q.sizes().slice(0, 3), at::kHalf, Q.device());
+  shared_prefix_attention_out(Q, K, V, as_i32(q_len),
+                              block_table.scalar_type() == at::kInt ? block_table : block_table.to(at::kInt),
+                              as_i32(num_blocks), as_i32(kv_len), as_i32(group_start), as_i32(prefix_len), k_scale, v_scale,
+                              softmax_scale, status, out, lse);
+  return {out, lse};
 }
 
 void write_kv(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& block_table,
@@ -458,11 +493,11 @@ pa_kv_new_t new_rows(const at::Tensor& k_new, const at::Tensor& v_new, const at:
   return nw;
 }
 
-void rotate_write_kv(const std::optional<at::Tensor>& q, const at::Tensor& k_new, const at::Tensor& v_new,
-                     const at::Tensor& cos_sin, bool interleaved, const at::Tensor& block_table,
-                     const at::Tensor& seq_index, const at::Tensor& positions, at::Tensor& k_cache, at::Tensor& v_cache,
-                     const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
-                     const std::optional<at::Tensor>& status, const std::optional<at::Tensor>& q_out) {
+void rotate_write_kv_out(const std::optional<at::Tensor>& q, const at::Tensor& k_new, const at::Tensor& v_new,
+                         const at::Tensor& cos_sin, bool interleaved, const at::Tensor& block_table,
+                         const at::Tensor& seq_index, const at::Tensor& positions, at::Tensor& k_cache, at::Tensor& v_cache,
+                         const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                         const std::optional<at::Tensor>& status, const std::optional<at::Tensor>& q_out) {
   TORCH_CHECK_VALUE(k_new.dim() == 3 && v_new.sizes() == k_new.sizes() && v_new.scalar_type() == k_new.scalar_type(),
                     "pie_b200: k_new / v_new must be [num_tokens, num_kv_heads, head_dim] of equal shape and dtype");
   TORCH_CHECK_VALUE(k_new.stride(2) == 1 && v_new.stride(2) == 1, "pie_b200: new rows need a contiguous head_dim");
@@ -517,6 +552,27 @@ void rotate_write_kv(const std::optional<at::Tensor>& q, const at::Tensor& k_new
   check_rc(kv_rotate_write(&nw, &r, &kv, &pg, opt_ptr<int32_t>(status), stream), "kv_rotate_write");
 }
 
+// Makes the rotated queries, and takes what the Python front end would convert (one token: 17 us a call with its checks,
+// 8 without).
+at::Tensor rotate_write_kv(const at::Tensor& q, const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& cos_sin,
+                           bool interleaved, const at::Tensor& block_table, const at::Tensor& seq_index,
+                           const at::Tensor& positions, at::Tensor& k_cache, at::Tensor& v_cache,
+                           const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale,
+                           const std::optional<at::Tensor>& status) {
+  TORCH_CHECK_VALUE(k_new.dim() == 3 && v_new.dim() == 3 && q.dim() == 3 && q.is_cuda(),
+                    "pie_b200: q, k_new and v_new must be CUDA tensors [num_tokens, heads, head_dim]");
+  TORCH_CHECK_VALUE(k_new.scalar_type() == at::kHalf || k_new.scalar_type() == at::kBFloat16 || k_new.scalar_type() == at::kFloat,
+                    "pie_b200: k_new / v_new must share a float16, bfloat16 or float32 dtype");
+  TORCH_CHECK_VALUE(cos_sin.dim() == 2 && cos_sin.size(1) >= 16 && cos_sin.size(1) <= k_new.size(2) && cos_sin.size(1) % 16 == 0,
+                    "pie_b200: cos_sin must be float32 [num_positions, rot_dim], rot_dim a multiple of 16 up to head_dim");
+  const auto rows = [](const at::Tensor& t) { return t.stride(2) == 1 ? t : t.contiguous(); };
+  const std::optional<at::Tensor> out = fresh(q.sizes(), q.scalar_type(), q.device());
+  rotate_write_kv_out(rows(q), rows(k_new), rows(v_new), cos_sin.stride(1) == 1 ? cos_sin : cos_sin.contiguous(), interleaved,
+                      block_table.scalar_type() == at::kInt ? block_table : block_table.to(at::kInt), flat_i32(seq_index),
+                      flat_i32(positions), k_cache, v_cache, k_scale, v_scale, status, out);
+  return *out;
+}
+
 void check_rows(const at::Tensor& ref, const std::optional<at::Tensor>& t, const char* name, at::ScalarType type,
                 int64_t rows) {
   if (!t.has_value()) return;
@@ -525,14 +581,14 @@ void check_rows(const at::Tensor& ref, const std::optional<at::Tensor>& t, const
                     name, " must be a contiguous vector of ", rows, type == at::kInt ? " int32" : " float32", " values");
 }
 
-void adjust_logits(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
-                   const std::optional<at::Tensor>& num_tokens, const std::optional<at::Tensor>& prompt_len,
-                   const std::optional<at::Tensor>& repetition, double repetition_value,
-                   const std::optional<at::Tensor>& presence, double presence_value,
-                   const std::optional<at::Tensor>& frequency, double frequency_value,
-                   const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& bias_row,
-                   const std::optional<at::Tensor>& mask, const std::optional<at::Tensor>& mask_row,
-                   const std::optional<at::Tensor>& status, at::Tensor& out) {
+void adjust_logits_out(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                       const std::optional<at::Tensor>& num_tokens, const std::optional<at::Tensor>& prompt_len,
+                       const std::optional<at::Tensor>& repetition, double repetition_value,
+                       const std::optional<at::Tensor>& presence, double presence_value,
+                       const std::optional<at::Tensor>& frequency, double frequency_value,
+                       const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& bias_row,
+                       const std::optional<at::Tensor>& mask, const std::optional<at::Tensor>& mask_row,
+                       const std::optional<at::Tensor>& status, at::Tensor& out) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1),
                     "pie_b200: logits must be a CUDA tensor [rows, vocab] with a contiguous vocabulary");
   check_device(logits, out, "out");
@@ -598,6 +654,71 @@ void adjust_logits(const at::Tensor& logits, const std::optional<at::Tensor>& to
   const c10::cuda::CUDAGuard guard(logits.device());
   void* stream = c10::cuda::getCurrentCUDAStream(logits.device().index()).stream();
   check_rc(logits_adjust(&a, opt_ptr<int32_t>(status), stream), "logits_adjust");
+}
+
+// Makes the new logits, and takes what the Python front end would convert (one row: 23 us a call with its checks, 8
+// without).
+at::Tensor adjust_logits(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                         const std::optional<at::Tensor>& num_tokens, const std::optional<at::Tensor>& prompt_len,
+                         const std::optional<at::Tensor>& repetition, double repetition_value,
+                         const std::optional<at::Tensor>& presence, double presence_value,
+                         const std::optional<at::Tensor>& frequency, double frequency_value,
+                         const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& bias_row,
+                         const std::optional<at::Tensor>& mask, const std::optional<at::Tensor>& mask_row,
+                         const std::optional<at::Tensor>& status) {
+  const auto type = logits.scalar_type();
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && (type == at::kFloat || type == at::kHalf || type == at::kBFloat16) && logits.is_cuda(),
+                    "pie_b200: logits must be float32, float16 or bfloat16 [..., vocab] on a CUDA device");
+  const int64_t V = logits.size(-1);
+  TORCH_CHECK_VALUE(V >= 1, "pie_b200: logits need a vocabulary");
+  TORCH_CHECK_VALUE(repetition.has_value() || repetition_value > 0, "pie_b200: repetition_penalty must be positive");
+  TORCH_CHECK_VALUE(tokens.has_value() || (!num_tokens.has_value() && !prompt_len.has_value()),
+                    "pie_b200: num_tokens and prompt_len come with tokens");
+  using Opt = std::optional<at::Tensor>;
+  const auto matrix = [](const at::Tensor& t, int64_t cols) {  // [..., cols] as rows
+    at::Tensor m = t.dim() == 2 ? t : t.reshape({t.numel() / (cols > 0 ? cols : 1), cols});
+    return m.size(1) < 2 || m.stride(1) == 1 ? m : m.contiguous();
+  };
+  const auto ints = [](const Opt& t) { return t.has_value() ? Opt(flat_i32(*t)) : t; };
+  const at::Tensor x = matrix(logits, V);
+  const int64_t R = x.size(0);
+  const auto values = [R](const Opt& t) {
+    if (!t.has_value() || (t->scalar_type() == at::kFloat && t->dim() == 1 && t->is_contiguous())) return t;
+    TORCH_CHECK_VALUE(t->numel() == R, "pie_b200: a penalty must be a number or ", R, " values");
+    return Opt(t->to(at::kFloat).reshape({R}).contiguous());
+  };
+  Opt seen = tokens, add = bias, bits = mask;
+  if (seen.has_value()) {
+    TORCH_CHECK_VALUE(seen->dim() == logits.dim() && seen->sizes().slice(0, seen->dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+                      "pie_b200: tokens must be shaped like logits, with their own last dimension");
+    at::Tensor i = seen->scalar_type() == at::kInt ? *seen : seen->to(at::kInt);
+    const int64_t L = i.size(-1);
+    if (i.dim() != 2) i = i.reshape({R, L});
+    seen = L < 2 || i.stride(1) == 1 ? i : i.contiguous();
+  }
+  const auto rows_of = [R](const Opt& t, const Opt& by, const char* name) {
+    TORCH_CHECK_VALUE(t.has_value() || !by.has_value(), "pie_b200: ", name, "_row without ", name);
+    TORCH_CHECK_VALUE(!t.has_value() || by.has_value() || t->size(0) == 1 || t->size(0) == R, "pie_b200: ", name, " has ",
+                      t.has_value() ? t->size(0) : 0, " rows for ", R, " rows of logits: pass ", name, "_row");
+  };
+  if (add.has_value()) {
+    at::Tensor b = add->scalar_type() == at::kFloat ? *add : add->to(at::kFloat);
+    TORCH_CHECK_VALUE((b.dim() == 1 || b.dim() == 2) && b.size(-1) == V, "pie_b200: bias must be [N, ", V, "] or [", V, "]");
+    add = matrix(b, V);
+  }
+  if (bits.has_value()) {
+    const int64_t W = (V + 31) / 32;
+    TORCH_CHECK_VALUE((bits->dim() == 1 || bits->dim() == 2) && bits->size(-1) == W && bits->scalar_type() == at::kInt,
+                      "pie_b200: mask must be int32 [M, ", W, "] or [", W, "]");
+    bits = matrix(*bits, W);
+  }
+  rows_of(add, bias_row, "bias");
+  rows_of(bits, mask_row, "mask");
+  at::Tensor out = fresh(logits.sizes(), type, logits.device());
+  at::Tensor o = out.dim() == 2 ? out : out.view({R, V});
+  adjust_logits_out(x, seen, ints(num_tokens), ints(prompt_len), values(repetition), repetition_value, values(presence),
+                    presence_value, values(frequency), frequency_value, add, ints(bias_row), bits, ints(mask_row), status, o);
+  return out;
 }
 
 // ---- shared blocks, page copies, beams ---------------------------------------
@@ -812,6 +933,26 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_meta(const at::Tensor& Q, con
           at::empty(Q.sizes().slice(0, 3), Q.options().dtype(at::kHalf))};
 }
 
+using Opt = std::optional<at::Tensor>;
+std::tuple<at::Tensor, at::Tensor> shared_prefix_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&,
+                                                      const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
+                                                      const at::Tensor&, const at::Tensor&, const at::Tensor&, const Opt&,
+                                                      const Opt&, double, const Opt&) {
+  return {at::empty_symint(Q.sym_sizes(), Q.options().dtype(at::kHalf)),
+          at::empty_symint(Q.sym_sizes().slice(0, 3), Q.options().dtype(at::kHalf))};
+}
+
+at::Tensor rotate_write_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool,
+                             const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&, const Opt&,
+                             const Opt&, const Opt&) {
+  return at::empty_symint(q.sym_sizes(), q.options());
+}
+
+at::Tensor adjust_logits_meta(const at::Tensor& logits, const Opt&, const Opt&, const Opt&, const Opt&, double, const Opt&,
+                              double, const Opt&, double, const Opt&, const Opt&, const Opt&, const Opt&, const Opt&) {
+  return at::empty_symint(logits.sym_sizes(), logits.options());
+}
+
 std::tuple<at::Tensor, at::Tensor> paged_attention_varlen_meta(
     const at::Tensor& Q, const at::Tensor&, const at::Tensor&, int64_t, const at::Tensor&, const at::Tensor&,
     const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
@@ -840,12 +981,21 @@ TORCH_LIBRARY(pie_b200, m) {
   m.def("project_write_kv(Tensor x, Tensor w, Tensor? bias, Tensor block_table, Tensor seq_index, Tensor positions, "
         "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(s!)? status) -> ()");
   m.def("shared_prefix_attention(Tensor Q, Tensor K, Tensor V, Tensor q_len, Tensor block_table, Tensor num_blocks, "
+        "int block_size, Tensor kv_len, Tensor group_start, Tensor prefix_len, Tensor? k_scale, Tensor? v_scale, "
+        "float softmax_scale, Tensor(s!)? status) -> (Tensor, Tensor)");
+  m.def("shared_prefix_attention_out(Tensor Q, Tensor K, Tensor V, Tensor q_len, Tensor block_table, Tensor num_blocks, "
         "Tensor kv_len, Tensor group_start, Tensor prefix_len, Tensor? k_scale, Tensor? v_scale, float softmax_scale, "
         "Tensor(s!)? status, Tensor(a!) out, Tensor(b!) lse) -> ()");
-  m.def("rotate_write_kv(Tensor? q, Tensor k_new, Tensor v_new, Tensor cos_sin, bool interleaved, Tensor block_table, "
+  m.def("rotate_write_kv(Tensor q, Tensor k_new, Tensor v_new, Tensor cos_sin, bool interleaved, Tensor block_table, "
+        "Tensor seq_index, Tensor positions, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, "
+        "Tensor(d!)? v_scale, Tensor(s!)? status) -> Tensor");
+  m.def("rotate_write_kv_out(Tensor? q, Tensor k_new, Tensor v_new, Tensor cos_sin, bool interleaved, Tensor block_table, "
         "Tensor seq_index, Tensor positions, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scale, "
         "Tensor(d!)? v_scale, Tensor(s!)? status, Tensor(e!)? q_out) -> ()");
   m.def("adjust_logits(Tensor logits, Tensor? tokens, Tensor? num_tokens, Tensor? prompt_len, Tensor? repetition, "
+        "float repetition_value, Tensor? presence, float presence_value, Tensor? frequency, float frequency_value, "
+        "Tensor? bias, Tensor? bias_row, Tensor? mask, Tensor? mask_row, Tensor(s!)? status) -> Tensor");
+  m.def("adjust_logits_out(Tensor logits, Tensor? tokens, Tensor? num_tokens, Tensor? prompt_len, Tensor? repetition, "
         "float repetition_value, Tensor? presence, float presence_value, Tensor? frequency, float frequency_value, "
         "Tensor? bias, Tensor? bias_row, Tensor? mask, Tensor? mask_row, Tensor(s!)? status, Tensor(a!) out) -> ()");
   m.def("copy_blocks(Tensor(a!)[] k_caches, Tensor(b!)[] v_caches, Tensor(c!)[] k_scales, Tensor(d!)[] v_scales, "
@@ -869,8 +1019,11 @@ TORCH_LIBRARY_IMPL(pie_b200, CUDA, m) {
   m.impl("write_kv", &write_kv);
   m.impl("project_write_kv", &project_write_kv);
   m.impl("shared_prefix_attention", &shared_prefix_attention);
+  m.impl("shared_prefix_attention_out", &shared_prefix_attention_out);
   m.impl("rotate_write_kv", &rotate_write_kv);
+  m.impl("rotate_write_kv_out", &rotate_write_kv_out);
   m.impl("adjust_logits", &adjust_logits);
+  m.impl("adjust_logits_out", &adjust_logits_out);
   m.impl("copy_blocks", &copy_blocks);
   m.impl("reorder_beams", &reorder_beams);
   m.impl("compact_blocks", &compact_blocks);
@@ -883,7 +1036,10 @@ TORCH_LIBRARY_IMPL(pie_b200, Meta, m) {
   m.impl("reorder_beams", &reorder_beams_meta);
   m.impl("compact_blocks", &compact_blocks_meta);
   m.impl("beam_select", &beam_select_meta);
-  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv", "shared_prefix_attention", "rotate_write_kv",
-                         "adjust_logits", "copy_blocks"})
+  m.impl("shared_prefix_attention", &shared_prefix_meta);
+  m.impl("rotate_write_kv", &rotate_write_meta);
+  m.impl("adjust_logits", &adjust_logits_meta);
+  for (const char* op : {"paged_attention_out", "paged_attention_varlen_out", "write_kv", "project_write_kv",
+                         "shared_prefix_attention_out", "rotate_write_kv_out", "adjust_logits_out", "copy_blocks"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&write_only_meta>());
 }

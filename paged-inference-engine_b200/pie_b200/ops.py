@@ -417,6 +417,10 @@ def shared_prefix_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, q
     what every row sees).  ``DeviceBlockManager.shared_prefixes`` and ``BeamSearch.step_inputs`` give both.  At most
     16 query rows times heads of a KV head (``max_q_len * Hq / Hkv``); fp16, bf16 and int8 pools.
     """
+    if BACKEND == "torch" and Q.is_cuda and out is None and lse is None and not _CHECK:  # the op checks and makes them
+        return _op("shared_prefix_attention")(Q, K, V, q_len_per_seq, block_table, num_blocks_per_seq, block_size,
+                                              kv_len_per_seq, group_start, prefix_len, k_scale, v_scale,
+                                              softmax_scale or 0.0, status)
     if Q.dim() != 4:
         raise ValueError("Q must be [num_seqs, num_q_heads, max_q_len, head_dim]")
     B, Hq, maxq, D = Q.shape
@@ -450,8 +454,8 @@ def shared_prefix_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, q
     scale = float(softmax_scale) if softmax_scale else 0.0
     if BACKEND == "torch":
         bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
-        _op("shared_prefix_attention")(Q, K, V, _i32(q_len_per_seq), bt, _i32(num_blocks_per_seq), _i32(kv_len_per_seq), gs,
-                                       pl, k_scale, v_scale, scale, status, out, lse)
+        _op("shared_prefix_attention_out")(Q, K, V, _i32(q_len_per_seq), bt, _i32(num_blocks_per_seq), _i32(kv_len_per_seq), gs,
+                                                           pl, k_scale, v_scale, scale, status, out, lse)
     else:
         for name, t in (("K", K), ("V", V), ("block_table", block_table), ("q_len_per_seq", q_len_per_seq),
                         ("kv_len_per_seq", kv_len_per_seq), ("num_blocks_per_seq", num_blocks_per_seq),
@@ -673,6 +677,9 @@ def rotate_write_kv(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch
     rot_dim on stay.  ``q``, ``k_new`` and ``v_new`` share a dtype; ``q_out`` may be ``q``.  A token whose position is
     outside ``cos_sin`` is left out (its row of the result too); see kv_rotate_write in the C header.
     """
+    if BACKEND == "torch" and k_cache.is_cuda and q is not None and q_out is None and not _CHECK:  # the op checks
+        return _op("rotate_write_kv")(q, k_new, v_new, cos_sin, interleaved, block_table, seq_index, positions, k_cache,
+                                      v_cache, k_scale, v_scale, status)
     if k_new.dim() != 3 or v_new.shape != k_new.shape:
         raise ValueError("k_new / v_new must be [num_tokens, num_kv_heads, head_dim] of equal shape")
     T, H, D = k_new.shape
@@ -712,8 +719,8 @@ def rotate_write_kv(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch
         status = status_word(k_cache.device)
     int8 = k_cache.dtype == torch.int8
     if BACKEND == "torch":
-        _op("rotate_write_kv")(q, k_new, v_new, cos_sin, bool(interleaved), bt, si.view(-1), ps.view(-1), k_cache, v_cache,
-                               k_scale if int8 else None, v_scale if int8 else None, status, q_out)
+        _op("rotate_write_kv_out")(q, k_new, v_new, cos_sin, bool(interleaved), bt, si.view(-1), ps.view(-1), k_cache, v_cache,
+                                   k_scale if int8 else None, v_scale if int8 else None, status, q_out)
     else:
         dev = k_cache.device
         for name, t in (("q", q), ("q_out", q_out), ("k_new", k_new), ("v_new", v_new), ("v_cache", v_cache),
@@ -1032,6 +1039,12 @@ def adjust_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None
     (token v: bit v % 32 of word v // 32, 1 = allowed) are one per row, one for all, or chosen by ``bias_row`` /
     ``mask_row`` (-1: none).  See logits_adjust in the C header.
     """
+    if BACKEND == "torch" and logits.is_cuda and out is None and not _CHECK:  # the op checks and makes the new logits
+        rep, rep_v = (repetition_penalty, 0.0) if isinstance(repetition_penalty, torch.Tensor) else (None, repetition_penalty)
+        pres, pres_v = (presence_penalty, 0.0) if isinstance(presence_penalty, torch.Tensor) else (None, presence_penalty)
+        freq, freq_v = (frequency_penalty, 0.0) if isinstance(frequency_penalty, torch.Tensor) else (None, frequency_penalty)
+        return _op("adjust_logits")(logits, tokens, num_tokens, prompt_len, rep, rep_v, pres, pres_v, freq, freq_v, bias,
+                                    bias_row, mask, mask_row, status)
     if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f"logits must be float32, float16 or bfloat16 [..., vocab], got {logits.dtype} {tuple(logits.shape)}")
     V = logits.shape[-1]
@@ -1084,8 +1097,8 @@ def adjust_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None
     if status is None and _CHECK:
         status = status_word(dev)
     if BACKEND == "torch":
-        _op("adjust_logits")(x, tokens, num_tokens, prompt_len, rep, rep_v, pres, pres_v, freq, freq_v, bias, bias_row, mask,
-                             mask_row, status, o)
+        _op("adjust_logits_out")(x, tokens, num_tokens, prompt_len, rep, rep_v, pres, pres_v, freq, freq_v, bias, bias_row,
+                                 mask, mask_row, status, o)
     else:
         for name, t in (("tokens", tokens), ("num_tokens", num_tokens), ("prompt_len", prompt_len), ("bias", bias),
                         ("bias_row", bias_row), ("mask", mask), ("mask_row", mask_row), ("out", o), ("status", status)):
