@@ -23,7 +23,10 @@
 //                csrc/kv_dequant.cu does for prompts; the raw bytes cross HBM once and the
 //                fp16 tile never leaves the SM
 //
-// Bound by HBM up to about 256 rows a kv head (16-bit pools), by the softmax chain beyond.
+// 16-bit pools: bound by HBM up to about 256 rows a kv head, by the issue of the two products beyond (128 keys of 128 rows
+// take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
+// INT8 pools: by the conversion of the tiles, 1100 cycles each; eight warps for it left 96 registers a thread and
+// gained nothing.
 #include <atomic>
 #include <type_traits>
 
@@ -38,14 +41,15 @@ constexpr uint32_t W_OCOL = 256;
 constexpr float W_THRESHOLD = 8.0f;  // growth of the maximum (log2) that rescales
 constexpr int W_SOFTMAX = 8;         // warps
 constexpr int W_PRODUCER = 8, W_MMA = 9, W_CONVERT = 10;
+constexpr int W_CONVERTERS = 4;      // warps, INT8
 
 template <int D, bool I8>
 struct WideCfg {
   static constexpr int TILE = (D / 64) * W_HALF;   // fp16 / bf16 operand tile of 128 rows
   static constexpr int RAW = 128 * D;              // int8 tile
   static constexpr int KST = D == 128 ? (I8 ? 2 : 3) : (I8 ? 3 : 5);  // K stages
-  static constexpr int VST = D == 128 ? (I8 ? 1 : 2) : (I8 ? 3 : 5);  // V stages
-  static constexpr int RST = I8 ? (D == 128 ? 4 : 8) : 0;  // raw tiles in flight, K and V alternating
+  static constexpr int VST = D == 128 ? 2 : (I8 ? 3 : 5);               // V stages
+  static constexpr int RST = I8 ? (D == 128 ? 2 : 8) : 0;  // raw tiles in flight, K and V alternating (4 and one V stage: 130 us, so 125)
   static constexpr int K0 = 2 * TILE;
   static constexpr int V0 = K0 + KST * TILE;
   static constexpr int R0 = V0 + VST * TILE;
@@ -55,9 +59,22 @@ struct WideCfg {
                        B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
   static constexpr int XCH = BAR + (D == 128 ? 256 : 512);
   static constexpr int SMEM = XCH + 1024 + 1024;  // exchange of the two streams, alignment
-  static constexpr int THREADS = 32 * (I8 ? W_CONVERT + 4 : W_CONVERT);
+  static constexpr int THREADS = 32 * (I8 ? W_CONVERT + W_CONVERTERS : W_CONVERT);
   static_assert(B_END * 8 <= XCH - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
 };
+
+// A scale's bits, where there is one: loaded without a branch or a conversion, so that nothing
+// waits for it before its use (4 groups of 32 over 16384 keys: 132 us with a wait of 1 us in every unit, 125 without).
+__device__ __forceinline__ uint32_t scale_bits(const void* base, long long at, bool is, bool f32) {
+  uint32_t v;
+  const char* a = static_cast<const char*>(base) + (at << (f32 ? 2 : 1));
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.s32 p, %2, 0;\nsetp.ne.s32 q, %3, 0;\nmov.b32 %0, 0;\n"
+      "@p ld.global.nc.u32 %0, [%1];\n@q ld.global.nc.u16 %0, [%1];\n}\n"
+      : "=&r"(v)
+      : "l"(a), "r"(static_cast<int>(is && f32)), "r"(static_cast<int>(is && !f32)));
+  return v;
+}
 
 __device__ unsigned int g_wide_abort = 0;  // launch generation in which a wait gave up
 
@@ -163,16 +180,16 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       mbar_init(bar(C::B_ODONE + x), 1);
     }
     for (int s = 0; s < KST; ++s) {
-      mbar_init(bar(C::B_KFULL + s), I8 ? 128 : 1);
+      mbar_init(bar(C::B_KFULL + s), I8 ? 32 * W_CONVERTERS : 1);
       mbar_init(bar(C::B_KEMPTY + s), 1);
     }
     for (int s = 0; s < VST; ++s) {
-      mbar_init(bar(C::B_VFULL + s), I8 ? 128 : 1);
+      mbar_init(bar(C::B_VFULL + s), I8 ? 32 * W_CONVERTERS : 1);
       mbar_init(bar(C::B_VEMPTY + s), 1);
     }
     for (int s = 0; s < C::RST; ++s) {
       mbar_init(bar(C::B_RFULL + s), 1);
-      mbar_init(bar(C::B_REMPTY + s), 128);
+      mbar_init(bar(C::B_REMPTY + s), 32 * W_CONVERTERS);
     }
     fence_mbar_init();
   }
@@ -307,12 +324,14 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
   } else if (warp >= W_CONVERT) {
     // ------------------------------------------------------------ INT8 -> fp16 tiles
     if constexpr (I8) {
-      // Warp c converts rows 32 c .. 32 c + 31 of every tile; lane l holds the scales of row 32 c + l.  A lane takes 16
+      // Warp c converts rows 16 c .. 16 c + 15 of every tile; lane l holds the scales of row 16 c + l % 16.  A lane takes 16
       // dims of a row at a time.  The eight lanes that a shared-memory access serves at once are four pieces of rows a
       // and a ^ 5: swizzled, those lie in different banks, in the raw tile (16 bytes a piece) as in the operand tile (twice
       // 16 bytes, two apart).
       constexpr int RPI = 32 / (D / 16);  // rows an iteration of a warp
-      const int c = warp - W_CONVERT;
+      constexpr int UNROLL = 4;
+      constexpr int ROWS = kWideKeys / W_CONVERTERS;  // of a tile, a warp
+      const int r0 = ROWS * (warp - W_CONVERT), mine_at = r0 + (lane & (ROWS - 1));
       const int half = D == 128 ? (lane >> 3) & 1 : 0;
       const int ch = 4 * half + (lane & 3);                    // 16-byte piece of the raw row
       const int pair = D == 128 ? lane >> 4 : lane >> 3;       // row pairs 0 5, 1 4, 2 7, 3 6 of eight rows
@@ -322,29 +341,29 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         const int* bt_row = p.bt + static_cast<long long>(it.grp.w) * p.bt_ss;
         const int n = it.n;
         auto block = [&](int j) {
-          const int key = (it.t + j) * kWideKeys + 32 * c + lane;
+          const int key = (it.t + j) * kWideKeys + mine_at;
           return j < n && key < it.grp.x ? bt_row[static_cast<long long>(key >> p.log2BS) * p.bt_sc] : -1;
         };
-        auto scales = [&](int j, int blk, float& k, float& v) {
-          k = v = 0.f;  // keys past the end, and of blocks outside the pool, are zeros
-          if (blk < 0 || blk >= p.NB) return;
-          const int slot = ((it.t + j) * kWideKeys + 32 * c + lane) & (p.BS - 1);
-          k = load_scale(p.ks, blk * p.ks_sblk + slot * p.ks_sslot + it.kvh * p.ks_shead, p.scale_f32);
-          v = load_scale(p.vs, blk * p.vs_sblk + slot * p.vs_sslot + it.kvh * p.vs_shead, p.scale_f32);
+        auto scales = [&](int j, int blk, uint32_t& k, uint32_t& v) {  // as they are stored; 0: no block, or past the end
+          const bool is = blk >= 0 && blk < p.NB;
+          const int slot = ((it.t + j) * kWideKeys + mine_at) & (p.BS - 1);
+          k = scale_bits(p.ks, is ? blk * p.ks_sblk + slot * p.ks_sslot + it.kvh * p.ks_shead : 0, is, p.scale_f32);
+          v = scale_bits(p.vs, is ? blk * p.vs_sblk + slot * p.vs_sslot + it.kvh * p.vs_shead : 0, is, p.scale_f32);
         };
-        auto convert = [&](int v, int j, float mine) {
+        auto convert = [&](int v, int j, uint32_t mine_bits) {
           const int st = v ? VST : KST, g = gt + j, s = g % st, rs = gr % C::RST;
           const unsigned char* src = sm + C::R0 + rs * C::RAW;
           unsigned char* dst = sm + (v ? C::V0 : C::K0) + s * TILE;
           wide_wait(p, bar(C::B_RFULL + rs), (gr / C::RST) & 1);
           if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
           ++gr;
+          const float mine = p.scale_f32 ? __uint_as_float(mine_bits) : __half2float(__ushort_as_half(static_cast<unsigned short>(mine_bits)));
           auto rows = [&](auto fp32_scale) {
-#pragma unroll
-            for (int k = 0; k < 32 / RPI; ++k) {
-              const int lr = (D == 128 ? 8 * (k >> 1) + 2 * (k & 1) : 8 * k) + pair;  // row within the warp's 32
+#pragma unroll UNROLL
+            for (int k = 0; k < ROWS / RPI; ++k) {
+              const int lr = (D == 128 ? 8 * (k >> 1) + 2 * (k & 1) : 8 * k) + pair;  // row within the warp's
               const int row = lr ^ flip;
-              const int r = 32 * c + row;
+              const int r = r0 + row;
               const float f = __shfl_sync(0xffffffffu, mine, row);
               const int at = D == 128 ? r * 128 + ((ch ^ (r & 7)) << 4) : r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
               const uint4 w = *reinterpret_cast<const uint4*>(src + at);
@@ -383,17 +402,18 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           mbar_arrive(bar((v ? C::B_VFULL : C::B_KFULL) + s));
           mbar_arrive(bar(C::B_REMPTY + rs));
         };
-        // in the order of the loads; the scales are fetched a tile ahead, the block ids two
-        float k0, v0, k1, v1, k2, v2;
-        scales(0, block(0), k0, v0);
-        scales(1, block(1), k1, v1);
-        int blk2 = block(2);
-        convert(0, 0, k0);
-        for (int j = 0; j < n; ++j) {
+        // In the order of the loads: K of a tile, V of the one before.  The scales are fetched a tile ahead, the block ids
+        // two.
+        uint32_t k1, v1, k2, v2, v0 = 0;
+        scales(0, block(0), k1, v1);
+        int blk2 = block(1);
+#pragma unroll 1
+        for (int j = -1; j < n; ++j) {
           scales(j + 2, blk2, k2, v2);
           blk2 = block(j + 3);
-          if (j + 1 < n) convert(0, j + 1, k1);
-          convert(1, j, v0);
+#pragma unroll 1
+          for (int v = 0; v < 2; ++v)
+            if (j + 1 - v >= 0 && j + 1 - v < n) convert(v, j + 1 - v, v ? v0 : k1);
           v0 = v1, k1 = k2, v1 = v2;
         }
         gt += n;
