@@ -20,12 +20,20 @@
 namespace pa {
 namespace {
 
-// Visible keys of sequence b's last row (0 for a sequence without rows).
-__device__ __forceinline__ int plan_keys(const SharedParams& p, int b, int rows) {
-  if (rows <= 0) return 0;
-  const long long cap = static_cast<long long>(max(0, min(p.nblk[b], p.bt_cols))) << p.log2BS;
-  return static_cast<int>(max(0LL, min(static_cast<long long>(p.kvlen[b]), cap)));
-}
+// Rows of sequence b, the keys that its last row sees (0 without rows), and the keys that its first does.  The
+// loads do not wait for one another.
+struct SeqKeys {
+  int rows, keys, first;
+  bool bad;
+  __device__ __forceinline__ SeqKeys(const SharedParams& p, int b) {
+    const int n = p.nblk[b], len = p.kvlen[b];
+    rows = seq_rows(p, b);
+    const long long cap = static_cast<long long>(max(0, min(n, p.bt_cols))) << p.log2BS;
+    keys = rows > 0 ? static_cast<int>(max(0LL, min(static_cast<long long>(len), cap))) : 0;
+    first = min(keys, max(0, len - rows + 1));
+    bad = rows > 0 && n > p.bt_cols;
+  }
+};
 
 // The group of sequence b in the rising starts s_start[0..G], or -1.
 __device__ __forceinline__ int group_of(const int* s_start, int G, int b) {
@@ -87,6 +95,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   __shared__ int s_warp[32];
   __shared__ int s_team, s_total, s_run;
 
+  const SeqKeys mine(p, min(tid, B - 1));  // asked for together with the groups
   int bad = 0;
   for (int i = tid; i <= G; i += T) {
     const int s = p.group_start[i];
@@ -103,12 +112,11 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   if (bad && tid == 0) set_status(p.status, ST_BAD_SEQ_INDEX);
 
   for (int b = tid; b < B; b += T) {
-    const int rows = seq_rows(p, b);
-    const int keys = plan_keys(p, b, rows);
-    if (rows > 0 && p.nblk[b] > p.bt_cols) set_status(p.status, ST_BAD_NUM_BLOCKS);
-    const int g = bad || keys == 0 ? -1 : group_of(s_start, G, b);
+    const SeqKeys s = b == tid ? mine : SeqKeys(p, b);
+    if (s.bad) set_status(p.status, ST_BAD_NUM_BLOCKS);
+    const int g = bad || s.keys == 0 ? -1 : group_of(s_start, G, b);
     if (g < 0) continue;
-    atomicMin(&s_keys[g], min(keys, max(0, p.kvlen[b] - rows + 1)));  // what its first row sees
+    atomicMin(&s_keys[g], s.first);
     atomicMin(&s_lead[g], b);
     atomicAdd(&s_count[g], 1);
   }
@@ -158,7 +166,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   }
 
   for (int b = tid; b < B; b += T) {
-    const int keys = plan_keys(p, b, seq_rows(p, b));
+    const int keys = (b == tid ? mine : SeqKeys(p, b)).keys;
     const int g = bad ? -1 : group_of(s_start, G, b);
     int4 chunk = make_int4(0, 0, 0, 0), own = make_int4(keys, 0, 0, 0);
     if (g >= 0 && s_keys[g] > 0) {
