@@ -101,7 +101,7 @@ struct SharedParams : AttnParams {
   int wide_ctas;
   int* step0;             // [groups + 1] first step of a group (wide)
   int4* grp;              // [groups] shared keys, first sequence, sequences, leader
-  int4* head;             // [1] CTAs of a team, steps of a team, total steps, whether entries are padded to whole runs (wide)
+  int4* head;             // [1] CTAs of a team, steps of a team, all steps (wide)
   int4* info;             // [B] what prefix_merge_kernel asks of a sequence's shared part: first tile and tiles of its chunk, or first step of its group
   long long prefix_row0;  // first partial row of the shared prefixes
 };
@@ -142,9 +142,6 @@ struct WideShape {
     lweight = RT > 1 ? 1 : 0;
   }
   __host__ __device__ int steps() const { return bundles << lweight; }  // of a (pass, kv head)
-  __host__ __device__ int padded(int run, bool pad) const {  // its length in the list
-    return pad ? (steps() + run - 1) / run * run : steps();
-  }
 };
 
 // First partial row of worker w's piece of a chunk, of a sequence's own keys, of a team's piece.

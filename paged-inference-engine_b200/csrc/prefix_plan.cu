@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
   int* s_unit = s_count + G;        // [G + 1]
   int* s_tile = s_unit + G + 1;     // [2 B + 1]
   __shared__ int s_warp[32];
-  __shared__ int s_team, s_total, s_run;
+  __shared__ int s_team;
 
   const SeqKeys mine(p, min(tid, B - 1));  // asked for together with the groups
   int bad = 0;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
       s_count[i] = 0;
     }
   }
-  if (tid == 0) s_team = 1, s_total = 0, s_run = INT_MAX;
+  if (tid == 0) s_team = 1;
   bad = __syncthreads_or(bad);
   if (bad && tid == 0) set_status(p.status, ST_BAD_SEQ_INDEX);
 
@@ -136,33 +136,16 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
       int steps = 0;
       if (s_keys[g] > 0) {
         const WideShape s(s_keys[g], s_start[g + 1] - s_start[g], per, team);
-        steps = s.steps();
-        s_lead[g] = s.passes;  // (the leader is in p.grp by now)
+        steps = s.passes * p.Hkv * s.steps();
       }
       s_unit[g] = steps;
-      atomicAdd(&s_total, steps > 0 ? s_lead[g] * p.Hkv * steps : 0);
     }
-    __syncthreads();
-    // A run that crosses from one list entry into the next pays for two beginnings and ends (7 us against 1 us a
-    // step).  So, for few groups, the shortest run of which every entry takes whole ones, if no more of them than teams
-    // come together and it is not much longer than an equal share.
-    const int share = (s_total + teams - 1) / teams;
-    const int run = share + tid;
-    if (G <= 32 && share > 0 && tid <= 8 + share / 16) {
-      int runs = 0;
-      for (int g = 0; g < G; ++g)
-        if (s_unit[g] > 0) runs += s_lead[g] * p.Hkv * ((s_unit[g] + run - 1) / run);
-      if (runs <= teams) atomicMin(&s_run, run);
-    }
-    __syncthreads();
-    const bool pad = s_run != INT_MAX;
-    const int length = pad ? s_run : share;
-    for (int g = tid; g < G; g += T)
-      if (s_unit[g] > 0) s_unit[g] = s_lead[g] * p.Hkv * (pad ? (s_unit[g] + length - 1) / length * length : s_unit[g]);
     __syncthreads();
     scan_cta(s_unit, G, s_warp);
     for (int g = tid; g <= G; g += T) p.step0[g] = s_unit[g];
-    if (tid == 0) p.head[0] = make_int4(team, length, s_unit[G], pad);
+    // (Runs made longer, so that none crosses from one list entry into the next, left more teams idle than the crossings
+    // cost: 54 against 51 us for 64 sequences over 8192 keys, 125 against 116 for 4 groups of 32 over 16384 INT8 keys.)
+    if (tid == 0) p.head[0] = make_int4(team, (s_unit[G] + teams - 1) / teams, s_unit[G], 0);
   }
 
   for (int b = tid; b < B; b += T) {
@@ -255,7 +238,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 3) prefix_merge_kernel(const
       seg += rp / shape.lanes * p.Hkv;
       rp %= shape.lanes;
     }
-    s0 = info.x + seg * shape.padded(head.y, head.w);
+    s0 = info.x + seg * shape.steps();
     f0 = s0 / head.y;
     cn = ((s0 + shape.steps() - 1) / head.y - f0 + 1) << shape.lparts;
     crow = static_cast<int>(shared_wide_row(p, shape, own.z, seg, f0, head.x, 0, rp)) + in_pair;

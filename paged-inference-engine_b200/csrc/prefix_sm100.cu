@@ -96,7 +96,6 @@ struct Pieces {
   int s, s1;          // steps of the team's run not walked yet
   int team, q, size;  // team, the CTA's place in it, CTAs of a team
   int run;
-  bool pad;
   int g, base;        // group and its first step
   int4 grp;           // shared keys, first sequence, sequences, leader
   WideShape sh;
@@ -111,7 +110,6 @@ struct Pieces {
     team = cta / size;
     q = cta - team * size;
     run = head.y;
-    pad = head.w != 0;
     s = min(team * run, head.z);
     s1 = min(s + run, head.z);
     g = g0 - 1;
@@ -128,7 +126,7 @@ struct Pieces {
   }
   __device__ __forceinline__ bool next(const SharedParams& p) {
     while (s < s1) {
-      const int len = sh.padded(run, pad);
+      const int len = sh.steps();
       if (s - base >= sh.passes * p.Hkv * len) {  // a group with steps is still ahead
         do {
           ++g;
@@ -435,41 +433,34 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       const int mine0 = two ? x * kWideRows : 0;                  // first row of this stream's tile
       const int live = min(kWideRows, it.live - mine0);           // rows of it
       const bool busy = 32 * (warp & 3) < live;                   // this warp holds one
-      // ---- Q: half a row a thread and tile, asked for at once, converted to the operand type, swizzled
+      // ---- Q: half a row a thread, converted to the operand type, swizzled
       if (done[0] > 0) wide_wait(p, bar(C::B_QEMPTY), q_done & 1), ++q_done;
-      const int row = tid >> 1, c0 = (tid & 1) * (D / 16);
-      uint4 w[2][D / 16];
-      int qn[2], m[2], rem[2];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
+#pragma unroll 1
+      for (int y = 0; y < (two ? 2 : 1); ++y) {
+        const int row = tid >> 1, c0 = (tid & 1) * (D / 16);
         const int R = it.row0 + y * kWideRows + row;
-        m[y] = R / per;
-        rem[y] = R - m[y] * per;
-        qn[y] = y * kWideRows + row < it.live ? seq_rows(p, it.grp.y + m[y]) : 0;
-      }
+        uint4 w[D / 16];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int qi = rem[y] / p.G;
-        const bool is = qi < qn[y];
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const unsigned short*>(p.q) + (is ? q_seq_base(p, it.grp.y + m[y]) + (it.kvh * p.G + rem[y] - qi * p.G) * p.q_sh +
-                                                                static_cast<long long>(qi) * p.q_sm
-                                                          : 0)) + c0;
+        for (int c = 0; c < D / 16; ++c) w[c] = make_uint4(0, 0, 0, 0);
+        if (y * kWideRows + row < it.live) {
+          const int m = R / per, rem = R - m * per;
+          const int qi = rem / p.G, b = it.grp.y + m;
+          if (qi < seq_rows(p, b)) {
+            const uint4* src = reinterpret_cast<const uint4*>(
+                static_cast<const unsigned short*>(p.q) + q_seq_base(p, b) + (it.kvh * p.G + rem - qi * p.G) * p.q_sh +
+                static_cast<long long>(qi) * p.q_sm) + c0;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) w[y][c] = is ? src[c] : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        if (y == 1 && !two) break;
+            for (int c = 0; c < D / 16; ++c) w[c] = src[c];
+          }
+        }
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          uint4& v = w[y][c];
-          v.x = cvt_pair<QBF16, MMA_BF16>(v.x);
-          v.y = cvt_pair<QBF16, MMA_BF16>(v.y);
-          v.z = cvt_pair<QBF16, MMA_BF16>(v.z);
-          v.w = cvt_pair<QBF16, MMA_BF16>(v.w);
+          w[c].x = cvt_pair<QBF16, MMA_BF16>(w[c].x);
+          w[c].y = cvt_pair<QBF16, MMA_BF16>(w[c].y);
+          w[c].z = cvt_pair<QBF16, MMA_BF16>(w[c].z);
+          w[c].w = cvt_pair<QBF16, MMA_BF16>(w[c].w);
           const int k = c0 + c;
-          *reinterpret_cast<uint4*>(sm + y * TILE + (k >> 3) * W_HALF + row * 128 + (((k & 7) ^ (row & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(sm + y * TILE + (k >> 3) * W_HALF + row * 128 + (((k & 7) ^ (row & 7)) << 4)) = w[c];
         }
       }
       fence_proxy_async_smem();
