@@ -391,6 +391,7 @@ int kv_write_copy(const pa_kv_new_t* nw, const pa_kv_cache_t* kv, const pa_pagin
  *   q        [num_tokens, num_q_heads, head_dim] in nw->dtype, written rotated
  *            to q_out (which may be q); num_q_heads 0: no queries
  *   cos_sin  fp32 [num_positions, rot_dim], row stride cs_stride
+ * Two tokens of a call may not have the same place in the cache.
  * A token whose position is outside cos_sin is left out (PA_STATUS_BAD_POSITION);
  * one whose K/V rows have no place has its query rows rotated all the same.
  * Limits: rot_dim a multiple of 16 up to head_dim; rows 16-byte aligned; an INT8
@@ -642,7 +643,8 @@ int beam_select(const pa_beam_select_t* args, void* workspace, size_t workspace_
  * reference samples from plain logits (core/model_runner.py:28-159).
  *   logits      [rows, vocab], PA_DTYPE_F32, F16 or BF16, any alignment; NaN stays NaN
  *               unless it is masked
- *   out         [rows, vocab], the same type or fp32; may be logits (same strides and type)
+ *   out         [rows, vocab], the same type or fp32; is logits (same strides and type) or does
+ *               not overlap it
  *   tokens      int32 [rows, max_tokens] or NULL (max_tokens 0): what each row has seen; the
  *               first prompt_len[r] (NULL: none) are its prompt, which counts as seen but not as
  *               generated, and those from num_tokens[r] (NULL: max_tokens) on do not count.

@@ -825,7 +825,7 @@ int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging
              !std::getenv("PIE_B200_NO_TCGEN05");
   c.p.wide_ctas = pa::device_sm_count();
   c.nt = c.p.wide ? (per <= 8 ? 1 : 2) : (c.p.cpm * per <= 8 || a.B * per <= 8 ? 1 : 2);
-  {
+  try {
     static std::mutex mu;
     static std::map<std::tuple<int, int, int, int, int, int, int>, pa::DecodeLaunch> cache;
     int dev = 0;
@@ -840,6 +840,8 @@ int shared_call(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_paging
     } else {
       c.plan = it->second;
     }
+  } catch (const std::exception&) {  // no exception leaves a C entry
+    return fail(PA_ERR_CUDA, "out of host memory");
   }
   c.p.num_warps_total = c.plan.ctas * c.plan.warps_per_cta;
   const long long base_rows = static_cast<long long>(a.B) * a.Hkv * per;

@@ -234,3 +234,63 @@ def test_both_backends_agree(ops):
     finally:
         ops.BACKEND = saved
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,L", [(80, 32003, 300), (20, 131072, 2600), (1200, 2100, 50)])
+def test_many_columns(ops, dtype, R, V, L):
+    """Enough columns for the wide pieces and for spans of several chunks; also in place."""
+    s = make(R, V, L, dtype, seed=R)
+    want = expect(s)
+    same(call(ops, s), want, dtype)
+    x = s["x"].cuda()
+    assert call(ops, s, x=x, out=x) is x
+    same(x, want, dtype)
+
+
+def test_spans_with_many_tokens(ops):
+    """A long history over several spans, each column seen more than once, counts of 32 bits."""
+    s = make(30, 90001, 66000, torch.bfloat16, seed=5)
+    s["count"][:] = 66000
+    s["prompt"][:15] = 0
+    got = call(ops, s)
+    rows = [0, 7, 16, 29]
+    part = {k: (v if k in ("bias", "allowed") else v[rows]) for k, v in s.items()}
+    same(got[rows], expect(part), torch.bfloat16)
+
+
+def test_what_is_converted(ops):
+    """Leading dimensions, 64-bit integers, penalties and biases of other types, one bias and one mask for all rows."""
+    V, L = 4099, 33
+    s = make(6, V, L, torch.float16, seed=8, biases=1, masks=1)
+    s["bias_row"][:] = 0
+    s["mask_row"][:] = 0
+    want = expect(s)
+    kw = dict(tokens=cuda(s["tokens"]).long().view(2, 3, L), num_tokens=cuda(s["count"]).long().view(2, 3), prompt_len=cuda(s["prompt"]).view(2, 3),
+              repetition_penalty=cuda(s["rep"]).double().view(2, 3), presence_penalty=cuda(s["pres"]).view(2, 3), frequency_penalty=cuda(s["freq"]).view(6, 1),
+              bias=cuda(s["bias"][0]).double(), mask=pack(s["allowed"])[0])
+    x = s["x"].cuda().view(2, 3, V)
+    got = ops.adjust_logits(x, **kw)
+    assert got.shape == (2, 3, V)
+    same(got.view(6, V), want, torch.float16)
+    out = torch.empty(2, 3, V, device="cuda")
+    same(ops.adjust_logits(x, out=out, **kw).view(6, V), want, torch.float32)
+    turned = x.view(6, V).t().contiguous().t()  # vocabulary not contiguous
+    flat = {k: v.reshape(6, -1) if k == "tokens" else v.reshape(6) if k not in ("bias", "mask") else v for k, v in kw.items()}
+    same(ops.adjust_logits(turned, **flat), want, torch.float16)
+
+
+def test_refusals_on_the_device(ops):
+    x = torch.zeros(2, 8, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for kw in (dict(repetition_penalty=0.0), dict(repetition_penalty=torch.ones(3, device="cuda")), dict(num_tokens=torch.zeros(2, **i32)),
+               dict(tokens=torch.zeros(3, 4, **i32)), dict(tokens=torch.zeros(4, **i32)), dict(tokens=torch.zeros(2, 4, dtype=torch.int32)),
+               dict(bias=torch.zeros(3, 8, device="cuda")), dict(bias=torch.zeros(2, 9, device="cuda")), dict(bias=torch.zeros(2, 8)),
+               dict(mask=torch.zeros(2, 2, **i32)), dict(mask=torch.zeros(2, 1, device="cuda")), dict(mask=torch.zeros(3, 1, **i32)),
+               dict(mask_row=torch.zeros(2, **i32)), dict(bias=torch.zeros(1, 8, device="cuda"), bias_row=torch.zeros(3, **i32))):
+        with pytest.raises(ValueError):
+            ops.adjust_logits(x, **kw)
+    for bad in (torch.zeros(2, 0, device="cuda"), torch.zeros(2, 8, device="cuda", dtype=torch.int32), torch.zeros(2, 8, device="cuda", dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            ops.adjust_logits(bad)
+    assert ops.adjust_logits(torch.zeros(0, 8, device="cuda")).shape == (0, 8)

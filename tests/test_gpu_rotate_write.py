@@ -258,3 +258,26 @@ def test_both_backends_agree(ops):
     for a, b in zip(got[:2], got[2:]):
         for x, y in zip(a, b):
             assert (x is None and y is None) or torch.equal(x, y)
+
+
+def test_what_is_converted_and_refused(ops):
+    """64-bit indexes, rows with other strides, and arguments that the op refuses."""
+    T, Hq, Hkv, D, BS = 5, 4, 2, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(T, h, D, device="cuda", generator=g).half() for h in (Hq, Hkv, Hkv))
+    table = ops.rope_table(40, D, device="cuda")
+    bt = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    row, pos = torch.zeros(T, dtype=torch.int32, device="cuda"), torch.arange(14, 14 + T, dtype=torch.int32, device="cuda")
+    pools = [torch.zeros(4, BS, Hkv, D, dtype=torch.float16, device="cuda") for _ in range(4)]
+    want = ops.rotate_write_kv(q, k, v, table, bt, row, pos, *pools[:2])
+    spread = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    got = ops.rotate_write_kv(spread(q), spread(k), spread(v), table.t().contiguous().t(), bt.long(), row.long().view(1, T), pos.long().view(1, T), *pools[2:])
+    assert torch.equal(got, want) and torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+    args = dict(q=q, k_new=k, v_new=v, cos_sin=table, block_table=bt, seq_index=row, positions=pos, k_cache=pools[0], v_cache=pools[1])
+    before = [t.clone() for t in pools[:2]]
+    for kw in (dict(q=q[:4]), dict(q=q.float()), dict(q=q.cpu()), dict(q=q[:, :, :32]), dict(k_new=k[:, :1]), dict(v_new=v.float()), dict(cos_sin=table.half()),
+               dict(cos_sin=table[:, :24]), dict(cos_sin=table.cpu()), dict(cos_sin=table[0]), dict(positions=pos[:3]), dict(seq_index=row.cpu()),
+               dict(block_table=bt[0]), dict(k_cache=pools[0].to(torch.int8), v_cache=pools[1].to(torch.int8)), dict(v_cache=pools[1][:3])):
+        with pytest.raises(ValueError):
+            ops.rotate_write_kv(**{**args, **kw})
+    assert all(torch.equal(a, b) for a, b in zip(before, pools))

@@ -358,3 +358,52 @@ def test_a_full_batch(ops, monkeypatch):
     with pytest.raises(RuntimeError, match="4096"):
         ops.shared_prefix_attention(torch.cat([p.Q, p.Q[:1]]), p.K, p.V, torch.cat([p.q_len, p.q_len[:1]]), torch.cat([p.table, p.table[:1]]),
                                     torch.cat([p.blocks, p.blocks[:1]]), 8, torch.cat([p.kv_len, p.kv_len[:1]]), p.group_start, p.prefix_len)
+
+
+def test_what_is_converted_and_refused(ops):
+    """64-bit metadata, float32 queries, the pool with heads in front, and arguments that the op refuses."""
+    p = Problem([(3, 64)], [[5, 20, 1]], seed=11)
+    Q, K, V, ql, bt, nb, BS, kl, gs, pl, _, _ = p.args()
+    want = ops.shared_prefix_attention(*p.args())
+    heads = [t.transpose(1, 2).contiguous() for t in (K, V)]
+    got = ops.shared_prefix_attention(Q.float(), *heads, ql.long(), bt.long(), nb.long(), BS, kl.long(), gs.long(), pl.long())
+    spread = ops.shared_prefix_attention(Q.transpose(1, 3).contiguous().transpose(1, 3), K, V, ql, bt, nb, BS, kl, gs, pl)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, spread))
+    args = dict(Q=Q, K=K, V=V, q_len_per_seq=ql, block_table=bt, num_blocks_per_seq=nb, block_size=BS, kv_len_per_seq=kl, group_start=gs, prefix_len=pl)
+    for kw in (dict(Q=Q[0]), dict(Q=Q[..., :64]), dict(K=K[:, :8], V=V[:, :8]), dict(K=K.cpu()), dict(V=V.bfloat16()), dict(block_table=bt[:2]),
+               dict(q_len_per_seq=ql[:2]), dict(kv_len_per_seq=kl.cpu()), dict(group_start=gs[:0]), dict(group_start=gs[:1]), dict(prefix_len=pl.view(1, 1)),
+               dict(prefix_len=pl.cpu()), dict(K=K.to(torch.int8), V=V.to(torch.int8))):
+        with pytest.raises(ValueError):
+            ops.shared_prefix_attention(**{**args, **kw})
+    with pytest.raises(RuntimeError, match="<= 16"):
+        ops.shared_prefix_attention(**{**args, "Q": Q.repeat(1, 1, 5, 1)})
+    with pytest.raises(RuntimeError, match="fp16, bf16 or int8"):
+        ops.shared_prefix_attention(**{**args, "K": K.float(), "V": V.float()})
+
+
+def test_two_calls_at_once(ops):
+    """Two streams, and two graphs replayed together: a call's workspace is its own."""
+    ps = [Problem([(40, 640), (9, 128)], [[3 + i % 50 for i in range(40)], [7] * 9], seed=s) for s in (1, 2)]
+    wants = [ops.shared_prefix_attention(*p.args()) for p in ps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ps]
+    gots = [[], []]
+    for _ in range(6):
+        for i, p in enumerate(ps):
+            with torch.cuda.stream(streams[i]):
+                gots[i].append(ops.shared_prefix_attention(*p.args()))
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for p in ps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.shared_prefix_attention(*p.args()))
+        graphs.append(g)
+    for _ in range(4):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for want, got, out in zip(wants, gots, outs):
+        for o, l in got + [out]:
+            assert torch.equal(o, want[0]) and torch.equal(l, want[1])
