@@ -18,7 +18,8 @@
 // Where whole heads are rotated by halves (FULL), a lane takes the same few dims of both halves, so both of a pair are
 // its own and a cos and a sin serve two dims.  With fewer dims rotated, the partner lies
 // in another lane of the same warp and comes by shuffles of packed words.  16384 tokens of 32 + 8 + 8 heads, INT8
-// pool: 120 us with shuffles for all, K and V rows in one warp and arithmetic a value at a time.
+// pool: 87 us (120 with shuffles for all, K and V rows in one warp and arithmetic a value at a time); 3001 tokens into a bf16
+// pool 17 us, 64 into INT8 3.6, one 2.4.
 #include "pa_common.cuh"
 #include "quant.cuh"
 

@@ -49,7 +49,7 @@ struct WideCfg {
   static constexpr int RAW = 128 * D;              // int8 tile
   static constexpr int KST = D == 128 ? (I8 ? 2 : 3) : (I8 ? 3 : 5);  // K stages
   static constexpr int VST = D == 128 ? 2 : (I8 ? 3 : 5);               // V stages
-  static constexpr int RST = I8 ? (D == 128 ? 2 : 8) : 0;  // raw tiles in flight, K and V alternating (4 and one V stage: 130 us, so 125)
+  static constexpr int RST = I8 ? (D == 128 ? 2 : 8) : 0;  // raw tiles in flight, K and V alternating (4 and one V stage: 120 us, so 115)
   static constexpr int K0 = 2 * TILE;
   static constexpr int V0 = K0 + KST * TILE;
   static constexpr int R0 = V0 + VST * TILE;
@@ -64,7 +64,7 @@ struct WideCfg {
 };
 
 // A scale's bits, where there is one: loaded without a branch or a conversion, so that nothing
-// waits for it before its use (4 groups of 32 over 16384 keys: 132 us with a wait of 1 us in every unit, 125 without).
+// waits for it before its use (4 groups of 32 over 16384 keys: 116 us with a wait in every unit, 115 without).
 __device__ __forceinline__ uint32_t scale_bits(const void* base, long long at, bool is, bool f32) {
   uint32_t v;
   const char* a = static_cast<const char*>(base) + (at << (f32 ? 2 : 1));
