@@ -23,6 +23,12 @@
 //                csrc/kv_dequant.cu does for prompts; the raw bytes cross HBM once and the
 //                fp16 tile never leaves the SM
 //
+// Roundings to 16 bits, as in the library's other attention kernels: the operands of a product have one type, so the
+// probabilities take the pool's (bf16: half a step of 2^-8, 1.6e-3 of the output over 65536 keys; fp16 and INT8 pools: fp16,
+// 2^-11), Q too where it differs, and INT8 keys and values fp16 once they carry their scales. A second
+// product with what the rounding left would halve the rate of a kernel that the products bound. Logits, maxima, sums (of the
+// unrounded probabilities) and outputs stay in fp32 until the join.
+//
 // 16-bit pools: bound by HBM up to about 256 rows a kv head, by the issue of the two products beyond (128 keys of 128 rows
 // take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
 // INT8 pools: by the conversion of the tiles, 1100 cycles each; eight warps for it left 96 registers a thread and
