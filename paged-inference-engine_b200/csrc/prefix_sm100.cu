@@ -24,8 +24,8 @@
 //                fp16 tile never leaves the SM
 //
 // Roundings to 16 bits, as in the library's other attention kernels: the operands of a product have one type, so the
-// probabilities take the pool's (bf16: half a step of 2^-8, 1.6e-3 of the output over 65536 keys; fp16 and INT8 pools: fp16,
-// 2^-11), Q too where it differs, and INT8 keys and values fp16 once they carry their scales. A second
+// probabilities take the pool's (bf16: off by up to 2^-8, which leaves 1.7e-3 in the output over 65536 keys; fp16 and INT8 pools:
+// fp16, 2^-11), Q too where it differs, and INT8 keys and values fp16 once they carry their scales. A second
 // product with what the rounding left would halve the rate of a kernel that the products bound. Logits, maxima, sums (of the
 // unrounded probabilities) and outputs stay in fp32 until the join.
 //

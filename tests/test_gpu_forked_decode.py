@@ -222,3 +222,53 @@ def test_beam_search_rules_refuse():
         search.advance(torch.zeros(2, 2, 30, device="cuda"), torch.zeros(4, 2, dtype=torch.int32, device="cuda"))
     search.advance(torch.zeros(2, 2, 30, device="cuda"))
     search.finish()
+
+
+@pytest.mark.parametrize("maxq", [1, 3])
+def test_an_eager_step_over_forks(maxq):
+    """The reference-named wrappers and DeviceBlockManager.shared_prefixes: several new tokens a sequence, forks of forks, one released."""
+    from kernels.flash_attention import flash_attention_shared_prefix, rotate_write_kv_cache
+    from pie_b200 import ops as o
+    from pie_b200.block_pool import DeviceBlockManager
+
+    BS, Hkv, D, Hq, NB, n = 16, 2, 64, 4, 120, 150
+    gen = torch.Generator(device="cuda").manual_seed(maxq)
+    k, v = (torch.full((NB, BS, Hkv, D), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pool = DeviceBlockManager(NB, BS, 12, 16)
+    pool.attach_caches(k, v)
+    table = o.rope_table(300, D, device="cuda")
+
+    def rows(count, heads):
+        return torch.randn(count, heads, D, device="cuda", generator=gen).bfloat16()
+
+    pool.allocate(0, -(-n // BS))
+    inp = pool.step_inputs([0], [n], [n])
+    rotate_write_kv_cache(None, rows(n, Hkv), rows(n, Hkv), table, inp["block_table"], inp["token_seq"], inp["positions"], k, v)
+    lens = {0: n, "a": n, "b": 70, "c": 70, 4: n}
+    pool.fork(0, "a", n)
+    pool.fork("a", "b", 70)
+    pool.fork("b", "c", 70)
+    pool.fork(0, 4, n)
+    pool.release_blocks(0)
+    del lens[0]
+    ids = ["a", 4, "b", "c"]
+    for _ in range(3):
+        for s in ids:
+            lens[s] += maxq
+            need = -(-lens[s] // BS) - pool.blocks_of(s)
+            if need:
+                pool.allocate(s, need)
+        inp = pool.step_inputs(ids, [maxq] * 4, [lens[s] for s in ids])
+        q = rotate_write_kv_cache(rows(4 * maxq, Hq), rows(4 * maxq, Hkv), rows(4 * maxq, Hkv), table, inp["block_table"], inp["token_seq"],
+                                  inp["positions"], k, v)
+        groups = pool.shared_prefixes(ids)
+        assert groups["group_start"].tolist() == [0, 2, 4] and groups["prefix_len"].tolist() == [n // BS * BS, 70 // BS * BS]
+        Q = q.view(4, maxq, Hq, D).transpose(1, 2)
+        out, lse = flash_attention_shared_prefix(Q, k, v, inp["q_len"], inp["block_table"], inp["num_blocks_per_seq"], BS, inp["kv_len"], **groups)
+        held = pool.block_table
+        p = Step(q.view(4, maxq, Hq, D)[:, 0], k, v, None, None, [held[s] for s in ids], [lens[s] for s in ids], BS)
+        p.Q, p.maxq, p.q_len = Q, maxq, inp["q_len"]
+        check(p, out, lse)
+    with pytest.raises(KeyError):
+        pool.shared_prefixes([0])
+    assert pool.status.item() == 0
