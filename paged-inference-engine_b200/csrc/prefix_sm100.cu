@@ -84,16 +84,23 @@ __device__ __forceinline__ uint32_t scale_bits(const void* base, long long at, b
 
 __device__ unsigned int g_wide_abort = 0;  // launch generation in which a wait gave up
 
-__device__ __noinline__ void wide_wait_slow(const SharedParams& p, uint32_t bar, uint32_t parity) {
+// False: gave up, by itself or since another wait of this launch did.  A CTA then walks to its end without its results
+// being good (the status word says so); only the producer stops, and waits for its copies before the CTA ends.
+__device__ __noinline__ bool wide_wait_slow(const SharedParams& p, uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 20); ++i) {
-    if (mbar_try_wait(bar, parity)) return;
-    if ((i & 1023) == 1023 && *reinterpret_cast<volatile unsigned int*>(&g_wide_abort) == p.abort_gen) return;
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 1023) == 1023 && *reinterpret_cast<volatile unsigned int*>(&g_wide_abort) == p.abort_gen) return false;
   }
   atomicExch(&g_wide_abort, p.abort_gen);
   set_status(p.status, ST_WAIT_TIMEOUT);
+  return false;
 }
-__device__ __forceinline__ void wide_wait(const SharedParams& p, uint32_t bar, uint32_t parity) {
-  if (!mbar_try_wait(bar, parity)) wide_wait_slow(p, bar, parity);
+__device__ __forceinline__ bool wide_wait(const SharedParams& p, uint32_t bar, uint32_t parity) {
+  return mbar_try_wait(bar, parity) || wide_wait_slow(p, bar, parity);
+}
+__device__ __noinline__ void wide_drain(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < (1 << 20); ++i)
+    if (mbar_try_wait(bar, parity)) return;
 }
 __device__ __forceinline__ void wide_barrier(int id, int n) { asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(n) : "memory"); }
 
@@ -230,8 +237,9 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
     // Lane i owns box i of every tile; the block ids of a tile are fetched one tile ahead.
     const int boxs = p.BS < 16 ? p.BS : 16;
     const int nbox = kWideKeys / boxs;  // <= 16 (block_size >= 8)
-    int gt = 0, gr = 0;  // tiles, and raw tiles, so far
-    while (it.next(p)) {
+    int issued[2] = {0, 0};  // K and V tiles (INT8: [0] raw tiles) so far
+    bool going = true;       // false: a wait gave up
+    while (going && it.next(p)) {
       const int* bt_row = p.bt + static_cast<long long>(it.grp.w) * p.bt_ss;
       auto fetch = [&](int j) {
         const int key = (it.t + j) * kWideKeys + lane * boxs;
@@ -246,27 +254,31 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       // The order of the loads is K0, K1 V0, K2 V1, ...: a key tile's K is wanted a product before its V, and a
       // V stage comes free late.
       auto load = [&](int v, int j, int blk) {
+        if (!going) return;
         const int slot = blk < p.NB ? ((it.t + j) * kWideKeys + lane * boxs) & (p.BS - 1) : 0;
-        uint32_t dst, full;
+        uint32_t dst, full, empty;
+        int turn;  // how often the stage was used
         if constexpr (I8) {
-          const int s = gr % C::RST;
+          const int s = issued[0] % C::RST;
+          turn = issued[0] / C::RST;
           full = bar(C::B_RFULL + s);
+          empty = bar(C::B_REMPTY + s);
           dst = base + C::R0 + s * C::RAW + lane * boxs * D;
-          if (lane == 0) {
-            if (gr >= C::RST) wide_wait(p, bar(C::B_REMPTY + s), (gr / C::RST - 1) & 1);
-            mbar_arrive_expect_tx(full, C::RAW);
-          }
-          ++gr;
         } else {
-          const int st = v ? VST : KST, g = gt + j, s = g % st;
+          const int st = v ? VST : KST, s = issued[v] % st;
+          turn = issued[v] / st;
           full = bar((v ? C::B_VFULL : C::B_KFULL) + s);
+          empty = bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s);
           dst = base + (v ? C::V0 : C::K0) + s * TILE + lane * boxs * 128;
-          if (lane == 0) {
-            if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
-            mbar_arrive_expect_tx(full, TILE);
-          }
         }
-        __syncwarp();
+        if (lane == 0) {
+          // free again, and its last copies have arrived (known, unless a reader gave up)
+          going = turn == 0 || (wide_wait(p, empty, (turn - 1) & 1) && wide_wait(p, full, (turn - 1) & 1));
+          if (going) mbar_arrive_expect_tx(full, I8 ? C::RAW : TILE);
+        }
+        going = __shfl_sync(0xffffffffu, going, 0);
+        if (!going) return;
+        ++issued[I8 ? 0 : v];
         if (lane < nbox) {
           const CUtensorMap* m = v ? &maps.v : &maps.k;
           tma_load_4d(dst, m, full, 0, it.kvh, slot, blk);
@@ -283,7 +295,11 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         b0 = b1;
         b1 = b2;
       }
-      gt += n;
+    }
+    if (lane == 0) {  // no copy is in flight when the CTA ends
+      const int k = issued[0], v = issued[1], kst = I8 ? C::RST : KST;
+      for (int s = 0; s < kst && s < k; ++s) wide_drain(bar((I8 ? C::B_RFULL : C::B_KFULL) + s), ((k - 1 - s) / kst) & 1);
+      for (int s = 0; s < VST && s < v; ++s) wide_drain(bar(C::B_VFULL + s), ((v - 1 - s) / VST) & 1);
     }
   } else if (warp == W_MMA) {
     // ------------------------------------------------------------ MMA issuer
