@@ -27,7 +27,8 @@
 // probabilities take the pool's (bf16: off by up to 2^-8, which leaves 1.7e-3 in the output over 65536 keys; fp16 and INT8 pools:
 // fp16, 2^-11), Q too where it differs, and INT8 keys and values fp16 once they carry their scales. A second
 // product with what the rounding left would halve the rate of a kernel that the products bound. Logits, maxima, sums (of the
-// unrounded probabilities) and outputs stay in fp32 until the join.
+// unrounded probabilities) and outputs stay in fp32 until the join.  fp16's range is that of values of INT8 pools (and of
+// bf16 queries over fp16 and INT8 pools), as it is that of the outputs; INT8 keys may lie beyond it (RANGE).
 //
 // 16-bit pools: bound by HBM up to about 256 rows a kv head, by the issue of the two products beyond (128 keys of 128 rows
 // take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
@@ -63,10 +64,15 @@ struct WideCfg {
   static constexpr int B_QREADY = 0, B_QEMPTY = 1, B_SFULL = 2, B_PFULL = 4, B_ODONE = 6, B_SLOT = 8, B_PLACE = 9,
                        B_KFULL = 10, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
                        B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
-  static constexpr int XCH = BAR + (D == 128 ? 256 : 512);
+  static constexpr int RANGE = BAR + (D == 128 ? 256 : 512);  // INT8: powers of two that the keys were divided by
+  // Tiles whose powers are held.  They are written with K of a tile and read with its logits.  Before K of tile t comes V of
+  // t - 2, which waits until the stage that tile t - 2 - VST had is free: its products, and so its probabilities, are done.
+  static constexpr int RANGES = I8 ? 8 : 0;
+  static_assert(!I8 || RANGES >= VST + 2, "a tile's powers are read before they are written again");
+  static constexpr int XCH = RANGE + RANGES * W_CONVERTERS * 4;
   static constexpr int SMEM = XCH + 1024 + 1024;  // exchange of the two streams, alignment
   static constexpr int THREADS = 32 * (I8 ? W_CONVERT + W_CONVERTERS : W_CONVERT);
-  static_assert(B_END * 8 <= XCH - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
+  static_assert(B_END * 8 <= RANGE - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
 };
 
 // A scale's bits, where there is one: loaded without a branch or a conversion, so that nothing
@@ -377,7 +383,19 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           wide_wait(p, bar(C::B_RFULL + rs), (gr / C::RST) & 1);
           if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
           ++gr;
-          const float mine = p.scale_f32 ? __uint_as_float(mine_bits) : __half2float(__ushort_as_half(static_cast<unsigned short>(mine_bits)));
+          float mine = p.scale_f32 ? __uint_as_float(mine_bits) : __half2float(__ushort_as_half(static_cast<unsigned short>(mine_bits)));
+          if (v == 0) {
+            // Keys that would leave fp16's range (a scale above 256) are divided by a power of two, one for the warp's keys of a
+            // tile, which their logits are multiplied by in turn.
+            const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(mine)));
+            float range = 1.f;
+            if (most > __float_as_uint(256.f) && most < 0x7f800000u) {
+              const unsigned e = (most >> 23) - 7u;  // exponent bits of the power
+              range = __uint_as_float(e << 23);
+              mine *= __uint_as_float((254u - e) << 23);
+            }
+            if (lane == 0) reinterpret_cast<float*>(sm + C::RANGE)[(g % C::RANGES) * W_CONVERTERS + warp - W_CONVERT] = range;
+          }
           auto rows = [&](auto fp32_scale) {
 #pragma unroll UNROLL
             for (int k = 0; k < ROWS / RPI; ++k) {
@@ -447,6 +465,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
     const uint32_t scol = trow + 128u * x, ocol = trow + W_OCOL + 128u * x;
     float* xch = reinterpret_cast<float*>(sm + C::XCH);  // [2 streams][128 rows]
     const int per = p.maxq * p.G;
+    int gt = 0;            // key tiles before the piece
     int done[2] = {0, 0};  // units of each stream
     int q_done = 0;
     for (; it.next(p);) {
@@ -497,6 +516,12 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           // first look: the row's maximum.  The logits are read again below: 128 of them do not fit the registers
           // beside the rest, and a second read of TMEM is cheap
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float range[4] = {1.f, 1.f, 1.f, 1.f};  // of the keys [32 c, 32 c + 32)
+          if constexpr (I8) {
+            static_assert(kWideKeys / W_CONVERTERS == 32, "a converting warp's keys are those of one step below");
+            const float4 w = reinterpret_cast<const float4*>(sm + C::RANGE)[(gt + it.tile(u)) % C::RANGES];
+            range[0] = w.x, range[1] = w.y, range[2] = w.z, range[3] = w.w;
+          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t r0[32], r1[32];
@@ -510,8 +535,20 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
                 if (64 * c + 32 + i >= left) r1[i] = 0xff800000u;
               }
             }
+            if constexpr (I8) {
+              float a[2] = {-INFINITY, -INFINITY}, b[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx4[i & 3] = fmax3f(mx4[i & 3], __uint_as_float(r0[i]), __uint_as_float(r1[i]));
+              for (int i = 0; i < 32; i += 2) {
+                const int k = (i >> 1) & 1;
+                a[k] = fmax3f(a[k], __uint_as_float(r0[i]), __uint_as_float(r0[i + 1]));
+                b[k] = fmax3f(b[k], __uint_as_float(r1[i]), __uint_as_float(r1[i + 1]));
+              }
+              mx4[2 * c] = fmaxf(a[0], a[1]) * range[2 * c];
+              mx4[2 * c + 1] = fmaxf(b[0], b[1]) * range[2 * c + 1];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mx4[i & 3] = fmax3f(mx4[i & 3], __uint_as_float(r0[i]), __uint_as_float(r1[i]));
+            }
           }
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
           float alpha = 1.f;
@@ -522,7 +559,6 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
             m_ref = mx;
           }
           const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-          const float c2 = p.scale_log2;
           uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
           // P of keys [32 c, 32 c + 32) takes TMEM columns [16 c, 16 c + 16): behind the logits still to be read
           uint32_t rr[2][32];
@@ -532,6 +568,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
             tmem_wait_ld();
             if (c < 3) tmem_ld32(scol + 32 * (c + 1), rr[(c + 1) & 1]);
             const uint32_t* s = rr[c & 1];
+            const float c2 = I8 ? p.scale_log2 * range[c] : p.scale_log2;
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -574,6 +611,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       }
       done[0] += (nu + 1) / 2;
       done[1] += nu / 2;
+      gt += it.n;
       // ---- end of the piece: its rows go to the workspace ---------------------------
       const long long prow = shared_wide_row(p, it.sh, it.grp.y, it.seg, it.team, it.size, it.part, it.lane) + mine0;
       const int rb = (warp & 3) * 32 + (lane & ~7);
