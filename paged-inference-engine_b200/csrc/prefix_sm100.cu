@@ -27,8 +27,8 @@
 // probabilities take the pool's (bf16: off by up to 2^-8, which leaves 1.7e-3 in the output over 65536 keys; fp16 and INT8 pools:
 // fp16, 2^-11), Q too where it differs, and INT8 keys and values fp16 once they carry their scales. A second
 // product with what the rounding left would halve the rate of a kernel that the products bound. Logits, maxima, sums (of the
-// unrounded probabilities) and outputs stay in fp32 until the join.  fp16's range is that of values of INT8 pools (and of
-// bf16 queries over fp16 and INT8 pools), as it is that of the outputs; INT8 keys may lie beyond it (RANGE).
+// unrounded probabilities) and outputs stay in fp32 until the join.  INT8 keys may lie beyond fp16's range, and values up to
+// 127 * 65536 (RANGE); it is the range of bf16 queries over fp16 and INT8 pools, as of the outputs.
 //
 // 16-bit pools: bound by HBM up to about 256 rows a kv head, by the issue of the two products beyond (128 keys of 128 rows
 // take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
@@ -64,12 +64,12 @@ struct WideCfg {
   static constexpr int B_QREADY = 0, B_QEMPTY = 1, B_SFULL = 2, B_PFULL = 4, B_ODONE = 6, B_SLOT = 8, B_PLACE = 9,
                        B_KFULL = 10, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
                        B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
-  static constexpr int RANGE = BAR + (D == 128 ? 256 : 512);  // INT8: powers of two that the keys were divided by
+  static constexpr int RANGE = BAR + (D == 128 ? 256 : 512);  // INT8: powers of two that keys and values were divided by
   // Tiles whose powers are held.  They are written with K of a tile and read with its logits.  Before K of tile t comes V of
   // t - 2, which waits until the stage that tile t - 2 - VST had is free: its products, and so its probabilities, are done.
   static constexpr int RANGES = I8 ? 8 : 0;
   static_assert(!I8 || RANGES >= VST + 2, "a tile's powers are read before they are written again");
-  static constexpr int XCH = RANGE + RANGES * W_CONVERTERS * 4;
+  static constexpr int XCH = RANGE + RANGES * W_CONVERTERS * 8;
   static constexpr int SMEM = XCH + 1024 + 1024;  // exchange of the two streams, alignment
   static constexpr int THREADS = 32 * (I8 ? W_CONVERT + W_CONVERTERS : W_CONVERT);
   static_assert(B_END * 8 <= RANGE - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
@@ -376,25 +376,32 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           k = scale_bits(p.ks, is ? blk * p.ks_sblk + slot * p.ks_sslot + it.kvh * p.ks_shead : 0, is, p.scale_f32);
           v = scale_bits(p.vs, is ? blk * p.vs_sblk + slot * p.vs_sslot + it.kvh * p.vs_shead : 0, is, p.scale_f32);
         };
-        auto convert = [&](int v, int j, uint32_t mine_bits) {
+        auto as_float = [&](uint32_t bits) {
+          return p.scale_f32 ? __uint_as_float(bits) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+        };
+        // Keys and values that would leave fp16's range (127 times a scale above 512) are divided by a power of two, one for the
+        // warp's rows of a tile, which the logits or probabilities are multiplied by in turn.
+        auto power = [&](float mine) {
+          if (!__any_sync(0xffffffffu, fabsf(mine) > 512.f)) return 1.f;
+          const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(mine)));
+          return most < 0x7f800000u ? __uint_as_float(((most >> 23) - 8u) << 23) : 1.f;
+        };
+        auto inverse = [&](float pow2) { return __uint_as_float((254u << 23) - __float_as_uint(pow2)); };
+        // later_bits: the scales of the same tile's V, at its K
+        auto convert = [&](int v, int j, uint32_t mine_bits, uint32_t later_bits) {
           const int st = v ? VST : KST, g = gt + j, s = g % st, rs = gr % C::RST;
           const unsigned char* src = sm + C::R0 + rs * C::RAW;
           unsigned char* dst = sm + (v ? C::V0 : C::K0) + s * TILE;
           wide_wait(p, bar(C::B_RFULL + rs), (gr / C::RST) & 1);
           if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
           ++gr;
-          float mine = p.scale_f32 ? __uint_as_float(mine_bits) : __half2float(__ushort_as_half(static_cast<unsigned short>(mine_bits)));
+          float mine = as_float(mine_bits);
+          const float range = power(mine);
+          mine *= inverse(range);
           if (v == 0) {
-            // Keys that would leave fp16's range (a scale above 256) are divided by a power of two, one for the warp's keys of a
-            // tile, which their logits are multiplied by in turn.
-            const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(mine)));
-            float range = 1.f;
-            if (most > __float_as_uint(256.f) && most < 0x7f800000u) {
-              const unsigned e = (most >> 23) - 7u;  // exponent bits of the power
-              range = __uint_as_float(e << 23);
-              mine *= __uint_as_float((254u - e) << 23);
-            }
-            if (lane == 0) reinterpret_cast<float*>(sm + C::RANGE)[(g % C::RANGES) * W_CONVERTERS + warp - W_CONVERT] = range;
+            const float later = power(as_float(later_bits));
+            float* at = reinterpret_cast<float*>(sm + C::RANGE) + (g % C::RANGES) * 2 * W_CONVERTERS + warp - W_CONVERT;
+            if (lane == 0) at[0] = range, at[W_CONVERTERS] = later;
           }
           auto rows = [&](auto fp32_scale) {
 #pragma unroll UNROLL
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           blk2 = block(j + 3);
 #pragma unroll 1
           for (int v = 0; v < 2; ++v)
-            if (j + 1 - v >= 0 && j + 1 - v < n) convert(v, j + 1 - v, v ? v0 : k1);
+            if (j + 1 - v >= 0 && j + 1 - v < n) convert(v, j + 1 - v, v ? v0 : k1, v1);
           v0 = v1, k1 = k2, v1 = v2;
         }
         gt += n;
@@ -516,12 +523,9 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           // first look: the row's maximum.  The logits are read again below: 128 of them do not fit the registers
           // beside the rest, and a second read of TMEM is cheap
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          float range[4] = {1.f, 1.f, 1.f, 1.f};  // of the keys [32 c, 32 c + 32)
-          if constexpr (I8) {
-            static_assert(kWideKeys / W_CONVERTERS == 32, "a converting warp's keys are those of one step below");
-            const float4 w = reinterpret_cast<const float4*>(sm + C::RANGE)[(gt + it.tile(u)) % C::RANGES];
-            range[0] = w.x, range[1] = w.y, range[2] = w.z, range[3] = w.w;
-          }
+          // INT8: of the keys [32 c, 32 c + 32), then of the values
+          static_assert(!I8 || kWideKeys / W_CONVERTERS == 32, "a converting warp's keys are those of one step below");
+          const float* range = reinterpret_cast<const float*>(sm + C::RANGE) + (I8 ? (gt + it.tile(u)) % C::RANGES * 2 * W_CONVERTERS : 0);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t r0[32], r1[32];
@@ -584,6 +588,14 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
               }
               sum[i & 1] = f2_add(sum[i & 1], f2_pack(p0, p1));
               pk[i] = pack2<MMA_BF16>(p0, p1);
+            }
+            if constexpr (I8) {
+              const float of_v = range[W_CONVERTERS + c];
+              if (of_v != 1.f) {  // the warp as one; exact, but for numbers below fp16's normal range
+                const __half2 h = __float2half2_rn(of_v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) reinterpret_cast<__half2*>(pk)[i] = __hmul2(reinterpret_cast<__half2*>(pk)[i], h);
+              }
             }
             tmem_st16(scol + 16 * c, pk);
           }

@@ -89,3 +89,20 @@ def test_keys_beyond_the_range_of_fp16(ops, monkeypatch, scale_dtype, big, D):
     p.Q = (p.Q.float() * 2.0 ** -math.ceil(math.log2(big * 127 / 4))).half()
     assert bool((p.Q != 0).any(-1).all())
     both_forms(p, ops, monkeypatch, parts(groups, 16), rows=[0, 7, 19, 20, 28], range_=1024.0)
+
+
+@pytest.mark.parametrize("scale_dtype,big", [(torch.float32, 512.0), (torch.float32, 600.0), (torch.float32, 65000.0), (torch.float16, 600.0),
+                                             (torch.float16, 65504.0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_beyond_the_range_of_fp16(ops, scale_dtype, big, D):
+    """INT8 values beyond 65504 of keys that weigh little (zeros: a logit of 0), so that the outputs are within fp16."""
+    groups = [(20, 700), (9, 320)]
+    p = Problem(groups, [[5] * 20, [40] * 9], pool=torch.int8, D=D, scale_dtype=scale_dtype, seed=int(big) % 1000 + D)
+    for b, at in ((0, (3, 300, 301, 640)), (20, (5, 200, 319))):
+        for i in at:
+            block, slot = p.table[b, i // p.BS].long(), i % p.BS
+            p.vs[block, slot] = big
+            p.K[block, slot] = 0
+    O, L = ops.shared_prefix_attention(*p.args())
+    assert big < 2000 or float(O.abs().max()) > 100  # they show
+    check_norms(p, O, L, parts(groups, 16), True, rows=[0, 7, 19, 20, 28], range_=1024.0)
