@@ -32,7 +32,6 @@
 // places in the row alone, not on its address, so equal rows have equal sums.
 #include "pa_common.cuh"
 
-#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -612,17 +611,6 @@ void beam_plan(BeamParams& p, int dtype) {
   p.row_units = static_cast<int>(units);
   p.log_span = 0;
   while ((p.part_units - 1) >> p.log_span >= kSpans) ++p.log_span;
-}
-
-// Shared memory past the default, allowed once per device.
-template <typename K>
-cudaError_t allow_smem(K* kernel, int bytes, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
-  return e;
 }
 
 template <int DT>

@@ -5,6 +5,7 @@
 // arithmetic.  No CUDA math-library routine is restated.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
@@ -23,6 +24,18 @@ namespace pa {
 __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
+// Shared memory past the default, allowed once per device.  `bytes` is the most that any launch of the kernel takes:
+// the attribute is the kernel's, so a launch's own size would fail a larger one that another thread is about to make.
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return e;
 }
 
 template <typename... KArgs, typename... Args>

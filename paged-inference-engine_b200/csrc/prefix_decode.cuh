@@ -25,7 +25,8 @@ struct SharedInst {
     return 0;
   }
   static cudaError_t launch(const SharedParams& p, const KvMaps& maps, const DecodeLaunch& pl, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pl.smem));
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = allow_smem(kern, SMEM_LIMIT, done);  // pl.smem goes by B
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3(pl.ctas), dim3(pl.warps_per_cta * 32), pl.smem, stream, p, maps);
   }

@@ -348,9 +348,11 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 3) prefix_merge_kernel(const
 }  // namespace
 
 cudaError_t launch_prefix_plan(const SharedParams& p, cudaStream_t stream) {
-  const size_t smem = (5 * static_cast<size_t>(p.groups) + 2 + 2 * static_cast<size_t>(p.B) + 1) * sizeof(int);
+  const auto bytes = [](size_t groups, size_t B) { return (5 * groups + 2 + 2 * B + 1) * sizeof(int); };
+  const size_t smem = bytes(p.groups, p.B);
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = allow_smem(prefix_plan_kernel, static_cast<int>(bytes(kMaxSharedSeqs, kMaxSharedSeqs)), done);
     if (e != cudaSuccess) return e;
   }
   // a thread for each work list entry: barriers cost more the more threads meet at them
