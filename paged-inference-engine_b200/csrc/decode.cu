@@ -87,6 +87,10 @@ __global__ void __launch_bounds__(128) pa_decode_merge_kernel(const AttnParams p
 template <int D, int KVT, int QT, int NT, bool TMA>
 struct DecodeInst {
   using Lay = DecLayout<D, KVT, NT>;
+  static cudaError_t allow() {  // launches' sizes go by B
+    static std::atomic<unsigned long long> done{0};
+    return allow_smem(pa_decode_kernel<D, KVT, QT, NT, TMA>, SMEM_LIMIT, done);
+  }
   static int plan(int B, DecodeLaunch* out) {
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return -1;
@@ -99,9 +103,7 @@ struct DecodeInst {
     out->warps_per_cta = nw;
     out->smem = static_cast<size_t>(fixed + nw * Lay::WARPB);
     auto kern = pa_decode_kernel<D, KVT, QT, NT, TMA>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(out->smem)) !=
-        cudaSuccess)
-      return -1;
+    if (allow() != cudaSuccess) return -1;
     int per_sm = 0;
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, nw * 32, out->smem);
     if (per_sm < 1) per_sm = 1;
@@ -113,7 +115,7 @@ struct DecodeInst {
     cudaError_t e;
     if (phase != DECODE_MERGE) {
       auto kern = pa_decode_kernel<D, KVT, QT, NT, TMA>;
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pl.smem));
+      e = allow();
       if (e != cudaSuccess) return e;
       e = launch_pdl(kern, dim3(pl.ctas), dim3(pl.warps_per_cta * 32), pl.smem, stream, p, maps);
       if (e != cudaSuccess) return e;

@@ -50,6 +50,21 @@ def test_batches_of_different_sizes(monkeypatch, backend):
         assert torch.equal(o, o2) and torch.equal(l, l2)
 
 
+@pytest.mark.parametrize("backend", ["torch", "ctypes"])
+def test_decode_batches_of_different_sizes(monkeypatch, backend):
+    """The same of paged_attention's split-K kernel."""
+    from pie_b200 import ops
+
+    monkeypatch.setattr(ops, "BACKEND", backend)
+    ps = [Problem([(1, 16)] * n, [[3]] * n, Hq=2, Hkv=1, D=64, seed=n) for n in (1, 33, 65, 97, 600, 900)]
+    calls = [lambda p=p: ops.paged_attention(*p.args()[:8], mode="decode") for p in ps]
+    want = [c() for c in calls]
+    got, raised = race(calls, 6000)
+    assert not raised, raised[0]
+    for (o, l), (o2, l2) in zip(want, got):
+        assert torch.equal(o, o2) and torch.equal(l, l2)
+
+
 def test_large_batches_of_groups():
     """The plan of more than some 1500 sequences and groups takes more shared memory than a kernel has by default."""
     from pie_b200 import ops
