@@ -101,7 +101,7 @@ struct SharedParams : AttnParams {
   int wide_ctas;
   int* step0;             // [groups + 1] first step of a group (wide)
   int4* grp;              // [groups] shared keys, first sequence, sequences, leader
-  int4* head;             // [1] CTAs of a team, steps of a team, all steps (wide)
+  int4* head;             // [1] CTAs of a team, steps of a team, all steps; 1 once a wait gave up (wide)
   int4* info;             // [B] what prefix_merge_kernel asks of a sequence's shared part: first tile and tiles of its chunk, or first step of its group
   long long prefix_row0;  // first partial row of the shared prefixes
 };

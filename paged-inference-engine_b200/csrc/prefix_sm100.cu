@@ -34,9 +34,9 @@
 // take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
 // INT8 pools: by the conversion of the tiles, 1100 cycles each; eight warps for it left 96 registers a thread and
 // gained nothing.
-#include <atomic>
 #include <type_traits>
 
+#include "bounded_wait.cuh"
 #include "pa_common.cuh"
 
 namespace pa {
@@ -64,7 +64,8 @@ struct WideCfg {
   static constexpr int B_QREADY = 0, B_QEMPTY = 1, B_SFULL = 2, B_PFULL = 4, B_ODONE = 6, B_SLOT = 8, B_PLACE = 9,
                        B_KFULL = 10, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
                        B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
-  static constexpr int RANGE = BAR + (D == 128 ? 256 : 512);  // INT8: powers of two that keys and values were divided by
+  static constexpr int BARS = D == 128 ? 256 : 512;  // bytes of the barriers, and what a wait that gives up writes (16 bytes)
+  static constexpr int RANGE = BAR + BARS;  // INT8: powers of two that keys and values were divided by
   // Tiles whose powers are held.  They are written with K of a tile and read with its logits.  Before K of tile t comes V of
   // t - 2, which waits until the stage that tile t - 2 - VST had is free: its products, and so its probabilities, are done.
   static constexpr int RANGES = I8 ? 8 : 0;
@@ -72,7 +73,7 @@ struct WideCfg {
   static constexpr int XCH = RANGE + RANGES * W_CONVERTERS * 8;
   static constexpr int SMEM = XCH + 1024 + 1024;  // exchange of the two streams, alignment
   static constexpr int THREADS = 32 * (I8 ? W_CONVERT + W_CONVERTERS : W_CONVERT);
-  static_assert(B_END * 8 <= RANGE - BAR && SMEM <= 227 * 1024, "shared memory per CTA");
+  static_assert(B_END * 8 + 16 <= BARS && BAR % BARS == 0 && SMEM <= 227 * 1024, "shared memory per CTA");
 };
 
 // A scale's bits, where there is one: loaded without a branch or a conversion, so that nothing
@@ -88,21 +89,31 @@ __device__ __forceinline__ uint32_t scale_bits(const void* base, long long at, b
   return v;
 }
 
-__device__ unsigned int g_wide_abort = 0;  // launch generation in which a wait gave up
-
-// False: gave up, by itself or since another wait of this launch did.  A CTA then walks to its end without its results
-// being good (the status word says so); only the producer stops, and waits for its copies before the CTA ends.
-__device__ __noinline__ bool wide_wait_slow(const SharedParams& p, uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < (1 << 20); ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 1023) == 1023 && *reinterpret_cast<volatile unsigned int*>(&g_wide_abort) == p.abort_gen) return false;
+// A wait that fails gave up, by itself or since another wait of this launch did (the plan clears their word in the call's workspace
+// on every run, a captured call's replays too).  A CTA then walks to its end without its results being good (the status
+// word says so); only the producer stops, and waits for its copies before the CTA ends.
+// The addresses of their word and of the status word lie at the end of the barriers' block, which a barrier's address gives: so
+// a wait has no other arguments (with the parameters for one, 128 sequences of 4 heads over 65536 keys took 192 us, so 187).
+template <int D>
+struct WideGiveUp {
+  uint32_t bar;
+  __device__ __forceinline__ uint64_t address(int i) const {
+    constexpr uint32_t BARS = WideCfg<D, false>::BARS;
+    uint64_t a;
+    asm volatile("ld.shared.b64 %0, [%1];\n" : "=l"(a) : "r"((bar & ~(BARS - 1)) + BARS - 16 + 8 * i));
+    return a;
   }
-  atomicExch(&g_wide_abort, p.abort_gen);
-  set_status(p.status, ST_WAIT_TIMEOUT);
-  return false;
+  __device__ __forceinline__ bool marked() const { return *reinterpret_cast<volatile int*>(address(0)) != 0; }
+  __device__ __forceinline__ void mark() const { atomicExch(reinterpret_cast<int*>(address(0)), 1); }
+  __device__ __forceinline__ void report() const { set_status(reinterpret_cast<int*>(address(1)), ST_WAIT_TIMEOUT); }
+};
+template <int D>
+__device__ __noinline__ bool wide_wait_slow(uint32_t bar, uint32_t parity) {
+  return bounded_wait<1 << 20, 64>(bar, parity, WideGiveUp<D>{bar});
 }
-__device__ __forceinline__ bool wide_wait(const SharedParams& p, uint32_t bar, uint32_t parity) {
-  return mbar_try_wait(bar, parity) || wide_wait_slow(p, bar, parity);
+template <int D>
+__device__ __forceinline__ bool wide_wait(uint32_t bar, uint32_t parity) {
+  return mbar_try_wait(bar, parity) || wide_wait_slow<D>(bar, parity);
 }
 __device__ __noinline__ void wide_drain(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 20); ++i)
@@ -208,6 +219,9 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       mbar_init(bar(C::B_RFULL + s), 1);
       mbar_init(bar(C::B_REMPTY + s), 32 * W_CONVERTERS);
     }
+    uint64_t* at = reinterpret_cast<uint64_t*>(sm + C::BAR + C::BARS - 16);
+    at[0] = reinterpret_cast<uint64_t>(&p.head[0].w);
+    at[1] = reinterpret_cast<uint64_t>(p.status);
     fence_mbar_init();
   }
   pdl_enter();
@@ -279,7 +293,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         }
         if (lane == 0) {
           // free again, and its last copies have arrived (known, unless a reader gave up)
-          going = turn == 0 || (wide_wait(p, empty, (turn - 1) & 1) && wide_wait(p, full, (turn - 1) & 1));
+          going = turn == 0 || (wide_wait<D>(empty, (turn - 1) & 1) && wide_wait<D>(full, (turn - 1) & 1));
           if (going) mbar_arrive_expect_tx(full, I8 ? C::RAW : TILE);
         }
         going = __shfl_sync(0xffffffffu, going, 0);
@@ -320,7 +334,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       const bool two = it.two;
       auto qk = [&](int u) {
         const int x = u & 1, tile = gt + it.tile(u), s = tile % KST;
-        wide_wait(p, bar(C::B_KFULL + s), (tile / KST) & 1);
+        wide_wait<D>(bar(C::B_KFULL + s), (tile / KST) & 1);
         tc_fence_after();
         tc_elect_mma_ss<D / 16, W_HALF / 16, W_HALF / 16>(tmem + 128u * x, smem_desc(base + (two ? x * TILE : 0), 16, 1024),
                                                           smem_desc(base + C::K0 + s * TILE, 16, 1024), IDESC_QK);
@@ -328,14 +342,14 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         if (!two || x) tc_elect_commit(bar(C::B_KEMPTY + s));
         if (u == nu - 1) tc_elect_commit(bar(C::B_QEMPTY));
       };
-      wide_wait(p, bar(C::B_QREADY), piece & 1);
+      wide_wait<D>(bar(C::B_QREADY), piece & 1);
       tc_fence_after();
       qk(0);
       if (nu > 1) qk(1);
       for (int u = 0; u < nu; ++u) {
         const int x = u & 1, tile = gt + it.tile(u), s = tile % VST;
-        wide_wait(p, bar(C::B_VFULL + s), (tile / VST) & 1);
-        wide_wait(p, bar(C::B_PFULL + x), (x ? px1 : px0) & 1);
+        wide_wait<D>(bar(C::B_VFULL + s), (tile / VST) & 1);
+        wide_wait<D>(bar(C::B_PFULL + x), (x ? px1 : px0) & 1);
         px0 += x ^ 1;
         px1 += x;
         tc_fence_after();
@@ -382,9 +396,8 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
         // Keys and values that would leave fp16's range (127 times a scale above 512) are divided by a power of two, one for the
         // warp's rows of a tile, which the logits or probabilities are multiplied by in turn.
         auto power = [&](float mine) {
-          if (!__any_sync(0xffffffffu, fabsf(mine) > 512.f)) return 1.f;
           const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(mine)));
-          return most < 0x7f800000u ? __uint_as_float(((most >> 23) - 8u) << 23) : 1.f;
+          return most > __float_as_uint(512.f) && most < 0x7f800000u ? __uint_as_float(((most >> 23) - 8u) << 23) : 1.f;
         };
         auto inverse = [&](float pow2) { return __uint_as_float((254u << 23) - __float_as_uint(pow2)); };
         // later_bits: the scales of the same tile's V, at its K
@@ -392,16 +405,19 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           const int st = v ? VST : KST, g = gt + j, s = g % st, rs = gr % C::RST;
           const unsigned char* src = sm + C::R0 + rs * C::RAW;
           unsigned char* dst = sm + (v ? C::V0 : C::K0) + s * TILE;
-          wide_wait(p, bar(C::B_RFULL + rs), (gr / C::RST) & 1);
-          if (g >= st) wide_wait(p, bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
+          wide_wait<D>(bar(C::B_RFULL + rs), (gr / C::RST) & 1);
+          if (g >= st) wide_wait<D>(bar((v ? C::B_VEMPTY : C::B_KEMPTY) + s), (g / st - 1) & 1);
           ++gr;
-          float mine = as_float(mine_bits);
-          const float range = power(mine);
-          mine *= inverse(range);
-          if (v == 0) {
-            const float later = power(as_float(later_bits));
+          float mine = as_float(mine_bits), range = 1.f, later = 1.f;
+          const float next = v == 0 ? as_float(later_bits) : 0.f;
+          if (__any_sync(0xffffffffu, fabsf(mine) > 512.f || fabsf(next) > 512.f)) {
+            range = power(mine);
+            later = power(next);
+            mine *= inverse(range);
+          }
+          if (v == 0 && lane == 0) {
             float* at = reinterpret_cast<float*>(sm + C::RANGE) + (g % C::RANGES) * 2 * W_CONVERTERS + warp - W_CONVERT;
-            if (lane == 0) at[0] = range, at[W_CONVERTERS] = later;
+            at[0] = range, at[W_CONVERTERS] = later;
           }
           auto rows = [&](auto fp32_scale) {
 #pragma unroll UNROLL
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       const int live = min(kWideRows, it.live - mine0);           // rows of it
       const bool busy = 32 * (warp & 3) < live;                   // this warp holds one
       // ---- Q: half a row a thread, converted to the operand type, swizzled
-      if (done[0] > 0) wide_wait(p, bar(C::B_QEMPTY), q_done & 1), ++q_done;
+      if (done[0] > 0) wide_wait<D>(bar(C::B_QEMPTY), q_done & 1), ++q_done;
 #pragma unroll 1
       for (int y = 0; y < (two ? 2 : 1); ++y) {
         const int row = tid >> 1, c0 = (tid & 1) * (D / 16);
@@ -516,14 +532,14 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
 
       float m_ref = -INFINITY, l = 0.f;
       for (int u = x; u < nu; u += 2) {
-        wide_wait(p, bar(C::B_SFULL + x), (done[x] + (u >> 1)) & 1);
+        wide_wait<D>(bar(C::B_SFULL + x), (done[x] + (u >> 1)) & 1);
         tc_fence_after();
         if (busy) {
           const int left = it.grp.x - (it.t + it.tile(u)) * kWideKeys;  // keys of this tile, maybe more than 128
           // first look: the row's maximum.  The logits are read again below: 128 of them do not fit the registers
           // beside the rest, and a second read of TMEM is cheap
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          // INT8: of the keys [32 c, 32 c + 32), then of the values
+          // INT8: the powers of the keys [32 c, 32 c + 32), then of the values
           static_assert(!I8 || kWideKeys / W_CONVERTERS == 32, "a converting warp's keys are those of one step below");
           const float* range = reinterpret_cast<const float*>(sm + C::RANGE) + (I8 ? (gt + it.tile(u)) % C::RANGES * 2 * W_CONVERTERS : 0);
 #pragma unroll
@@ -635,7 +651,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
           if (rb + k < live) *reinterpret_cast<uint4*>(p.part_o + (prow + rb + k) * D + col + 4 * (lane & 7)) = ov[k];
       };
       if (two) {
-        wide_wait(p, bar(C::B_ODONE + x), (done[x] - 1) & 1);  // the stream's last P*V
+        wide_wait<D>(bar(C::B_ODONE + x), (done[x] - 1) & 1);  // the stream's last P*V
         tc_fence_after();
         if (busy) {
 #pragma unroll 1
@@ -670,8 +686,8 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       const float f0 = x ? fo : fm, f1 = x ? fm : fo;
       // every stream's last P*V; past the exchange both have seen the S of their last unit, so that neither
       // barrier is more than one phase behind
-      wide_wait(p, bar(C::B_ODONE), (done[0] - 1) & 1);
-      if (both) wide_wait(p, bar(C::B_ODONE + 1), (done[1] - 1) & 1);
+      wide_wait<D>(bar(C::B_ODONE), (done[0] - 1) & 1);
+      if (both) wide_wait<D>(bar(C::B_ODONE + 1), (done[1] - 1) & 1);
       tc_fence_after();
       if (busy) {
         // this thread's stream names its half of the columns
@@ -730,12 +746,7 @@ bool prefix_wide_supported(int kv_kind, int D, int BS) {
   return (kv_kind == KV_F16 || kv_kind == KV_BF16 || kv_kind == KV_I8) && (D == 64 || D == 128) && BS >= 8;
 }
 
-cudaError_t launch_prefix_wide(const SharedParams& p_in, const KvMaps& maps, int kv_kind, int D, cudaStream_t stream) {
-  static std::atomic<unsigned int> generation{0};
-  SharedParams p = p_in;
-  do {
-    p.abort_gen = ++generation;
-  } while (p.abort_gen == 0);
+cudaError_t launch_prefix_wide(const SharedParams& p, const KvMaps& maps, int kv_kind, int D, cudaStream_t stream) {
   return D == 64 ? launch_wide_d<64>(p, maps, kv_kind, stream) : launch_wide_d<128>(p, maps, kv_kind, stream);
 }
 
