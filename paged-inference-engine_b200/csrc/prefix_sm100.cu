@@ -62,7 +62,7 @@ struct WideCfg {
   static constexpr int R0 = V0 + VST * TILE;
   static constexpr int BAR = R0 + RST * RAW;
   static constexpr int B_QREADY = 0, B_QEMPTY = 1, B_SFULL = 2, B_PFULL = 4, B_ODONE = 6, B_SLOT = 8, B_PLACE = 9,
-                       B_KFULL = 10, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
+                       B_LAST = 10, B_KFULL = 11, B_KEMPTY = B_KFULL + KST, B_VFULL = B_KEMPTY + KST, B_VEMPTY = B_VFULL + VST,
                        B_RFULL = B_VEMPTY + VST, B_REMPTY = B_RFULL + RST, B_END = B_REMPTY + RST;
   static constexpr int BARS = D == 128 ? 256 : 512;  // bytes of the barriers, and what a wait that gives up writes (16 bytes)
   static constexpr int RANGE = BAR + BARS;  // INT8: powers of two that keys and values were divided by
@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t scale_bits(const void* base, long long at, b
 
 // A wait that fails gave up, by itself or since another wait of this launch did (the plan clears their word in the call's workspace
 // on every run, a captured call's replays too).  A CTA then walks to its end without its results being good (the status
-// word says so); only the producer stops, and waits for its copies before the CTA ends.
+// word says so); the producer stops, and it and the issuer of the products wait for theirs before the CTA ends.
 // The addresses of their word and of the status word lie at the end of the barriers' block, which a barrier's address gives: so
 // a wait has no other arguments (with the parameters for one, 128 sequences of 4 heads over 65536 keys took 192 us, so 187).
 template <int D>
@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
   if (tid == 32) {
     mbar_init(bar(C::B_QREADY), 32 * W_SOFTMAX);
     mbar_init(bar(C::B_QEMPTY), 1);
+    mbar_init(bar(C::B_LAST), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(bar(C::B_SFULL + x), 1);
       mbar_init(bar(C::B_PFULL + x), 16 * W_SOFTMAX);
@@ -361,6 +362,10 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
       }
       gt += it.n;
     }
+    // No product is in flight when the CTA gives its tensor memory back and ends.  (The softmax has waited for the last ones,
+    // unless a wait of its gave up.)
+    tc_elect_commit(bar(C::B_LAST));
+    wide_drain(bar(C::B_LAST), 0);
   } else if (warp >= W_CONVERT) {
     // ------------------------------------------------------------ INT8 -> fp16 tiles
     if constexpr (I8) {
