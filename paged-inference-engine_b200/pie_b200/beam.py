@@ -129,6 +129,8 @@ class BeamSearch:
             rule.update(bias=self.bias, bias_row=rows if self.bias.shape[0] > 1 else None)
         if mask is not None:
             if mask.dim() == 3:
+                if tuple(mask.shape[:2]) not in ((B, K), (B, 1), (1, 1)):
+                    raise ValueError(f"mask must be [{B}, {K}, words], [{B}, words] or [words], got {tuple(mask.shape)}")
                 mask = mask.reshape(-1, mask.shape[-1])
             rule.update(mask=mask, mask_row=rows if mask.dim() == 2 and mask.shape[0] == B > 1 and K > 1 else None)
         out = torch.empty(B * K, V, dtype=torch.float32, device=logits.device)
