@@ -146,7 +146,7 @@ class DecodeStepGraph:
 
         ``seq_lens[i]``: tokens of sequence i including this step's;
         Beams of a search are refused (they are extended together, by ``BeamSearch``), and so is a position inside a
-        block that a fork shares: it would overwrite the other sequence's token.
+        block that a fork shares: it would overwrite the other sequence's token.  So is a position behind ``rope``'s last.
         ``q`` [n, Hq, D], ``k_new`` / ``v_new`` [n, Hkv, D] on the device.
         Returns O [n, Hq, D] (float16), a view of the graph's output buffer:
         consume it before the next ``step``.
@@ -160,6 +160,8 @@ class DecodeStepGraph:
             for sid, ln in zip(seq_ids, seq_lens):
                 if (int(ln) - 1) // self.BS < ledger.shared_columns(int(sid)):
                     raise ValueError(f"token {int(ln) - 1} of sequence {sid} lies in a block that another sequence holds")
+        if self.rope is not None and any(int(ln) > self.rope.shape[0] for ln in seq_lens):
+            raise ValueError(f"rope holds {self.rope.shape[0]} positions, a sequence would have {max(int(n) for n in seq_lens)} tokens")
         if self.graphs is None:
             self.capture()
         for sid, ln in zip(seq_ids, seq_lens):

@@ -50,3 +50,26 @@ def test_masks_of_each_shape():
         for seq in range(2):
             assert set(got[seq]) <= allowed[seq] | {0}, (tuple(mask.shape), got)  # (a finished beam goes on with 0)
         s.finish()
+
+
+def test_a_step_beyond_the_rotation_table():
+    """A position without a row of the table would leave the token out and attend to what its slot held."""
+    from pie_b200 import ops
+    from pie_b200.block_pool import DeviceBlockManager
+    from pie_b200.decode_step import DecodeStepGraph
+
+    BS, H, D, NB = 4, 1, 64, 20
+    k, v = (torch.zeros(NB, BS, H, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    pool = DeviceBlockManager(NB, BS, 4, 12)
+    pool.attach_caches(k, v)
+    graph = DecodeStepGraph(pool, k, v, None, None, 2, 2, rope=ops.rope_table(9, D, device="cuda"), share_prefixes=True)
+    pool.allocate(0, 2)
+    pool.allocate(1, 2)
+    q, kn, vn = (torch.randn(2, h, D, device="cuda").half() for h in (2, 1, 1))
+    graph.step([0, 1], [8, 9], q, kn, vn)
+    free, cache = pool.num_free_blocks(), k.clone()
+    with pytest.raises(ValueError, match="rope"):
+        graph.step([0, 1], [9, 10], q, kn, vn)
+    assert pool.num_free_blocks() == free and torch.equal(k, cache)
+    graph.step([0], [9], q[:1], kn[:1], vn[:1])
+    graph.check()
