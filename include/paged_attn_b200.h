@@ -63,6 +63,7 @@ enum {
   PA_STATUS_BAD_POSITION = 2,
   PA_STATUS_BAD_NUM_BLOCKS = 4,
   PA_STATUS_BAD_SEQ_INDEX = 8,
+  PA_STATUS_WAIT_TIMEOUT = 16, /* a kernel's wait for its own copies or products gave up: the outputs are not good */
   PA_STATUS_PEER_TIMEOUT = 32,
   PA_STATUS_COPY_OVERLAP = 64, /* a page copy into another copy's source or target  */
   PA_STATUS_BAD_POOL = 128     /* block pool arrays that contradict each other      */

@@ -28,6 +28,7 @@ PA_STATUS_BAD_BLOCK_ID = 1
 PA_STATUS_BAD_POSITION = 2
 PA_STATUS_BAD_NUM_BLOCKS = 4
 PA_STATUS_BAD_SEQ_INDEX = 8
+PA_STATUS_WAIT_TIMEOUT = 16
 PA_STATUS_PEER_TIMEOUT = 32
 PA_STATUS_COPY_OVERLAP = 64
 PA_STATUS_BAD_POOL = 128

@@ -227,6 +227,8 @@ def _raise_status_value(fn: str, v: int) -> None:
             bits.append("num_blocks_per_seq wider than the block table")
         if v & _lib.PA_STATUS_BAD_SEQ_INDEX:
             bits.append("sequence index outside the block table")
+        if v & _lib.PA_STATUS_WAIT_TIMEOUT:
+            bits.append("a wait inside a kernel gave up")
         if v & _lib.PA_STATUS_PEER_TIMEOUT:
             bits.append("a peer GPU never reached the output-exchange barrier")
         if v & _lib.PA_STATUS_COPY_OVERLAP:

@@ -10,7 +10,7 @@ from conftest import PKG, ROOT
 
 pytestmark = pytest.mark.gpu
 
-TIMEOUT = 16  # PA_STATUS: a bounded wait gave up
+TIMEOUT = 16  # PA_STATUS_WAIT_TIMEOUT
 
 SOURCE = """
 #include "bounded_wait.cuh"
