@@ -80,6 +80,38 @@ class _Prefix:
         self.n, self.holders, self.up = n, holders, up
 
 
+def _best_cuts(widths: Sequence[int]) -> list[int]:
+    """Where the runs begin into which ``len(widths) + 1`` neighbours are cut, ``widths[i]`` columns common to i and i + 1.
+
+    A run's columns are the fewest between its neighbours, and it saves them for all members but one.  With best[j] the most that the
+    first j save, best[j] = max(best[j - 1], best[i] + (j - 1 - i) w over the runs i..j-1 whose neighbours all share w or
+    more): for each w the largest best[i] - i w of the places i where such a run may have begun.
+    """
+    levels = sorted(set(widths))
+    if len(levels) > 16:  # some of them: still runs of what their members share, perhaps not the best
+        levels = [levels[i * (len(levels) - 1) // 15] for i in range(16)]
+    lead = [(0, 0)] * len(levels)  # of each level: best[i] - i w, i
+    best, begin = [0, 0], [0, 0]   # of the first j: what they save, where their last run begins
+    for j in range(2, len(widths) + 2):
+        most, first = best[j - 1], j - 1
+        for k, w in enumerate(levels):
+            if widths[j - 2] < w:  # a run over these two ends
+                lead[k] = (best[j - 1] - (j - 1) * w, j - 1)
+                continue
+            value = lead[k][0] + (j - 1) * w
+            if value > most:
+                most, first = value, lead[k][1]
+            if best[j - 1] - (j - 1) * w > lead[k][0]:
+                lead[k] = (best[j - 1] - (j - 1) * w, j - 1)
+        best.append(most)
+        begin.append(first)
+    cuts, j = [], len(widths) + 1
+    while j > 0:
+        cuts.append(begin[j])
+        j = begin[j]
+    return cuts[::-1]
+
+
 class BlockLedger:
     """Host half of the pool: the decisions the reference's BlockManager makes, without the ids.
 
@@ -206,31 +238,46 @@ class BlockLedger:
     def shared_runs(self, seq_ids: Sequence[int]) -> tuple[list[int], list[int]]:
         """Neighbours in ``seq_ids`` whose first columns are the same: (where each run begins, and the end; its columns).
 
-        A sequence joins the run before it where the run's sequences then read no fewer columns together than without it.
+        A run's columns are read once instead of once per member; the order is cut so that this saves the most columns
+        (``_best_cuts``; exactly so for up to 16 different widths between neighbours that share anything).
         """
-        starts, columns = [0], []
-        run: list[_Prefix] = []
-        width = 0
+        starts: list[int] = []
+        columns: list[int] = []
+        begin = 0                 # of the neighbours that share something
+        widths: list[int] = []    # shared by each of them and the one before
+        last: list[_Prefix] = []
+
+        def close(end: int) -> None:
+            if not widths:
+                starts.append(begin)
+                columns.append(0)
+                return
+            cuts = [0] if min(widths) == max(widths) else _best_cuts(widths)
+            for i, j in zip(cuts, [*cuts[1:], end - begin]):
+                starts.append(begin + i)
+                columns.append(min(widths[i:j - 1], default=0))
+
         for i, s in enumerate(seq_ids):
             path, node = [], self.prefix.get(s)
             while node is not None:
                 path.append(node)
                 node = node.up
             path.reverse()
-            n = i - starts[-1]
-            if n:
-                both = [a for a, b in zip(run, path) if a is b]
-                shared = sum(a.n for a in both)
-                if shared and shared * n >= width * (n - 1):
-                    run, width = both, shared
-                    continue
-                starts.append(i)
-                columns.append(width if n > 1 else 0)
-            run, width = path, sum(a.n for a in path)
+            if i:
+                width = 0
+                for x, y in zip(last, path):
+                    if x is not y:
+                        break
+                    width += x.n
+                if width:
+                    widths.append(width)
+                else:
+                    close(i)
+                    begin, widths = i, []
+            last = path
         if seq_ids:
-            columns.append(width if len(seq_ids) - starts[-1] > 1 else 0)
-            starts.append(len(seq_ids))
-        return starts, columns
+            close(len(seq_ids))
+        return [*starts, len(seq_ids)], columns
 
     def fork(self, parent_id: int, child_id: int, num_tokens: int, block_size: int) -> tuple[AllocStatus, int]:
         """The child gets the parent's first tokens: (status, the child's slot); queues the operation on success."""
