@@ -16,7 +16,8 @@ step with one graph replay:
      the new queries by their positions;
   4. paged attention of every sequence's new query over its whole cache, or with
      ``share_prefixes`` ``shared_prefix_attention``: sequences forked from one
-     another that stand side by side in a step read their common blocks once.
+     another that stand side by side in a step read their common blocks once
+     (one level of them: of forks of forks, what saves the most).
 
 Decode positions follow the sequence: a sequence holding ``n`` tokens after
 this step's append writes its new token at position ``n - 1`` and attends to
@@ -44,6 +45,7 @@ class DecodeStepGraph:
     """Decode rows of one attention layer as a captured CUDA graph (see the module docstring)."""
 
     PAD_SEQ = -1  # the reserved padding sequence's id in the pool
+    rope: Optional[torch.Tensor] = None
 
     def __init__(self, pool: DeviceBlockManager, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], num_q_heads: int, max_seqs: int,
