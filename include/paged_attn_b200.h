@@ -257,7 +257,12 @@ int paged_attn_varlen(const pa_attn_io_t* io, const pa_kv_cache_t* kv, const pa_
  * group_start[g] .. group_start[g + 1] - 1 of the batch are group g, and the
  * first prefix_len[g] keys of all of them are the same: their block tables name
  * the same blocks there, as block_pool_apply_shared's forks do.  The result is
- * that of paged_attn_forward up to the order of sums.
+ * that of paged_attn_forward up to the order of sums and to roundings: as there,
+ * probabilities take the pool's 16-bit type (fp16 for I8 pools); beyond 16
+ * (sequence, query row, group head) rows in the batch, I8 keys and values of a
+ * shared part, code times scale, and Q of another type than the pool's (bf16 for I8 pools) are rounded
+ * to it too, where paged_attn_forward keeps codes as they are.  Shared I8 values go up
+ * to 127 * 65536 in magnitude, keys as far as fp32; bf16 Q over F16 and I8 pools to 65504.
  *   group_start   int32 [num_groups + 1] on the device, rising, within 0..num_seqs
  *                 (else nothing is shared and PA_STATUS_BAD_SEQ_INDEX is set);
  *                 sequences outside every group share nothing

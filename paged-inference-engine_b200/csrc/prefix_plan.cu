@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(1024) prefix_plan_kernel(const SharedParams p)
     scan_cta(s_unit, G, s_warp);
     for (int g = tid; g <= G; g += T) p.step0[g] = s_unit[g];
     // (Runs made longer, so that none crosses from one list entry into the next, left more teams idle than the crossings
-    // cost: 54 against 51 us for 64 sequences over 8192 keys, 125 against 116 for 4 groups of 32 over 16384 INT8 keys.)
+    // cost: 54 against 50-51 us for 64 sequences over 8192 keys, 125 against 113-116 for 4 groups of 32 over 16384 INT8 keys.)
     if (tid == 0) p.head[0] = make_int4(team, (s_unit[G] + teams - 1) / teams, s_unit[G], 0);  // no wait has given up
   }
 

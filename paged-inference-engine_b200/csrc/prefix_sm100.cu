@@ -30,10 +30,12 @@
 // unrounded probabilities) and outputs stay in fp32 until the join.  INT8 keys may lie beyond fp16's range, and values up to
 // 127 * 65536 (RANGE); it is the range of bf16 queries over fp16 and INT8 pools, as of the outputs.
 //
-// 16-bit pools: bound by HBM up to about 256 rows a kv head, by the issue of the two products beyond (128 keys of 128 rows
-// take 1995 cycles; 128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 51 %, the exponentials' unit 51 %).
-// INT8 pools: by the conversion of the tiles, 1100 cycles each; eight warps for it left 96 registers a thread and
-// gained nothing.
+// 16-bit pools with many rows: 128 keys of 128 rows take 1995 cycles, about 1000 of the products and 1000 of the exponentials, one
+// after the other for most of it (128 sequences of 4 heads over 65536 bf16 keys: tensor pipe 49 %, the exponentials'
+// unit 50 %, DRAM 24 %).  With few rows (64 sequences of 4 heads over 8192 fp16 keys: 20 %, 21 %, 14 %) by latency: the first tiles, and pieces
+// of 256 rows that every CTA writes.
+// INT8 pools: by the conversion of the tiles, 1100 cycles each (tensor pipe 21 %, issue slots 40 %); eight warps for
+// it left 96 registers a thread and gained nothing.
 #include <type_traits>
 
 #include "bounded_wait.cuh"
@@ -56,7 +58,7 @@ struct WideCfg {
   static constexpr int RAW = 128 * D;              // int8 tile
   static constexpr int KST = D == 128 ? (I8 ? 2 : 3) : (I8 ? 3 : 5);  // K stages
   static constexpr int VST = D == 128 ? 2 : (I8 ? 3 : 5);               // V stages
-  static constexpr int RST = I8 ? (D == 128 ? 2 : 8) : 0;  // raw tiles in flight, K and V alternating (4 and one V stage: 120 us, so 115)
+  static constexpr int RST = I8 ? (D == 128 ? 2 : 8) : 0;  // raw tiles in flight, K and V alternating (4 and one V stage: 120 us where this took 115)
   static constexpr int K0 = 2 * TILE;
   static constexpr int V0 = K0 + KST * TILE;
   static constexpr int R0 = V0 + VST * TILE;
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(WideCfg<D, I8>::THREADS, 1)
   } else if (warp >= W_CONVERT) {
     // ------------------------------------------------------------ INT8 -> fp16 tiles
     if constexpr (I8) {
-      // Warp c converts rows 16 c .. 16 c + 15 of every tile; lane l holds the scales of row 16 c + l % 16.  A lane takes 16
+      // Warp c converts rows ROWS c .. ROWS c + ROWS - 1 of every tile; lane l holds the scales of row ROWS c + l % ROWS.  A lane takes 16
       // dims of a row at a time.  The eight lanes that a shared-memory access serves at once are four pieces of rows a
       // and a ^ 5: swizzled, those lie in different banks, in the raw tile (16 bytes a piece) as in the operand tile (twice
       // 16 bytes, two apart).
